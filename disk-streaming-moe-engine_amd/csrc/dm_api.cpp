@@ -56,9 +56,10 @@ hipEvent_t g_noalloc_ev[kMaxDevices];
 bool g_noalloc_recorded[kMaxDevices];
 std::mutex g_scratch_mu;
 // first-error key slots: [0, kMaxLayers) uploaded 4-bit layers, kMaxLayers
-// the unit calls, then one per GGUF layer
+// the unit calls, then one per GGUF layer, then the token mixer's calls
 constexpr int kGgufSlot0 = kMaxLayers + 1;
-constexpr int kStatusSlots = kGgufSlot0 + kMaxLayers;
+constexpr int kMixerSlot = kGgufSlot0 + kMaxLayers;
+constexpr int kStatusSlots = kMixerSlot + 1;
 
 // One MoE layer uploaded from a GGUF file: one device block holding the fp32
 // router and shared gate, the expert offset table and the expert payloads.
@@ -280,6 +281,19 @@ struct dmh_ctx {
   long spin_limit = dm::kDefaultSpinLimit;
   // host-pointer calls rerun through the multi-kernel path after a time-out
   int64_t sync_fallbacks = 0;
+  // the token mixer's device memory, and what grew out of use but is held by
+  // captured graphs
+  struct MixerBuf {
+    void* p = nullptr;
+    size_t cap = 0;
+    bool captured = false;
+  } mixer[dm::kMixerBuffers];
+  std::vector<void*> mixer_held;
+  ~dmh_ctx() {
+    for (const MixerBuf& b : mixer)
+      if (b.p) (void)hipFree(b.p);
+    for (void* p : mixer_held) (void)hipFree(p);
+  }
 };
 
 namespace {
@@ -397,6 +411,50 @@ int dm::api_moe_dims_check(const dmh_moe_dims* d, int layer, char* err, size_t e
                    " E=%d K=%d I=%d Ish=%d (need G in {32, 64, 128, 256}, H/I/Ish multiples of"
                    " 128, E<=2048, K<=32, H/I/Ish<=8192)\",\"stage\":\"config\",\"layer\":%d}",
                    G, H, E, K, I, Ish, layer);
+  return DMH_OK;
+}
+
+int dm::api_mixer_begin(dmh_ctx* c, hipStream_t* st, unsigned long long** status, char* err,
+                        size_t errlen) {
+  HIP_TRY(hipSetDevice(c->device));
+  *st = c->cur;
+  *status = c->status + kMixerSlot;
+  return DMH_OK;
+}
+
+int dm::api_mixer_buffer(dmh_ctx* c, MixerBuffer which, size_t bytes, void** p, char* err,
+                         size_t errlen) {
+  auto& b = c->mixer[which];
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  HIP_TRY(hipStreamIsCapturing(c->cur, &cap));
+  const bool capturing = cap != hipStreamCaptureStatusNone;
+  if (bytes > b.cap) {
+    if (capturing)
+      return set_err(err, errlen, DMH_ERR_INVALID_ARG,
+                     "{\"error_type\":\"CONFIG_ERROR\",\"detail\":\"the call needs %zu bytes of"
+                     " device memory, which a captured call cannot allocate: make a call of its"
+                     " sizes before the capture\",\"stage\":\"mixer\"}", bytes);
+    if (b.p && b.captured) {
+      try {
+        c->mixer_held.push_back(b.p);
+      } catch (const std::bad_alloc&) {
+        return set_err(err, errlen, DMH_ERR_NO_MEMORY, "out of host memory");
+      }
+    } else if (b.p) {
+      (void)hipFree(b.p);  // (waits for the work queued on it)
+    }
+    b = {};
+    const hipError_t e = dev_malloc(&b.p, bytes);
+    if (e != hipSuccess) {
+      b.p = nullptr;
+      (void)hipGetLastError();  // (the failed allocation is not the next launch's error)
+      return set_err(err, errlen, DMH_ERR_NO_MEMORY, "hipMalloc(%zu): %s", bytes,
+                     hipGetErrorString(e));
+    }
+    b.cap = bytes;
+  }
+  b.captured = b.captured || capturing;
+  *p = b.p;
   return DMH_OK;
 }
 
@@ -952,7 +1010,7 @@ int dmh_sync(dmh_ctx* c, char* err, size_t errlen) {
   HIP_TRY(hipMemcpy(keys.data(), c->status, sizeof(unsigned long long) * keys.size(),
                     hipMemcpyDeviceToHost));
   int rc = DMH_OK;
-  for (int l = kGgufSlot0; l < kStatusSlots && rc == DMH_OK; ++l)
+  for (int l = kGgufSlot0; l < kMixerSlot && rc == DMH_OK; ++l)
     if (keys[l] != dm::kNoError) rc = gguf_finish(c, l - kGgufSlot0, keys[l], err, errlen);
   for (int l = 0; l <= kMaxLayers && rc == DMH_OK; ++l) {
     Layer* Ly = l < (int)c->layers.size() ? c->layers[l] : nullptr;
@@ -969,6 +1027,8 @@ int dmh_sync(dmh_ctx* c, char* err, size_t errlen) {
     }
     rc = finish_status(c, Ly, l, key, ids.empty() ? nullptr : ids.data(), err, errlen, idk);
   }
+  if (rc == DMH_OK && keys[kMixerSlot] != dm::kNoError)
+    rc = dm::api_mixer_error(keys[kMixerSlot], err, errlen);
   HIP_TRY(hipMemset(c->status, 0xFF, sizeof(unsigned long long) * keys.size()));
   return rc;
 }

@@ -96,6 +96,7 @@ enum : uint32_t {
   kPhSync = 0,  // a wait between workgroups gave up: the outputs are not valid
   kPhX = 1, kPhRouterW = 2, kPhLogit = 3, kPhSoftmax = 4, kPhTopk = 5,
   kPhExpert = 6, kPhShared = 7, kPhGate = 8, kPhAgg = 9,
+  kPhSeq = 10,  // a mixer call's sequences, pos: the sequence (a status word of their own)
 };
 enum : uint32_t {  // kinds
   kTkSum = 0, kTkLeak = 1,                          // top-k
@@ -103,6 +104,7 @@ enum : uint32_t {  // kinds
   kEkBadId = 4,     // an expert id outside [0, E) given to the experts entry point
   kEkRecheck = 15,  // fused decode: a non-finite output whose first failing check is re-derived
   kGkLogit = 0, kGkRange = 1,                       // shared gate
+  kSqOffsets = 0, kSqLength = 1, kSqSlot = 2, kSqTwice = 3, kSqCount = 4,  // sequences
 };
 constexpr uint64_t kNoError = ~0ull;
 

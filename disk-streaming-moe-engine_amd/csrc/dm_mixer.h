@@ -1,0 +1,35 @@
+// dm_mixer.h -- host-side launchers of the token mixer's kernels: the short
+// convolution and the norms (dm_mixer.hip), the gated delta rule row by row
+// (dm_mixer.hip) and in chunks (dm_delta.hip).
+//
+// Every array is device memory; sizes, strides and alignment have been checked
+// (dm_mixer_api.cpp).  What only the device knows, the sequences, is checked by
+// the kernels (seq_range) before any row or state is touched.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/dismoen_hip.h"
+
+namespace dm {
+
+// dmh_seq_batch on the device.
+struct SeqDev {
+  int num, rows, max_len, slots_n;
+  const int32_t* off;
+  const int32_t* slots;
+  const int32_t* fresh;
+  unsigned long long* status;
+};
+
+// `wide`: the rows, their strides and the state are aligned for 16-byte
+// accesses.
+hipError_t launch_short_conv(const dmh_short_conv& a, const SeqDev& s, bool wide, hipStream_t st);
+hipError_t launch_gated_norm(const dmh_gated_norm& a, bool wide, hipStream_t st);
+
+// Sequences of at most max_rows rows (the others are left alone).
+hipError_t launch_delta_rows(const dmh_gated_delta& a, const SeqDev& s, int max_rows, bool wide,
+                             hipStream_t st);
+
+}  // namespace dm

@@ -37,7 +37,8 @@ EXPORTS = (
     "dmh_gguf_read", "dmh_dequant_gguf", "dmh_gguf_stream_tensor_f32",
     "dmh_upload_moe_layer_gguf", "dmh_free_layer_gguf", "dmh_moe_forward_gguf",
     "dmh_set_layer_norm", "dmh_port_moe_forward", "dmh_moe_forward_noalloc",
-    "dmh_set_spin_limit", "dmh_sync_fallbacks", "dmh_xcd_rotation",
+    "dmh_set_spin_limit", "dmh_sync_fallbacks", "dmh_xcd_rotation", "dmh_short_conv_forward",
+    "dmh_gated_delta_forward", "dmh_gated_norm_forward",
 )
 
 
@@ -70,6 +71,39 @@ class DmhGgufHeader(C.Structure):
     _fields_ = [("version", C.c_int32), ("tensor_count", C.c_int64),
                 ("metadata_kv_count", C.c_int64), ("data_section_offset", C.c_int64),
                 ("expected_file_size", C.c_int64), ("alignment", C.c_int64)]
+
+
+class DmhSeqBatch(C.Structure):
+    _fields_ = [("num_seqs", C.c_int32), ("total_tokens", C.c_int32), ("max_seq_len", C.c_int32),
+                ("num_slots", C.c_int32), ("offsets", C.c_void_p), ("slots", C.c_void_p),
+                ("fresh", C.c_void_p)]
+
+
+class DmhShortConv(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("channels", C.c_int32), ("width", C.c_int32),
+                ("silu", C.c_int32), ("x", C.c_void_p), ("x_stride", C.c_int64),
+                ("weight", C.c_void_p), ("bias", C.c_void_p), ("state", C.c_void_p),
+                ("y", C.c_void_p), ("y_stride", C.c_int64)]
+
+
+class DmhGatedDelta(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "k_heads", "v_heads", "k_dim", "v_dim",
+                                          "qk_norm")]
+                + [("eps", C.c_float), ("scale", C.c_float)]
+                + [(n, C.c_void_p) for n in "qkvab"]
+                + [(n + "_stride", C.c_int64) for n in "qkvab"]
+                + [("a_log", C.c_void_p), ("dt_bias", C.c_void_p), ("state", C.c_void_p),
+                   ("o", C.c_void_p), ("o_stride", C.c_int64)])
+
+
+class DmhGatedNorm(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "stream_dtype", "rows", "groups", "dim", "post",
+                                          "gate_act")]
+                + [("scale", C.c_float), ("eps", C.c_float)]
+                + [(n, C.c_void_p) for n in ("x", "gate", "residual", "stream", "y")]
+                + [(n, C.c_int64) for n in ("x_stride", "gate_stride", "residual_stride",
+                                            "stream_stride", "y_stride")]
+                + [(n, C.c_void_p) for n in ("gamma", "edge_gamma", "scale_vec")])
 
 
 class DismoenError(RuntimeError):
@@ -156,6 +190,9 @@ def lib():
     L.dmh_set_layer_norm.argtypes = [vp, i32, vp, i32, u32, C.c_char_p, sz]
     L.dmh_port_moe_forward.argtypes = [vp, i32, vp, i32, C.c_float, vp, vp, vp, vp, u32,
                                        C.c_char_p, sz]
+    L.dmh_short_conv_forward.argtypes = [vp, vp, vp, u32, vp, sz]
+    L.dmh_gated_delta_forward.argtypes = [vp, vp, vp, u32, vp, sz]
+    L.dmh_gated_norm_forward.argtypes = [vp, vp, u32, vp, sz]
     _lib = L
     return L
 

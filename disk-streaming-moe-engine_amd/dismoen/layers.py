@@ -86,6 +86,7 @@ class MoEBlock:
         e = errbuf()
         check(self._lib.dmh_create(device, C.byref(h), e, len(e)), e)
         self._h = h
+        self.device = device
         self.dims = {}
         self.gguf_dims = {}
         self._ebuf = None  # error buffer reused by forward_into

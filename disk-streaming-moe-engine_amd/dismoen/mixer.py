@@ -1,0 +1,351 @@
+"""The token mixer of the port block's linear-attention layers over libdismoen_hip.so.
+
+Between the mixer's two projections (src/layers/port_scheduler.mojo:286-372):
+  ShortConv        causal depthwise convolution with a state per sequence
+  GatedDelta       the gated delta rule with a state per sequence
+  GatedNorm        norms after and before a block, with its gate and residual
+  GatedDeltaMixer  the three together, as a layer runs them
+A SeqBatch says which rows are which sequence's.  An operator is made once per
+layer, with its weights, and called once per step.
+
+Arrays are torch tensors on the block's device (the call is queued on the
+block's stream and returns at once; errors in the sequences are reported by
+MoEBlock.sync()), or numpy arrays, all of them (the call is synchronous; bf16
+rows are their uint16 bit patterns).  Outputs are arrays of the caller's.  A
+block's stream is its own: order work of other streams against it, or give it
+theirs (MoEBlock.set_stream).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from ._lib import (DMH_F_DEVICE, DismoenError, DmhGatedDelta, DmhGatedNorm, DmhSeqBatch,
+                   DmhShortConv, check, errbuf)
+
+F32, F16, BF16 = 0, 1, 2
+GATES = {None: 0, "silu": 1, "sigmoid": 2}
+_NP = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint16): BF16}
+_TORCH: dict = {}
+
+
+def _torch_types():
+    import torch
+    _TORCH.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    return _TORCH
+
+
+def _bad(text: str) -> DismoenError:
+    return DismoenError(1, '{"error_type":"CONFIG_ERROR","detail":"' + text + '","stage":"mixer"}')
+
+
+def _type(a) -> int:
+    t = _NP.get(a.dtype) if isinstance(a, np.ndarray) else (_TORCH or _torch_types()).get(a.dtype)
+    if t is None:
+        raise _bad(f"rows are float32, float16 or bfloat16, not {a.dtype}")
+    return t
+
+
+def _packed(a, dims: int) -> bool:
+    """Whether the last `dims` dimensions lie one behind the other."""
+    want = 1
+    for n, s in zip(reversed(a.shape[-dims:]), reversed(_strides(a)[-dims:])):
+        if n != 1 and s != want:
+            return False
+        want *= n
+    return True
+
+
+def _strides(a):
+    return tuple(s // a.itemsize for s in a.strides) if isinstance(a, np.ndarray) else a.stride()
+
+
+def _address(a, device: int):
+    """(address, whether it is device memory)."""
+    if isinstance(a, np.ndarray):
+        return a.ctypes.data, False
+    if not a.is_cuda or a.device.index != device:
+        raise _bad(f"tensors must be on the block's device, cuda:{device}")
+    return a.data_ptr(), True
+
+
+class _Operator:
+    """A call's argument block, filled field by field; checks that all of its
+    arrays are on one side."""
+
+    def __init__(self, blk):
+        self._blk = blk
+        self._err = errbuf()
+        self._host = None  # numpy (True), torch (False), not known yet (None)
+        self._kept = []
+
+    def _side(self, a):
+        p, dev = _address(a, self._blk.device)
+        if self._host is None:
+            self._host = not dev
+        elif self._host is dev:
+            raise _bad("numpy arrays and device tensors in one call")
+        return p
+
+    def _weight(self, a, shape, what):
+        """The address of an fp32 weight that the operator keeps."""
+        if a is None:
+            return None
+        if tuple(a.shape) != shape or _type(a) != F32 or not _packed(a, len(shape)):
+            raise _bad(f"{what} must be a contiguous float32 array of shape {list(shape)}")
+        self._kept.append(a)
+        return self._side(a)
+
+    def _rows(self, a, shape, dtype, what):
+        """(address, stride between rows) of a row array [rows][...]."""
+        if tuple(a.shape[1:]) != shape or _type(a) != dtype or not _packed(a, len(shape)):
+            raise _bad(f"{what} must be rows of shape {list(shape)}, packed, of the call's type")
+        width = 1
+        for n in shape:
+            width *= n
+        return self._side(a), max(_strides(a)[0], width) if a.shape[0] <= 1 else _strides(a)[0]
+
+    def _state(self, a, shape, dtype, what, batch):
+        if tuple(a.shape) != (batch.num_slots, *shape) or _type(a) != dtype \
+                or not _packed(a, a.ndim):
+            raise _bad(f"{what} must be a contiguous array [num_slots]{list(shape)}")
+        return self._side(a)
+
+    def _flags(self, batch=None):
+        if batch is not None and batch.host is not self._host:
+            raise _bad("numpy arrays and device tensors in one call")
+        return 0 if self._host else DMH_F_DEVICE
+
+
+class SeqBatch:
+    """The sequences of a step: rows offsets[i] .. offsets[i + 1] - 1 are sequence
+    i's, its state is state slots[i] (None: i; negative: the sequence is
+    skipped), and one marked in `fresh` starts from zeros.  offsets, slots and
+    fresh are int32, torch tensors or numpy arrays; total_tokens and max_len
+    bound the rows and any sequence's length.  The arrays are read by each call,
+    so their values may change between steps."""
+
+    def __init__(self, offsets, total_tokens: int, max_len: int, num_slots: int, slots=None,
+                 fresh=None):
+        n = offsets.shape[0] - 1
+        self.total_tokens, self.num_slots = int(total_tokens), int(num_slots)
+        self.host = isinstance(offsets, np.ndarray)
+        self.arrays = (offsets, slots, fresh)
+        ptrs = []
+        for a, want, what in ((offsets, n + 1, "offsets"), (slots, n, "slots"),
+                              (fresh, n, "fresh")):
+            if a is None:
+                ptrs.append(None)
+                continue
+            if a.ndim != 1 or a.shape[0] != want or str(a.dtype).split(".")[-1] != "int32" \
+                    or not _packed(a, 1) or isinstance(a, np.ndarray) is not self.host:
+                raise _bad(f"{what} must be {want} int32 values on the side of offsets")
+            if not self.host and (not a.is_cuda or a.device != offsets.device):
+                raise _bad(f"{what} must be on the device")
+            ptrs.append(a.ctypes.data if self.host else a.data_ptr())
+        self._c = DmhSeqBatch(n, self.total_tokens, int(max_len), self.num_slots, *ptrs)
+        self._ref = C.addressof(self._c)
+
+    def _rows_in(self, a, what):
+        if a.shape[0] < self.total_tokens:
+            raise _bad(f"{what} has fewer rows than total_tokens")
+
+
+class ShortConv(_Operator):
+    """Causal depthwise convolution: weight [channels][width] and bias [channels]
+    fp32, SiLU where `silu`."""
+
+    def __init__(self, blk, weight, bias=None, silu: bool = True):
+        super().__init__(blk)
+        if weight.ndim != 2:
+            raise _bad("weight must be [channels][width]")
+        self.channels, self.width = weight.shape
+        a = self._c = DmhShortConv()
+        a.channels, a.width, a.silu = self.channels, self.width, int(silu)
+        a.weight = self._weight(weight, (self.channels, self.width), "weight")
+        a.bias = self._weight(bias, (self.channels,), "bias")
+        self._ref = C.addressof(a)
+
+    def __call__(self, x, state, batch: SeqBatch, out):
+        """out[t] for the rows x [rows][channels]; state [num_slots][width - 1]
+        [channels], the last rows of each sequence, is brought up to date."""
+        a, shape = self._c, (self.channels,)
+        a.dtype = t = _type(x)
+        a.x, a.x_stride = self._rows(x, shape, t, "x")
+        a.y, a.y_stride = self._rows(out, shape, t, "out")
+        a.state = self._state(state, (self.width - 1, self.channels), t, "state", batch)
+        batch._rows_in(x, "x")
+        batch._rows_in(out, "out")
+        e = self._err
+        rc = self._blk._lib.dmh_short_conv_forward(self._blk.handle, self._ref, batch._ref,
+                                                   self._flags(batch), e, len(e))
+        if rc:
+            check(rc, e)
+        return out
+
+
+class GatedDelta(_Operator):
+    """The gated delta rule on v_heads heads (v_heads / k_heads of them share a
+    key head).  With a_log [v_heads] the gates come raw: log decay =
+    -exp(a_log) softplus(a + dt_bias), beta = sigmoid(b); without it a is the log
+    decay and b is beta, in fp32.  scale: None is k_dim ** -0.5."""
+
+    def __init__(self, blk, k_heads: int, v_heads: int, k_dim: int, v_dim: int, a_log=None,
+                 dt_bias=None, qk_norm: bool = True, eps: float = 1e-6, scale: float | None = None):
+        super().__init__(blk)
+        a = self._c = DmhGatedDelta()
+        a.k_heads, a.v_heads, a.k_dim, a.v_dim = k_heads, v_heads, k_dim, v_dim
+        a.qk_norm, a.eps = int(qk_norm), eps
+        a.scale = k_dim ** -0.5 if scale is None else scale
+        a.a_log = self._weight(a_log, (v_heads,), "a_log")
+        a.dt_bias = self._weight(dt_bias, (v_heads,), "dt_bias")
+        self._raw = a_log is not None
+        self._k, self._v, self._g = (k_heads, k_dim), (v_heads, v_dim), (v_heads,)
+        self._s = (v_heads, k_dim, v_dim)
+        self._ref = C.addressof(a)
+
+    def __call__(self, q, k, v, a, b, state, batch: SeqBatch, out):
+        """out[t] [v_heads][v_dim] for rows q, k [rows][k_heads][k_dim], v
+        [rows][v_heads][v_dim] and gates a, b [rows][v_heads]; state [num_slots]
+        [v_heads][k_dim][v_dim] fp32 is brought up to date."""
+        c = self._c
+        c.dtype = t = _type(v)
+        g = t if self._raw else F32
+        c.q, c.q_stride = self._rows(q, self._k, t, "q")
+        c.k, c.k_stride = self._rows(k, self._k, t, "k")
+        c.v, c.v_stride = self._rows(v, self._v, t, "v")
+        c.a, c.a_stride = self._rows(a, self._g, g, "a")
+        c.b, c.b_stride = self._rows(b, self._g, g, "b")
+        c.o, c.o_stride = self._rows(out, self._v, t, "out")
+        c.state = self._state(state, self._s, F32, "state", batch)
+        n = batch.total_tokens
+        if min(q.shape[0], k.shape[0], v.shape[0], a.shape[0], b.shape[0], out.shape[0]) < n:
+            raise _bad("a row array has fewer rows than total_tokens")
+        e = self._err
+        rc = self._blk._lib.dmh_gated_delta_forward(self._blk.handle, self._ref, batch._ref,
+                                                    self._flags(batch), e, len(e))
+        if rc:
+            check(rc, e)
+        return out
+
+
+class GatedNorm(_Operator):
+    """Norms after and before a block with its gate and residual, over rows of
+    `groups` groups of `dim`:
+      u      = rmsnorm(x) * gamma where `post`, else x; times silu or sigmoid of the gate
+      stream = residual + scale * u      (scale: a number, or [groups][dim])
+      y      = rmsnorm(stream) * edge_gamma where `edge`"""
+
+    def __init__(self, blk, dim: int, groups: int = 1, gamma=None, edge_gamma=None,
+                 post: bool = True, edge: bool = False, gate: str | None = None, scale=1.0,
+                 eps: float = 1e-6):
+        super().__init__(blk)
+        if gate not in GATES:
+            raise _bad("gate must be None, silu or sigmoid")
+        if (gamma is not None and not post) or (edge_gamma is not None and not edge):
+            raise _bad("gamma without post, or edge_gamma without edge")
+        a = self._c = DmhGatedNorm()
+        a.groups, a.dim, a.post, a.gate_act, a.eps = groups, dim, int(post), GATES[gate], eps
+        a.gamma = self._weight(gamma, (dim,), "gamma")
+        a.edge_gamma = self._weight(edge_gamma, (dim,), "edge_gamma")
+        if isinstance(scale, (int, float)):
+            a.scale = scale
+        else:
+            a.scale = 1.0
+            a.scale_vec = self._weight(scale, (groups, dim), "scale")
+        self._shape, self._edge, self._gate = (groups, dim), edge, gate is not None
+        self._ref = C.addressof(a)
+
+    def __call__(self, x, stream=None, y=None, gate=None, residual=None):
+        """Writes stream and (where `edge`) y, arrays of the rows' shape [rows]
+        [groups][dim]; stream may be the residual itself."""
+        if (gate is None) == self._gate or (y is None) == self._edge:
+            raise _bad("gate and y are given exactly where the operator has them")
+        a, shape, n = self._c, self._shape, x.shape[0]
+        a.dtype = t = _type(x)
+        out = y if stream is None else stream
+        if out is None:
+            raise _bad("neither stream nor y is given")
+        a.stream_dtype = st = _type(out)
+        a.rows = n
+        a.x, a.x_stride = self._rows(x, shape, t, "x")
+        a.gate, a.gate_stride = self._rows(gate, shape, t, "gate") if self._gate else (None, 0)
+        a.residual, a.residual_stride = ((None, 0) if residual is None
+                                         else self._rows(residual, shape, st, "residual"))
+        a.stream, a.stream_stride = ((None, 0) if stream is None
+                                     else self._rows(stream, shape, st, "stream"))
+        a.y, a.y_stride = (None, 0) if y is None else self._rows(y, shape, st, "y")
+        for r in (gate, residual, stream, y):
+            if r is not None and r.shape[0] != n:
+                raise _bad("the row arrays differ in their rows")
+        e = self._err
+        rc = self._blk._lib.dmh_gated_norm_forward(self._blk.handle, self._ref, self._flags(), e,
+                                                   len(e))
+        if rc:
+            check(rc, e)
+        return stream, y
+
+
+class GatedDeltaMixer:
+    """One linear-attention layer between its projections: the convolution over
+    the mixed rows [q | k | v], the gated delta rule, and the norm of each head's
+    output, gated by silu(z).  conv_state [num_slots][width - 1][channels] and
+    state [num_slots][v_heads][k_dim][v_dim] belong to the caller."""
+
+    def __init__(self, blk, k_heads: int, v_heads: int, k_dim: int, v_dim: int, conv_weight,
+                 a_log, dt_bias, norm_gamma, conv_bias=None, eps: float = 1e-6):
+        self.channels = 2 * k_heads * k_dim + v_heads * v_dim
+        self.k, self.v = (k_heads, k_dim), (v_heads, v_dim)
+        self.conv = ShortConv(blk, conv_weight, bias=conv_bias)
+        if self.conv.channels != self.channels:
+            raise _bad(f"conv_weight must have {self.channels} channels")
+        self.delta = GatedDelta(blk, k_heads, v_heads, k_dim, v_dim, a_log=a_log, dt_bias=dt_bias,
+                                eps=eps)
+        self.norm = GatedNorm(blk, v_dim, v_heads, gamma=norm_gamma, gate="silu", eps=eps)
+
+    def __call__(self, mixed, z, b, a, conv_state, state, batch: SeqBatch, work, out):
+        """out [rows][v_heads][v_dim], the input of the output projection, from the
+        input projection's rows mixed [rows][channels], z [rows][v_heads][v_dim]
+        and b, a [rows][v_heads].  work: rows like mixed, overwritten.  What out
+        holds in rows of no sequence has no meaning."""
+        n, kw = batch.total_tokens, self.k[0] * self.k[1]
+        work, out = work[:n], out[:n]
+        self.conv(mixed, conv_state, batch, work)
+        if isinstance(work, np.ndarray):
+            q, k, v = (np.lib.stride_tricks.as_strided(
+                work[:, at:], (n, *s), (work.strides[0], s[1] * work.itemsize, work.itemsize))
+                for at, s in ((0, self.k), (kw, self.k), (2 * kw, self.v)))
+        else:
+            q, k, v = (work[:, at:at + s[0] * s[1]].unflatten(1, s)
+                       for at, s in ((0, self.k), (kw, self.k), (2 * kw, self.v)))
+        self.delta(q, k, v, a, b, state, batch, out)
+        self.norm(out, out, gate=z[:n])
+        return out
+
+
+class PortBlock:
+    """forward_port_block (src/layers/port_scheduler.mojo:286-482) on fp32 device
+    rows, its token mixer the caller's:
+      x_mid = x + mix(rmsnorm(x) * input_gamma)
+      y     = x_mid + MoE(rmsnorm(x_mid) * post_gamma)
+    with the MoE section of an uploaded 4-bit layer.  The mixer's residual and the
+    MoE section's norm are one pass."""
+
+    def __init__(self, blk, layer_idx: int, input_gamma=None, post_gamma=None, eps: float = 1e-6):
+        self._blk, self._layer = blk, layer_idx
+        self._h = h = blk.dims[layer_idx][0]
+        self._before = GatedNorm(blk, h, post=False, edge=True, edge_gamma=input_gamma, eps=eps)
+        self._after = GatedNorm(blk, h, post=False, edge=True, edge_gamma=post_gamma, eps=eps)
+
+    def __call__(self, x, mix, xn, x_mid, y):
+        """x, xn, x_mid, y [rows][hidden] fp32 device tensors (xn and x_mid are
+        overwritten); mix(xn) -> the mixer's output rows [rows][hidden], in fp32,
+        fp16 or bf16."""
+        rows = (x.shape[0], 1, self._h)
+        self._before(x.view(rows), y=xn.view(rows))
+        out = mix(xn)
+        self._after(out.reshape(rows), x_mid.view(rows), xn.view(rows), residual=x.view(rows))
+        self._blk.forward_device(self._layer, xn.data_ptr(), x.shape[0], y.data_ptr(),
+                                 residual_ptr=x_mid.data_ptr())
+        return y

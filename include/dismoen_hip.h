@@ -445,6 +445,143 @@ int dmh_moe_forward_gguf(dmh_ctx* ctx, int layer, const float* x, const float* r
                          int seq_len, float* y, int32_t* ids, float* probs, float* shg,
                          unsigned flags, char* err, size_t errlen);
 
+/* ---- the token mixer of the linear-attention layers --------------------------
+ * What the port block (src/layers/port_scheduler.mojo:286-372) runs between the
+ * two projections of a linear-attention mixer and at the block's edges: a short
+ * causal convolution over the mixed q, k, v rows, the gated delta rule on its
+ * heads with one state per sequence, the gated norm of its output, and the norm
+ * that joins the mixer's output to the residual stream for the MoE section.
+ * The calls take plain arrays and no uploaded layer.
+ *
+ * Rows (x, q, k, v, y, o, gates) have one of these types; weights, decays and
+ * the delta rule's states are fp32, and everything is computed in fp32 or more
+ * and rounded once, on output. */
+#define DMH_DTYPE_F32 0
+#define DMH_DTYPE_F16 1
+#define DMH_DTYPE_BF16 2
+
+/* The sequences of one call, their rows back to back: sequence i has the rows
+ * offsets[i] .. offsets[i + 1] - 1 (none is allowed) of every row array, in
+ * order, and its state is state slots[i].  Rows outside every sequence, and
+ * states that no sequence names, stay as they are.  A sequence with a negative
+ * slot is skipped (the padding of a captured graph's batch); so is one without
+ * rows: its state stays, whatever fresh says.
+ *
+ * With DMH_F_DEVICE the arrays are device memory, read when the kernels run, so
+ * a captured graph takes each replay's values.  A sequence whose offsets
+ * decrease or leave [0, total_tokens], that is longer than max_seq_len, or whose
+ * slot is num_slots or more, is left out, and the next dmh_sync reports a
+ * SEQUENCE_ERROR; what the sequences behind decreasing offsets give is not valid.
+ * It also reports two sequences with rows that name one slot, whose state and
+ * rows are then not valid.  With host memory the call itself fails
+ * with that error, before anything is written. */
+typedef struct {
+  int32_t num_seqs;
+  int32_t total_tokens;    /* rows that the sequences may use */
+  int32_t max_seq_len;     /* no sequence is longer (>= 1) */
+  int32_t num_slots;       /* states in the state array */
+  const int32_t* offsets;  /* [num_seqs + 1] */
+  const int32_t* slots;    /* [num_seqs], or NULL: sequence i uses state i */
+  const int32_t* fresh;    /* [num_seqs] nonzero: starts from a state of zeros; or NULL: none */
+} dmh_seq_batch;
+
+/* Causal depthwise convolution of width taps: with x(p) the row at position p
+ * of a sequence, and x(-1), x(-2), ... the last row, the one before it, ... of
+ * its state,
+ *   y(p)[c] = act(bias[c] + sum_j weight[c][j] * x(p - (width - 1) + j)[c]),
+ * and the state becomes the last width - 1 rows seen.  Strides are in elements
+ * between rows.  y must not overlap x. */
+typedef struct {
+  int32_t dtype;        /* of x, state and y */
+  int32_t channels;
+  int32_t width;        /* 2, 3 or 4 */
+  int32_t silu;         /* act: 1 SiLU, 0 none */
+  const void* x;        /* [total_tokens][channels] */
+  int64_t x_stride;
+  const float* weight;  /* [channels][width] */
+  const float* bias;    /* [channels] or NULL */
+  void* state;          /* [num_slots][width - 1][channels], the oldest row first */
+  void* y;
+  int64_t y_stride;
+} dmh_short_conv;
+
+int dmh_short_conv_forward(dmh_ctx* ctx, const dmh_short_conv* args, const dmh_seq_batch* batch,
+                           unsigned flags, char* err, size_t errlen);
+
+/* The gated delta rule.  Value head h works with key head
+ * h / (v_heads / k_heads); with k, q its key and query (each divided by
+ * sqrt(sum of squares + eps) where qk_norm is set), the state S [k_dim][v_dim]
+ * takes a row as
+ *   S  = exp(g) * S
+ *   S += k (beta * (v - S^T k))^T
+ *   o  = scale * S^T q.
+ * Gates: with a_log set, a and b are raw rows of dtype and
+ *   g = -exp(a_log[h]) * softplus(a + dt_bias[h]),  beta = sigmoid(b);
+ * without it a is g and b is beta, fp32 rows.
+ * Sequences of up to 32 rows take the recurrence row by row; longer ones take it
+ * 64 rows at a time as matrix products.  Which one a sequence takes goes by its
+ * length alone, so its results do not depend on what else is in the call.
+ * o must not overlap the inputs.  A row with a value that is not finite leaves
+ * NaN in its head of its own sequence, from up to 63 rows before it on, and in
+ * no other sequence. */
+typedef struct {
+  int32_t dtype;       /* of q, k, v, o, and of raw a, b */
+  int32_t k_heads, v_heads;  /* v_heads a multiple of k_heads */
+  int32_t k_dim, v_dim;      /* multiples of 8, 8 to 256 */
+  int32_t qk_norm;
+  float eps;
+  float scale;
+  const void* q;       /* [total_tokens][k_heads][k_dim] */
+  const void* k;
+  const void* v;       /* [total_tokens][v_heads][v_dim] */
+  const void* a;       /* [total_tokens][v_heads] */
+  const void* b;
+  int64_t q_stride, k_stride, v_stride, a_stride, b_stride;  /* elements between rows */
+  const float* a_log;    /* [v_heads], or NULL */
+  const float* dt_bias;  /* [v_heads], or NULL: zeros */
+  float* state;        /* [num_slots][v_heads][k_dim][v_dim], 16-byte aligned */
+  void* o;             /* [total_tokens][v_heads][v_dim] */
+  int64_t o_stride;
+} dmh_gated_delta;
+
+int dmh_gated_delta_forward(dmh_ctx* ctx, const dmh_gated_delta* args, const dmh_seq_batch* batch,
+                            unsigned flags, char* err, size_t errlen);
+
+/* Norms after and before a block, with the block's gate and residual, in one
+ * pass over rows of groups * dim elements, each group on its own:
+ *   u      = x, or with post set x / sqrt(mean(x^2) + eps) * gamma
+ *   u      = u * silu(gate) or u * sigmoid(gate)       (gate_act)
+ *   stream = residual + scale * scale_vec * u          (residual NULL: 0)
+ *   y      = stream / sqrt(mean(stream^2) + eps) * edge_gamma
+ * where y takes the stream before its rounding.  stream or y may be NULL, and
+ * stream may be the residual itself, or x where their types are one; apart from
+ * that the outputs must not overlap the inputs. */
+#define DMH_GATE_NONE 0
+#define DMH_GATE_SILU 1
+#define DMH_GATE_SIGMOID 2
+typedef struct {
+  int32_t dtype;         /* of x and gate */
+  int32_t stream_dtype;  /* of residual, stream and y: dtype or DMH_DTYPE_F32 */
+  int32_t rows, groups;
+  int32_t dim;           /* 1 to 8192 */
+  int32_t post;
+  int32_t gate_act;
+  float scale;
+  float eps;             /* > 0 */
+  const void* x;
+  const void* gate;
+  const void* residual;
+  void* stream;
+  void* y;
+  int64_t x_stride, gate_stride, residual_stride, stream_stride, y_stride;
+  const float* gamma;       /* [dim], or NULL: ones */
+  const float* edge_gamma;  /* [dim], or NULL: ones */
+  const float* scale_vec;   /* [groups][dim], or NULL: ones */
+} dmh_gated_norm;
+
+int dmh_gated_norm_forward(dmh_ctx* ctx, const dmh_gated_norm* args, unsigned flags, char* err,
+                           size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif
