@@ -9,6 +9,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 #include <new>
@@ -22,6 +23,11 @@
 namespace {
 
 using dm::SeqDev;
+
+// Sequences of up to kRowsMost rows take the delta rule row by row.
+constexpr int kRowsMost = 32;
+// Chunks whose factors are in memory at once (40 KB to 130 KB a head).
+constexpr int64_t kChunkRoom = 512;
 
 struct Err {
   char* p;
@@ -262,7 +268,7 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
     return err.arg("q, k, v, a, b, state or o is NULL");
   if (!aligned(a.state, 16)) return err.arg("state must be 16-byte aligned");
   // (2^32 threads are the most that a launch holds)
-  if ((int64_t)b.num_seqs * a.v_heads * ((a.v_dim + 15) / 16) >= (int64_t)1 << 24)
+  if ((int64_t)b.num_seqs * a.v_heads * ((a.v_dim + 15) / 16) >= (int64_t)1 << 23)
     return err(DMH_ERR_CONFIG, "CONFIG_ERROR", "too many sequences for one call: %d", b.num_seqs);
   const size_t es = elem(a.dtype), gs = a.a_log ? es : 4;
   const int64_t kw = (int64_t)a.k_heads * a.k_dim, vw = (int64_t)a.v_heads * a.v_dim;
@@ -302,7 +308,15 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
   }
   const bool wide = q.wide() && k.wide() && v.wide() && o.wide();
   const SeqDev s = seq_dev(b, status);
-  const hipError_t e = dm::launch_delta_rows(a, s, b.max_seq_len, wide, st);
+  const int64_t chunks = b.max_seq_len > kRowsMost ? dm::delta_chunk_count(s, kRowsMost + 1) : 0;
+  const int64_t room = std::min(chunks, kChunkRoom);
+  void* ws = nullptr;
+  if (chunks && (rc = dm::api_mixer_buffer(c, dm::kMixerChunks, room * dm::delta_chunk_bytes(a, wide),
+                                           &ws, errp, errlen)))
+    return rc;
+  hipError_t e = dm::launch_delta_rows(a, s, kRowsMost, wide, st);
+  if (e == hipSuccess && chunks)
+    e = dm::launch_delta_chunks(a, s, kRowsMost + 1, chunks, room, ws, wide, st);
   if (e != hipSuccess) return err.hip(e);
   return dev ? DMH_OK : stage.out(st, err);
 }
