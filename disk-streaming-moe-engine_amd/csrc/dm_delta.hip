@@ -18,6 +18,7 @@
 // their norms and decays as factors of rows in fp32.  Sums of log decays are
 // kept in 64 bits: e^(G_i - G_j) of two large sums would lose what the
 // difference holds.
+#include <cstdlib>
 #include "dm_mixer_device.h"
 
 namespace dm {
@@ -36,17 +37,19 @@ constexpr size_t frag_bytes(int n) { return (size_t)n * 1024; }  // 64 lanes of 
 
 // What k_delta_prep leaves per chunk: for each value head (I + A)^-1 diag(beta)
 // in three parts, the query-key matrix in NPO, and the rows' factors; for each
-// key head K^T, and K and Q where the rows cannot be read in place.
-template <int DKT, int NPK, int NPO, bool DIRECT>
+// key head K^T, and K and Q where the rows cannot be read in place (they are not
+// bf16, or not aligned: WIDE is false).
+template <int DKT, int NPK, int NPO, bool WIDE>
 struct Layout {
+  static constexpr bool direct = WIDE && NPK == 1;  // K and Q are read in place
   static constexpr int KS = DKT / 32;  // steps of 32 along the key dimension
   static constexpr int NPQ = NPK < NPO ? NPK : NPO;
   static constexpr size_t qk = frag_bytes(kTiles * 3);
   static constexpr size_t rows = qk + frag_bytes(kTiles * NPO);
   static constexpr size_t v_head = rows + 4 * kChunk * sizeof(float);
   static constexpr size_t k_rows = frag_bytes(DKT / 16 * 2 * NPK);
-  static constexpr size_t q_rows = k_rows + (DIRECT ? 0 : frag_bytes(4 * KS * NPK));
-  static constexpr size_t k_head = q_rows + (DIRECT ? 0 : frag_bytes(4 * KS * NPQ));
+  static constexpr size_t q_rows = k_rows + (direct ? 0 : frag_bytes(4 * KS * NPK));
+  static constexpr size_t k_head = q_rows + (direct ? 0 : frag_bytes(4 * KS * NPQ));
 };
 
 struct ChunkWork {
@@ -54,6 +57,7 @@ struct ChunkWork {
   uint8_t* k_heads;
   int rank0, count;  // the chunks of this pass, counted over all long sequences
   int min_rows;      // sequences of fewer rows are not taken
+  uint8_t* nowhere;  // 4 KB: where a lane without an output row stores
 };
 
 __device__ __forceinline__ int chunks_of(const SeqDev& s, int i, int min_rows) {
@@ -111,23 +115,29 @@ __device__ __forceinline__ void store_frag(void* base, size_t frag, int lane, ui
 
 // ---- what does not depend on the state ---------------------------------------------
 // One workgroup per chunk and value head; wave w has rows 16 w .. 16 w + 15.
-// The products of rows with rows take each wave's rows as the left factor and
-// all waves' rows, from LDS, as the right one.  (I + A)^-1 comes by forward
-// substitution in the 16 x 16 diagonal blocks (a column per lane) and, as
-// -T22 A21 T11, in the blocks below them, 16 and then 32 wide, on the fp32
-// matrix cores: products of powers of A would take fewer steps and lose all
-// precision for keys that resemble each other.
-template <typename T, int DKT, int NPK, int NPO, bool DIRECT>
+// The products of rows with rows take each wave's rows as one factor and all
+// waves' rows, from LDS, as the other.  (I + A)^-1 comes by substitution in the
+// 16 x 16 diagonal blocks (a row per lane) and, as -T22 A21 T11, in the blocks
+// below them, 16 and then 32 wide, on the fp32 matrix cores: products of powers
+// of A would take fewer steps and lose all precision for keys that resemble each
+// other.  The chain of loads, products and substitution bounds it, so everything
+// is loaded at once, unconditionally, and LDS is kept small for more workgroups
+// per CU: T takes the place of the keys.
+template <typename T, int DKT, int NPK, int NPO, bool WIDE>
 __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s, ChunkWork cw) {
-  using L = Layout<DKT, NPK, NPO, DIRECT>;
+  using L = Layout<DKT, NPK, NPO, WIDE>;
   constexpr int KS = L::KS;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int local = blockIdx.x / d.v_heads, h = blockIdx.x - local * d.v_heads;
   const int rep = d.v_heads / d.k_heads, kh = h / rep;
 
-  __shared__ __align__(16) uint8_t kfrag[frag_bytes(4 * KS * NPK)];
-  __shared__ __align__(16) float am[kChunk * kPad], qm[kChunk * kPad], tm[kChunk * kPad];
+  constexpr size_t kMat = kChunk * kPad * sizeof(float);
+  constexpr size_t kKeys = frag_bytes(4 * KS * NPK);
+  __shared__ __align__(16) uint8_t shared[kKeys > kMat ? kKeys : kMat];
+  __shared__ __align__(16) float am[kChunk * kPad];
+  uint8_t* const kfrag = shared;
+  float* const tm = reinterpret_cast<float*>(shared);
   __shared__ double decay[kChunk];
   __shared__ float beta_s[kChunk], rk_s[kChunk], rq_s[kChunk];
   __shared__ int scan[4], found[2];
@@ -149,27 +159,39 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
     for (int i = 0; i < w; ++i) sum += scan[i];
     const int all = scan[0] + scan[1] + scan[2] + scan[3];
     if (rank < base + sum && rank >= base + sum - own) {
-      found[0] = j0 + tid;
-      found[1] = rank - (base + sum - own);
+      found[0] = s.off[j0 + tid] + (rank - (base + sum - own)) * kChunk;
+      found[1] = s.off[j0 + tid + 1];
     }
     base += all;
     if (rank < base) break;
   }
   __syncthreads();
-  if (found[0] < 0) return;
-  const int begin = s.off[found[0]] + found[1] * kChunk;
-  const int rows = min(s.off[found[0] + 1] - begin, kChunk);
+  const int begin = __builtin_amdgcn_readfirstlane(found[0]);
+  if (begin < 0) return;
+  const int rows = min(__builtin_amdgcn_readfirstlane(found[1]) - begin, kChunk);
   uint8_t* const vws = cw.v_heads + (size_t)blockIdx.x * L::v_head;
   uint8_t* const kws = cw.k_heads + ((size_t)local * d.k_heads + kh) * L::k_head;
 
-  // gates and decays: a row per lane
-  double since = 0.0;
-  float beta = 0.0f;
-  if (lane < rows) {
-    const Gates gt = load_gates<T>(d, begin + lane, h);
-    since = gt.log_decay < -10000.0f ? -10000.0 : (double)gt.log_decay;  // e^-10000 is 0 as well
-    beta = gt.beta;
+  // the rows' values; of a row or column that is not there, another's, cleared
+  // below
+  const int row = 16 * w + n;
+  const bool row_in = row < rows;
+  float kv[KS][8], qv[KS][8];
+  {
+    const int64_t at = begin + min(row, rows - 1);
+    const T* kp = static_cast<const T*>(d.k) + at * d.k_stride + kh * d.k_dim;
+    const T* qp = static_cast<const T*>(d.q) + at * d.q_stride + kh * d.k_dim;
+#pragma unroll
+    for (int st = 0; st < KS; ++st) {
+      const int c = 32 * st + 8 * g < d.k_dim ? 32 * st + 8 * g : 0;
+      load_f32<8>(kp + c, WIDE, kv[st]);
+      load_f32<8>(qp + c, WIDE, qv[st]);
+    }
   }
+  // gates and decays: a row per lane
+  const Gates gt = load_gates<T>(d, begin + min(lane, rows - 1), h);
+  double since = lane < rows ? (double)gt.log_decay : 0.0;
+  if (since < -10000.0) since = -10000.0;  // (e^-10000 is 0 as well)
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) {
     const double v = __shfl_up(since, m);
@@ -178,94 +200,124 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   const double last = __shfl(since, 63);
   if (w == 0) {
     decay[lane] = since;
-    beta_s[lane] = beta;
+    beta_s[lane] = lane < rows ? gt.beta : 0.0f;
   }
 
-  // keys and queries of the wave's rows: norms and parts
+  // norms and parts of keys and queries
   bf16x8 qf[KS][NPK], kf[KS][NPK];
-  {
-    const int row = 16 * w + n;
-    const T* kp = static_cast<const T*>(d.k) + (int64_t)(begin + row) * d.k_stride + kh * d.k_dim;
-    const T* qp = static_cast<const T*>(d.q) + (int64_t)(begin + row) * d.q_stride + kh * d.k_dim;
-    float ksum = 0.0f, qsum = 0.0f;
+  float ksum = 0.0f, qsum = 0.0f;
 #pragma unroll
-    for (int st = 0; st < KS; ++st) {
-      const int c = 32 * st + 8 * g;
-      float kv[8] = {}, qv[8] = {};
-      if (row < rows && c < d.k_dim) {
-        load_f32<8>(kp + c, DIRECT, kv);
-        load_f32<8>(qp + c, DIRECT, qv);
-      }
+  for (int st = 0; st < KS; ++st) {
+    const bool in = row_in && 32 * st + 8 * g < d.k_dim;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ksum = __builtin_fmaf(kv[i], kv[i], ksum);
-        qsum = __builtin_fmaf(qv[i], qv[i], qsum);
-      }
-      uint4 kp4[NPK], qp4[NPK];
-      split8<NPK>(kv, kp4);
-      split8<NPK>(qv, qp4);
+    for (int i = 0; i < 8; ++i) {
+      kv[st][i] = in ? kv[st][i] : 0.0f;
+      qv[st][i] = in ? qv[st][i] : 0.0f;
+      ksum = __builtin_fmaf(kv[st][i], kv[st][i], ksum);
+      qsum = __builtin_fmaf(qv[st][i], qv[st][i], qsum);
+    }
+    uint4 kp4[NPK], qp4[NPK];
+    split8<NPK>(kv[st], kp4);
+    split8<NPK>(qv[st], qp4);
 #pragma unroll
-      for (int p = 0; p < NPK; ++p) {
-        store_frag(kfrag, (w * KS + st) * NPK + p, lane, kp4[p]);
-        kf[st][p] = __builtin_bit_cast(bf16x8, kp4[p]);
-        qf[st][p] = __builtin_bit_cast(bf16x8, qp4[p]);
-        if (!DIRECT && h == kh * rep) {
-          store_frag(kws + L::k_rows, (w * KS + st) * NPK + p, lane, kp4[p]);
-          if (p < L::NPQ) store_frag(kws + L::q_rows, (w * KS + st) * L::NPQ + p, lane, qp4[p]);
-        }
+    for (int p = 0; p < NPK; ++p) {
+      store_frag(kfrag, (w * KS + st) * NPK + p, lane, kp4[p]);
+      kf[st][p] = __builtin_bit_cast(bf16x8, kp4[p]);
+      qf[st][p] = __builtin_bit_cast(bf16x8, qp4[p]);
+      if (!L::direct && h == kh * rep) {
+        store_frag(kws + L::k_rows, (w * KS + st) * NPK + p, lane, kp4[p]);
+        if (p < L::NPQ) store_frag(kws + L::q_rows, (w * KS + st) * L::NPQ + p, lane, qp4[p]);
       }
     }
-    ksum += __shfl_xor(ksum, 16);
-    qsum += __shfl_xor(qsum, 16);
-    ksum += __shfl_xor(ksum, 32);
-    qsum += __shfl_xor(qsum, 32);
-    if (g == 0) {
-      rk_s[row] = d.qk_norm ? 1.0f / sqrtf(ksum + d.eps) : 1.0f;
-      rq_s[row] = d.qk_norm ? d.scale / sqrtf(qsum + d.eps) : d.scale;
-    }
+  }
+  ksum += __shfl_xor(ksum, 16);
+  qsum += __shfl_xor(qsum, 16);
+  ksum += __shfl_xor(ksum, 32);
+  qsum += __shfl_xor(qsum, 32);
+  const float rk = d.qk_norm ? 1.0f / sqrtf(ksum + d.eps) : 1.0f;
+  const float rq = d.qk_norm ? d.scale / sqrtf(qsum + d.eps) : d.scale;
+  if (g == 0) {
+    rk_s[row] = rk;
+    rq_s[row] = rq;
   }
   __syncthreads();
 
-  // A and the query-key matrix
+  // A, with the wave's rows on the left; and the transposed query-key matrix,
+  // with its rows on the right: four consecutive keys of a row per lane, which
+  // is a piece of the left factor that k_delta_chunks loads
+  const double since_q = decay[row];
   for (int j = 0; j <= w; ++j) {
-    f32x4 kk = {}, qk = {};
+    f32x4 kk = {}, kq = {};
 #pragma unroll
     for (int st = 0; st < KS; ++st) {
       bf16x8 b[NPK];
 #pragma unroll
       for (int p = 0; p < NPK; ++p) b[p] = load_frag(kfrag, (j * KS + st) * NPK + p, lane);
       kk = mfma_parts<3>(kf[st], b, kk);
-      qk = mfma_parts<3>(qf[st], b, qk);
+      kq = mfma_parts<3>(b, qf[st], kq);
     }
     const int col = 16 * j + n;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = 16 * w + 4 * g + r;
-      const float e = row >= col ? expf((float)(decay[row] - decay[col])) * rk_s[col] : 0.0f;
-      am[row * kPad + col] = row > col && row < rows ? beta_s[row] * rk_s[row] * e * kk[r] : 0.0f;
-      qm[row * kPad + col] = row >= col && row < rows ? rq_s[row] * e * qk[r] : 0.0f;
+      const int rr = 16 * w + 4 * g + r, cc = 16 * j + 4 * g + r;
+      const float e = rr > col ? expf((float)(decay[rr] - decay[col])) : 0.0f;
+      am[rr * kPad + col] =
+          rr > col && rr < rows ? beta_s[rr] * rk_s[rr] * (e * rk_s[col]) * kk[r] : 0.0f;
+      const float eq = row >= cc ? expf((float)(since_q - decay[cc])) : 0.0f;
+      kq[r] = row >= cc && row_in ? rq * (eq * rk_s[cc]) * kq[r] : 0.0f;
     }
-  }
-  if ((w & 1) == 0) {  // the upper halves of the tiles on the diagonal
+    uint2 p[NPO];
+    split4<NPO>(kq, p);
+    uint8_t* const to = vws + L::qk + (n + 16 * ((j & 1) * 2 + (g >> 1))) * 16 + (g & 1) * 8;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      qm[(16 * w + 4 * g + r) * kPad + 16 * w + 16 + n] = 0.0f;
-      tm[(16 * w + 4 * g + r) * kPad + 16 * w + 16 + n] = 0.0f;
+    for (int i = 0; i < NPO; ++i)
+      *reinterpret_cast<uint2*>(to + (tile_of(w, j >> 1) * NPO + i) * 1024) = p[i];
+  }
+  if ((w & 1) == 0) {  // the empty half of the tile on the diagonal
+    uint8_t* const to = vws + L::qk + (n + 32 + 16 * (g >> 1)) * 16 + (g & 1) * 8;
+#pragma unroll
+    for (int i = 0; i < NPO; ++i)
+      *reinterpret_cast<uint2*>(to + (tile_of(w, w >> 1) * NPO + i) * 1024) = make_uint2(0, 0);
+  }
+  if (h == kh * rep) {  // K^T
+    for (int i = tid; i < DKT / 16 * 2 * NPK * 64; i += 256) {
+      const int frag = i >> 6, p = frag % NPK, half = frag / NPK & 1, t = frag / (2 * NPK);
+      const int c = 16 * t + n;  // key dimension
+      uint16_t v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int tok = 32 * half + 8 * g + e;
+        const int from = (((tok >> 4) * KS + (c >> 5)) * NPK + p) * 1024 +
+                         ((tok & 15) + 16 * ((c & 31) >> 3)) * 16 + (c & 7) * 2;
+        v[e] = *reinterpret_cast<const uint16_t*>(kfrag + from);
+      }
+      store_frag(kws, frag, lane,
+                 make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16,
+                            v[6] | v[7] << 16));
     }
   }
   __syncthreads();
 
-  // the diagonal blocks of T = (I + A)^-1, a column per lane
+  // the diagonal blocks of T = (I + A)^-1 from T (I + A) = I, a row per lane
   {
     float x[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float v = i == n ? 1.0f : 0.0f;
+    for (int j = 0; j < 16; ++j) x[j] = j == n ? 1.0f : 0.0f;
 #pragma unroll
-      for (int m = 0; m < i; ++m)
-        v = __builtin_fmaf(-am[(16 * w + i) * kPad + 16 * w + m], x[m], v);
-      x[i] = v;
-      if (g == 0) tm[(16 * w + i) * kPad + 16 * w + n] = v;
+    for (int m = 15; m > 0; --m) {
+      const float* a = am + (16 * w + m) * kPad + 16 * w;
+#pragma unroll
+      for (int j = 0; j < m; ++j) x[j] = __builtin_fmaf(-x[m], a[j], x[j]);
+    }
+    if (g == 0) {
+#pragma unroll
+      for (int j = 0; j < 16; j += 4)
+        *reinterpret_cast<f32x4*>(tm + row * kPad + 16 * w + j) = f32x4{x[j], x[j + 1], x[j + 2],
+                                                                        x[j + 3]};
+    } else if (g == 1 && (w & 1) == 0) {  // the empty half of the tile on the diagonal
+#pragma unroll
+      for (int j = 0; j < 16; j += 4)
+        *reinterpret_cast<f32x4*>(tm + row * kPad + 16 * w + 16 + j) = f32x4{};
     }
   }
   __syncthreads();
@@ -304,24 +356,18 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   }
   __syncthreads();
 
-  // parts of both matrices, as left factors
+  // its parts, as a left factor
   for (int i = tid; i < kTiles * 64; i += 256) {
     const int tile = i >> 6;  // (lane is i & 63)
     const int blk = tile < 2 ? tile : (tile + 2) / 2, half = tile < 2 ? 0 : tile & 1;
     const int at = (16 * blk + n) * kPad + 32 * half + 8 * g;
-    float v[8], q[8];
+    float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = tm[at + e] * beta_s[32 * half + 8 * g + e];
-      q[e] = qm[at + e];
-    }
-    uint4 vp[3], qp[NPO];
+    for (int e = 0; e < 8; ++e) v[e] = tm[at + e] * beta_s[32 * half + 8 * g + e];
+    uint4 vp[3];
     split8<3>(v, vp);
-    split8<NPO>(q, qp);
 #pragma unroll
     for (int p = 0; p < 3; ++p) store_frag(vws, tile * 3 + p, lane, vp[p]);
-#pragma unroll
-    for (int p = 0; p < NPO; ++p) store_frag(vws + L::qk, tile * NPO + p, lane, qp[p]);
   }
   if (w == 0) {
     float* f = reinterpret_cast<float*>(vws + L::rows);
@@ -331,23 +377,6 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
     f[kChunk + lane] = in ? grown * rq_s[lane] : 0.0f;
     f[2 * kChunk + lane] = in ? expf((float)(last - since)) * rk_s[lane] : 0.0f;
     f[3 * kChunk + lane] = expf((float)last);
-  }
-  if (h == kh * rep) {
-    for (int i = tid; i < DKT / 16 * 2 * NPK * 64; i += 256) {
-      const int frag = i >> 6, p = frag % NPK, half = frag / NPK & 1, t = frag / (2 * NPK);
-      const int c = 16 * t + n;  // key dimension
-      uint16_t v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int row = 32 * half + 8 * g + e;
-        const int from = (((row >> 4) * KS + (c >> 5)) * NPK + p) * 1024 +
-                         ((row & 15) + 16 * ((c & 31) >> 3)) * 16 + (c & 7) * 2;
-        v[e] = *reinterpret_cast<const uint16_t*>(kfrag + from);
-      }
-      store_frag(kws, frag, lane,
-                 make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16,
-                            v[6] | v[7] << 16));
-    }
   }
 }
 
@@ -362,9 +391,9 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
 // chunk's is used up.  A chunk takes about as long as this chain of products and
 // exchanges, whatever the number of columns; more heads or sequences run beside
 // it.
-template <typename T, int DKT, int NC, int NPK, int NPO, bool DIRECT>
+template <typename T, int DKT, int NC, int NPK, int NPO, bool WIDE>
 __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev s, ChunkWork cw) {
-  using L = Layout<DKT, NPK, NPO, DIRECT>;
+  using L = Layout<DKT, NPK, NPO, WIDE>;
   constexpr int KS = L::KS, NT = DKT / 64, NPQ = L::NPQ;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -390,13 +419,15 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
   for (int j = tid; j < seq; j += 256) mine += chunks_of(s, j, cw.min_rows);
   if (mine) atomicAdd(&before, mine);
   __syncthreads();
-  const int first = cw.rank0 - before;  // of this pass, counted in this sequence
+  const int first = cw.rank0 - __builtin_amdgcn_readfirstlane(before);  // of this pass, counted in this sequence
   const int c0 = max(first, 0);
   const int c1 = min((r.end - r.begin + kChunk - 1) / kChunk, first + cw.count);
   if (c0 >= c1) return;
 
-  // an element of a C tile: row 4 g + i of 16, column n
-  const int col = cb * 16 * NC + n;
+  // an element of a C tile: row 4 g + i of 16, column n.  O is held transposed, a
+  // row and four columns per lane.
+  const int col = cb * 16 * NC + n, ocol = cb * 16 * NC + 4 * g;
+  T* const nowhere = reinterpret_cast<T*>(cw.nowhere + tid * 16);
   float* const sp = d.state + (((size_t)r.slot * d.v_heads + h) * d.k_dim + 16 * NT * w + 4 * g) *
                                   d.v_dim + col;
   f32x4 S[NT][NC];
@@ -411,88 +442,95 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
       }
 
   bf16x8 kf[KS][NPK], qf[KS][NPQ], tf[2][3], af[2][NPO], gf[NT][2][NPK];
-  float v[NC][4], pk[4], pq[4], pr[4], fade;
+  T v[NC][4];
+  f32x4 pk, pr;
+  float pq, fade;
   const bool two = w >= 2;  // rows 32 on: two tiles of the triangular factors
-  const auto v_ws = [&](int c) {
-    return cw.v_heads + ((size_t)(c - first) * d.v_heads + h) * L::v_head;
+  // Loads are unconditional, so that none waits for another: behind the last row
+  // or dimension they read one that is there (what comes of it meets a factor of
+  // zero or is not stored).  Addresses are a uniform base of the chunk and 32-bit
+  // offsets of the lane that hold for all chunks.
+  const uint32_t at16 = lane * 16;
+  const uint32_t t_at[2] = {tile_of(w, 0) * 3 * 1024 + at16, tile_of(w, two) * 3 * 1024 + at16};
+  const uint32_t a_at[2] = {(uint32_t)L::qk + tile_of(w, 0) * NPO * 1024 + at16,
+                            (uint32_t)L::qk + tile_of(w, two) * NPO * 1024 + at16};
+  const uint32_t g_at = NT * w * 2 * NPK * 1024 + at16;
+  const uint32_t kr_at = (uint32_t)L::k_rows + w * KS * NPK * 1024 + at16;
+  const uint32_t qr_at = (uint32_t)L::q_rows + w * KS * NPQ * 1024 + at16;
+  const uint32_t f4_at = (uint32_t)L::rows + (16 * w + 4 * g) * 4;
+  const uint32_t f1_at = (uint32_t)L::rows + (kChunk + 16 * w + n) * 4;
+  uint32_t k_at[KS], v_at[NC];
+#pragma unroll
+  for (int st = 0; st < KS; ++st)
+    k_at[st] = (32 * st + 8 * g < d.k_dim ? 32 * st + 8 * g : 0) * sizeof(T);
+#pragma unroll
+  for (int nc = 0; nc < NC; ++nc) v_at[nc] = min(col + 16 * nc, d.v_dim - 1) * sizeof(T);
+  const auto frag = [](const uint8_t* base, uint32_t at) {
+    return *reinterpret_cast<const bf16x8*>(base + at);
   };
-  const auto k_ws = [&](int c) {
-    return cw.k_heads + ((size_t)(c - first) * d.k_heads + kh) * L::k_head;
-  };
-  const auto load_rows = [&](int c) {  // K and Q
-    if constexpr (DIRECT) {
-      const int row = r.begin + c * kChunk + 16 * w + n;
-      const T* kp = static_cast<const T*>(d.k) + (int64_t)row * d.k_stride + kh * d.k_dim;
-      const T* qp = static_cast<const T*>(d.q) + (int64_t)row * d.q_stride + kh * d.k_dim;
+  const uint8_t* const k0 = reinterpret_cast<const uint8_t*>(
+      static_cast<const T*>(d.k) + (int64_t)r.begin * d.k_stride + kh * d.k_dim);
+  const uint8_t* const q0 = reinterpret_cast<const uint8_t*>(
+      static_cast<const T*>(d.q) + (int64_t)r.begin * d.q_stride + kh * d.k_dim);
+  const uint8_t* const v0 = reinterpret_cast<const uint8_t*>(
+      static_cast<const T*>(d.v) + (int64_t)r.begin * d.v_stride + h * d.v_dim);
+  const int64_t k_pitch = d.k_stride * sizeof(T), q_pitch = d.q_stride * sizeof(T);
+  const int64_t v_pitch = d.v_stride * sizeof(T);
+  T* const o0 = static_cast<T*>(d.o) + (int64_t)r.begin * d.o_stride + h * d.v_dim + ocol;
+  const int len = r.end - r.begin;
+  const auto load_rows = [&](int c, const uint8_t* kws) {  // K and Q
+    if constexpr (L::direct) {
+      const int row = min(c * kChunk + 16 * w + n, len - 1);
+      const uint8_t *kp = k0 + row * k_pitch, *qp = q0 + row * q_pitch;
 #pragma unroll
       for (int st = 0; st < KS; ++st) {
-        const int at = 32 * st + 8 * g;
-        uint4 k4 = {}, q4 = {};
-        if (row < r.end && at < d.k_dim) {
-          k4 = *reinterpret_cast<const uint4*>(kp + at);
-          q4 = *reinterpret_cast<const uint4*>(qp + at);
-        }
-        kf[st][0] = __builtin_bit_cast(bf16x8, k4);
-        qf[st][0] = __builtin_bit_cast(bf16x8, q4);
+        kf[st][0] = frag(kp, k_at[st]);
+        qf[st][0] = frag(qp, k_at[st]);
       }
     } else {
-      const uint8_t* p = k_ws(c);
 #pragma unroll
       for (int st = 0; st < KS; ++st) {
 #pragma unroll
-        for (int i = 0; i < NPK; ++i)
-          kf[st][i] = load_frag(p + L::k_rows, (w * KS + st) * NPK + i, lane);
+        for (int i = 0; i < NPK; ++i) kf[st][i] = frag(kws, kr_at + (st * NPK + i) * 1024);
 #pragma unroll
-        for (int i = 0; i < NPQ; ++i)
-          qf[st][i] = load_frag(p + L::q_rows, (w * KS + st) * NPQ + i, lane);
+        for (int i = 0; i < NPQ; ++i) qf[st][i] = frag(kws, qr_at + (st * NPQ + i) * 1024);
       }
     }
   };
   const auto load_v = [&](int c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = r.begin + c * kChunk + 16 * w + 4 * g + i;
-      const T* vp = static_cast<const T*>(d.v) + (int64_t)row * d.v_stride + h * d.v_dim + col;
+      const uint8_t* vp = v0 + min(c * kChunk + 16 * w + 4 * g + i, len - 1) * v_pitch;
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc)
-        v[nc][i] = row < r.end && col + 16 * nc < d.v_dim ? (float)vp[16 * nc] : 0.0f;
+      for (int nc = 0; nc < NC; ++nc) v[nc][i] = *reinterpret_cast<const T*>(vp + v_at[nc]);
     }
   };
-  const auto load_factors = [&](int c) {
-    const float* f = reinterpret_cast<const float*>(v_ws(c) + L::rows);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pk[i] = f[16 * w + 4 * g + i];
-      pq[i] = f[kChunk + 16 * w + 4 * g + i];
-      pr[i] = f[2 * kChunk + 16 * w + 4 * g + i];
-    }
-    fade = f[3 * kChunk];
+  const auto load_factors = [&](const uint8_t* vws) {
+    pk = *reinterpret_cast<const f32x4*>(vws + f4_at);
+    pq = *reinterpret_cast<const float*>(vws + f1_at);
+    pr = *reinterpret_cast<const f32x4*>(vws + f4_at + 2 * kChunk * 4);
+    fade = *reinterpret_cast<const float*>(vws + L::rows + 3 * kChunk * 4);
   };
-  const auto load_t = [&](int c) {
-    const uint8_t* p = v_ws(c);
+  const auto load_t = [&](const uint8_t* vws) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      tf[0][i] = load_frag(p, tile_of(w, 0) * 3 + i, lane);
-      if (two) tf[1][i] = load_frag(p, tile_of(w, 1) * 3 + i, lane);
-    }
-  };
-  const auto load_a = [&](int c) {
-    const uint8_t* p = v_ws(c) + L::qk;
+    for (int st = 0; st < 2; ++st)
 #pragma unroll
-    for (int i = 0; i < NPO; ++i) {
-      af[0][i] = load_frag(p, tile_of(w, 0) * NPO + i, lane);
-      if (two) af[1][i] = load_frag(p, tile_of(w, 1) * NPO + i, lane);
-    }
+      for (int i = 0; i < 3; ++i) tf[st][i] = frag(vws, t_at[st] + i * 1024);
   };
-  const auto load_kt = [&](int c) {
-    const uint8_t* p = k_ws(c);
+  const auto load_a = [&](const uint8_t* vws) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int i = 0; i < NPO; ++i) af[st][i] = frag(vws, a_at[st] + i * 1024);
+  };
+  const auto load_kt = [&](const uint8_t* kws) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int i = 0; i < NPK; ++i)
-          gf[t][st][i] = load_frag(p, ((NT * w + t) * 2 + st) * NPK + i, lane);
+          gf[t][st][i] = frag(kws, g_at + ((t * 2 + st) * NPK + i) * 1024);
   };
   // tile t of a right factor's rows to LDS: fragment [step][column tile][part]
   const auto put = [&](uint8_t* base, int t, int nc, auto parts, f32x4 x) {
@@ -512,43 +550,55 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
   using P3 = std::integral_constant<int, 3>;
   using PO = std::integral_constant<int, NPO>;
 
-  load_rows(c0);
+  size_t vws_at = ((size_t)(c0 - first) * d.v_heads + h) * L::v_head;
+  size_t kws_at = ((size_t)(c0 - first) * d.k_heads + kh) * L::k_head;
+  const uint8_t *vws = cw.v_heads + vws_at, *kws = cw.k_heads + kws_at;
+  load_rows(c0, kws);
   load_v(c0);
-  load_factors(c0);
-  load_t(c0);
-  load_a(c0);
-  load_kt(c0);
+  load_factors(vws);
+  load_t(vws);
+  load_a(vws);
+  load_kt(kws);
+  // All loads here (vmcnt 0): the waits that the compiler places in the loop
+  // would otherwise have to hold for the order of these as well, and wait for
+  // every load there.
+  __builtin_amdgcn_s_waitcnt(0x0F70);
   for (int c = c0; c < c1; ++c) {
-    const bool more = c + 1 < c1;
+    const int next = min(c + 1, c1 - 1), row0 = c * kChunk + 16 * w + 4 * g;
+    vws_at += next > c ? (size_t)d.v_heads * L::v_head : 0;
+    kws_at += next > c ? (size_t)d.k_heads * L::k_head : 0;
+    asm("" : "+s"(vws_at), "+s"(kws_at));  // one base each: not one for every load
+    vws = cw.v_heads + vws_at;
+    kws = cw.k_heads + kws_at;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) put(sb, NT * w + t, nc, P3{}, S[t][nc]);
     lds_barrier();
-    f32x4 p[NC] = {}, o[NC] = {};
+    // (two chains each: a product waits for the last one of its own sum)
+    f32x4 p[NC][2] = {}, o[NC][2] = {};
 #pragma unroll
     for (int st = 0; st < KS; ++st)
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) {
         bf16x8 b[3];
         get(sb, st, nc, b);
-        p[nc] = mfma_parts<3>(kf[st], b, p[nc]);
-        o[nc] = mfma_parts<NPO>(qf[st], b, o[nc]);
+        p[nc][st & 1] = mfma_parts<3>(kf[st], b, p[nc][st & 1]);
+        o[nc][st & 1] = mfma_parts<NPO>(b, qf[st], o[nc][st & 1]);
       }
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
+      p[nc][0] += p[nc][1];
       f32x4 x;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i] = __builtin_fmaf(-pk[i], p[nc][i], v[nc][i]);
-        o[nc][i] *= pq[i];
+        x[i] = __builtin_fmaf(-pk[i], p[nc][0][i], row0 + i < len ? (float)v[nc][i] : 0.0f);
+        o[nc][0][i] = (o[nc][0][i] + o[nc][1][i]) * pq;
       }
       put(rb, w, nc, P3{}, x);
     }
-    if (more) {
-      load_rows(c + 1);
-      load_v(c + 1);
-    }
+    load_rows(next, kws);
+    load_v(next);
     lds_barrier();
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
@@ -557,15 +607,17 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
       get(rb, 0, nc, b);
       u = mfma_parts<3>(tf[0], b, u);
       if (two) {
+        f32x4 u1 = {};
         get(rb, 1, nc, b);
-        u = mfma_parts<3>(tf[1], b, u);
+        u1 = mfma_parts<3>(tf[1], b, u1);
+        u += u1;
       }
       put(ub, w, nc, PO{}, u);
 #pragma unroll
       for (int i = 0; i < 4; ++i) u[i] *= pr[i];
       put(gb, w, nc, P3{}, u);
     }
-    if (more) load_t(c + 1);
+    load_t(vws);
     lds_barrier();
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
@@ -581,25 +633,23 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
       }
       bf16x8 b[NPO];
       get(ub, 0, nc, b);
-      o[nc] = mfma_parts<NPO>(af[0], b, o[nc]);
+      o[nc][0] = mfma_parts<NPO>(b, af[0], o[nc][0]);
       if (two) {
         get(ub, 1, nc, b);
-        o[nc] = mfma_parts<NPO>(af[1], b, o[nc]);
+        o[nc][0] = mfma_parts<NPO>(b, af[1], o[nc][0]);
       }
     }
-    if (more) {
-      load_kt(c + 1);
-      load_a(c + 1);
-      load_factors(c + 1);
-    }
+    load_kt(kws);
+    load_a(vws);
+    load_factors(vws);
+    // (not a branch, which would make the waits in the loop longer)
+    const int row = c * kChunk + 16 * w + n;
+    T* const op = o0 + row * d.o_stride;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = r.begin + c * kChunk + 16 * w + 4 * g + i;
-      T* op = static_cast<T*>(d.o) + (int64_t)row * d.o_stride + h * d.v_dim + col;
-      if (row < r.end)
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc)
-          if (col + 16 * nc < d.v_dim) op[16 * nc] = (T)o[nc][i];
+    for (int nc = 0; nc < NC; ++nc) {
+      const bool in = row < len && ocol + 16 * nc < d.v_dim;
+      const float y[4] = {o[nc][0][0], o[nc][0][1], o[nc][0][2], o[nc][0][3]};
+      store_f32<4>(in ? op + 16 * nc : nowhere, WIDE, y);
     }
   }
 #pragma unroll
@@ -613,38 +663,44 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
 }
 
 // ---- launches ----------------------------------------------------------------------
-template <typename T, bool DIRECT, typename F>
+template <typename T, bool WIDE, typename F>
 auto with_dims(const dmh_gated_delta& a, F f) {
   constexpr int NPK = std::is_same_v<T, bf16_t> ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
   constexpr int NPO = std::is_same_v<T, float> ? 3 : 2;
-  if (a.k_dim <= 64) return f(T{}, Layout<64, NPK, NPO, DIRECT>{});
-  if (a.k_dim <= 128) return f(T{}, Layout<128, NPK, NPO, DIRECT>{});
-  return f(T{}, Layout<256, NPK, NPO, DIRECT>{});
+  if (a.k_dim <= 64) return f(T{}, Layout<64, NPK, NPO, WIDE>{});
+  if (a.k_dim <= 128) return f(T{}, Layout<128, NPK, NPO, WIDE>{});
+  return f(T{}, Layout<256, NPK, NPO, WIDE>{});
 }
 template <typename F>
 auto with_form(const dmh_gated_delta& a, bool wide, F f) {
   if (a.dtype == DMH_DTYPE_BF16)
     return wide ? with_dims<bf16_t, true>(a, f) : with_dims<bf16_t, false>(a, f);
-  if (a.dtype == DMH_DTYPE_F16) return with_dims<half_t, false>(a, f);
-  return with_dims<float, false>(a, f);
+  if (a.dtype == DMH_DTYPE_F16)
+    return wide ? with_dims<half_t, true>(a, f) : with_dims<half_t, false>(a, f);
+  return wide ? with_dims<float, true>(a, f) : with_dims<float, false>(a, f);
 }
 
-template <typename T, int DKT, int NPK, int NPO, bool DIRECT>
-hipError_t run(T, Layout<DKT, NPK, NPO, DIRECT>, const dmh_gated_delta& a, const SeqDev& s,
+template <typename T, int DKT, int NPK, int NPO, bool WIDE>
+hipError_t run(T, Layout<DKT, NPK, NPO, WIDE>, const dmh_gated_delta& a, const SeqDev& s,
                int min_rows, int64_t chunks, int64_t room, void* ws, hipStream_t st) {
-  using L = Layout<DKT, NPK, NPO, DIRECT>;
+  using L = Layout<DKT, NPK, NPO, WIDE>;
   ChunkWork cw;
   cw.v_heads = static_cast<uint8_t*>(ws);
   cw.k_heads = cw.v_heads + (size_t)room * a.v_heads * L::v_head;
   cw.min_rows = min_rows;
+  cw.nowhere = cw.k_heads + (size_t)room * a.k_heads * L::k_head;
   const int64_t units = ((int64_t)s.num * a.v_heads + 7) / 8 * 8;
   for (int64_t at = 0; at < chunks; at += room) {
     cw.rank0 = (int)at;
     cw.count = (int)(chunks - at < room ? chunks - at : room);
-    k_delta_prep<T, DKT, NPK, NPO, DIRECT>
+    k_delta_prep<T, DKT, NPK, NPO, WIDE>
         <<<dim3((unsigned)cw.count * a.v_heads), 256, 0, st>>>(a, s, cw);
-    k_delta_chunks<T, DKT, 1, NPK, NPO, DIRECT>
-        <<<dim3((unsigned)(units * ((a.v_dim + 15) / 16))), 256, 0, st>>>(a, s, cw);
+    const char* e = getenv("DM_NC");
+    const int nc = e ? atoi(e) : 1;
+    const unsigned ncb = (a.v_dim + 16 * nc - 1) / (16 * nc);
+    if (nc == 1) k_delta_chunks<T, DKT, 1, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 256, 0, st>>>(a, s, cw);
+    if (nc == 2) k_delta_chunks<T, DKT, 2, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 256, 0, st>>>(a, s, cw);
+    if (nc == 4) k_delta_chunks<T, DKT, DKT == 256 ? 2 : 4, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 256, 0, st>>>(a, s, cw);
   }
   return hipGetLastError();
 }

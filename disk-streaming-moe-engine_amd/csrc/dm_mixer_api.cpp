@@ -311,7 +311,7 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
   const int64_t chunks = b.max_seq_len > kRowsMost ? dm::delta_chunk_count(s, kRowsMost + 1) : 0;
   const int64_t room = std::min(chunks, kChunkRoom);
   void* ws = nullptr;
-  if (chunks && (rc = dm::api_mixer_buffer(c, dm::kMixerChunks, room * dm::delta_chunk_bytes(a, wide),
+  if (chunks && (rc = dm::api_mixer_buffer(c, dm::kMixerChunks, room * dm::delta_chunk_bytes(a, wide) + 4096,
                                            &ws, errp, errlen)))
     return rc;
   hipError_t e = dm::launch_delta_rows(a, s, kRowsMost, wide, st);
