@@ -37,19 +37,23 @@ constexpr size_t frag_bytes(int n) { return (size_t)n * 1024; }  // 64 lanes of 
 
 // What k_delta_prep leaves per chunk: for each value head (I + A)^-1 diag(beta)
 // in three parts, the query-key matrix in NPO, and the rows' factors; for each
-// key head K^T, and K and Q where the rows cannot be read in place (they are not
-// bf16, or not aligned: WIDE is false).
+// key head K^T, K and Q (copied: read in place, rows a power of two apart meet in
+// the same channels of the L2, and two thirds of the loads' time goes there).
+// The key dimension comes in steps of a matrix product, in the order in which a
+// wave of k_delta_chunks has it in its part of the state: element e of lane
+// group g is 4 g + e of the step's first 16 and, from e = 4 on, of its second.
+// At 64 dimensions a wave has only 16, and its step is half empty.
 template <int DKT, int NPK, int NPO, bool WIDE>
 struct Layout {
-  static constexpr bool direct = WIDE && NPK == 1;  // K and Q are read in place
-  static constexpr int KS = DKT / 32;  // steps of 32 along the key dimension
+  static constexpr int SW = DKT == 64 ? 16 : 32;  // dimensions of a step
+  static constexpr int KS = DKT / SW;
   static constexpr int NPQ = NPK < NPO ? NPK : NPO;
   static constexpr size_t qk = frag_bytes(kTiles * 3);
   static constexpr size_t rows = qk + frag_bytes(kTiles * NPO);
   static constexpr size_t v_head = rows + 4 * kChunk * sizeof(float);
   static constexpr size_t k_rows = frag_bytes(DKT / 16 * 2 * NPK);
-  static constexpr size_t q_rows = k_rows + (direct ? 0 : frag_bytes(4 * KS * NPK));
-  static constexpr size_t k_head = q_rows + (direct ? 0 : frag_bytes(4 * KS * NPQ));
+  static constexpr size_t q_rows = k_rows + frag_bytes(4 * KS * NPK);
+  static constexpr size_t k_head = q_rows + frag_bytes(4 * KS * NPQ);
 };
 
 struct ChunkWork {
@@ -57,7 +61,6 @@ struct ChunkWork {
   uint8_t* k_heads;
   int rank0, count;  // the chunks of this pass, counted over all long sequences
   int min_rows;      // sequences of fewer rows are not taken
-  uint8_t* nowhere;  // 4 KB: where a lane without an output row stores
 };
 
 __device__ __forceinline__ int chunks_of(const SeqDev& s, int i, int min_rows) {
@@ -69,6 +72,14 @@ __device__ __forceinline__ int chunks_of(const SeqDev& s, int i, int min_rows) {
 __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
+
+// A matrix product's result may be read only some cycles after the product was
+// issued, which the compiler sees to by counting instructions.  It does not do
+// so where a branch lies between the two: there, results of a wave that took the
+// branch were read before they were written.  So wherever a branch or the end of
+// a loop may come between a product and the first other use of its result, the
+// result passes through here: 16 cycles, more than any product used takes.
+__device__ __forceinline__ void settle(f32x4& c) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(c)); }
 
 // Four fp32 values as NP parts of four bf16.
 template <int NP>
@@ -114,93 +125,117 @@ __device__ __forceinline__ void store_frag(void* base, size_t frag, int lane, ui
 }
 
 // ---- what does not depend on the state ---------------------------------------------
-// One workgroup per chunk and value head; wave w has rows 16 w .. 16 w + 15.
-// The products of rows with rows take each wave's rows as one factor and all
-// waves' rows, from LDS, as the other.  (I + A)^-1 comes by substitution in the
-// 16 x 16 diagonal blocks (a row per lane) and, as -T22 A21 T11, in the blocks
-// below them, 16 and then 32 wide, on the fp32 matrix cores: products of powers
-// of A would take fewer steps and lose all precision for keys that resemble each
-// other.  The chain of loads, products and substitution bounds it, so everything
-// is loaded at once, unconditionally, and LDS is kept small for more workgroups
-// per CU: T takes the place of the keys.
-template <typename T, int DKT, int NPK, int NPO, bool WIDE>
+// One workgroup per chunk and HB value heads of a key head (two, where there
+// are; their keys' products are the same up to factors); wave w has rows 16 w ..
+// 16 w + 15.  Products of rows with rows are taken transposed: four consecutive
+// keys of one row per lane are a piece of the left factor that k_delta_chunks
+// loads, and of a row of A.  T = (I + A)^-1 comes by substitution in the 16 x 16
+// diagonal blocks (a row per lane) and, as -T22 A21 T11, in the blocks below
+// them, 16 and then 32 wide, on the fp32 matrix cores: products of powers of A
+// would take fewer steps and lose all precision for keys that resemble each
+// other.
+// The chain of loads, products and substitution bounds it, not bytes, so
+// everything is loaded at once, unconditionally, and T takes A's place in LDS,
+// for three workgroups per CU.
+template <typename T, int DKT, int NPK, int NPO, bool WIDE, int HB>
 __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s, ChunkWork cw) {
   using L = Layout<DKT, NPK, NPO, WIDE>;
   constexpr int KS = L::KS;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int local = blockIdx.x / d.v_heads, h = blockIdx.x - local * d.v_heads;
-  const int rep = d.v_heads / d.k_heads, kh = h / rep;
+  const int rep = d.v_heads / d.k_heads, groups = (rep + HB - 1) / HB;
+  const int local = blockIdx.x / (d.k_heads * groups);
+  const int unit = blockIdx.x - local * d.k_heads * groups;
+  const int kh = unit / groups, group = unit - kh * groups;
+  const int h0 = kh * rep + group * HB, heads = min(HB, rep - group * HB);
 
-  constexpr size_t kMat = kChunk * kPad * sizeof(float);
-  constexpr size_t kKeys = frag_bytes(4 * KS * NPK);
-  __shared__ __align__(16) uint8_t shared[kKeys > kMat ? kKeys : kMat];
-  __shared__ __align__(16) float am[kChunk * kPad];
-  uint8_t* const kfrag = shared;
-  float* const tm = reinterpret_cast<float*>(shared);
-  __shared__ double decay[kChunk];
-  __shared__ float beta_s[kChunk], rk_s[kChunk], rq_s[kChunk];
-  __shared__ int scan[4], found[2];
+  constexpr int kMat = kChunk * kPad;
+  __shared__ __align__(16) uint8_t kfrag[frag_bytes(4 * KS * NPK)];
+  __shared__ __align__(16) float am[HB * kMat];  // A, and then T in its place
+  __shared__ __align__(16) float2 decay[HB][kChunk];
+  __shared__ __align__(16) float beta_s[HB][kChunk], rk_s[kChunk];
+  __shared__ float rq_s[kChunk];
+
+  // head h0 + w's constants (of waves without a head: another's)
+  const int hw = h0 + min(w, heads - 1);
+  const float a_log = d.a_log ? d.a_log[hw] : 0.0f, dt = d.dt_bias ? d.dt_bias[hw] : 0.0f;
 
   // the chunk: sequence and place in it
   const int rank = cw.rank0 + local;
-  if (tid == 0) found[0] = -1;
-  for (int j0 = 0, base = 0; j0 < s.num; j0 += 256) {
-    const int own = j0 + tid < s.num ? chunks_of(s, j0 + tid, cw.min_rows) : 0;
+  int begin = -1, end = 0;
+  for (int j0 = 0, base = 0; j0 < s.num && begin < 0; j0 += 64) {
+    const int own = j0 + lane < s.num ? chunks_of(s, j0 + lane, cw.min_rows) : 0;
     int sum = own;
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) {
       const int v = __shfl_up(sum, m);
       if (lane >= m) sum += v;
     }
-    __syncthreads();
-    if (lane == 63) scan[w] = sum;
-    __syncthreads();
-    for (int i = 0; i < w; ++i) sum += scan[i];
-    const int all = scan[0] + scan[1] + scan[2] + scan[3];
-    if (rank < base + sum && rank >= base + sum - own) {
-      found[0] = s.off[j0 + tid] + (rank - (base + sum - own)) * kChunk;
-      found[1] = s.off[j0 + tid + 1];
+    const unsigned long long past = __ballot(base + sum > rank);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      begin = s.off[j0 + at] + (rank - base - __shfl(sum - own, at)) * kChunk;
+      end = s.off[j0 + at + 1];
     }
-    base += all;
-    if (rank < base) break;
+    base += __shfl(sum, 63);
   }
-  __syncthreads();
-  const int begin = __builtin_amdgcn_readfirstlane(found[0]);
+  begin = __builtin_amdgcn_readfirstlane(begin);
   if (begin < 0) return;
-  const int rows = min(__builtin_amdgcn_readfirstlane(found[1]) - begin, kChunk);
-  uint8_t* const vws = cw.v_heads + (size_t)blockIdx.x * L::v_head;
+  const int rows = min(__builtin_amdgcn_readfirstlane(end) - begin, kChunk);
+  uint8_t* const vws = cw.v_heads + ((size_t)local * d.v_heads + h0) * L::v_head;
   uint8_t* const kws = cw.k_heads + ((size_t)local * d.k_heads + kh) * L::k_head;
 
-  // the rows' values; of a row or column that is not there, another's, cleared
-  // below
+  // the rows' values and gates, all loads at once; of a row or column that is not
+  // there, another's, cleared below
   const int row = 16 * w + n;
   const bool row_in = row < rows;
+  const int64_t gate_at = begin + min(lane, rows - 1);
+  float ga, gb;
+  if (d.a_log) {
+    ga = (float)static_cast<const T*>(d.a)[gate_at * d.a_stride + hw];
+    gb = (float)static_cast<const T*>(d.b)[gate_at * d.b_stride + hw];
+  } else {
+    ga = static_cast<const float*>(d.a)[gate_at * d.a_stride + hw];
+    gb = static_cast<const float*>(d.b)[gate_at * d.b_stride + hw];
+  }
   float kv[KS][8], qv[KS][8];
   {
     const int64_t at = begin + min(row, rows - 1);
     const T* kp = static_cast<const T*>(d.k) + at * d.k_stride + kh * d.k_dim;
     const T* qp = static_cast<const T*>(d.q) + at * d.q_stride + kh * d.k_dim;
 #pragma unroll
-    for (int st = 0; st < KS; ++st) {
-      const int c = 32 * st + 8 * g < d.k_dim ? 32 * st + 8 * g : 0;
-      load_f32<8>(kp + c, WIDE, kv[st]);
-      load_f32<8>(qp + c, WIDE, qv[st]);
-    }
-  }
-  // gates and decays: a row per lane
-  const Gates gt = load_gates<T>(d, begin + min(lane, rows - 1), h);
-  double since = lane < rows ? (double)gt.log_decay : 0.0;
-  if (since < -10000.0) since = -10000.0;  // (e^-10000 is 0 as well)
+    for (int st = 0; st < KS; ++st)
 #pragma unroll
-  for (int m = 1; m < 64; m *= 2) {
-    const double v = __shfl_up(since, m);
-    if (lane >= m) since += v;
+      for (int e = 0; e < L::SW / 4; e += 4) {
+        const int c = L::SW * st + 4 * e + 4 * g < d.k_dim ? L::SW * st + 4 * e + 4 * g : 0;
+        float k4[4], q4[4];
+        load_f32<4>(kp + c, WIDE, k4);
+        load_f32<4>(qp + c, WIDE, q4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          kv[st][e + i] = k4[i];
+          qv[st][e + i] = q4[i];
+        }
+      }
   }
-  const double last = __shfl(since, 63);
-  if (w == 0) {
-    decay[lane] = since;
-    beta_s[lane] = lane < rows ? gt.beta : 0.0f;
+  // gates and decays of head h0 + w, a row per lane; e^-10000 is 0 as well as
+  // e^-inf, and does not turn into NaN in a difference
+  double since = 0.0;
+  if (w < heads) {
+    const Gates gt = d.a_log ? gates_of(ga + dt, gb, a_log) : Gates{ga, gb};
+    since = lane < rows ? (double)gt.log_decay : 0.0;
+    if (since < -10000.0) since = -10000.0;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const double v = __shfl_up(since, m);
+      if (lane >= m) since += v;
+    }
+    // in powers of two and two fp32 parts: a difference of two sums is then
+    // exact to its own last bit
+    const double e2 = since * 0x1.71547652b82fep+0;
+    const float hi = (float)e2;
+    decay[w][lane] = make_float2(hi, (float)(e2 - (double)hi));
+    beta_s[w][lane] = lane < rows ? gt.beta : 0.0f;
   }
 
   // norms and parts of keys and queries
@@ -208,9 +243,9 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   float ksum = 0.0f, qsum = 0.0f;
 #pragma unroll
   for (int st = 0; st < KS; ++st) {
-    const bool in = row_in && 32 * st + 8 * g < d.k_dim;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      const bool in = row_in && i < L::SW / 4 && L::SW * st + 4 * (i & 4) + 4 * g < d.k_dim;
       kv[st][i] = in ? kv[st][i] : 0.0f;
       qv[st][i] = in ? qv[st][i] : 0.0f;
       ksum = __builtin_fmaf(kv[st][i], kv[st][i], ksum);
@@ -224,7 +259,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
       store_frag(kfrag, (w * KS + st) * NPK + p, lane, kp4[p]);
       kf[st][p] = __builtin_bit_cast(bf16x8, kp4[p]);
       qf[st][p] = __builtin_bit_cast(bf16x8, qp4[p]);
-      if (!L::direct && h == kh * rep) {
+      if (group == 0) {
         store_frag(kws + L::k_rows, (w * KS + st) * NPK + p, lane, kp4[p]);
         if (p < L::NPQ) store_frag(kws + L::q_rows, (w * KS + st) * L::NPQ + p, lane, qp4[p]);
       }
@@ -242,10 +277,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   }
   __syncthreads();
 
-  // A, with the wave's rows on the left; and the transposed query-key matrix,
-  // with its rows on the right: four consecutive keys of a row per lane, which
-  // is a piece of the left factor that k_delta_chunks loads
-  const double since_q = decay[row];
+  // A and the query-key matrix
   for (int j = 0; j <= w; ++j) {
     f32x4 kk = {}, kq = {};
 #pragma unroll
@@ -253,42 +285,56 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
       bf16x8 b[NPK];
 #pragma unroll
       for (int p = 0; p < NPK; ++p) b[p] = load_frag(kfrag, (j * KS + st) * NPK + p, lane);
-      kk = mfma_parts<3>(kf[st], b, kk);
+      kk = mfma_parts<3>(b, kf[st], kk);
       kq = mfma_parts<3>(b, qf[st], kq);
     }
-    const int col = 16 * j + n;
+    settle(kk);
+    settle(kq);
+    const int c0 = 16 * j + 4 * g;  // the lane's keys c0 .. c0 + 3 of row `row`
+    const f32x4 rkc = *reinterpret_cast<const f32x4*>(rk_s + c0);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int rr = 16 * w + 4 * g + r, cc = 16 * j + 4 * g + r;
-      const float e = rr > col ? expf((float)(decay[rr] - decay[col])) : 0.0f;
-      am[rr * kPad + col] =
-          rr > col && rr < rows ? beta_s[rr] * rk_s[rr] * (e * rk_s[col]) * kk[r] : 0.0f;
-      const float eq = row >= cc ? expf((float)(since_q - decay[cc])) : 0.0f;
-      kq[r] = row >= cc && row_in ? rq * (eq * rk_s[cc]) * kq[r] : 0.0f;
+    for (int i = 0; i < HB; ++i) {
+      if (i >= heads) break;
+      const float2 dr = decay[i][row];
+      const float bk = beta_s[i][row] * rk;
+      f32x4 a, q;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float2 dc = decay[i][c0 + r];
+        const float e = __builtin_amdgcn_exp2f((dr.x - dc.x) + (dr.y - dc.y)) * rkc[r];
+        a[r] = c0 + r < row && row_in ? bk * (e * kk[r]) : 0.0f;
+        q[r] = c0 + r <= row && row_in ? rq * (e * kq[r]) : 0.0f;
+      }
+      *reinterpret_cast<f32x4*>(am + i * kMat + row * kPad + c0) = a;
+      uint2 p[NPO];
+      split4<NPO>(q, p);
+      uint8_t* const to = vws + i * L::v_head + L::qk +
+                          (n + 16 * ((j & 1) * 2 + (g >> 1))) * 16 + (g & 1) * 8;
+#pragma unroll
+      for (int o = 0; o < NPO; ++o)
+        *reinterpret_cast<uint2*>(to + (tile_of(w, j >> 1) * NPO + o) * 1024) = p[o];
     }
-    uint2 p[NPO];
-    split4<NPO>(kq, p);
-    uint8_t* const to = vws + L::qk + (n + 16 * ((j & 1) * 2 + (g >> 1))) * 16 + (g & 1) * 8;
-#pragma unroll
-    for (int i = 0; i < NPO; ++i)
-      *reinterpret_cast<uint2*>(to + (tile_of(w, j >> 1) * NPO + i) * 1024) = p[i];
   }
-  if ((w & 1) == 0) {  // the empty half of the tile on the diagonal
-    uint8_t* const to = vws + L::qk + (n + 32 + 16 * (g >> 1)) * 16 + (g & 1) * 8;
+  if ((w & 1) == 0) {  // the empty halves of the tiles on the diagonal
+    for (int i = 0; i < heads; ++i) {
+      *reinterpret_cast<f32x4*>(am + i * kMat + row * kPad + 16 * w + 16 + 4 * g) = f32x4{};
+      uint8_t* const to = vws + i * L::v_head + L::qk + (n + 32 + 16 * (g >> 1)) * 16 + (g & 1) * 8;
 #pragma unroll
-    for (int i = 0; i < NPO; ++i)
-      *reinterpret_cast<uint2*>(to + (tile_of(w, w >> 1) * NPO + i) * 1024) = make_uint2(0, 0);
+      for (int o = 0; o < NPO; ++o)
+        *reinterpret_cast<uint2*>(to + (tile_of(w, w >> 1) * NPO + o) * 1024) = make_uint2(0, 0);
+    }
   }
-  if (h == kh * rep) {  // K^T
-    for (int i = tid; i < DKT / 16 * 2 * NPK * 64; i += 256) {
-      const int frag = i >> 6, p = frag % NPK, half = frag / NPK & 1, t = frag / (2 * NPK);
+  if (group == 0 && w < 2) {  // K^T, by the waves with fewer products
+    for (int frag = w; frag < DKT / 16 * 2 * NPK; frag += 2) {
+      const int p = frag % NPK, half = frag / NPK & 1, t = frag / (2 * NPK);
       const int c = 16 * t + n;  // key dimension
       uint16_t v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int tok = 32 * half + 8 * g + e;
-        const int from = (((tok >> 4) * KS + (c >> 5)) * NPK + p) * 1024 +
-                         ((tok & 15) + 16 * ((c & 31) >> 3)) * 16 + (c & 7) * 2;
+        const int in = c % L::SW;  // the dimension's place in its step
+        const int from = (((tok >> 4) * KS + c / L::SW) * NPK + p) * 1024 +
+                         ((tok & 15) + 16 * ((in & 15) >> 2)) * 16 + ((in >> 4) * 4 + (in & 3)) * 2;
         v[e] = *reinterpret_cast<const uint16_t*>(kfrag + from);
       }
       store_frag(kws, frag, lane,
@@ -298,80 +344,91 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   }
   __syncthreads();
 
-  // the diagonal blocks of T = (I + A)^-1 from T (I + A) = I, a row per lane
+  // the diagonal blocks of T from T (I + A) = I, a row per lane, a head per group
+  // of lanes
   {
+    float* const a = am + (HB == 2 ? g & 1 : 0) * kMat + 16 * w * kPad + 16 * w;
     float x[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) x[j] = j == n ? 1.0f : 0.0f;
 #pragma unroll
-    for (int m = 15; m > 0; --m) {
-      const float* a = am + (16 * w + m) * kPad + 16 * w;
+    for (int m = 15; m > 0; --m)
 #pragma unroll
-      for (int j = 0; j < m; ++j) x[j] = __builtin_fmaf(-x[m], a[j], x[j]);
-    }
-    if (g == 0) {
-#pragma unroll
-      for (int j = 0; j < 16; j += 4)
-        *reinterpret_cast<f32x4*>(tm + row * kPad + 16 * w + j) = f32x4{x[j], x[j + 1], x[j + 2],
-                                                                        x[j + 3]};
-    } else if (g == 1 && (w & 1) == 0) {  // the empty half of the tile on the diagonal
+      for (int j = 0; j < m; ++j) x[j] = __builtin_fmaf(-x[m], a[m * kPad + j], x[j]);
+    // (in place: the wave has read its block)
+    if (g < HB) {
 #pragma unroll
       for (int j = 0; j < 16; j += 4)
-        *reinterpret_cast<f32x4*>(tm + row * kPad + 16 * w + 16 + j) = f32x4{};
+        *reinterpret_cast<f32x4*>(a + n * kPad + j) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
     }
   }
   __syncthreads();
-  // C tiles as right factors: step r of a product over 16 takes row 4 g + r of it
-  const auto a_blk = [&](const float* m, int bi, int bj, int st) {
-    return m[(16 * bi + n) * kPad + 16 * bj + st];
+  // block (bi, bj) from the left; C tiles as right factors: step r of a product
+  // over 16 takes row 4 g + r of it
+  const auto left = [&](const float* m, int bi, int bj, int k) {
+    return m[(16 * bi + n) * kPad + 16 * bj + k];
   };
-  if (w < 2) {
-    const int b0 = 2 * w, b1 = b0 + 1;
+  if (w < 2 * HB) {
+    float* const a = am + (w >> 1) * kMat;
+    const int b0 = 2 * (w & 1), b1 = b0 + 1;
     f32x4 x = {}, y = {};
 #pragma unroll
     for (int st = 0; st < 4; ++st)
-      x = mfma_f32(a_blk(am, b1, b0, 4 * st + g),
-                   tm[(16 * b0 + 4 * st + g) * kPad + 16 * b0 + n], x);
+      x = mfma_f32(left(a, b1, b0, 4 * st + g), a[(16 * b0 + 4 * st + g) * kPad + 16 * b0 + n], x);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) y = mfma_f32(a_blk(tm, b1, b1, 4 * g + r), x[r], y);
+    for (int r = 0; r < 4; ++r) y = mfma_f32(left(a, b1, b1, 4 * g + r), x[r], y);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) tm[(16 * b1 + 4 * g + r) * kPad + 16 * b0 + n] = -y[r];
+    for (int r = 0; r < 4; ++r) a[(16 * b1 + 4 * g + r) * kPad + 16 * b0 + n] = -y[r];
   }
   __syncthreads();
-  {
-    const int bi = w >> 1, bj = w & 1;
-    f32x4 y = {};
+  // the 2 x 2 blocks below: with two heads, a wave has a long and a short one
+  const int fi = HB == 2 ? w & 1 : 0;
+  float* const fa = am + fi * kMat;
+  f32x4 fy[HB] = {};
+#pragma unroll
+  for (int task = 0; task < HB; ++task) {
+    const int bi = HB == 2 ? (task == 0) : w >> 1, bj = HB == 2 ? (w >> 1) ^ task : w & 1;
     for (int k = 0; k <= bi; ++k) {
       f32x4 x = {};
       for (int kk = bj; kk < 2; ++kk)
 #pragma unroll
         for (int st = 0; st < 4; ++st)
-          x = mfma_f32(a_blk(am, 2 + k, kk, 4 * st + g),
-                       tm[(16 * kk + 4 * st + g) * kPad + 16 * bj + n], x);
+          x = mfma_f32(left(fa, 2 + k, kk, 4 * st + g),
+                       fa[(16 * kk + 4 * st + g) * kPad + 16 * bj + n], x);
+      settle(x);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) y = mfma_f32(a_blk(tm, 2 + bi, 2 + k, 4 * g + r), x[r], y);
+      for (int r = 0; r < 4; ++r)
+        fy[task] = mfma_f32(left(fa, 2 + bi, 2 + k, 4 * g + r), x[r], fy[task]);
     }
+    settle(fy[task]);
+  }
+  __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 4; ++r) tm[(32 + 16 * bi + 4 * g + r) * kPad + 16 * bj + n] = -y[r];
+  for (int task = 0; task < HB; ++task) {
+    const int bi = HB == 2 ? (task == 0) : w >> 1, bj = HB == 2 ? (w >> 1) ^ task : w & 1;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) fa[(32 + 16 * bi + 4 * g + r) * kPad + 16 * bj + n] = -fy[task][r];
   }
   __syncthreads();
 
-  // its parts, as a left factor
-  for (int i = tid; i < kTiles * 64; i += 256) {
-    const int tile = i >> 6;  // (lane is i & 63)
+  // T diag(beta) in parts, as a left factor
+  for (int q = tid; q < heads * kTiles * 64; q += 256) {
+    const int i = q / (kTiles * 64), tile = (q >> 6) % kTiles;  // (lane is q & 63)
     const int blk = tile < 2 ? tile : (tile + 2) / 2, half = tile < 2 ? 0 : tile & 1;
-    const int at = (16 * blk + n) * kPad + 32 * half + 8 * g;
+    const float* const t = am + i * kMat + (16 * blk + n) * kPad + 32 * half + 8 * g;
+    const float* const b = beta_s[i] + 32 * half + 8 * g;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tm[at + e] * beta_s[32 * half + 8 * g + e];
+    for (int e = 0; e < 8; ++e) v[e] = t[e] * b[e];
     uint4 vp[3];
     split8<3>(v, vp);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) store_frag(vws, tile * 3 + p, lane, vp[p]);
+    for (int p = 0; p < 3; ++p) store_frag(vws + i * L::v_head, tile * 3 + p, lane, vp[p]);
   }
-  if (w == 0) {
-    float* f = reinterpret_cast<float*>(vws + L::rows);
+  if (w < heads) {
+    float* f = reinterpret_cast<float*>(vws + w * L::v_head + L::rows);
     const bool in = lane < rows;
+    const double last = __shfl(since, 63);
     const float grown = expf((float)since);
     f[lane] = in ? grown * rk_s[lane] : 0.0f;
     f[kChunk + lane] = in ? grown * rq_s[lane] : 0.0f;
@@ -381,21 +438,52 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
 }
 
 // ---- the chunks of a head, in order ----------------------------------------------
-// One workgroup per head and 16 NC columns of its state, which four waves hold
-// in registers, each the rows of DKT / 64 tiles of 16.  In a chunk wave w
-// computes rows 16 w .. 16 w + 15: K S and Q S (all of S needed), R = V - K S,
-// U = T R (rows of R up to its own), O; and then its rows of K^T U (all of U).
-// S, R and U pass between the waves through LDS, already split into parts and
-// in the order in which a right factor is held, so a chunk has three barriers.
-// Every left factor is loaded straight into registers, as soon as the previous
-// chunk's is used up.  A chunk takes about as long as this chain of products and
-// exchanges, whatever the number of columns; more heads or sequences run beside
-// it.
-template <typename T, int DKT, int NC, int NPK, int NPO, bool WIDE>
-__global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev s, ChunkWork cw) {
+// One workgroup per head and 16 NC columns of its state, eight waves.  Waves 0-3
+// walk the chain from chunk to chunk: each holds the rows of DKT / 64 tiles of
+// 16 of the state in registers, where they are a right factor as they stand, and
+//   1  P   of all 64 rows over its part of the key dimension, summed through LDS,
+//   2  R = V - e^G P and
+//   3  U = T R of rows 16 w .. 16 w + 15 (rows of R up to its own),
+//   4  its rows of S' = e^G_last S + K^T U,
+// with a barrier behind 1, 2 and 3.  Waves 4-7 bring the factors of the chain
+// from memory into LDS, without registers where they fit (STAGE), and make the
+// outputs of 16 rows each, O = e^G Q S + (Q K^T) U, from the parts of S and U that
+// the others leave in LDS.  So the chain never waits for memory: with its loads
+// its own, a third of its time went into their issue, 64 bytes a cycle and CU.
+// A factor is used in one step only, so one copy of each is enough: the next
+// chunk's K arrives from the barrier behind step 1 to the one behind 3, K^T as
+// well, T from there to the next one.  Where they do not fit, the chain loads K,
+// T and K^T into registers itself.
+constexpr size_t kLds = 160 * 1024 - 512;
+
+template <int DKT, int NC, int NPK, int NPO, bool WIDE>
+struct Shared {
   using L = Layout<DKT, NPK, NPO, WIDE>;
-  constexpr int KS = L::KS, NT = DKT / 64, NPQ = L::NPQ;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  static constexpr int KS = L::KS;
+  static constexpr size_t s = 0;                               // S: [step][column tile][part]
+  static constexpr size_t p = s + frag_bytes(KS * NC * NPO);   // P: [column tile][row block][wave]
+  static constexpr size_t r = p + frag_bytes(16 * NC);         // R: [half][column tile][part]
+  static constexpr size_t u = r + frag_bytes(3 * 2 * NC);      // U
+  static constexpr size_t g = u + frag_bytes(NPO * 2 * NC);    // U as S' takes it
+  static constexpr size_t v = g + frag_bytes(3 * 2 * NC);      // V: [row][column] fp32
+  static constexpr size_t f = v + (size_t)kChunk * 16 * NC * 4;  // factors of rows, twice
+  static constexpr size_t common = f + 2 * 3 * kChunk * 4;
+  static constexpr size_t k = common;                          // K, T, K^T as k_delta_prep left them
+  static constexpr size_t t = k + frag_bytes(4 * KS * NPK);
+  static constexpr size_t kt = t + frag_bytes(kTiles * 3);
+  static constexpr size_t all = kt + frag_bytes(DKT / 16 * 2 * NPK);
+  static constexpr bool stage = all <= kLds;
+  static constexpr size_t bytes = stage ? all : common;
+};
+
+template <typename T, int DKT, int NC, int NPK, int NPO, bool WIDE>
+__global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev s, ChunkWork cw) {
+  using L = Layout<DKT, NPK, NPO, WIDE>;
+  using M = Shared<DKT, NC, NPK, NPO, WIDE>;
+  constexpr int KS = L::KS, KW = KS / 4, NT = DKT / 64, NPQ = L::NPQ;
+  constexpr int kKT = DKT / 16 * 2 * NPK;  // fragments of K^T
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3;
   const int n = lane & 15, g = lane >> 4;
   // the column blocks of a head on one XCD (workgroups go round the XCDs): they
   // read the same factors
@@ -407,27 +495,192 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
   const SeqRange r = seq_range(s, seq, false);
   if (!r.live || r.end - r.begin < cw.min_rows) return;
 
-  __shared__ __align__(16) uint8_t sb[frag_bytes(3 * KS * NC)];
-  __shared__ __align__(16) uint8_t rb[frag_bytes(3 * 2 * NC)];
-  __shared__ __align__(16) uint8_t ub[frag_bytes(NPO * 2 * NC)], gb[frag_bytes(3 * 2 * NC)];
+  __shared__ __align__(16) uint8_t lds[M::bytes];
   __shared__ int before;
+  uint8_t* const sb = lds + M::s;
+  uint8_t* const pb = lds + M::p;
+  uint8_t* const rb = lds + M::r;
+  uint8_t* const ub = lds + M::u;
+  uint8_t* const gb = lds + M::g;
+  float* const vb = reinterpret_cast<float*>(lds + M::v);
+  float* const fb = reinterpret_cast<float*>(lds + M::f);  // [chunk & 1][R | U | fade][row]
 
   // chunks of the sequences before this one
   if (tid == 0) before = 0;
   __syncthreads();
   int mine = 0;
-  for (int j = tid; j < seq; j += 256) mine += chunks_of(s, j, cw.min_rows);
+  for (int j = tid; j < seq; j += 512) mine += chunks_of(s, j, cw.min_rows);
   if (mine) atomicAdd(&before, mine);
   __syncthreads();
-  const int first = cw.rank0 - __builtin_amdgcn_readfirstlane(before);  // of this pass, counted in this sequence
-  const int c0 = max(first, 0);
-  const int c1 = min((r.end - r.begin + kChunk - 1) / kChunk, first + cw.count);
+  // (of this pass, counted in this sequence)
+  const int first = cw.rank0 - __builtin_amdgcn_readfirstlane(before);
+  const int len = r.end - r.begin;
+  const int c0 = max(first, 0), c1 = min((len + kChunk - 1) / kChunk, first + cw.count);
   if (c0 >= c1) return;
 
-  // an element of a C tile: row 4 g + i of 16, column n.  O is held transposed, a
-  // row and four columns per lane.
-  const int col = cb * 16 * NC + n, ocol = cb * 16 * NC + 4 * g;
-  T* const nowhere = reinterpret_cast<T*>(cw.nowhere + tid * 16);
+  // Loads have a uniform base per chunk and 32-bit offsets of the lane that hold
+  // for all chunks, and are not conditional, so that none waits for another.
+  size_t vws_at = ((size_t)(c0 - first) * d.v_heads + h) * L::v_head;
+  size_t kws_at = ((size_t)(c0 - first) * d.k_heads + kh) * L::k_head;
+  const uint8_t *vws = cw.v_heads + vws_at, *kws = cw.k_heads + kws_at;
+  const auto step = [&](int c) {  // from chunk c to the next one's factors (the last one's again)
+    vws_at += c + 1 < c1 ? (size_t)d.v_heads * L::v_head : 0;
+    kws_at += c + 1 < c1 ? (size_t)d.k_heads * L::k_head : 0;
+    asm("" : "+s"(vws_at), "+s"(kws_at));  // one base each: not one for every load
+    vws = cw.v_heads + vws_at;
+    kws = cw.k_heads + kws_at;
+  };
+  const uint32_t at16 = lane * 16;
+  const auto frag = [](const uint8_t* base, uint32_t at) {
+    return *reinterpret_cast<const bf16x8*>(base + at);
+  };
+  const bool two = w >= 2;  // rows 32 on: two tiles of the triangular factors
+  const auto get = [&](const uint8_t* base, int st, int nc, auto& b) {
+    constexpr int NP = sizeof(b) / sizeof(b[0]);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) b[i] = load_frag(base, (st * NC + nc) * NP + i, lane);
+  };
+
+  if (wave >= 4) {  // ---- loads, and the outputs of rows 16 w .. 16 w + 15
+    // O and V are held transposed: a row (n) and four columns per lane
+    const int col = cb * 16 * NC + 4 * g, row = 16 * w + n;
+    const uint32_t q_at = (uint32_t)L::q_rows + w * KS * NPQ * 1024 + at16;
+    const uint32_t a_at[2] = {(uint32_t)L::qk + tile_of(w, 0) * NPO * 1024 + at16,
+                              (uint32_t)L::qk + tile_of(w, two) * NPO * 1024 + at16};
+    // the rows' factors in one load: of lane group 0 for R, 1 for O, 2 for U, 3 fade
+    const uint32_t f_at = (uint32_t)L::rows + (g * kChunk + (g < 3 ? row : 0)) * 4;
+    T* const o0 = static_cast<T*>(d.o) + (int64_t)(r.begin + row) * d.o_stride + h * d.v_dim + col;
+    const T* const v0 = static_cast<const T*>(d.v) + (int64_t)r.begin * d.v_stride + h * d.v_dim;
+    bf16x8 qf[KS][NPQ], af[2][NPO];
+    float f;
+    // V as it comes: a conversion would wait for it
+    using Bits = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
+    Vec<T, 4> v4[NC];
+    uint32_t v1[NC][4];
+    const auto load_q = [&] {
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+#pragma unroll
+        for (int i = 0; i < NPQ; ++i) qf[st][i] = frag(kws, q_at + (st * NPQ + i) * 1024);
+    };
+    const auto load_a = [&] {
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int i = 0; i < NPO; ++i) af[st][i] = frag(vws, a_at[st] + i * 1024);
+    };
+    const auto load_v = [&](int c) {
+      f = *reinterpret_cast<const float*>(vws + f_at);
+      // (a row or columns that are not there: the chunk's first)
+      const T* const vp = v0 + ((int64_t)c * kChunk + (c * kChunk + row < len ? row : 0)) * d.v_stride;
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) {
+        const T* const at = vp + (col + 16 * nc < d.v_dim ? col + 16 * nc : 0);
+        if constexpr (WIDE) {
+          v4[nc] = *reinterpret_cast<const Vec<T, 4>*>(at);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v1[nc][i] = reinterpret_cast<const Bits*>(at)[i];
+        }
+      }
+    };
+    const auto put_v = [&](int c) {
+      const bool in = c * kChunk + row < len;
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          T e;
+          if constexpr (WIDE) e = v4[nc].v[i];
+          else e = __builtin_bit_cast(T, (Bits)v1[nc][i]);
+          x[i] = in ? (float)e : 0.0f;
+        }
+        *reinterpret_cast<f32x4*>(vb + row * 16 * NC + 16 * nc + 4 * g) = x;
+      }
+      if (g != 1) fb[((c & 1) * 3 + (g == 0 ? 0 : g - 1)) * kChunk + row] = f;
+    };
+    // fragments of the chain, a quarter of them per wave
+    const auto bring = [&](const uint8_t* from, size_t to, int count) {
+#pragma unroll
+      for (int i = 0; i < (count + 3) / 4; ++i) {
+        const int j = 4 * i + w;
+        if (count % 4 == 0 || j < count) dma16_lds(from + j * 1024 + at16, lds_u32(lds + to + j * 1024));
+      }
+    };
+    load_q();
+    load_a();
+    load_v(c0);
+    if constexpr (M::stage) {
+      bring(kws + L::k_rows, M::k, 4 * KS * NPK);
+      bring(vws, M::t, kTiles * 3);
+    }
+    put_v(c0);
+    wait_vm();
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // (vmcnt 0, which the compiler takes note of)
+    lds_barrier();
+    for (int c = c0; c < c1; ++c) {
+      const float pq = __shfl(f, 16 + n);
+      lds_barrier();  // 1
+      const uint8_t* const kt_from = kws;
+      step(c);
+      if constexpr (M::stage) {
+        bring(kws + L::k_rows, M::k, 4 * KS * NPK);
+        bring(kt_from, M::kt, kKT);
+      }
+      load_v(min(c + 1, c1 - 1));
+      lds_barrier();  // 2
+      f32x4 o[NC][2] = {};
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+          bf16x8 b[NPO];
+          get(sb, st, nc, b);
+          o[nc][st & 1] = mfma_parts<NPO>(b, qf[st], o[nc][st & 1]);
+        }
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) {
+        settle(o[nc][0]);
+        settle(o[nc][1]);
+        o[nc][0] = (o[nc][0] + o[nc][1]) * pq;
+      }
+      load_q();
+      // K and K^T are there: only what was issued behind them, Q, may be under way
+      if constexpr (M::stage) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KS * NPQ) : "memory");
+      lds_barrier();  // 3
+      if constexpr (M::stage) bring(vws, M::t, kTiles * 3);
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) {
+        bf16x8 b[NPO];
+        get(ub, 0, nc, b);
+        o[nc][0] = mfma_parts<NPO>(b, af[0], o[nc][0]);
+        if (two) {
+          get(ub, 1, nc, b);
+          o[nc][0] = mfma_parts<NPO>(b, af[1], o[nc][0]);
+        }
+        settle(o[nc][0]);
+      }
+      load_a();
+      put_v(c + 1);
+      if (c * kChunk + row < len) {
+        T* const op = o0 + (int64_t)c * kChunk * d.o_stride;
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+          const float y[4] = {o[nc][0][0], o[nc][0][1], o[nc][0][2], o[nc][0][3]};
+          if (col + 16 * nc < d.v_dim) store_f32<4>(op + 16 * nc, WIDE, y);
+        }
+      }
+      // T is there: only what was issued behind it, the stores, may be under way
+      if constexpr (M::stage) asm volatile("s_waitcnt vmcnt(1)" ::: "memory");
+    }
+    return;
+  }
+
+  // ---- the chain
+  __builtin_amdgcn_s_setprio(3);
+  // an element of a C tile: row 4 g + i of 16, column n
+  const int col = cb * 16 * NC + n;
   float* const sp = d.state + (((size_t)r.slot * d.v_heads + h) * d.k_dim + 16 * NT * w + 4 * g) *
                                   d.v_dim + col;
   f32x4 S[NT][NC];
@@ -440,99 +693,7 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
         const bool in = 16 * (NT * w + t) + 4 * g + i < d.k_dim && col + 16 * nc < d.v_dim;
         S[t][nc][i] = in && !(c0 == 0 && r.fresh) ? sp[(size_t)(16 * t + i) * d.v_dim + 16 * nc] : 0.0f;
       }
-
-  bf16x8 kf[KS][NPK], qf[KS][NPQ], tf[2][3], af[2][NPO], gf[NT][2][NPK];
-  T v[NC][4];
-  f32x4 pk, pr;
-  float pq, fade;
-  const bool two = w >= 2;  // rows 32 on: two tiles of the triangular factors
-  // Loads are unconditional, so that none waits for another: behind the last row
-  // or dimension they read one that is there (what comes of it meets a factor of
-  // zero or is not stored).  Addresses are a uniform base of the chunk and 32-bit
-  // offsets of the lane that hold for all chunks.
-  const uint32_t at16 = lane * 16;
-  const uint32_t t_at[2] = {tile_of(w, 0) * 3 * 1024 + at16, tile_of(w, two) * 3 * 1024 + at16};
-  const uint32_t a_at[2] = {(uint32_t)L::qk + tile_of(w, 0) * NPO * 1024 + at16,
-                            (uint32_t)L::qk + tile_of(w, two) * NPO * 1024 + at16};
-  const uint32_t g_at = NT * w * 2 * NPK * 1024 + at16;
-  const uint32_t kr_at = (uint32_t)L::k_rows + w * KS * NPK * 1024 + at16;
-  const uint32_t qr_at = (uint32_t)L::q_rows + w * KS * NPQ * 1024 + at16;
-  const uint32_t f4_at = (uint32_t)L::rows + (16 * w + 4 * g) * 4;
-  const uint32_t f1_at = (uint32_t)L::rows + (kChunk + 16 * w + n) * 4;
-  uint32_t k_at[KS], v_at[NC];
-#pragma unroll
-  for (int st = 0; st < KS; ++st)
-    k_at[st] = (32 * st + 8 * g < d.k_dim ? 32 * st + 8 * g : 0) * sizeof(T);
-#pragma unroll
-  for (int nc = 0; nc < NC; ++nc) v_at[nc] = min(col + 16 * nc, d.v_dim - 1) * sizeof(T);
-  const auto frag = [](const uint8_t* base, uint32_t at) {
-    return *reinterpret_cast<const bf16x8*>(base + at);
-  };
-  const uint8_t* const k0 = reinterpret_cast<const uint8_t*>(
-      static_cast<const T*>(d.k) + (int64_t)r.begin * d.k_stride + kh * d.k_dim);
-  const uint8_t* const q0 = reinterpret_cast<const uint8_t*>(
-      static_cast<const T*>(d.q) + (int64_t)r.begin * d.q_stride + kh * d.k_dim);
-  const uint8_t* const v0 = reinterpret_cast<const uint8_t*>(
-      static_cast<const T*>(d.v) + (int64_t)r.begin * d.v_stride + h * d.v_dim);
-  const int64_t k_pitch = d.k_stride * sizeof(T), q_pitch = d.q_stride * sizeof(T);
-  const int64_t v_pitch = d.v_stride * sizeof(T);
-  T* const o0 = static_cast<T*>(d.o) + (int64_t)r.begin * d.o_stride + h * d.v_dim + ocol;
-  const int len = r.end - r.begin;
-  const auto load_rows = [&](int c, const uint8_t* kws) {  // K and Q
-    if constexpr (L::direct) {
-      const int row = min(c * kChunk + 16 * w + n, len - 1);
-      const uint8_t *kp = k0 + row * k_pitch, *qp = q0 + row * q_pitch;
-#pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        kf[st][0] = frag(kp, k_at[st]);
-        qf[st][0] = frag(qp, k_at[st]);
-      }
-    } else {
-#pragma unroll
-      for (int st = 0; st < KS; ++st) {
-#pragma unroll
-        for (int i = 0; i < NPK; ++i) kf[st][i] = frag(kws, kr_at + (st * NPK + i) * 1024);
-#pragma unroll
-        for (int i = 0; i < NPQ; ++i) qf[st][i] = frag(kws, qr_at + (st * NPQ + i) * 1024);
-      }
-    }
-  };
-  const auto load_v = [&](int c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t* vp = v0 + min(c * kChunk + 16 * w + 4 * g + i, len - 1) * v_pitch;
-#pragma unroll
-      for (int nc = 0; nc < NC; ++nc) v[nc][i] = *reinterpret_cast<const T*>(vp + v_at[nc]);
-    }
-  };
-  const auto load_factors = [&](const uint8_t* vws) {
-    pk = *reinterpret_cast<const f32x4*>(vws + f4_at);
-    pq = *reinterpret_cast<const float*>(vws + f1_at);
-    pr = *reinterpret_cast<const f32x4*>(vws + f4_at + 2 * kChunk * 4);
-    fade = *reinterpret_cast<const float*>(vws + L::rows + 3 * kChunk * 4);
-  };
-  const auto load_t = [&](const uint8_t* vws) {
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int i = 0; i < 3; ++i) tf[st][i] = frag(vws, t_at[st] + i * 1024);
-  };
-  const auto load_a = [&](const uint8_t* vws) {
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int i = 0; i < NPO; ++i) af[st][i] = frag(vws, a_at[st] + i * 1024);
-  };
-  const auto load_kt = [&](const uint8_t* kws) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int i = 0; i < NPK; ++i)
-          gf[t][st][i] = frag(kws, g_at + ((t * 2 + st) * NPK + i) * 1024);
-  };
-  // tile t of a right factor's rows to LDS: fragment [step][column tile][part]
+  // row block t of a right factor to LDS
   const auto put = [&](uint8_t* base, int t, int nc, auto parts, f32x4 x) {
     constexpr int NP = decltype(parts)::value;
     uint2 p[NP];
@@ -542,85 +703,119 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
     for (int i = 0; i < NP; ++i)
       *reinterpret_cast<uint2*>(base + (((t >> 1) * NC + nc) * NP + i) * 1024 + at) = p[i];
   };
-  const auto get = [&](const uint8_t* base, int st, int nc, auto& b) {
-    constexpr int NP = sizeof(b) / sizeof(b[0]);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) b[i] = load_frag(base, (st * NC + nc) * NP + i, lane);
-  };
   using P3 = std::integral_constant<int, 3>;
   using PO = std::integral_constant<int, NPO>;
 
-  size_t vws_at = ((size_t)(c0 - first) * d.v_heads + h) * L::v_head;
-  size_t kws_at = ((size_t)(c0 - first) * d.k_heads + kh) * L::k_head;
-  const uint8_t *vws = cw.v_heads + vws_at, *kws = cw.k_heads + kws_at;
-  load_rows(c0, kws);
-  load_v(c0);
-  load_factors(vws);
-  load_t(vws);
-  load_a(vws);
-  load_kt(kws);
-  // All loads here (vmcnt 0): the waits that the compiler places in the loop
-  // would otherwise have to hold for the order of these as well, and wait for
-  // every load there.
-  __builtin_amdgcn_s_waitcnt(0x0F70);
-  for (int c = c0; c < c1; ++c) {
-    const int next = min(c + 1, c1 - 1), row0 = c * kChunk + 16 * w + 4 * g;
-    vws_at += next > c ? (size_t)d.v_heads * L::v_head : 0;
-    kws_at += next > c ? (size_t)d.k_heads * L::k_head : 0;
-    asm("" : "+s"(vws_at), "+s"(kws_at));  // one base each: not one for every load
-    vws = cw.v_heads + vws_at;
-    kws = cw.k_heads + kws_at;
+  // a factor: from LDS where a step begins, or into registers for the next chunk
+  bf16x8 kf[4][KW][NPK], tf[2][3], gf[NT][2][NPK];
+  const auto take_k = [&](const uint8_t* base) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < KW * NPK; ++i)
+        kf[b][i / NPK][i % NPK] = frag(base, (b * KS + w * KW) * NPK * 1024 + i * 1024 + at16);
+  };
+  const auto take_t = [&](const uint8_t* base) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      tf[0][i] = frag(base, tile_of(w, 0) * 3 * 1024 + i * 1024 + at16);
+      tf[1][i] = frag(base, tile_of(w, two) * 3 * 1024 + i * 1024 + at16);
+    }
+  };
+  const auto take_kt = [&](const uint8_t* base) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc) put(sb, NT * w + t, nc, P3{}, S[t][nc]);
-    lds_barrier();
-    // (two chains each: a product waits for the last one of its own sum)
-    f32x4 p[NC][2] = {}, o[NC][2] = {};
+      for (int i = 0; i < 2 * NPK; ++i)
+        gf[t][i / NPK][i % NPK] = frag(base, (NT * w + t) * 2 * NPK * 1024 + i * 1024 + at16);
+  };
+  if constexpr (!M::stage) {
+    take_k(kws + L::k_rows);
+    take_t(vws);
+    take_kt(kws);
+    // All loads here (vmcnt 0): the waits that the compiler places in the loop
+    // would otherwise have to hold for the order of these as well, and wait for
+    // every load there.
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+  }
+  lds_barrier();
+  for (int c = c0; c < c1; ++c) {
+    const float* const fc = fb + (c & 1) * 3 * kChunk;
+    if constexpr (M::stage) take_k(lds + M::k);
+    f32x4 p[NC][4] = {};
 #pragma unroll
-    for (int st = 0; st < KS; ++st)
+    for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc) {
+      for (int kw = 0; kw < KW; ++kw) {
+        uint2 lo[3], hi[3] = {};
+        split4<3>(S[NT == 1 ? 0 : 2 * kw][nc], lo);
+        if constexpr (NT > 1) split4<3>(S[2 * kw + 1][nc], hi);
         bf16x8 b[3];
-        get(sb, st, nc, b);
-        p[nc][st & 1] = mfma_parts<3>(kf[st], b, p[nc][st & 1]);
-        o[nc][st & 1] = mfma_parts<NPO>(b, qf[st], o[nc][st & 1]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const uint4 q = make_uint4(lo[i].x, lo[i].y, hi[i].x, hi[i].y);
+          if (i < NPO) store_frag(sb, ((w * KW + kw) * NC + nc) * NPO + i, lane, q);
+          b[i] = __builtin_bit_cast(bf16x8, q);
+        }
+#pragma unroll
+        for (int i = 0; i < NPK; ++i)  // (part by part: four sums in turn)
+#pragma unroll
+          for (int j = 0; j < 3 - i; ++j)
+#pragma unroll
+            for (int blk = 0; blk < 4; ++blk) p[nc][blk] = mfma16(kf[blk][kw][i], b[j], p[nc][blk]);
       }
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+      for (int blk = 0; blk < 4; ++blk)
+        *reinterpret_cast<f32x4*>(pb + ((nc * 4 + blk) * 4 + w) * 1024 + at16) = p[nc][blk];
+    lds_barrier();
+    const f32x4 pk = *reinterpret_cast<const f32x4*>(fc + 16 * w + 4 * g);
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
-      p[nc][0] += p[nc][1];
-      f32x4 x;
+      f32x4 q[4], x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = __builtin_fmaf(-pk[i], p[nc][0][i], row0 + i < len ? (float)v[nc][i] : 0.0f);
-        o[nc][0][i] = (o[nc][0][i] + o[nc][1][i]) * pq;
-      }
+      for (int i = 0; i < 4; ++i)
+        q[i] = *reinterpret_cast<const f32x4*>(pb + ((nc * 4 + w) * 4 + i) * 1024 + at16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = vb[(16 * w + 4 * g + i) * 16 * NC + 16 * nc + n];
+      q[0] = (q[0] + q[1]) + (q[2] + q[3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-pk[i], q[0][i], x[i]);
       put(rb, w, nc, P3{}, x);
     }
-    load_rows(next, kws);
-    load_v(next);
+    if constexpr (M::stage) take_t(lds + M::t);
+    const f32x4 pr = *reinterpret_cast<const f32x4*>(fc + kChunk + 16 * w + 4 * g);
+    const float fade = fc[2 * kChunk + 16 * w];
     lds_barrier();
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
-      f32x4 u = {};
-      bf16x8 b[3];
+      f32x4 u = {}, u1 = {};
+      bf16x8 b[3], b1[3];
       get(rb, 0, nc, b);
-      u = mfma_parts<3>(tf[0], b, u);
       if (two) {
-        f32x4 u1 = {};
-        get(rb, 1, nc, b);
-        u1 = mfma_parts<3>(tf[1], b, u1);
+        get(rb, 1, nc, b1);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int j = 0; j < 3 - i; ++j) {
+            u = mfma16(tf[0][i], b[j], u);
+            u1 = mfma16(tf[1][i], b1[j], u1);
+          }
+        settle(u);
+        settle(u1);
         u += u1;
+      } else {
+        u = mfma_parts<3>(tf[0], b, u);
+        settle(u);
       }
+      put(gb, w, nc, P3{}, u * pr);
       put(ub, w, nc, PO{}, u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] *= pr[i];
-      put(gb, w, nc, P3{}, u);
     }
-    load_t(vws);
     lds_barrier();
+    if constexpr (M::stage) take_kt(lds + M::kt);
 #pragma unroll
-    for (int nc = 0; nc < NC; ++nc) {
+    for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         bf16x8 b[3];
@@ -631,26 +826,16 @@ __global__ __launch_bounds__(256) void k_delta_chunks(dmh_gated_delta d, SeqDev 
           S[t][nc] = mfma_parts<3>(gf[t][st], b, S[t][nc]);
         }
       }
-      bf16x8 b[NPO];
-      get(ub, 0, nc, b);
-      o[nc][0] = mfma_parts<NPO>(b, af[0], o[nc][0]);
-      if (two) {
-        get(ub, 1, nc, b);
-        o[nc][0] = mfma_parts<NPO>(b, af[1], o[nc][0]);
-      }
+    if constexpr (!M::stage) {
+      step(c);
+      take_k(kws + L::k_rows);
+      take_t(vws);
+      take_kt(kws);
     }
-    load_kt(kws);
-    load_a(vws);
-    load_factors(vws);
-    // (not a branch, which would make the waits in the loop longer)
-    const int row = c * kChunk + 16 * w + n;
-    T* const op = o0 + row * d.o_stride;
 #pragma unroll
-    for (int nc = 0; nc < NC; ++nc) {
-      const bool in = row < len && ocol + 16 * nc < d.v_dim;
-      const float y[4] = {o[nc][0][0], o[nc][0][1], o[nc][0][2], o[nc][0][3]};
-      store_f32<4>(in ? op + 16 * nc : nowhere, WIDE, y);
-    }
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) settle(S[t][nc]);
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -688,19 +873,22 @@ hipError_t run(T, Layout<DKT, NPK, NPO, WIDE>, const dmh_gated_delta& a, const S
   cw.v_heads = static_cast<uint8_t*>(ws);
   cw.k_heads = cw.v_heads + (size_t)room * a.v_heads * L::v_head;
   cw.min_rows = min_rows;
-  cw.nowhere = cw.k_heads + (size_t)room * a.k_heads * L::k_head;
   const int64_t units = ((int64_t)s.num * a.v_heads + 7) / 8 * 8;
   for (int64_t at = 0; at < chunks; at += room) {
     cw.rank0 = (int)at;
     cw.count = (int)(chunks - at < room ? chunks - at : room);
-    k_delta_prep<T, DKT, NPK, NPO, WIDE>
-        <<<dim3((unsigned)cw.count * a.v_heads), 256, 0, st>>>(a, s, cw);
+    const int rep = a.v_heads / a.k_heads;
+    if (rep > 1)
+      k_delta_prep<T, DKT, NPK, NPO, WIDE, 2>
+          <<<dim3((unsigned)cw.count * a.k_heads * ((rep + 1) / 2)), 256, 0, st>>>(a, s, cw);
+    else
+      k_delta_prep<T, DKT, NPK, NPO, WIDE, 1>
+          <<<dim3((unsigned)cw.count * a.k_heads), 256, 0, st>>>(a, s, cw);
     const char* e = getenv("DM_NC");
     const int nc = e ? atoi(e) : 1;
     const unsigned ncb = (a.v_dim + 16 * nc - 1) / (16 * nc);
-    if (nc == 1) k_delta_chunks<T, DKT, 1, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 256, 0, st>>>(a, s, cw);
-    if (nc == 2) k_delta_chunks<T, DKT, 2, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 256, 0, st>>>(a, s, cw);
-    if (nc == 4) k_delta_chunks<T, DKT, DKT == 256 ? 2 : 4, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 256, 0, st>>>(a, s, cw);
+    if (nc == 1) k_delta_chunks<T, DKT, 1, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 512, 0, st>>>(a, s, cw);
+    if (nc == 2) k_delta_chunks<T, DKT, 2, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 512, 0, st>>>(a, s, cw);
   }
   return hipGetLastError();
 }

@@ -34,7 +34,7 @@ hipError_t launch_delta_rows(const dmh_gated_delta& a, const SeqDev& s, int max_
 
 // Sequences of min_rows rows and more, in chunks of kDeltaChunk: delta_chunk_count
 // is the most there can be, room of them are worked on at a time, in ws of room
-// times delta_chunk_bytes, and 4096 more.
+// times delta_chunk_bytes.
 constexpr int kDeltaChunk = 64;
 int64_t delta_chunk_count(const SeqDev& s, int min_rows);
 size_t delta_chunk_bytes(const dmh_gated_delta& a, bool wide);

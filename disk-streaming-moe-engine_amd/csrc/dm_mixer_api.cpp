@@ -279,7 +279,8 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
   const Rows gb{a.b, b.total_tokens, a.v_heads, a.b_stride, gs};
   const Rows state{a.state, b.num_slots, sw, sw, 4};
   for (const Rows* r : std::initializer_list<const Rows*>{&q, &k, &v, &o, &ga, &gb})
-    if (!r->ok()) return err.arg("a stride is shorter than its row");
+    if (!r->ok() || r->stride >= 1 << 24)
+      return err.arg("a stride is shorter than its row, or 2^24 or more");
   for (const Rows* r : std::initializer_list<const Rows*>{&q, &k, &v, &ga, &gb})
     if (overlap(o, *r) || overlap(state, *r))
       return err.arg("o and state must not overlap the inputs");
@@ -311,7 +312,7 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
   const int64_t chunks = b.max_seq_len > kRowsMost ? dm::delta_chunk_count(s, kRowsMost + 1) : 0;
   const int64_t room = std::min(chunks, kChunkRoom);
   void* ws = nullptr;
-  if (chunks && (rc = dm::api_mixer_buffer(c, dm::kMixerChunks, room * dm::delta_chunk_bytes(a, wide) + 4096,
+  if (chunks && (rc = dm::api_mixer_buffer(c, dm::kMixerChunks, room * dm::delta_chunk_bytes(a, wide),
                                            &ws, errp, errlen)))
     return rc;
   hipError_t e = dm::launch_delta_rows(a, s, kRowsMost, wide, st);

@@ -103,19 +103,17 @@ __device__ __forceinline__ float sigmoid_hw(float z) {
 struct Gates {
   float log_decay, beta;
 };
-__device__ __forceinline__ Gates delta_gates(float a, float b, const float* a_log,
-                                             const float* dt_bias, int h) {
-  if (!a_log) return {a, b};
-  const float z = a + (dt_bias ? dt_bias[h] : 0.0f);
-  return {-expf(a_log[h]) * (z > 20.0f ? z : log1pf(expf(z))), 1.0f / (1.0f + expf(-b))};
+__device__ __forceinline__ Gates gates_of(float a_dt, float b, float a_log) {
+  return {-expf(a_log) * (a_dt > 20.0f ? a_dt : log1pf(expf(a_dt))), 1.0f / (1.0f + expf(-b))};
 }
 template <typename T>
 __device__ __forceinline__ Gates load_gates(const dmh_gated_delta& d, int64_t t, int h) {
   if (!d.a_log)
     return {static_cast<const float*>(d.a)[t * d.a_stride + h],
             static_cast<const float*>(d.b)[t * d.b_stride + h]};
-  return delta_gates((float)static_cast<const T*>(d.a)[t * d.a_stride + h],
-                     (float)static_cast<const T*>(d.b)[t * d.b_stride + h], d.a_log, d.dt_bias, h);
+  return gates_of((float)static_cast<const T*>(d.a)[t * d.a_stride + h] +
+                      (d.dt_bias ? d.dt_bias[h] : 0.0f),
+                  (float)static_cast<const T*>(d.b)[t * d.b_stride + h], d.a_log[h]);
 }
 
 }  // namespace dm

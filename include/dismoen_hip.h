@@ -536,7 +536,7 @@ typedef struct {
   const void* v;       /* [total_tokens][v_heads][v_dim] */
   const void* a;       /* [total_tokens][v_heads] */
   const void* b;
-  int64_t q_stride, k_stride, v_stride, a_stride, b_stride;  /* elements between rows */
+  int64_t q_stride, k_stride, v_stride, a_stride, b_stride;  /* elements between rows, < 2^24 */
   const float* a_log;    /* [v_heads], or NULL */
   const float* dt_bias;  /* [v_heads], or NULL: zeros */
   float* state;        /* [num_slots][v_heads][k_dim][v_dim], 16-byte aligned */
