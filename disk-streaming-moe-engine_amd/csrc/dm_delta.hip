@@ -18,7 +18,9 @@
 // their norms and decays as factors of rows in fp32.  Sums of log decays are
 // kept in 64 bits: e^(G_i - G_j) of two large sums would lose what the
 // difference holds.
-#include <cstdlib>
+#include <algorithm>
+#include <type_traits>
+
 #include "dm_mixer_device.h"
 
 namespace dm {
@@ -37,17 +39,23 @@ constexpr size_t frag_bytes(int n) { return (size_t)n * 1024; }  // 64 lanes of 
 
 // What k_delta_prep leaves per chunk: for each value head (I + A)^-1 diag(beta)
 // in three parts, the query-key matrix in NPO, and the rows' factors; for each
-// key head K^T, K and Q (copied: read in place, rows a power of two apart meet in
-// the same channels of the L2, and two thirds of the loads' time goes there).
-// The key dimension comes in steps of a matrix product, in the order in which a
-// wave of k_delta_chunks has it in its part of the state: element e of lane
-// group g is 4 g + e of the step's first 16 and, from e = 4 on, of its second.
-// At 64 dimensions a wave has only 16, and its step is half empty.
+// key head K^T, K and Q (copied: rows a power of two apart meet in the same
+// channels of the L2, and read in place they hold up all the other loads: 2048
+// rows of 32 heads took 62 us instead of 57).
+// The key dimension comes in steps of a matrix product, SW dimensions each, of
+// which lane group g of a factor has SW / 4 in a row.  In the state, whose tiles
+// of 16 rows are a right factor as they stand, row 4 g + i of a step's first tile
+// is the lane group's dimension i, of its second one 4 + i.  At 64 dimensions a
+// wave of the chain has only one tile, and its step is half empty.
 template <int DKT, int NPK, int NPO, bool WIDE>
 struct Layout {
-  static constexpr int SW = DKT == 64 ? 16 : 32;  // dimensions of a step
+  static constexpr int SW = DKT == 64 ? 16 : 32;
   static constexpr int KS = DKT / SW;
   static constexpr int NPQ = NPK < NPO ? NPK : NPO;
+  // the dimension that row m of tile t is
+  static __device__ __forceinline__ int dim(int t, int m) {
+    return SW == 32 ? 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3) : 16 * t + m;
+  }
   static constexpr size_t qk = frag_bytes(kTiles * 3);
   static constexpr size_t rows = qk + frag_bytes(kTiles * NPO);
   static constexpr size_t v_head = rows + 4 * kChunk * sizeof(float);
@@ -137,20 +145,28 @@ __device__ __forceinline__ void store_frag(void* base, size_t frag, int lane, ui
 // The chain of loads, products and substitution bounds it, not bytes, so
 // everything is loaded at once, unconditionally, and T takes A's place in LDS,
 // for three workgroups per CU.
+// The first `short_blocks` workgroups take the short sequences, row by row: they
+// have the longest way, and no chunk waits for them.
 template <typename T, int DKT, int NPK, int NPO, bool WIDE, int HB>
-__global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s, ChunkWork cw) {
+__global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s, ChunkWork cw,
+                                                    unsigned short_blocks) {
+  if (blockIdx.x < short_blocks) {
+    delta_rows<T, DKT / 8>(d, s, cw.min_rows - 1, WIDE, blockIdx.x);
+    return;
+  }
   using L = Layout<DKT, NPK, NPO, WIDE>;
   constexpr int KS = L::KS;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int rep = d.v_heads / d.k_heads, groups = (rep + HB - 1) / HB;
-  const int local = blockIdx.x / (d.k_heads * groups);
-  const int unit = blockIdx.x - local * d.k_heads * groups;
+  const int block = blockIdx.x - short_blocks, local = block / (d.k_heads * groups);
+  const int unit = block - local * d.k_heads * groups;
   const int kh = unit / groups, group = unit - kh * groups;
   const int h0 = kh * rep + group * HB, heads = min(HB, rep - group * HB);
 
   constexpr int kMat = kChunk * kPad;
-  __shared__ __align__(16) uint8_t kfrag[frag_bytes(4 * KS * NPK)];
+  constexpr int kPiece = L::SW / 2;  // bytes of a lane's part of a step: no empty half in LDS
+  __shared__ __align__(16) uint8_t kfrag[4 * KS * NPK * 64 * kPiece];
   __shared__ __align__(16) float am[HB * kMat];  // A, and then T in its place
   __shared__ __align__(16) float2 decay[HB][kChunk];
   __shared__ __align__(16) float beta_s[HB][kChunk], rk_s[kChunk];
@@ -204,19 +220,18 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
     const T* kp = static_cast<const T*>(d.k) + at * d.k_stride + kh * d.k_dim;
     const T* qp = static_cast<const T*>(d.q) + at * d.q_stride + kh * d.k_dim;
 #pragma unroll
-    for (int st = 0; st < KS; ++st)
+    for (int st = 0; st < KS; ++st) {
+      constexpr int N = L::SW / 4;
+      const int c = L::SW * st + N * g < d.k_dim ? L::SW * st + N * g : 0;
+      float kn[N], qn[N];
+      load_f32<N>(kp + c, WIDE, kn);
+      load_f32<N>(qp + c, WIDE, qn);
 #pragma unroll
-      for (int e = 0; e < L::SW / 4; e += 4) {
-        const int c = L::SW * st + 4 * e + 4 * g < d.k_dim ? L::SW * st + 4 * e + 4 * g : 0;
-        float k4[4], q4[4];
-        load_f32<4>(kp + c, WIDE, k4);
-        load_f32<4>(qp + c, WIDE, q4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          kv[st][e + i] = k4[i];
-          qv[st][e + i] = q4[i];
-        }
+      for (int i = 0; i < N; ++i) {
+        kv[st][i] = kn[i];
+        qv[st][i] = qn[i];
       }
+    }
   }
   // gates and decays of head h0 + w, a row per lane; e^-10000 is 0 as well as
   // e^-inf, and does not turn into NaN in a difference
@@ -245,7 +260,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   for (int st = 0; st < KS; ++st) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool in = row_in && i < L::SW / 4 && L::SW * st + 4 * (i & 4) + 4 * g < d.k_dim;
+      const bool in = row_in && i < L::SW / 4 && L::SW * st + L::SW / 4 * g < d.k_dim;
       kv[st][i] = in ? kv[st][i] : 0.0f;
       qv[st][i] = in ? qv[st][i] : 0.0f;
       ksum = __builtin_fmaf(kv[st][i], kv[st][i], ksum);
@@ -256,7 +271,11 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
     split8<NPK>(qv[st], qp4);
 #pragma unroll
     for (int p = 0; p < NPK; ++p) {
-      store_frag(kfrag, (w * KS + st) * NPK + p, lane, kp4[p]);
+      if constexpr (kPiece == 16)
+        store_frag(kfrag, (w * KS + st) * NPK + p, lane, kp4[p]);
+      else
+        *reinterpret_cast<uint2*>(kfrag + (((w * KS + st) * NPK + p) * 64 + lane) * 8) =
+            make_uint2(kp4[p].x, kp4[p].y);
       kf[st][p] = __builtin_bit_cast(bf16x8, kp4[p]);
       qf[st][p] = __builtin_bit_cast(bf16x8, qp4[p]);
       if (group == 0) {
@@ -284,7 +303,15 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
     for (int st = 0; st < KS; ++st) {
       bf16x8 b[NPK];
 #pragma unroll
-      for (int p = 0; p < NPK; ++p) b[p] = load_frag(kfrag, (j * KS + st) * NPK + p, lane);
+      for (int p = 0; p < NPK; ++p) {
+        if constexpr (kPiece == 16) {
+          b[p] = load_frag(kfrag, (j * KS + st) * NPK + p, lane);
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(
+              kfrag + (((j * KS + st) * NPK + p) * 64 + lane) * 8);
+          b[p] = __builtin_bit_cast(bf16x8, make_uint4(v.x, v.y, 0, 0));
+        }
+      }
       kk = mfma_parts<3>(b, kf[st], kk);
       kq = mfma_parts<3>(b, qf[st], kq);
     }
@@ -327,14 +354,13 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   if (group == 0 && w < 2) {  // K^T, by the waves with fewer products
     for (int frag = w; frag < DKT / 16 * 2 * NPK; frag += 2) {
       const int p = frag % NPK, half = frag / NPK & 1, t = frag / (2 * NPK);
-      const int c = 16 * t + n;  // key dimension
+      const int c = L::dim(t, n);
       uint16_t v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int tok = 32 * half + 8 * g + e;
-        const int in = c % L::SW;  // the dimension's place in its step
-        const int from = (((tok >> 4) * KS + c / L::SW) * NPK + p) * 1024 +
-                         ((tok & 15) + 16 * ((in & 15) >> 2)) * 16 + ((in >> 4) * 4 + (in & 3)) * 2;
+        const int from = ((((tok >> 4) * KS + c / L::SW) * NPK + p) * 64 + (tok & 15) +
+                          16 * (c % L::SW / (L::SW / 4))) * kPiece + c % (L::SW / 4) * 2;
         v[e] = *reinterpret_cast<const uint16_t*>(kfrag + from);
       }
       store_frag(kws, frag, lane,
@@ -466,7 +492,8 @@ struct Shared {
   static constexpr size_t u = r + frag_bytes(3 * 2 * NC);      // U
   static constexpr size_t g = u + frag_bytes(NPO * 2 * NC);    // U as S' takes it
   static constexpr size_t v = g + frag_bytes(3 * 2 * NC);      // V: [row][column] fp32
-  static constexpr size_t f = v + (size_t)kChunk * 16 * NC * 4;  // factors of rows, twice
+  static constexpr int vp = 16 * NC + 4;  // a row's pitch: four rows apart, other banks
+  static constexpr size_t f = v + (size_t)kChunk * vp * 4;     // factors of rows, twice
   static constexpr size_t common = f + 2 * 3 * kChunk * 4;
   static constexpr size_t k = common;                          // K, T, K^T as k_delta_prep left them
   static constexpr size_t t = k + frag_bytes(4 * KS * NPK);
@@ -596,7 +623,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
           else e = __builtin_bit_cast(T, (Bits)v1[nc][i]);
           x[i] = in ? (float)e : 0.0f;
         }
-        *reinterpret_cast<f32x4*>(vb + row * 16 * NC + 16 * nc + 4 * g) = x;
+        *reinterpret_cast<f32x4*>(vb + row * M::vp + 16 * nc + 4 * g) = x;
       }
       if (g != 1) fb[((c & 1) * 3 + (g == 0 ? 0 : g - 1)) * kChunk + row] = f;
     };
@@ -681,8 +708,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
   __builtin_amdgcn_s_setprio(3);
   // an element of a C tile: row 4 g + i of 16, column n
   const int col = cb * 16 * NC + n;
-  float* const sp = d.state + (((size_t)r.slot * d.v_heads + h) * d.k_dim + 16 * NT * w + 4 * g) *
-                                  d.v_dim + col;
+  float* const sp = d.state + ((size_t)r.slot * d.v_heads + h) * d.k_dim * d.v_dim + col;
   f32x4 S[NT][NC];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -690,8 +716,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
     for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool in = 16 * (NT * w + t) + 4 * g + i < d.k_dim && col + 16 * nc < d.v_dim;
-        S[t][nc][i] = in && !(c0 == 0 && r.fresh) ? sp[(size_t)(16 * t + i) * d.v_dim + 16 * nc] : 0.0f;
+        const int dim = L::dim(NT * w + t, 4 * g + i);
+        const bool in = dim < d.k_dim && col + 16 * nc < d.v_dim;
+        S[t][nc][i] = in && !(c0 == 0 && r.fresh) ? sp[(size_t)dim * d.v_dim + 16 * nc] : 0.0f;
       }
   // row block t of a right factor to LDS
   const auto put = [&](uint8_t* base, int t, int nc, auto parts, f32x4 x) {
@@ -719,7 +746,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
       tf[0][i] = frag(base, tile_of(w, 0) * 3 * 1024 + i * 1024 + at16);
-      tf[1][i] = frag(base, tile_of(w, two) * 3 * 1024 + i * 1024 + at16);
+      if (two || !M::stage) tf[1][i] = frag(base, tile_of(w, two) * 3 * 1024 + i * 1024 + at16);
     }
   };
   const auto take_kt = [&](const uint8_t* base) {
@@ -739,9 +766,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
     __builtin_amdgcn_s_waitcnt(0x0F70);
   }
   lds_barrier();
+  if constexpr (M::stage) take_k(lds + M::k);
   for (int c = c0; c < c1; ++c) {
     const float* const fc = fb + (c & 1) * 3 * kChunk;
-    if constexpr (M::stage) take_k(lds + M::k);
     f32x4 p[NC][4] = {};
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc)
@@ -770,23 +797,27 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
       for (int blk = 0; blk < 4; ++blk)
         *reinterpret_cast<f32x4*>(pb + ((nc * 4 + blk) * 4 + w) * 1024 + at16) = p[nc][blk];
     lds_barrier();
+    // (all of the step's reads ahead of its arithmetic, T's for the next step last)
     const f32x4 pk = *reinterpret_cast<const f32x4*>(fc + 16 * w + 4 * g);
+    f32x4 q[NC][4], x[NC];
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
-      f32x4 q[4], x;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        q[i] = *reinterpret_cast<const f32x4*>(pb + ((nc * 4 + w) * 4 + i) * 1024 + at16);
+        q[nc][i] = *reinterpret_cast<const f32x4*>(pb + ((nc * 4 + w) * 4 + i) * 1024 + at16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = vb[(16 * w + 4 * g + i) * 16 * NC + 16 * nc + n];
-      q[0] = (q[0] + q[1]) + (q[2] + q[3]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-pk[i], q[0][i], x[i]);
-      put(rb, w, nc, P3{}, x);
+      for (int i = 0; i < 4; ++i) x[nc][i] = vb[(16 * w + 4 * g + i) * M::vp + 16 * nc + n];
     }
-    if constexpr (M::stage) take_t(lds + M::t);
     const f32x4 pr = *reinterpret_cast<const f32x4*>(fc + kChunk + 16 * w + 4 * g);
     const float fade = fc[2 * kChunk + 16 * w];
+    if constexpr (M::stage) take_t(lds + M::t);
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+      q[nc][0] = (q[nc][0] + q[nc][1]) + (q[nc][2] + q[nc][3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[nc][i] = __builtin_fmaf(-pk[i], q[nc][0][i], x[nc][i]);
+      put(rb, w, nc, P3{}, x[nc]);
+    }
     lds_barrier();
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
@@ -814,18 +845,28 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
     }
     lds_barrier();
     if constexpr (M::stage) take_kt(lds + M::kt);
+    bf16x8 ug[NC][2][3];
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        bf16x8 b[3];
-        get(gb, st, nc, b);
+      for (int st = 0; st < 2; ++st) get(gb, st, nc, ug[nc][st]);
+    if constexpr (M::stage) take_k(lds + M::k);  // (the next chunk's)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (st == 0) S[t][nc] *= fade;
-          S[t][nc] = mfma_parts<3>(gf[t][st], b, S[t][nc]);
-        }
-      }
+    for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) S[t][nc] *= fade;
+    // (part by part: all the sums in turn)
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int i = 0; i < NPK; ++i)
+#pragma unroll
+        for (int j = 0; j < 3 - i; ++j)
+#pragma unroll
+          for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              S[t][nc] = mfma16(gf[t][st][i], ug[nc][st][j], S[t][nc]);
     if constexpr (!M::stage) {
       step(c);
       take_k(kws + L::k_rows);
@@ -842,9 +883,11 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (16 * (NT * w + t) + 4 * g + i < d.k_dim && col + 16 * nc < d.v_dim)
-          sp[(size_t)(16 * t + i) * d.v_dim + 16 * nc] = S[t][nc][i];
+      for (int i = 0; i < 4; ++i) {
+        const int dim = L::dim(NT * w + t, 4 * g + i);
+        if (dim < d.k_dim && col + 16 * nc < d.v_dim)
+          sp[(size_t)dim * d.v_dim + 16 * nc] = S[t][nc][i];
+      }
 }
 
 // ---- launches ----------------------------------------------------------------------
@@ -874,21 +917,24 @@ hipError_t run(T, Layout<DKT, NPK, NPO, WIDE>, const dmh_gated_delta& a, const S
   cw.k_heads = cw.v_heads + (size_t)room * a.v_heads * L::v_head;
   cw.min_rows = min_rows;
   const int64_t units = ((int64_t)s.num * a.v_heads + 7) / 8 * 8;
+  const int rep = a.v_heads / a.k_heads;
+  // Two column tiles per workgroup take 1.5 times as long as one (2048 rows of 32
+  // heads: 83 us instead of 57), so they pay where single tiles would come to
+  // more than one workgroup per CU (four long prompts: 420 us instead of 590).
+  const int64_t longs = std::min<int64_t>(s.num, s.rows / min_rows);
+  const bool pairs = longs * a.v_heads * ((a.v_dim + 15) / 16) > 256;
+  const auto chain = pairs ? k_delta_chunks<T, DKT, 2, NPK, NPO, WIDE>
+                           : k_delta_chunks<T, DKT, 1, NPK, NPO, WIDE>;
+  const int64_t ncb = pairs ? (a.v_dim + 31) / 32 : (a.v_dim + 15) / 16;
   for (int64_t at = 0; at < chunks; at += room) {
     cw.rank0 = (int)at;
     cw.count = (int)(chunks - at < room ? chunks - at : room);
-    const int rep = a.v_heads / a.k_heads;
-    if (rep > 1)
-      k_delta_prep<T, DKT, NPK, NPO, WIDE, 2>
-          <<<dim3((unsigned)cw.count * a.k_heads * ((rep + 1) / 2)), 256, 0, st>>>(a, s, cw);
-    else
-      k_delta_prep<T, DKT, NPK, NPO, WIDE, 1>
-          <<<dim3((unsigned)cw.count * a.k_heads), 256, 0, st>>>(a, s, cw);
-    const char* e = getenv("DM_NC");
-    const int nc = e ? atoi(e) : 1;
-    const unsigned ncb = (a.v_dim + 16 * nc - 1) / (16 * nc);
-    if (nc == 1) k_delta_chunks<T, DKT, 1, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 512, 0, st>>>(a, s, cw);
-    if (nc == 2) k_delta_chunks<T, DKT, 2, NPK, NPO, WIDE><<<dim3((unsigned)(units * ncb)), 512, 0, st>>>(a, s, cw);
+    const unsigned blocks = (unsigned)cw.count * a.k_heads * (rep > 1 ? (rep + 1) / 2 : 1);
+    const unsigned rows = at == 0 ? delta_rows_blocks(a, s) : 0;
+    const auto prep = rep > 1 ? k_delta_prep<T, DKT, NPK, NPO, WIDE, 2>
+                              : k_delta_prep<T, DKT, NPK, NPO, WIDE, 1>;
+    prep<<<dim3(rows + blocks), 256, 0, st>>>(a, s, cw, rows);
+    chain<<<dim3((unsigned)(units * ncb)), 512, 0, st>>>(a, s, cw);
   }
   return hipGetLastError();
 }
@@ -907,8 +953,8 @@ size_t delta_chunk_bytes(const dmh_gated_delta& a, bool wide) {
   });
 }
 
-hipError_t launch_delta_chunks(const dmh_gated_delta& a, const SeqDev& s, int min_rows,
-                               int64_t chunks, int64_t room, void* ws, bool wide, hipStream_t st) {
+hipError_t launch_delta(const dmh_gated_delta& a, const SeqDev& s, int min_rows, int64_t chunks,
+                        int64_t room, void* ws, bool wide, hipStream_t st) {
   return with_form(a, wide, [&](auto t, auto l) {
     return run(t, l, a, s, min_rows, chunks, room, ws, st);
   });

@@ -25,7 +25,7 @@ namespace {
 using dm::SeqDev;
 
 // Sequences of up to kRowsMost rows take the delta rule row by row.
-constexpr int kRowsMost = 32;
+constexpr int kRowsMost = 16;
 // Chunks whose factors are in memory at once (40 KB to 130 KB a head).
 constexpr int64_t kChunkRoom = 512;
 
@@ -315,9 +315,8 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
   if (chunks && (rc = dm::api_mixer_buffer(c, dm::kMixerChunks, room * dm::delta_chunk_bytes(a, wide),
                                            &ws, errp, errlen)))
     return rc;
-  hipError_t e = dm::launch_delta_rows(a, s, kRowsMost, wide, st);
-  if (e == hipSuccess && chunks)
-    e = dm::launch_delta_chunks(a, s, kRowsMost + 1, chunks, room, ws, wide, st);
+  const hipError_t e = chunks ? dm::launch_delta(a, s, kRowsMost + 1, chunks, room, ws, wide, st)
+                              : dm::launch_delta_rows(a, s, wide, st);
   if (e != hipSuccess) return err.hip(e);
   return dev ? DMH_OK : stage.out(st, err);
 }

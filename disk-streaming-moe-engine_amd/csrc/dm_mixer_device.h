@@ -116,4 +116,127 @@ __device__ __forceinline__ Gates load_gates(const dmh_gated_delta& d, int64_t t,
                   (float)static_cast<const T*>(d.b)[t * d.b_stride + h], d.a_log[h]);
 }
 
+// ---- the delta rule, row by row -----------------------------------------------------
+// A wave keeps 32 columns of one head's state in registers for the length of a
+// sequence: lane (rg, cg) holds columns 4 cg .. 4 cg + 3 of the RPL rows
+// RPL rg .. RPL rg + RPL - 1.  Columns never meet, so waves share nothing.
+// Both products with the old state, S^T k and S^T q, run in one pass over the
+// registers, and the new state's S'^T q = g S^T q + (k . q) u needs no second
+// one.  A row's three sums of squares and eight column sums are then added over
+// the eight row groups.  One read and one write of the state bound a single row
+// per sequence: 128 bytes per row and wave, whole lines.
+// Sequences of more than max_rows rows are left alone; block: of the workgroups
+// that delta_rows_blocks counts.
+inline unsigned delta_rows_blocks(const dmh_gated_delta& d, const SeqDev& s) {
+  return (unsigned)(((int64_t)s.num * d.v_heads * ((d.v_dim + 31) / 32) + 3) / 4);
+}
+template <typename T, int RPL>
+__device__ __forceinline__ void delta_rows(const dmh_gated_delta& d, const SeqDev& s, int max_rows,
+                                           bool wide, unsigned block) {
+  const int lane = threadIdx.x & 63;
+  const int cg = lane & 7, rg = lane >> 3;
+  const int ncb = (d.v_dim + 31) / 32;
+  const int64_t unit = (int64_t)block * 4 + (threadIdx.x >> 6);
+  const int per_seq = ncb * d.v_heads;
+  const int seq = (int)(unit / per_seq);
+  if (seq >= s.num) return;
+  const int in_seq = (int)(unit - (int64_t)seq * per_seq);
+  const int h = in_seq / ncb, cb = in_seq - h * ncb;
+  const SeqRange r = seq_range(s, seq, in_seq == 0 && lane == 0);
+  if (!r.live) return;
+  if (in_seq == 0 && s.slots) report_shared_slot(s, seq, r.slot, lane);
+  if (r.end - r.begin > max_rows) return;
+
+  const int kh = h / (d.v_heads / d.k_heads);
+  const int row0 = rg * RPL, col0 = cb * 32 + cg * 4;
+  const bool col_in = col0 < d.v_dim;
+  float* sp = d.state + (((size_t)r.slot * d.v_heads + h) * d.k_dim + row0) * d.v_dim + col0;
+  float S[RPL][4];
+#pragma unroll
+  for (int i = 0; i < RPL; ++i) {
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!r.fresh && col_in && row0 + i < d.k_dim)
+      v = *reinterpret_cast<const f32x4*>(sp + (size_t)i * d.v_dim);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) S[i][j] = v[j];
+  }
+  const T* qp = static_cast<const T*>(d.q) + (int64_t)kh * d.k_dim + row0;
+  const T* kp = static_cast<const T*>(d.k) + (int64_t)kh * d.k_dim + row0;
+  const T* vp = static_cast<const T*>(d.v) + (int64_t)h * d.v_dim + col0;
+  T* op = static_cast<T*>(d.o) + (int64_t)h * d.v_dim + col0;
+
+  float qn[RPL], kn[RPL], vn[4];
+  Gates gn;
+  const auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < RPL; i += 8) {
+      float q8[8] = {}, k8[8] = {};
+      if (row0 + i < d.k_dim) {
+        load_f32<8>(qp + t * d.q_stride + i, wide, q8);
+        load_f32<8>(kp + t * d.k_stride + i, wide, k8);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        qn[i + j] = q8[j];
+        kn[i + j] = k8[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vn[j] = 0.0f;
+    if (col_in) load_f32<4>(vp + t * d.v_stride, wide, vn);
+    gn = load_gates<T>(d, t, h);
+  };
+  fetch(r.begin);
+  for (int t = r.begin; t < r.end; ++t) {
+    float q[RPL], k[RPL], v[4];
+#pragma unroll
+    for (int i = 0; i < RPL; ++i) {
+      q[i] = qn[i];
+      k[i] = kn[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = vn[j];
+    const Gates g = gn;
+    if (t + 1 < r.end) fetch(t + 1);
+
+    float sum[11] = {};  // k.S and q.S of the four columns, k.k, q.q, k.q
+#pragma unroll
+    for (int i = 0; i < RPL; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sum[j] = __builtin_fmaf(k[i], S[i][j], sum[j]);
+        sum[4 + j] = __builtin_fmaf(q[i], S[i][j], sum[4 + j]);
+      }
+      sum[8] = __builtin_fmaf(k[i], k[i], sum[8]);
+      sum[9] = __builtin_fmaf(q[i], q[i], sum[9]);
+      sum[10] = __builtin_fmaf(k[i], q[i], sum[10]);
+    }
+#pragma unroll
+    for (int m = 8; m < 64; m *= 2)
+#pragma unroll
+      for (int j = 0; j < 11; ++j) sum[j] += __shfl_xor(sum[j], m);
+    const float rk = d.qk_norm ? 1.0f / sqrtf(sum[8] + d.eps) : 1.0f;
+    const float rq = d.qk_norm ? d.scale / sqrtf(sum[9] + d.eps) : d.scale;
+    const float decay = expf(g.log_decay);
+    float u[4], o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u[j] = g.beta * (v[j] - decay * (rk * sum[j])) * rk;
+      o[j] = rq * (decay * sum[4 + j] + sum[10] * u[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < RPL; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) S[i][j] = __builtin_fmaf(k[i], u[j], decay * S[i][j]);
+    if (rg == 0 && col_in) store_f32<4>(op + t * d.o_stride, wide, o);
+  }
+  if (!col_in) return;
+#pragma unroll
+  for (int i = 0; i < RPL; ++i)
+    if (row0 + i < d.k_dim) {
+      const f32x4 v = {S[i][0], S[i][1], S[i][2], S[i][3]};
+      *reinterpret_cast<f32x4*>(sp + (size_t)i * d.v_dim) = v;
+    }
+}
+
 }  // namespace dm

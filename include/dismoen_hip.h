@@ -518,7 +518,7 @@ int dmh_short_conv_forward(dmh_ctx* ctx, const dmh_short_conv* args, const dmh_s
  * Gates: with a_log set, a and b are raw rows of dtype and
  *   g = -exp(a_log[h]) * softplus(a + dt_bias[h]),  beta = sigmoid(b);
  * without it a is g and b is beta, fp32 rows.
- * Sequences of up to 32 rows take the recurrence row by row; longer ones take it
+ * Sequences of up to 16 rows take the recurrence row by row; longer ones take it
  * 64 rows at a time as matrix products.  Which one a sequence takes goes by its
  * length alone, so its results do not depend on what else is in the call.
  * o must not overlap the inputs.  A row with a value that is not finite leaves
