@@ -26,96 +26,121 @@ from ._lib import (DMH_F_DEVICE, DismoenError, DmhGatedDelta, DmhGatedNorm, DmhS
 
 F32, F16, BF16 = 0, 1, 2
 GATES = {None: 0, "silu": 1, "sigmoid": 2}
-_NP = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint16): BF16}
-_TORCH: dict = {}
+_TYPES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint16): BF16}
 
 
-def _torch_types():
-    import torch
-    _TORCH.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-    return _TORCH
+def _type(a) -> int:
+    t = _TYPES.get(a.dtype)
+    if t is None and not isinstance(a, np.ndarray) and len(_TYPES) == 3:
+        import torch
+        _TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        t = _TYPES.get(a.dtype)
+    if t is None:
+        raise _bad(f"rows are float32, float16 or bfloat16, not {a.dtype}")
+    return t
 
 
 def _bad(text: str) -> DismoenError:
     return DismoenError(1, '{"error_type":"CONFIG_ERROR","detail":"' + text + '","stage":"mixer"}')
 
 
-def _type(a) -> int:
-    t = _NP.get(a.dtype) if isinstance(a, np.ndarray) else (_TORCH or _torch_types()).get(a.dtype)
-    if t is None:
-        raise _bad(f"rows are float32, float16 or bfloat16, not {a.dtype}")
-    return t
+def _strides(a):
+    return tuple(s // a.itemsize for s in a.strides) if isinstance(a, np.ndarray) else a.stride()
 
 
-def _packed(a, dims: int) -> bool:
-    """Whether the last `dims` dimensions lie one behind the other."""
+def _packed(shape, strides) -> bool:
+    """Whether the elements of these dimensions lie one behind the other."""
     want = 1
-    for n, s in zip(reversed(a.shape[-dims:]), reversed(_strides(a)[-dims:])):
+    for n, s in zip(reversed(shape), reversed(strides)):
         if n != 1 and s != want:
             return False
         want *= n
     return True
 
 
-def _strides(a):
-    return tuple(s // a.itemsize for s in a.strides) if isinstance(a, np.ndarray) else a.stride()
-
-
-def _address(a, device: int):
-    """(address, whether it is device memory)."""
-    if isinstance(a, np.ndarray):
-        return a.ctypes.data, False
-    if not a.is_cuda or a.device.index != device:
-        raise _bad(f"tensors must be on the block's device, cuda:{device}")
-    return a.data_ptr(), True
-
-
 class _Operator:
     """A call's argument block, filled field by field; checks that all of its
-    arrays are on one side."""
+    arrays are on one side, the host's (device None) or the block's device."""
 
     def __init__(self, blk):
         self._blk = blk
         self._err = errbuf()
-        self._host = None  # numpy (True), torch (False), not known yet (None)
+        self._sides = set()
         self._kept = []
-
-    def _side(self, a):
-        p, dev = _address(a, self._blk.device)
-        if self._host is None:
-            self._host = not dev
-        elif self._host is dev:
-            raise _bad("numpy arrays and device tensors in one call")
-        return p
 
     def _weight(self, a, shape, what):
         """The address of an fp32 weight that the operator keeps."""
         if a is None:
             return None
-        if tuple(a.shape) != shape or _type(a) != F32 or not _packed(a, len(shape)):
+        if tuple(a.shape) != shape or _type(a) != F32 or not _packed(a.shape, _strides(a)):
             raise _bad(f"{what} must be a contiguous float32 array of shape {list(shape)}")
+        host = isinstance(a, np.ndarray)
+        if not host and a.get_device() != self._blk.device:
+            raise _bad(f"{what} must be on the block's device, cuda:{self._blk.device}")
         self._kept.append(a)
-        return self._side(a)
+        self._sides.add(host)
+        if len(self._sides) > 1:
+            raise _bad("numpy arrays and device tensors in one operator")
+        return a.ctypes.data if host else a.data_ptr()
 
-    def _rows(self, a, shape, dtype, what):
-        """(address, stride between rows) of a row array [rows][...]."""
-        if tuple(a.shape[1:]) != shape or _type(a) != dtype or not _packed(a, len(shape)):
-            raise _bad(f"{what} must be rows of shape {list(shape)}, packed, of the call's type")
-        width = 1
-        for n in shape:
-            width *= n
-        return self._side(a), max(_strides(a)[0], width) if a.shape[0] <= 1 else _strides(a)[0]
-
-    def _state(self, a, shape, dtype, what, batch):
-        if tuple(a.shape) != (batch.num_slots, *shape) or _type(a) != dtype \
-                or not _packed(a, a.ndim):
-            raise _bad(f"{what} must be a contiguous array [num_slots]{list(shape)}")
-        return self._side(a)
-
-    def _flags(self, batch=None):
-        if batch is not None and batch.host is not self._host:
+    def _side(self, a):
+        """Whether the call's arrays are the host's, as `a` and the weights are."""
+        host = isinstance(a, np.ndarray)
+        if self._sides and host not in self._sides:
             raise _bad("numpy arrays and device tensors in one call")
-        return 0 if self._host else DMH_F_DEVICE
+        return host
+
+    # (called for each array of each call: no more Python than it takes)
+    def _rows(self, a, heads, dim, dtype, device, what):
+        """(rows, address, stride) of a row array [rows][heads][dim]."""
+        if device is None:
+            if not isinstance(a, np.ndarray) or a.ndim != 3:
+                raise _bad(f"{what} must be a numpy array as the others, [rows][{heads}][{dim}]")
+            (n, h, d), (s, sh, sd), p = a.shape, _strides(a), a.ctypes.data
+        else:
+            try:
+                n, h, d = a.shape
+                s, sh, sd = a.stride()
+                if a.get_device() != device:
+                    raise ValueError
+            except (ValueError, AttributeError, TypeError):
+                raise _bad(f"{what} must be a tensor on cuda:{device}, [rows][{heads}][{dim}]") \
+                    from None
+            p = a.data_ptr()
+        if h != heads or d != dim or a.dtype != dtype or (sd != 1 and d != 1) \
+                or (sh != d and h != 1):
+            raise _bad(f"{what} must be rows of {heads} times {dim} elements, packed, of the"
+                       " call's type")
+        return n, p, s if n > 1 else max(s, h * d)
+
+    def _rows1(self, a, dim, dtype, device, what):
+        """The same of [rows][dim]."""
+        if device is None:
+            if not isinstance(a, np.ndarray) or a.ndim != 2:
+                raise _bad(f"{what} must be a numpy array as the others, [rows][{dim}]")
+            (n, d), (s, sd), p = a.shape, _strides(a), a.ctypes.data
+        else:
+            try:
+                n, d = a.shape
+                s, sd = a.stride()
+                if a.get_device() != device:
+                    raise ValueError
+            except (ValueError, AttributeError, TypeError):
+                raise _bad(f"{what} must be a tensor on cuda:{device}, [rows][{dim}]") from None
+            p = a.data_ptr()
+        if d != dim or a.dtype != dtype or (sd != 1 and d != 1):
+            raise _bad(f"{what} must be rows of {dim} elements, packed, of the call's type")
+        return n, p, s if n > 1 else max(s, d)
+
+    def _state(self, a, shape, dtype, device, batch):
+        host = isinstance(a, np.ndarray)
+        if host is not (device is None) or a.shape != (batch.num_slots, *shape) \
+                or _type(a) != dtype or not (a.flags.c_contiguous if host else a.is_contiguous()) \
+                or (not host and a.get_device() != device):
+            raise _bad(f"state must be a contiguous array [num_slots]{list(shape)}")
+        if batch.host is not host:
+            raise _bad("numpy arrays and device tensors in one call")
+        return a.ctypes.data if host else a.data_ptr()
 
 
 class SeqBatch:
@@ -138,18 +163,14 @@ class SeqBatch:
             if a is None:
                 ptrs.append(None)
                 continue
-            if a.ndim != 1 or a.shape[0] != want or str(a.dtype).split(".")[-1] != "int32" \
-                    or not _packed(a, 1) or isinstance(a, np.ndarray) is not self.host:
+            if isinstance(a, np.ndarray) is not self.host or a.ndim != 1 or a.shape[0] != want \
+                    or str(a.dtype).split(".")[-1] != "int32" or not _packed(a.shape, _strides(a)):
                 raise _bad(f"{what} must be {want} int32 values on the side of offsets")
             if not self.host and (not a.is_cuda or a.device != offsets.device):
                 raise _bad(f"{what} must be on the device")
             ptrs.append(a.ctypes.data if self.host else a.data_ptr())
         self._c = DmhSeqBatch(n, self.total_tokens, int(max_len), self.num_slots, *ptrs)
         self._ref = C.addressof(self._c)
-
-    def _rows_in(self, a, what):
-        if a.shape[0] < self.total_tokens:
-            raise _bad(f"{what} has fewer rows than total_tokens")
 
 
 class ShortConv(_Operator):
@@ -170,16 +191,16 @@ class ShortConv(_Operator):
     def __call__(self, x, state, batch: SeqBatch, out):
         """out[t] for the rows x [rows][channels]; state [num_slots][width - 1]
         [channels], the last rows of each sequence, is brought up to date."""
-        a, shape = self._c, (self.channels,)
-        a.dtype = t = _type(x)
-        a.x, a.x_stride = self._rows(x, shape, t, "x")
-        a.y, a.y_stride = self._rows(out, shape, t, "out")
-        a.state = self._state(state, (self.width - 1, self.channels), t, "state", batch)
-        batch._rows_in(x, "x")
-        batch._rows_in(out, "out")
-        e = self._err
-        rc = self._blk._lib.dmh_short_conv_forward(self._blk.handle, self._ref, batch._ref,
-                                                   self._flags(batch), e, len(e))
+        c, t, w, e, blk = self._c, x.dtype, self.channels, self._err, self._blk
+        dev = None if self._side(x) else blk.device
+        c.dtype = code = _type(x)
+        nx, c.x, c.x_stride = self._rows1(x, w, t, dev, "x")
+        ny, c.y, c.y_stride = self._rows1(out, w, t, dev, "out")
+        c.state = self._state(state, (self.width - 1, w), code, dev, batch)
+        if min(nx, ny) < batch.total_tokens:
+            raise _bad("x or out has fewer rows than total_tokens")
+        rc = blk._lib.dmh_short_conv_forward(blk.handle, self._ref, batch._ref,
+                                             0 if dev is None else DMH_F_DEVICE, e, 2048)
         if rc:
             check(rc, e)
         return out
@@ -201,7 +222,6 @@ class GatedDelta(_Operator):
         a.a_log = self._weight(a_log, (v_heads,), "a_log")
         a.dt_bias = self._weight(dt_bias, (v_heads,), "dt_bias")
         self._raw = a_log is not None
-        self._k, self._v, self._g = (k_heads, k_dim), (v_heads, v_dim), (v_heads,)
         self._s = (v_heads, k_dim, v_dim)
         self._ref = C.addressof(a)
 
@@ -209,22 +229,25 @@ class GatedDelta(_Operator):
         """out[t] [v_heads][v_dim] for rows q, k [rows][k_heads][k_dim], v
         [rows][v_heads][v_dim] and gates a, b [rows][v_heads]; state [num_slots]
         [v_heads][k_dim][v_dim] fp32 is brought up to date."""
-        c = self._c
-        c.dtype = t = _type(v)
-        g = t if self._raw else F32
-        c.q, c.q_stride = self._rows(q, self._k, t, "q")
-        c.k, c.k_stride = self._rows(k, self._k, t, "k")
-        c.v, c.v_stride = self._rows(v, self._v, t, "v")
-        c.a, c.a_stride = self._rows(a, self._g, g, "a")
-        c.b, c.b_stride = self._rows(b, self._g, g, "b")
-        c.o, c.o_stride = self._rows(out, self._v, t, "out")
-        c.state = self._state(state, self._s, F32, "state", batch)
-        n = batch.total_tokens
-        if min(q.shape[0], k.shape[0], v.shape[0], a.shape[0], b.shape[0], out.shape[0]) < n:
+        c, t, e, blk = self._c, v.dtype, self._err, self._blk
+        dev = None if self._side(v) else blk.device
+        c.dtype = _type(v)
+        g = t if self._raw else a.dtype
+        if not self._raw and _type(a) != F32:
+            raise _bad("without a_log, a and b must be float32")
+        hk, hv, dk, dv = c.k_heads, c.v_heads, c.k_dim, c.v_dim
+        rows = self._rows
+        nq, c.q, c.q_stride = rows(q, hk, dk, t, dev, "q")
+        nk, c.k, c.k_stride = rows(k, hk, dk, t, dev, "k")
+        nv, c.v, c.v_stride = rows(v, hv, dv, t, dev, "v")
+        na, c.a, c.a_stride = self._rows1(a, hv, g, dev, "a")
+        nb, c.b, c.b_stride = self._rows1(b, hv, g, dev, "b")
+        no, c.o, c.o_stride = rows(out, hv, dv, t, dev, "out")
+        c.state = self._state(state, self._s, F32, dev, batch)
+        if min(nq, nk, nv, na, nb, no) < batch.total_tokens:
             raise _bad("a row array has fewer rows than total_tokens")
-        e = self._err
-        rc = self._blk._lib.dmh_gated_delta_forward(self._blk.handle, self._ref, batch._ref,
-                                                    self._flags(batch), e, len(e))
+        rc = blk._lib.dmh_gated_delta_forward(blk.handle, self._ref, batch._ref,
+                                              0 if dev is None else DMH_F_DEVICE, e, 2048)
         if rc:
             check(rc, e)
         return out
@@ -262,26 +285,35 @@ class GatedNorm(_Operator):
         [groups][dim]; stream may be the residual itself."""
         if (gate is None) == self._gate or (y is None) == self._edge:
             raise _bad("gate and y are given exactly where the operator has them")
-        a, shape, n = self._c, self._shape, x.shape[0]
-        a.dtype = t = _type(x)
         out = y if stream is None else stream
         if out is None:
             raise _bad("neither stream nor y is given")
-        a.stream_dtype = st = _type(out)
-        a.rows = n
-        a.x, a.x_stride = self._rows(x, shape, t, "x")
-        a.gate, a.gate_stride = self._rows(gate, shape, t, "gate") if self._gate else (None, 0)
-        a.residual, a.residual_stride = ((None, 0) if residual is None
-                                         else self._rows(residual, shape, st, "residual"))
-        a.stream, a.stream_stride = ((None, 0) if stream is None
-                                     else self._rows(stream, shape, st, "stream"))
-        a.y, a.y_stride = (None, 0) if y is None else self._rows(y, shape, st, "y")
-        for r in (gate, residual, stream, y):
-            if r is not None and r.shape[0] != n:
-                raise _bad("the row arrays differ in their rows")
-        e = self._err
-        rc = self._blk._lib.dmh_gated_norm_forward(self._blk.handle, self._ref, self._flags(), e,
-                                                   len(e))
+        c, t, so, e, blk = self._c, x.dtype, out.dtype, self._err, self._blk
+        dev = None if self._side(x) else blk.device
+        c.dtype, c.stream_dtype = _type(x), _type(out)
+        h, d = self._shape
+        rows = self._rows
+        n, c.x, c.x_stride = rows(x, h, d, t, dev, "x")
+        c.rows = m = n
+        if gate is not None:
+            m, c.gate, c.gate_stride = rows(gate, h, d, t, dev, "gate")
+        if residual is not None:
+            k, c.residual, c.residual_stride = rows(residual, h, d, so, dev, "residual")
+            m = m if k == n else k
+        else:
+            c.residual = None
+        if stream is not None:
+            k, c.stream, c.stream_stride = rows(stream, h, d, so, dev, "stream")
+            m = m if k == n else k
+        else:
+            c.stream = None
+        if y is not None:
+            k, c.y, c.y_stride = rows(y, h, d, so, dev, "y")
+            m = m if k == n else k
+        if m != n:
+            raise _bad("the row arrays differ in their rows")
+        rc = blk._lib.dmh_gated_norm_forward(blk.handle, self._ref, 0 if dev is None else DMH_F_DEVICE,
+                                             e, 2048)
         if rc:
             check(rc, e)
         return stream, y
