@@ -47,7 +47,7 @@ constexpr size_t frag_bytes(int n) { return (size_t)n * 1024; }  // 64 lanes of 
 // of 16 rows are a right factor as they stand, row 4 g + i of a step's first tile
 // is the lane group's dimension i, of its second one 4 + i.  At 64 dimensions a
 // wave of the chain has only one tile, and its step is half empty.
-template <int DKT, int NPK, int NPO, bool WIDE>
+template <int DKT, int NPK, int NPO>
 struct Layout {
   static constexpr int SW = DKT == 64 ? 16 : 32;
   static constexpr int KS = DKT / SW;
@@ -147,14 +147,14 @@ __device__ __forceinline__ void store_frag(void* base, size_t frag, int lane, ui
 // for three workgroups per CU.
 // The first `short_blocks` workgroups take the short sequences, row by row: they
 // have the longest way, and no chunk waits for them.
-template <typename T, int DKT, int NPK, int NPO, bool WIDE, int HB>
+template <typename T, int DKT, int NPK, int NPO, int HB>
 __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s, ChunkWork cw,
                                                     unsigned short_blocks) {
   if (blockIdx.x < short_blocks) {
-    delta_rows<T, DKT / 8>(d, s, cw.min_rows - 1, WIDE, blockIdx.x);
+    delta_rows<T, DKT / 8>(d, s, cw.min_rows - 1, blockIdx.x);
     return;
   }
-  using L = Layout<DKT, NPK, NPO, WIDE>;
+  using L = Layout<DKT, NPK, NPO>;
   constexpr int KS = L::KS;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -167,6 +167,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   constexpr int kMat = kChunk * kPad;
   constexpr int kPiece = L::SW / 2;  // bytes of a lane's part of a step: no empty half in LDS
   __shared__ __align__(16) uint8_t kfrag[4 * KS * NPK * 64 * kPiece];
+  __shared__ __align__(16) uint8_t qfrag[frag_bytes(KS * NPK)];  // the last rows' queries
   __shared__ __align__(16) float am[HB * kMat];  // A, and then T in its place
   __shared__ __align__(16) float2 decay[HB][kChunk];
   __shared__ __align__(16) float beta_s[HB][kChunk], rk_s[kChunk];
@@ -224,8 +225,8 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
       constexpr int N = L::SW / 4;
       const int c = L::SW * st + N * g < d.k_dim ? L::SW * st + N * g : 0;
       float kn[N], qn[N];
-      load_f32<N>(kp + c, WIDE, kn);
-      load_f32<N>(qp + c, WIDE, qn);
+      load_f32<N>(kp + c, kn);
+      load_f32<N>(qp + c, qn);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         kv[st][i] = kn[i];
@@ -271,6 +272,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
     split8<NPK>(qv[st], qp4);
 #pragma unroll
     for (int p = 0; p < NPK; ++p) {
+      if (w == 3) store_frag(qfrag, st * NPK + p, lane, qp4[p]);
       if constexpr (kPiece == 16)
         store_frag(kfrag, (w * KS + st) * NPK + p, lane, kp4[p]);
       else
@@ -296,51 +298,88 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   }
   __syncthreads();
 
-  // A and the query-key matrix
-  for (int j = 0; j <= w; ++j) {
-    f32x4 kk = {}, kq = {};
+  const auto load_key = [&](int rb, int st, int p) -> bf16x8 {
+    const int at = ((rb * KS + st) * NPK + p) * 64 + lane;
+    if constexpr (kPiece == 16) {
+      return load_frag(kfrag, (rb * KS + st) * NPK + p, lane);
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(kfrag + at * 8);
+      return __builtin_bit_cast(bf16x8, make_uint4(v.x, v.y, 0, 0));
+    }
+  };
+  // K^T: the products of the wave's rows with unit vectors give a dimension's
+  // values for four rows in a row, exactly
+  if (group == 0) {
 #pragma unroll
-    for (int st = 0; st < KS; ++st) {
-      bf16x8 b[NPK];
+    for (int t = 0; t < DKT / 16; ++t) {
+      bf16x8 unit;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        unit[e] = (__bf16)(e < L::SW / 4 && L::SW / 4 * g + e == L::dim(t, n) % L::SW ? 1.0f : 0.0f);
 #pragma unroll
       for (int p = 0; p < NPK; ++p) {
-        if constexpr (kPiece == 16) {
-          b[p] = load_frag(kfrag, (j * KS + st) * NPK + p, lane);
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(
-              kfrag + (((j * KS + st) * NPK + p) * 64 + lane) * 8);
-          b[p] = __builtin_bit_cast(bf16x8, make_uint4(v.x, v.y, 0, 0));
+        f32x4 k4 = mfma16(kf[L::SW == 32 ? t >> 1 : t][p], unit, f32x4{});
+        uint2 v[1];
+        split4<1>(k4, v);
+        *reinterpret_cast<uint2*>(kws + ((t * 2 + (w >> 1)) * NPK + p) * 1024 +
+                                  (n + 16 * ((w & 1) * 2 + (g >> 1))) * 16 + (g & 1) * 8) = v[0];
+      }
+    }
+  }
+
+  // A and the query-key matrix: wave 0 takes the first two of the last rows' four
+  // tiles, besides its own one
+  const auto tiles = [&](int rb, int j0, int j1, float rk_row, float rq_row) {
+    const int qrow = 16 * rb + n;
+    const bool here = qrow < rows;
+    for (int j = j0; j <= j1; ++j) {
+      f32x4 kk = {}, kq = {};
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        bf16x8 b[NPK];
+#pragma unroll
+        for (int p = 0; p < NPK; ++p) b[p] = load_key(j, st, p);
+        kk = mfma_parts<3>(b, kf[st], kk);
+        kq = mfma_parts<3>(b, qf[st], kq);
+      }
+      settle(kk);
+      settle(kq);
+      const int c0 = 16 * j + 4 * g;  // the lane's keys c0 .. c0 + 3 of row qrow
+      const f32x4 rkc = *reinterpret_cast<const f32x4*>(rk_s + c0);
+#pragma unroll
+      for (int i = 0; i < HB; ++i) {
+        if (i >= heads) break;
+        const float2 dr = decay[i][qrow];
+        const float bk = beta_s[i][qrow] * rk_row;
+        f32x4 a, q;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float2 dc = decay[i][c0 + r];
+          const float e = __builtin_amdgcn_exp2f((dr.x - dc.x) + (dr.y - dc.y)) * rkc[r];
+          a[r] = c0 + r < qrow && here ? bk * (e * kk[r]) : 0.0f;
+          q[r] = c0 + r <= qrow && here ? rq_row * (e * kq[r]) : 0.0f;
         }
+        *reinterpret_cast<f32x4*>(am + i * kMat + qrow * kPad + c0) = a;
+        uint2 p[NPO];
+        split4<NPO>(q, p);
+        uint8_t* const to = vws + i * L::v_head + L::qk +
+                            (n + 16 * ((j & 1) * 2 + (g >> 1))) * 16 + (g & 1) * 8;
+#pragma unroll
+        for (int o = 0; o < NPO; ++o)
+          *reinterpret_cast<uint2*>(to + (tile_of(rb, j >> 1) * NPO + o) * 1024) = p[o];
       }
-      kk = mfma_parts<3>(b, kf[st], kk);
-      kq = mfma_parts<3>(b, qf[st], kq);
     }
-    settle(kk);
-    settle(kq);
-    const int c0 = 16 * j + 4 * g;  // the lane's keys c0 .. c0 + 3 of row `row`
-    const f32x4 rkc = *reinterpret_cast<const f32x4*>(rk_s + c0);
+  };
+  tiles(w, w == 3 ? 2 : 0, w, rk, rq);
+  if (w == 0) {
 #pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      if (i >= heads) break;
-      const float2 dr = decay[i][row];
-      const float bk = beta_s[i][row] * rk;
-      f32x4 a, q;
+    for (int st = 0; st < KS; ++st)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float2 dc = decay[i][c0 + r];
-        const float e = __builtin_amdgcn_exp2f((dr.x - dc.x) + (dr.y - dc.y)) * rkc[r];
-        a[r] = c0 + r < row && row_in ? bk * (e * kk[r]) : 0.0f;
-        q[r] = c0 + r <= row && row_in ? rq * (e * kq[r]) : 0.0f;
+      for (int p = 0; p < NPK; ++p) {
+        kf[st][p] = load_key(3, st, p);
+        qf[st][p] = load_frag(qfrag, st * NPK + p, lane);
       }
-      *reinterpret_cast<f32x4*>(am + i * kMat + row * kPad + c0) = a;
-      uint2 p[NPO];
-      split4<NPO>(q, p);
-      uint8_t* const to = vws + i * L::v_head + L::qk +
-                          (n + 16 * ((j & 1) * 2 + (g >> 1))) * 16 + (g & 1) * 8;
-#pragma unroll
-      for (int o = 0; o < NPO; ++o)
-        *reinterpret_cast<uint2*>(to + (tile_of(w, j >> 1) * NPO + o) * 1024) = p[o];
-    }
+    tiles(3, 0, 1, rk_s[48 + n], rq_s[48 + n]);
   }
   if ((w & 1) == 0) {  // the empty halves of the tiles on the diagonal
     for (int i = 0; i < heads; ++i) {
@@ -349,23 +388,6 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
 #pragma unroll
       for (int o = 0; o < NPO; ++o)
         *reinterpret_cast<uint2*>(to + (tile_of(w, w >> 1) * NPO + o) * 1024) = make_uint2(0, 0);
-    }
-  }
-  if (group == 0 && w < 2) {  // K^T, by the waves with fewer products
-    for (int frag = w; frag < DKT / 16 * 2 * NPK; frag += 2) {
-      const int p = frag % NPK, half = frag / NPK & 1, t = frag / (2 * NPK);
-      const int c = L::dim(t, n);
-      uint16_t v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int tok = 32 * half + 8 * g + e;
-        const int from = ((((tok >> 4) * KS + c / L::SW) * NPK + p) * 64 + (tok & 15) +
-                          16 * (c % L::SW / (L::SW / 4))) * kPiece + c % (L::SW / 4) * 2;
-        v[e] = *reinterpret_cast<const uint16_t*>(kfrag + from);
-      }
-      store_frag(kws, frag, lane,
-                 make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16,
-                            v[6] | v[7] << 16));
     }
   }
   __syncthreads();
@@ -482,9 +504,9 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
 // T and K^T into registers itself.
 constexpr size_t kLds = 160 * 1024 - 512;
 
-template <int DKT, int NC, int NPK, int NPO, bool WIDE>
+template <int DKT, int NC, int NPK, int NPO>
 struct Shared {
-  using L = Layout<DKT, NPK, NPO, WIDE>;
+  using L = Layout<DKT, NPK, NPO>;
   static constexpr int KS = L::KS;
   static constexpr size_t s = 0;                               // S: [step][column tile][part]
   static constexpr size_t p = s + frag_bytes(KS * NC * NPO);   // P: [column tile][row block][wave]
@@ -503,10 +525,10 @@ struct Shared {
   static constexpr size_t bytes = stage ? all : common;
 };
 
-template <typename T, int DKT, int NC, int NPK, int NPO, bool WIDE>
+template <typename T, int DKT, int NC, int NPK, int NPO>
 __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev s, ChunkWork cw) {
-  using L = Layout<DKT, NPK, NPO, WIDE>;
-  using M = Shared<DKT, NC, NPK, NPO, WIDE>;
+  using L = Layout<DKT, NPK, NPO>;
+  using M = Shared<DKT, NC, NPK, NPO>;
   constexpr int KS = L::KS, KW = KS / 4, NT = DKT / 64, NPQ = L::NPQ;
   constexpr int kKT = DKT / 16 * 2 * NPK;  // fragments of K^T
   const int tid = threadIdx.x, lane = tid & 63;
@@ -580,10 +602,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
     const T* const v0 = static_cast<const T*>(d.v) + (int64_t)r.begin * d.v_stride + h * d.v_dim;
     bf16x8 qf[KS][NPQ], af[2][NPO];
     float f;
-    // V as it comes: a conversion would wait for it
-    using Bits = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
-    Vec<T, 4> v4[NC];
-    uint32_t v1[NC][4];
+    Vec<T, 4> v4[NC];  // (as it comes: a conversion would wait for it)
     const auto load_q = [&] {
 #pragma unroll
       for (int st = 0; st < KS; ++st)
@@ -603,12 +622,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) {
         const T* const at = vp + (col + 16 * nc < d.v_dim ? col + 16 * nc : 0);
-        if constexpr (WIDE) {
-          v4[nc] = *reinterpret_cast<const Vec<T, 4>*>(at);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v1[nc][i] = reinterpret_cast<const Bits*>(at)[i];
-        }
+        v4[nc] = load_raw<4>(at);
       }
     };
     const auto put_v = [&](int c) {
@@ -618,10 +632,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
         f32x4 x;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          T e;
-          if constexpr (WIDE) e = v4[nc].v[i];
-          else e = __builtin_bit_cast(T, (Bits)v1[nc][i]);
-          x[i] = in ? (float)e : 0.0f;
+          x[i] = in ? (float)v4[nc][i] : 0.0f;
         }
         *reinterpret_cast<f32x4*>(vb + row * M::vp + 16 * nc + 4 * g) = x;
       }
@@ -695,7 +706,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
           const float y[4] = {o[nc][0][0], o[nc][0][1], o[nc][0][2], o[nc][0][3]};
-          if (col + 16 * nc < d.v_dim) store_f32<4>(op + 16 * nc, WIDE, y);
+          if (col + 16 * nc < d.v_dim) store_f32<4>(op + 16 * nc, y);
         }
       }
       // T is there: only what was issued behind it, the stores, may be under way
@@ -891,27 +902,25 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
 }
 
 // ---- launches ----------------------------------------------------------------------
-template <typename T, bool WIDE, typename F>
+template <typename T, typename F>
 auto with_dims(const dmh_gated_delta& a, F f) {
   constexpr int NPK = std::is_same_v<T, bf16_t> ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
   constexpr int NPO = std::is_same_v<T, float> ? 3 : 2;
-  if (a.k_dim <= 64) return f(T{}, Layout<64, NPK, NPO, WIDE>{});
-  if (a.k_dim <= 128) return f(T{}, Layout<128, NPK, NPO, WIDE>{});
-  return f(T{}, Layout<256, NPK, NPO, WIDE>{});
+  if (a.k_dim <= 64) return f(T{}, Layout<64, NPK, NPO>{});
+  if (a.k_dim <= 128) return f(T{}, Layout<128, NPK, NPO>{});
+  return f(T{}, Layout<256, NPK, NPO>{});
 }
 template <typename F>
-auto with_form(const dmh_gated_delta& a, bool wide, F f) {
-  if (a.dtype == DMH_DTYPE_BF16)
-    return wide ? with_dims<bf16_t, true>(a, f) : with_dims<bf16_t, false>(a, f);
-  if (a.dtype == DMH_DTYPE_F16)
-    return wide ? with_dims<half_t, true>(a, f) : with_dims<half_t, false>(a, f);
-  return wide ? with_dims<float, true>(a, f) : with_dims<float, false>(a, f);
+auto with_form(const dmh_gated_delta& a, F f) {
+  if (a.dtype == DMH_DTYPE_BF16) return with_dims<bf16_t>(a, f);
+  if (a.dtype == DMH_DTYPE_F16) return with_dims<half_t>(a, f);
+  return with_dims<float>(a, f);
 }
 
-template <typename T, int DKT, int NPK, int NPO, bool WIDE>
-hipError_t run(T, Layout<DKT, NPK, NPO, WIDE>, const dmh_gated_delta& a, const SeqDev& s,
+template <typename T, int DKT, int NPK, int NPO>
+hipError_t run(T, Layout<DKT, NPK, NPO>, const dmh_gated_delta& a, const SeqDev& s,
                int min_rows, int64_t chunks, int64_t room, void* ws, hipStream_t st) {
-  using L = Layout<DKT, NPK, NPO, WIDE>;
+  using L = Layout<DKT, NPK, NPO>;
   ChunkWork cw;
   cw.v_heads = static_cast<uint8_t*>(ws);
   cw.k_heads = cw.v_heads + (size_t)room * a.v_heads * L::v_head;
@@ -923,16 +932,16 @@ hipError_t run(T, Layout<DKT, NPK, NPO, WIDE>, const dmh_gated_delta& a, const S
   // more than one workgroup per CU (four long prompts: 420 us instead of 590).
   const int64_t longs = std::min<int64_t>(s.num, s.rows / min_rows);
   const bool pairs = longs * a.v_heads * ((a.v_dim + 15) / 16) > 256;
-  const auto chain = pairs ? k_delta_chunks<T, DKT, 2, NPK, NPO, WIDE>
-                           : k_delta_chunks<T, DKT, 1, NPK, NPO, WIDE>;
+  const auto chain = pairs ? k_delta_chunks<T, DKT, 2, NPK, NPO>
+                           : k_delta_chunks<T, DKT, 1, NPK, NPO>;
   const int64_t ncb = pairs ? (a.v_dim + 31) / 32 : (a.v_dim + 15) / 16;
   for (int64_t at = 0; at < chunks; at += room) {
     cw.rank0 = (int)at;
     cw.count = (int)(chunks - at < room ? chunks - at : room);
     const unsigned blocks = (unsigned)cw.count * a.k_heads * (rep > 1 ? (rep + 1) / 2 : 1);
     const unsigned rows = at == 0 ? delta_rows_blocks(a, s) : 0;
-    const auto prep = rep > 1 ? k_delta_prep<T, DKT, NPK, NPO, WIDE, 2>
-                              : k_delta_prep<T, DKT, NPK, NPO, WIDE, 1>;
+    const auto prep = rep > 1 ? k_delta_prep<T, DKT, NPK, NPO, 2>
+                              : k_delta_prep<T, DKT, NPK, NPO, 1>;
     prep<<<dim3(rows + blocks), 256, 0, st>>>(a, s, cw, rows);
     chain<<<dim3((unsigned)(units * ncb)), 512, 0, st>>>(a, s, cw);
   }
@@ -946,16 +955,16 @@ int64_t delta_chunk_count(const SeqDev& s, int min_rows) {
   return s.rows / kChunk + (most < s.num ? most : s.num);
 }
 
-size_t delta_chunk_bytes(const dmh_gated_delta& a, bool wide) {
-  return with_form(a, wide, [&](auto, auto l) {
+size_t delta_chunk_bytes(const dmh_gated_delta& a) {
+  return with_form(a, [&](auto, auto l) {
     using L = decltype(l);
     return a.v_heads * L::v_head + a.k_heads * L::k_head;
   });
 }
 
 hipError_t launch_delta(const dmh_gated_delta& a, const SeqDev& s, int min_rows, int64_t chunks,
-                        int64_t room, void* ws, bool wide, hipStream_t st) {
-  return with_form(a, wide, [&](auto t, auto l) {
+                        int64_t room, void* ws, hipStream_t st) {
+  return with_form(a, [&](auto t, auto l) {
     return run(t, l, a, s, min_rows, chunks, room, ws, st);
   });
 }

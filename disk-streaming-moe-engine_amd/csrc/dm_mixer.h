@@ -23,21 +23,19 @@ struct SeqDev {
   unsigned long long* status;
 };
 
-// `wide`: the rows, their strides and the state are aligned for 16-byte
-// accesses.
-hipError_t launch_short_conv(const dmh_short_conv& a, const SeqDev& s, bool wide, hipStream_t st);
-hipError_t launch_gated_norm(const dmh_gated_norm& a, bool wide, hipStream_t st);
+hipError_t launch_short_conv(const dmh_short_conv& a, const SeqDev& s, hipStream_t st);
+hipError_t launch_gated_norm(const dmh_gated_norm& a, hipStream_t st);
 
 // The delta rule row by row.
-hipError_t launch_delta_rows(const dmh_gated_delta& a, const SeqDev& s, bool wide, hipStream_t st);
+hipError_t launch_delta_rows(const dmh_gated_delta& a, const SeqDev& s, hipStream_t st);
 
 // Sequences of min_rows rows and more in chunks of kDeltaChunk, the others row by
 // row.  delta_chunk_count is the most chunks there can be; room of them are worked
 // on at a time, in ws of room times delta_chunk_bytes.
 constexpr int kDeltaChunk = 64;
 int64_t delta_chunk_count(const SeqDev& s, int min_rows);
-size_t delta_chunk_bytes(const dmh_gated_delta& a, bool wide);
+size_t delta_chunk_bytes(const dmh_gated_delta& a);
 hipError_t launch_delta(const dmh_gated_delta& a, const SeqDev& s, int min_rows, int64_t chunks,
-                        int64_t room, void* ws, bool wide, hipStream_t st);
+                        int64_t room, void* ws, hipStream_t st);
 
 }  // namespace dm

@@ -78,8 +78,9 @@ struct Rows {
   int64_t rows, width, stride;
   size_t size;
   size_t bytes() const { return rows ? ((size_t)(rows - 1) * stride + width) * size : 0; }
-  bool ok() const { return stride >= width && stride < ((int64_t)1 << 40); }
-  bool wide() const { return aligned(p, 16) && stride * size % 16 == 0; }
+  bool ok() const {
+    return stride >= width && stride < ((int64_t)1 << 40) && aligned(p, size);
+  }
 };
 
 // Whether two row arrays share an element.  Rows of one pitch whose columns
@@ -217,7 +218,7 @@ int dmh_short_conv_forward(dmh_ctx* c, const dmh_short_conv* args, const dmh_seq
   Rows x{a.x, b.total_tokens, a.channels, a.x_stride, es};
   Rows y{a.y, b.total_tokens, a.channels, a.y_stride, es};
   const Rows state{a.state, b.num_slots, state_row, state_row, es};
-  if (!x.ok() || !y.ok()) return err.arg("x_stride and y_stride must be channels or more");
+  if (!x.ok() || !y.ok() || !state.ok()) return err.arg("a stride is shorter than its row, or an array is misaligned");
   if (overlap(x, y) || overlap(state, x) || overlap(state, y))
     return err.arg("x, y and state must not overlap");
   if (!c) return err.arg("ctx is NULL");
@@ -233,11 +234,8 @@ int dmh_short_conv_forward(dmh_ctx* c, const dmh_short_conv* args, const dmh_seq
     stage.add(a.y, y.bytes(), true);
     stage_batch(stage, b);
     if ((rc = stage.in(c, st, err))) return rc;
-    x.p = a.x;
-    y.p = a.y;
   }
-  const bool wide = x.wide() && y.wide() && aligned(a.state, 16) && a.channels * es % 16 == 0;
-  const hipError_t e = dm::launch_short_conv(a, seq_dev(b, status), wide, st);
+  const hipError_t e = dm::launch_short_conv(a, seq_dev(b, status), st);
   if (e != hipSuccess) return err.hip(e);
   return dev ? DMH_OK : stage.out(st, err);
 }
@@ -280,7 +278,7 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
   const Rows state{a.state, b.num_slots, sw, sw, 4};
   for (const Rows* r : std::initializer_list<const Rows*>{&q, &k, &v, &o, &ga, &gb})
     if (!r->ok() || r->stride >= 1 << 24)
-      return err.arg("a stride is shorter than its row, or 2^24 or more");
+      return err.arg("a stride is shorter than its row, or 2^24 or more, or an array is misaligned");
   for (const Rows* r : std::initializer_list<const Rows*>{&q, &k, &v, &ga, &gb})
     if (overlap(o, *r) || overlap(state, *r))
       return err.arg("o and state must not overlap the inputs");
@@ -302,21 +300,16 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
     stage.add(a.o, o.bytes(), true);
     stage_batch(stage, b);
     if ((rc = stage.in(c, st, err))) return rc;
-    q.p = a.q;
-    k.p = a.k;
-    v.p = a.v;
-    o.p = a.o;
   }
-  const bool wide = q.wide() && k.wide() && v.wide() && o.wide();
   const SeqDev s = seq_dev(b, status);
   const int64_t chunks = b.max_seq_len > kRowsMost ? dm::delta_chunk_count(s, kRowsMost + 1) : 0;
   const int64_t room = std::min(chunks, kChunkRoom);
   void* ws = nullptr;
-  if (chunks && (rc = dm::api_mixer_buffer(c, dm::kMixerChunks, room * dm::delta_chunk_bytes(a, wide),
+  if (chunks && (rc = dm::api_mixer_buffer(c, dm::kMixerChunks, room * dm::delta_chunk_bytes(a),
                                            &ws, errp, errlen)))
     return rc;
-  const hipError_t e = chunks ? dm::launch_delta(a, s, kRowsMost + 1, chunks, room, ws, wide, st)
-                              : dm::launch_delta_rows(a, s, wide, st);
+  const hipError_t e = chunks ? dm::launch_delta(a, s, kRowsMost + 1, chunks, room, ws, st)
+                              : dm::launch_delta_rows(a, s, st);
   if (e != hipSuccess) return err.hip(e);
   return dev ? DMH_OK : stage.out(st, err);
 }
@@ -345,7 +338,7 @@ int dmh_gated_norm_forward(dmh_ctx* c, const dmh_gated_norm* args, unsigned flag
   Rows res{a.residual, a.rows, w, a.residual_stride, ss};
   Rows stream{a.stream, a.rows, w, a.stream_stride, ss}, y{a.y, a.rows, w, a.y_stride, ss};
   for (const Rows* r : {&x, &gate, &res, &stream, &y})
-    if (r->p && !r->ok()) return err.arg("a stride is shorter than its row");
+    if (r->p && !r->ok()) return err.arg("a stride is shorter than its row, or an array is misaligned");
   // (a thread reads the elements that it writes before it writes them)
   const bool on_res = a.stream == a.residual && a.stream_stride == a.residual_stride;
   const bool on_x = a.stream == a.x && a.stream_stride == a.x_stride && es == ss;
@@ -369,16 +362,8 @@ int dmh_gated_norm_forward(dmh_ctx* c, const dmh_gated_norm* args, unsigned flag
     stage.add(a.edge_gamma, 4 * (size_t)a.dim);
     stage.add(a.scale_vec, 4 * (size_t)w);
     if ((rc = stage.in(c, st, err))) return rc;
-    x.p = a.x;
-    gate.p = a.gate;
-    res.p = a.residual;
-    stream.p = a.stream;
-    y.p = a.y;
   }
-  bool wide = a.dim % 8 == 0 && aligned(a.gamma, 16) && aligned(a.edge_gamma, 16) &&
-              aligned(a.scale_vec, 16);
-  for (const Rows* r : {&x, &gate, &res, &stream, &y}) wide = wide && (!r->p || r->wide());
-  const hipError_t e = dm::launch_gated_norm(a, wide, st);
+  const hipError_t e = dm::launch_gated_norm(a, st);
   if (e != hipSuccess) return err.hip(e);
   return dev ? DMH_OK : stage.out(st, err);
 }

@@ -13,34 +13,45 @@ namespace dm {
 typedef _Float16 half_t;
 typedef __bf16 bf16_t;
 
+// N consecutive elements, aligned as one is: global memory takes such an access
+// of up to 16 bytes at any element's address as it does an aligned one, so rows
+// need no alignment or pitch of their own.
 template <typename T, int N>
-struct alignas(sizeof(T) * N >= 16 ? 16 : sizeof(T) * N) Vec {
-  T v[N];
+struct VecOf {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
-
-// N consecutive elements as fp32: one or two 16-byte loads where `wide`, else
-// element by element.
+template <typename T>
+struct VecOf<T, 1> {
+  typedef T type;
+};
+template <typename T, int N>
+using Vec = typename VecOf<T, N>::type;
 template <int N, typename T>
-__device__ __forceinline__ void load_f32(const T* p, bool wide, float (&f)[N]) {
-  if (wide) {
-    const Vec<T, N> r = *reinterpret_cast<const Vec<T, N>*>(p);
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = (float)r.v[i];
+__device__ __forceinline__ Vec<T, N> load_raw(const T* p) {
+  return *reinterpret_cast<const Vec<T, N>*>(p);
+}
+template <int N, typename T>
+__device__ __forceinline__ void to_f32(const T& v, float (&f)[N]) {
+  if constexpr (N == 1) {
+    f[0] = (float)v;
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = (float)p[i];
+    for (int i = 0; i < N; ++i) f[i] = (float)v[i];
   }
 }
 template <int N, typename T>
-__device__ __forceinline__ void store_f32(T* p, bool wide, const float (&f)[N]) {
-  if (wide) {
+__device__ __forceinline__ void load_f32(const T* p, float (&f)[N]) {
+  to_f32<N>(load_raw<N>(p), f);
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_f32(T* p, const float (&f)[N]) {
+  if constexpr (N == 1) {
+    *p = (T)f[0];
+  } else {
     Vec<T, N> r;
 #pragma unroll
-    for (int i = 0; i < N; ++i) r.v[i] = (T)f[i];
+    for (int i = 0; i < N; ++i) r[i] = (T)f[i];
     *reinterpret_cast<Vec<T, N>*>(p) = r;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) p[i] = (T)f[i];
   }
 }
 
@@ -132,7 +143,7 @@ inline unsigned delta_rows_blocks(const dmh_gated_delta& d, const SeqDev& s) {
 }
 template <typename T, int RPL>
 __device__ __forceinline__ void delta_rows(const dmh_gated_delta& d, const SeqDev& s, int max_rows,
-                                           bool wide, unsigned block) {
+                                           unsigned block) {
   const int lane = threadIdx.x & 63;
   const int cg = lane & 7, rg = lane >> 3;
   const int ncb = (d.v_dim + 31) / 32;
@@ -172,8 +183,8 @@ __device__ __forceinline__ void delta_rows(const dmh_gated_delta& d, const SeqDe
     for (int i = 0; i < RPL; i += 8) {
       float q8[8] = {}, k8[8] = {};
       if (row0 + i < d.k_dim) {
-        load_f32<8>(qp + t * d.q_stride + i, wide, q8);
-        load_f32<8>(kp + t * d.k_stride + i, wide, k8);
+        load_f32<8>(qp + t * d.q_stride + i, q8);
+        load_f32<8>(kp + t * d.k_stride + i, k8);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -183,7 +194,7 @@ __device__ __forceinline__ void delta_rows(const dmh_gated_delta& d, const SeqDe
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) vn[j] = 0.0f;
-    if (col_in) load_f32<4>(vp + t * d.v_stride, wide, vn);
+    if (col_in) load_f32<4>(vp + t * d.v_stride, vn);
     gn = load_gates<T>(d, t, h);
   };
   fetch(r.begin);
@@ -228,7 +239,7 @@ __device__ __forceinline__ void delta_rows(const dmh_gated_delta& d, const SeqDe
     for (int i = 0; i < RPL; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) S[i][j] = __builtin_fmaf(k[i], u[j], decay * S[i][j]);
-    if (rg == 0 && col_in) store_f32<4>(op + t * d.o_stride, wide, o);
+    if (rg == 0 && col_in) store_f32<4>(op + t * d.o_stride, o);
   }
   if (!col_in) return;
 #pragma unroll
