@@ -115,11 +115,13 @@ int check_batch(const dmh_seq_batch* b, bool dev, const Err& err) {
   } catch (const std::bad_alloc&) {
     return err(DMH_ERR_NO_MEMORY, "HIP_ERROR", "out of host memory");
   }
+  int64_t most = 0;  // the largest offset so far
   for (int64_t i = 0; i < b->num_seqs; ++i) {
     const int64_t begin = b->offsets[i], end = b->offsets[i + 1];
+    most = std::max(most, begin);
     const int64_t slot = b->slots ? b->slots[i] : i;
     if (slot < 0) continue;
-    if (begin < 0 || end < begin || end > b->total_tokens) return seq_error(err, dm::kSqOffsets, i);
+    if (begin < most || end < begin || end > b->total_tokens) return seq_error(err, dm::kSqOffsets, i);
     if (end - begin > b->max_seq_len) return seq_error(err, dm::kSqLength, i);
     if (slot >= b->num_slots) return seq_error(err, dm::kSqSlot, i);
     if (end == begin) continue;

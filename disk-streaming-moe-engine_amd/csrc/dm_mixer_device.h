@@ -72,7 +72,8 @@ __device__ __forceinline__ SeqRange seq_range(const SeqDev& s, int i, bool repor
   r.live = r.slot >= 0;
   uint32_t kind = kSqCount;
   if (r.live) {
-    if (r.begin < 0 || r.end < r.begin || r.end > s.rows) kind = kSqOffsets;
+    if (r.begin < 0 || r.end < r.begin || r.end > s.rows || (i && s.off[i - 1] > r.begin))
+      kind = kSqOffsets;
     else if (r.end - r.begin > s.max_len) kind = kSqLength;
     else if (r.slot >= s.slots_n) kind = kSqSlot;
   }

@@ -464,8 +464,9 @@ int dmh_moe_forward_gguf(dmh_ctx* ctx, int layer, const float* x, const float* r
  * offsets[i] .. offsets[i + 1] - 1 (none is allowed) of every row array, in
  * order, and its state is state slots[i].  Rows outside every sequence, and
  * states that no sequence names, stay as they are.  A sequence with a negative
- * slot is skipped (the padding of a captured graph's batch); so is one without
- * rows: its state stays, whatever fresh says.
+ * slot is skipped (the padding of a captured graph's batch; offsets behind the
+ * last sequence that is not are not looked at); so is one without rows: its state
+ * stays, whatever fresh says.
  *
  * With DMH_F_DEVICE the arrays are device memory, read when the kernels run, so
  * a captured graph takes each replay's values.  A sequence whose offsets
@@ -473,8 +474,14 @@ int dmh_moe_forward_gguf(dmh_ctx* ctx, int layer, const float* x, const float* r
  * slot is num_slots or more, is left out, and the next dmh_sync reports a
  * SEQUENCE_ERROR; what the sequences behind decreasing offsets give is not valid.
  * It also reports two sequences with rows that name one slot, whose state and
- * rows are then not valid.  With host memory the call itself fails
- * with that error, before anything is written. */
+ * rows are then not valid.  With host memory the call itself fails with that
+ * error, before anything is written.
+ *
+ * The delta rule of sequences of more than 16 rows works in device memory of the
+ * context (some 55 KB per value head and 64 rows at 128 dimensions in bf16, for
+ * 512 times 64 rows at once at most), kept from call to call: make a call of the
+ * same sizes before one is captured.  Replays of graphs that one context captured
+ * must not overlap each other or its other calls. */
 typedef struct {
   int32_t num_seqs;
   int32_t total_tokens;    /* rows that the sequences may use */

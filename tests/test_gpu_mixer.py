@@ -380,6 +380,8 @@ def test_delta_bad_values_stay_in_their_sequence(block):
 @pytest.mark.parametrize("off,slots,text,lost", [
     ([0, 4, 2, 80], [0, 1, 2], "sequence 1: offsets", (1, 2)),  # (2's rows are partly 0's)
     ([-3, 4, 9, 80], [0, 1, 2], "sequence 0: offsets", (0,)),
+    ([0, 9, 4, 50], [0, -1, 2], "sequence 2: offsets", (2,)),  # rows of sequence 0, behind a skipped one
+    ([0, 9, 0, 0], [0, -1, -1], None, ()),  # padding
     ([0, 4, 9, 2000000000], [0, 1, 2], "sequence 2: offsets", (2,)),
     ([0, 4, 9, 90], [0, 1, 2], "sequence 2: longer", (2,)),
     ([0, 4, 9, 80], [0, 6, 2], "sequence 1: slot outside", (1,)),
@@ -571,6 +573,72 @@ def test_mixer_on_another_stream_captured_and_replayed(block):
         assert torch.equal(live[4], wc) and torch.equal(live[5], ws)
         run_delta(block, [x * (i + 1) for x in big], 1, 2, 64, 64, t)
     del graph
+
+
+def test_capture_needs_the_buffers(block):
+    """A captured call that would have to allocate is refused and leaves the
+    capture whole; after an eager call of its sizes it is taken."""
+    from dismoen import MoEBlock
+    g = gen("capture")
+    with MoEBlock(0) as blk:  # without buffers of other calls
+        s = Seqs([70, 30], g, fresh=False)
+        q, k, v, a, b, gates = delta_inputs(g, s.rows, 1, 2, 64, 64, torch.bfloat16)
+        op = GatedDelta(blk, 1, 2, 64, 64, **gates)
+        state, o = rand(g, s.num_slots, 2, 64, 64), torch.zeros_like(v)
+        mark = torch.zeros(1, device="cuda")
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        blk.set_stream(stream.cuda_stream)
+        with torch.cuda.graph(graph, stream=stream):
+            with pytest.raises(DismoenError, match="before the capture"):
+                op(q, k, v, a, b, state, s.batch, o)
+            mark.add_(1)
+        blk.set_stream(None)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert mark.item() == 1 and not o.any()
+        start, eager = state.clone(), torch.zeros_like(v)
+        torch.cuda.synchronize()
+        op(q, k, v, a, b, state, s.batch, eager)
+        blk.sync()
+        want = state.clone()
+        graph2 = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        blk.set_stream(stream.cuda_stream)
+        with torch.cuda.graph(graph2, stream=stream):
+            op(q, k, v, a, b, state, s.batch, o)
+        blk.set_stream(None)
+        for _ in range(3):
+            state.copy_(start)
+            o.zero_()
+            torch.cuda.synchronize()
+            graph2.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, eager) and torch.equal(state, want)
+        blk.sync()
+        del graph, graph2
+
+
+def test_delta_many_chunks(block):
+    """More chunks than are worked on at once: the state passes from one part of
+    the call to the next in memory."""
+    g = gen("parts")
+    lens = [20000, 33, 14000]  # 313 + 1 + 219 chunks of 64
+    s = Seqs(lens, g, fresh=False)
+    q, k, v, a, b, gates = delta_inputs(g, s.rows, 1, 1, 8, 8, torch.float32)
+    state, o = rand(g, s.num_slots, 1, 8, 8), torch.zeros_like(v)
+    old = state.clone()
+    torch.cuda.synchronize()
+    op = GatedDelta(block, 1, 1, 8, 8, **gates)
+    op(q, k, v, a, b, state, s.batch, o)
+    block.sync()
+    want, new, largest = R.delta(q, k, v, a, b, old, *s.args, **gates)
+    # (a row's roundings fade with the state: those of the last 2000 rows are far
+    # more than are left)
+    m = float(largest.max())
+    live = ~want.isnan()
+    R.close(o.cpu()[live], want[live], m * 8 ** -0.5, 64 * 2000)
+    R.close(state, new, m, 64 * 2000)
 
 
 def test_port_block(block, oracle):

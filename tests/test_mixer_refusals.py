@@ -116,6 +116,9 @@ def test_conv_overlap():
     (dict(offsets=(0, 2, 7)), "sequence 1: offsets"),
     (dict(offsets=(-1, 2, 5)), "sequence 0: offsets"),
     (dict(offsets=(3, 2, 5)), "sequence 0: offsets"),
+    (dict(offsets=(0, 4, 2, 5), slots=(0, -1, 1)), "sequence 2: offsets"),  # rows of sequence 0
+    (dict(offsets=(0, 4, 2, 3, 5), slots=(0, -1, -1, 1)), "sequence 3: offsets"),
+    (dict(offsets=(0, 4, 0, 0), slots=(0, -1, -1)), CTX[1]),  # padding
     (dict(offsets=(0, 5, 5)), "sequence 0: longer than max_seq_len"),
     (dict(slots=(0, 3)), "sequence 1: slot outside"),
     (dict(slots=(1, 1)), "sequence 1: names the state"),
