@@ -28,6 +28,8 @@ using dm::SeqDev;
 constexpr int kRowsMost = 16;
 // Chunks whose factors are in memory at once (40 KB to 130 KB a head).
 constexpr int64_t kChunkRoom = 512;
+// Rows of a call, whose numbers the kernels count on from in 32 bits.
+constexpr int32_t kRowsLimit = 1 << 30;
 
 struct Err {
   char* p;
@@ -103,6 +105,7 @@ int check_batch(const dmh_seq_batch* b, bool dev, const Err& err) {
   if (!b) return err.arg("batch is NULL");
   if (b->num_seqs < 0 || b->total_tokens < 0 || b->num_slots < 0)
     return err.arg("num_seqs, total_tokens and num_slots must not be negative");
+  if (b->total_tokens >= kRowsLimit) return err.arg("total_tokens must be below 2^30");
   if (b->num_seqs == 0) return DMH_OK;
   if (b->max_seq_len < 1) return err.arg("max_seq_len must be positive");
   if (!b->offsets) return err.arg("offsets is NULL");
@@ -132,15 +135,23 @@ int check_batch(const dmh_seq_batch* b, bool dev, const Err& err) {
 }
 
 // Host arrays of a call, laid out in one device block: all are copied there,
-// the written ones come back.
+// the written ones come back, without what lies between their rows (another
+// output, where two are slices of one buffer).
 class Stage {
  public:
   template <typename P>
-  void add(P*& p, size_t bytes, bool out = false) {
+  void add(P*& p, size_t bytes) {
     if (!p || !bytes) return;
-    items_[n_++] = {const_cast<void*>(static_cast<const void*>(p)), bytes, total_, out,
+    items_[n_++] = {const_cast<void*>(static_cast<const void*>(p)), bytes, total_, nullptr,
                     [](void* field, void* v) { *static_cast<P**>(field) = static_cast<P*>(v); }, &p};
     total_ += (bytes + 255) & ~(size_t)255;
+  }
+  // (r outlives the stage)
+  template <typename P>
+  void add_out(P*& p, const Rows& r) {
+    const int n = n_;
+    add(p, r.bytes());
+    if (n_ > n) items_[n].out = &r;
   }
   int in(dmh_ctx* c, hipStream_t st, const Err& err) {
     void* base = nullptr;
@@ -159,8 +170,13 @@ class Stage {
   int out(hipStream_t st, const Err& err) {
     for (int i = 0; i < n_; ++i) {
       const Item& it = items_[i];
-      if (!it.is_out) continue;
-      const hipError_t e = hipMemcpyAsync(it.host, it.dev, it.bytes, hipMemcpyDeviceToHost, st);
+      if (!it.out) continue;
+      const Rows& r = *it.out;
+      const hipError_t e =
+          r.stride == r.width || r.rows == 1
+              ? hipMemcpyAsync(it.host, it.dev, it.bytes, hipMemcpyDeviceToHost, st)
+              : hipMemcpy2DAsync(it.host, r.stride * r.size, it.dev, r.stride * r.size,
+                                 r.width * r.size, r.rows, hipMemcpyDeviceToHost, st);
       if (e != hipSuccess) return err.hip(e);
     }
     const hipError_t e = hipStreamSynchronize(st);
@@ -171,7 +187,7 @@ class Stage {
   struct Item {
     void* host;
     size_t bytes, at;
-    bool is_out;
+    const Rows* out;  // the rows to copy back, or NULL
     void (*set)(void*, void*);
     void* field;
     void* dev;
@@ -232,8 +248,8 @@ int dmh_short_conv_forward(dmh_ctx* c, const dmh_short_conv* args, const dmh_seq
     stage.add(a.x, x.bytes());
     stage.add(a.weight, 4 * (size_t)a.channels * a.width);
     stage.add(a.bias, 4 * (size_t)a.channels);
-    stage.add(a.state, state.bytes(), true);
-    stage.add(a.y, y.bytes(), true);
+    stage.add_out(a.state, state);
+    stage.add_out(a.y, y);
     stage_batch(stage, b);
     if ((rc = stage.in(c, st, err))) return rc;
   }
@@ -298,8 +314,8 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
     stage.add(a.b, gb.bytes());
     stage.add(a.a_log, 4 * (size_t)a.v_heads);
     stage.add(a.dt_bias, 4 * (size_t)a.v_heads);
-    stage.add(a.state, state.bytes(), true);
-    stage.add(a.o, o.bytes(), true);
+    stage.add_out(a.state, state);
+    stage.add_out(a.o, o);
     stage_batch(stage, b);
     if ((rc = stage.in(c, st, err))) return rc;
   }
@@ -331,6 +347,7 @@ int dmh_gated_norm_forward(dmh_ctx* c, const dmh_gated_norm* args, unsigned flag
   if (a.gate_act < DMH_GATE_NONE || a.gate_act > DMH_GATE_SIGMOID) return err.arg("unknown gate_act");
   // (rmsnorm's check of its eps)
   if (!(a.eps > 0.0f) || !std::isfinite(a.eps)) return err.arg("eps must be finite and positive");
+  if (a.rows == 0) return c ? DMH_OK : err.arg("ctx is NULL");
   if (!a.x || (a.gate_act && !a.gate)) return err.arg("x or gate is NULL");
   if (!a.stream && !a.y) return err.arg("stream and y are both NULL");
   if (!a.gate_act) a.gate = nullptr;
@@ -348,7 +365,6 @@ int dmh_gated_norm_forward(dmh_ctx* c, const dmh_gated_norm* args, unsigned flag
       overlap(y, x) || overlap(y, gate) || overlap(y, res) || overlap(y, stream))
     return err.arg("stream and y must not overlap each other or the inputs");
   if (!c) return err.arg("ctx is NULL");
-  if (a.rows == 0) return DMH_OK;
   hipStream_t st;
   unsigned long long* status;
   int rc = dm::api_mixer_begin(c, &st, &status, errp, errlen);
@@ -358,8 +374,8 @@ int dmh_gated_norm_forward(dmh_ctx* c, const dmh_gated_norm* args, unsigned flag
     stage.add(a.x, x.bytes());
     stage.add(a.gate, gate.bytes());
     stage.add(a.residual, res.bytes());
-    stage.add(a.stream, stream.bytes(), true);
-    stage.add(a.y, y.bytes(), true);
+    stage.add_out(a.stream, stream);
+    stage.add_out(a.y, y);
     stage.add(a.gamma, 4 * (size_t)a.dim);
     stage.add(a.edge_gamma, 4 * (size_t)a.dim);
     stage.add(a.scale_vec, 4 * (size_t)w);

@@ -31,7 +31,7 @@ __device__ __forceinline__ Vec<T, N> load_raw(const T* p) {
   return *reinterpret_cast<const Vec<T, N>*>(p);
 }
 template <int N, typename T>
-__device__ __forceinline__ void to_f32(const T& v, float (&f)[N]) {
+__device__ __forceinline__ void to_f32(T v, float (&f)[N]) {
   if constexpr (N == 1) {
     f[0] = (float)v;
   } else {

@@ -138,8 +138,8 @@ class _Operator:
                 or _type(a) != dtype or not (a.flags.c_contiguous if host else a.is_contiguous()) \
                 or (not host and a.get_device() != device):
             raise _bad(f"state must be a contiguous array [num_slots]{list(shape)}")
-        if batch.host is not host:
-            raise _bad("numpy arrays and device tensors in one call")
+        if batch.device != device:
+            raise _bad("the batch's arrays are not where the call's are")
         return a.ctypes.data if host else a.data_ptr()
 
 
@@ -155,7 +155,11 @@ class SeqBatch:
                  fresh=None):
         n = offsets.shape[0] - 1
         self.total_tokens, self.num_slots = int(total_tokens), int(num_slots)
+        if not all(0 <= v < 1 << 31 for v in (n, self.total_tokens, self.num_slots, int(max_len))):
+            raise _bad("total_tokens, max_len, num_slots and the number of sequences are int32"
+                       " values from 0 on")
         self.host = isinstance(offsets, np.ndarray)
+        self.device = None if self.host else offsets.get_device()
         self.arrays = (offsets, slots, fresh)
         ptrs = []
         for a, want, what in ((offsets, n + 1, "offsets"), (slots, n, "slots"),
@@ -166,7 +170,7 @@ class SeqBatch:
             if isinstance(a, np.ndarray) is not self.host or a.ndim != 1 or a.shape[0] != want \
                     or str(a.dtype).split(".")[-1] != "int32" or not _packed(a.shape, _strides(a)):
                 raise _bad(f"{what} must be {want} int32 values on the side of offsets")
-            if not self.host and (not a.is_cuda or a.device != offsets.device):
+            if not self.host and (not a.is_cuda or a.get_device() != self.device):
                 raise _bad(f"{what} must be on the device")
             ptrs.append(a.ctypes.data if self.host else a.data_ptr())
         self._c = DmhSeqBatch(n, self.total_tokens, int(max_len), self.num_slots, *ptrs)
@@ -310,8 +314,8 @@ class GatedNorm(_Operator):
         if y is not None:
             k, c.y, c.y_stride = rows(y, h, d, so, dev, "y")
             m = m if k == n else k
-        if m != n:
-            raise _bad("the row arrays differ in their rows")
+        if m != n or n >= 1 << 31:
+            raise _bad("the row arrays differ in their rows, or have 2^31 or more")
         rc = blk._lib.dmh_gated_norm_forward(blk.handle, self._ref, 0 if dev is None else DMH_F_DEVICE,
                                              e, 2048)
         if rc:
@@ -374,6 +378,11 @@ class PortBlock:
         """x, xn, x_mid, y [rows][hidden] fp32 device tensors (xn and x_mid are
         overwritten); mix(xn) -> the mixer's output rows [rows][hidden], in fp32,
         fp16 or bf16."""
+        for a, what in ((x, "x"), (xn, "xn"), (x_mid, "x_mid"), (y, "y")):
+            if isinstance(a, np.ndarray) or _type(a) != F32 or a.shape != (x.shape[0], self._h) \
+                    or not a.is_contiguous() or a.get_device() != self._blk.device:
+                raise _bad(f"{what} must be contiguous float32 rows of {self._h} on"
+                           f" cuda:{self._blk.device}")
         rows = (x.shape[0], 1, self._h)
         self._before(x.view(rows), y=xn.view(rows))
         out = mix(xn)

@@ -484,7 +484,7 @@ int dmh_moe_forward_gguf(dmh_ctx* ctx, int layer, const float* x, const float* r
  * must not overlap each other or its other calls. */
 typedef struct {
   int32_t num_seqs;
-  int32_t total_tokens;    /* rows that the sequences may use */
+  int32_t total_tokens;    /* rows that the sequences may use, < 2^30 */
   int32_t max_seq_len;     /* no sequence is longer (>= 1) */
   int32_t num_slots;       /* states in the state array */
   const int32_t* offsets;  /* [num_seqs + 1] */

@@ -478,6 +478,36 @@ def test_host_arrays_give_the_same_bits(block, t):
     assert np.array_equal(hout, to_np(out)) and np.array_equal(hy, to_np(y))
 
 
+def test_host_outputs_side_by_side(block):
+    """Two outputs that are columns of one host buffer, and rows with something
+    else between them: neither takes back what lies between its rows."""
+    g = gen("side")
+    x, gm = rand(g, 9, 2, 48), rand(g, 48)
+    both = np.full((9, 3, 2, 48), 7.0, np.float32)
+    norm = GatedNorm(block, 48, 2, gamma=to_np(gm), edge=True)
+    norm(to_np(x), both[:, 0], both[:, 2])
+    apart = [np.zeros((9, 2, 48), np.float32) for _ in range(2)]
+    norm(to_np(x), *apart)
+    assert np.array_equal(both[:, 0], apart[0]) and np.array_equal(both[:, 2], apart[1])
+    assert (both[:, 1] == 7.0).all()
+
+
+def test_calls_without_rows(block):
+    """Empty tensors, which have no address."""
+    e = torch.empty(0, 2, 48, device="cuda")
+    GatedNorm(block, 48, 2, edge=True, gate="silu")(e, e, e, gate=e)
+    g = gen("empty")
+    mixer, p, ch = mixer_layer(block, g)
+    t = torch.bfloat16
+    cs, st = rand(g, 3, 3, ch, t=t), rand(g, 3, 4, 64, 64)
+    before = cs.clone(), st.clone()
+    s = SeqBatch(torch.zeros(3, dtype=torch.int32, device="cuda"), 0, 1, 3)
+    r = lambda *d: torch.empty(0, *d, dtype=t, device="cuda")
+    mixer(r(ch), r(4, 64), r(4), r(4), cs, st, s, r(ch), r(4, 64))
+    block.sync()
+    assert torch.equal(cs, before[0]) and torch.equal(st, before[1])
+
+
 def mixer_layer(block, g, hk=2, hv=4, dk=64, dv=64, t=torch.bfloat16):
     ch = 2 * hk * dk + hv * dv
     p = {"conv_weight": rand(g, ch, 4) * 0.5, "a_log": rand(g, hv), "dt_bias": rand(g, hv) - 2,

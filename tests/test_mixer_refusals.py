@@ -287,3 +287,72 @@ def test_operators_refuse_wrong_arrays():
                {"gamma": z(5)}):
         with pytest.raises(DismoenError, match="CONFIG_ERROR"):
             GatedNorm(Blk, 4, 2, **kw)
+
+
+@pytest.mark.parametrize("name,make", [("short_conv", conv), ("gated_delta", delta)])
+def test_rows_of_a_call(name, make):
+    """Row numbers are 32 bits wide, with room for a step past the last one."""
+    assert "below 2^30" in call(name, make(), batch(total=1 << 30))[1]
+    # (addresses that rows of 64 bytes leave apart; not read on the host)
+    far = {f: (2 + i) << 40 for i, f in enumerate(
+        ["x", "y", "state"] if name == "short_conv" else [*"qkvabo", "state"])}
+    assert CTX[1] in call(name, make(**far), batch(total=(1 << 30) - 1), F_DEVICE)[1]
+
+
+def test_no_rows():
+    """A call without rows needs no arrays (an empty tensor has no address)."""
+    a = norm(rows=0, x=None, gate=None, residual=None, stream=None, y=None)
+    assert CTX[1] in call("gated_norm", a)[1]
+    for name, make, fields in (("short_conv", conv, "xy"), ("gated_delta", delta, "qkvabo")):
+        a = make(**{f: None for f in fields})
+        assert CTX[1] in call(name, a, batch((0, 0, 0), total=0))[1]
+
+
+def test_batch_values_and_places():
+    """Python's integers are wider than the call's, and a batch has a device."""
+    from dismoen import DismoenError, SeqBatch, ShortConv
+
+    class Blk:
+        device, handle, _lib = 0, None, lib()
+
+    off = np.array([0, 2, 5], np.int32)
+    for args in ((off, 1 << 32, 4, 3), (off, 5, 1 << 31, 3), (off, 5, 4, (1 << 32) + 3),
+                 (off, -1, 4, 3), (off[:0], 5, 4, 3)):
+        with pytest.raises(DismoenError, match="CONFIG_ERROR"):
+            SeqBatch(*args)
+    b = SeqBatch(off, 5, 4, 3)
+    conv = ShortConv(Blk, np.zeros((8, 4), np.float32))
+    args = [np.zeros((5, 8), np.float32), np.zeros((3, 3, 8), np.float32), b,
+            np.zeros((5, 8), np.float32)]
+    with pytest.raises(DismoenError, match="ctx is NULL"):
+        conv(*args)
+    b.device = 1
+    with pytest.raises(DismoenError, match="batch"):
+        conv(*args)
+
+
+def test_port_block_refuses_wrong_arrays():
+    torch = pytest.importorskip("torch")
+    from dismoen import DismoenError, PortBlock
+
+    class Blk:  # (a CPU tensor's device is -1)
+        device, handle, _lib, dims = -1, None, lib(), {0: (8, 4, 2, 4, 4)}
+
+    port = PortBlock(Blk, 0)
+    ok = [torch.zeros(3, 8) for _ in range(4)]
+
+    def run(i=None, other=None):
+        a = list(ok)
+        if i is not None:
+            a[i] = other
+        port(a[0], lambda v: v, *a[1:])
+
+    with pytest.raises(DismoenError, match="ctx is NULL"):
+        run()
+    for i in range(4):
+        for other in (torch.zeros(3, 8, dtype=torch.float16), torch.zeros(3, 9),
+                      torch.zeros(3, 16)[:, ::2], torch.zeros(24), np.zeros((3, 8), np.float32)):
+            with pytest.raises(DismoenError, match="CONFIG_ERROR.*must be contiguous float32"):
+                run(i, other)
+    with pytest.raises(DismoenError, match="CONFIG_ERROR"):
+        run(3, torch.zeros(2, 8))
