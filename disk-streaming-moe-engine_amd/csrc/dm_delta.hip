@@ -142,9 +142,11 @@ __device__ __forceinline__ void store_frag(void* base, size_t frag, int lane, ui
 // them, 16 and then 32 wide, on the fp32 matrix cores: products of powers of A
 // would take fewer steps and lose all precision for keys that resemble each
 // other.
-// The chain of loads, products and substitution bounds it, not bytes, so
-// everything is loaded at once, unconditionally, and T takes A's place in LDS,
-// for three workgroups per CU.
+// With few chunks the way through loads, products and substitution bounds it, so
+// everything is loaded at once, unconditionally, and T takes A's place in LDS (57
+// KB at 128 dimensions in bf16: two workgroups per CU): 2048 rows of 16 key and 32
+// value heads in 18.5 us.  With many, what it writes does: 465 MB of factors for
+// 16384 rows in 130 us, 4.2 TB/s with what it reads.
 // The first `short_blocks` workgroups take the short sequences, row by row: they
 // have the longest way, and no chunk waits for them.
 template <typename T, int DKT, int NPK, int NPO, int HB>
@@ -172,10 +174,6 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   __shared__ __align__(16) float2 decay[HB][kChunk];
   __shared__ __align__(16) float beta_s[HB][kChunk], rk_s[kChunk];
   __shared__ float rq_s[kChunk];
-
-  // head h0 + w's constants (of waves without a head: another's)
-  const int hw = h0 + min(w, heads - 1);
-  const float a_log = d.a_log ? d.a_log[hw] : 0.0f, dt = d.dt_bias ? d.dt_bias[hw] : 0.0f;
 
   // the chunk: sequence and place in it
   const int rank = cw.rank0 + local;
@@ -206,15 +204,8 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   // there, another's, cleared below
   const int row = 16 * w + n;
   const bool row_in = row < rows;
-  const int64_t gate_at = begin + min(lane, rows - 1);
-  float ga, gb;
-  if (d.a_log) {
-    ga = (float)static_cast<const T*>(d.a)[gate_at * d.a_stride + hw];
-    gb = (float)static_cast<const T*>(d.b)[gate_at * d.b_stride + hw];
-  } else {
-    ga = static_cast<const float*>(d.a)[gate_at * d.a_stride + hw];
-    gb = static_cast<const float*>(d.b)[gate_at * d.b_stride + hw];
-  }
+  // (a wave without a head: another one's gates)
+  const RawGates<T> raw = load_gates<T>(d, begin + min(lane, rows - 1), h0 + min(w, heads - 1));
   float kv[KS][8], qv[KS][8];
   {
     const int64_t at = begin + min(row, rows - 1);
@@ -238,7 +229,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
   // e^-inf, and does not turn into NaN in a difference
   double since = 0.0;
   if (w < heads) {
-    const Gates gt = d.a_log ? gates_of(ga + dt, gb, a_log) : Gates{ga, gb};
+    const Gates gt = gates_of(d, raw);
     since = lane < rows ? (double)gt.log_decay : 0.0;
     if (since < -10000.0) since = -10000.0;
 #pragma unroll
@@ -494,10 +485,13 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
 //   3  U = T R of rows 16 w .. 16 w + 15 (rows of R up to its own),
 //   4  its rows of S' = e^G_last S + K^T U,
 // with a barrier behind 1, 2 and 3.  Waves 4-7 bring the factors of the chain
-// from memory into LDS, without registers where they fit (STAGE), and make the
+// from memory into LDS, without registers where they fit (M::stage), and make the
 // outputs of 16 rows each, O = e^G Q S + (Q K^T) U, from the parts of S and U that
 // the others leave in LDS.  So the chain never waits for memory: with its loads
-// its own, a third of its time went into their issue, 64 bytes a cycle and CU.
+// its own, a third of its time went into their issue, 64 bytes a cycle and CU
+// (75 us instead of 57 for 2048 rows of 32 heads).  What bounds it is the way
+// from barrier to barrier, 1.75 us a chunk with one column tile and 2.6 with two;
+// the matrix cores are busy 17 to 19% of it.
 // A factor is used in one step only, so one copy of each is enough: the next
 // chunk's K arrives from the barrier behind step 1 to the one behind 3, K^T as
 // well, T from there to the next one.  Where they do not fit, the chain loads K,
@@ -928,8 +922,8 @@ hipError_t run(T, Layout<DKT, NPK, NPO>, const dmh_gated_delta& a, const SeqDev&
   const int64_t units = ((int64_t)s.num * a.v_heads + 7) / 8 * 8;
   const int rep = a.v_heads / a.k_heads;
   // Two column tiles per workgroup take 1.5 times as long as one (2048 rows of 32
-  // heads: 83 us instead of 57), so they pay where single tiles would come to
-  // more than one workgroup per CU (four long prompts: 420 us instead of 590).
+  // heads: 82 us instead of 56), so they pay where single tiles would come to
+  // more than one workgroup per CU (four long prompts: 408 us instead of 590).
   const int64_t longs = std::min<int64_t>(s.num, s.rows / min_rows);
   const bool pairs = longs * a.v_heads * ((a.v_dim + 15) / 16) > 256;
   const auto chain = pairs ? k_delta_chunks<T, DKT, 2, NPK, NPO>
