@@ -89,6 +89,17 @@ __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
 // result passes through here: 16 cycles, more than any product used takes.
 __device__ __forceinline__ void settle(f32x4& c) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(c)); }
 
+// Several results with one wait: all of them pass through before it, as they are
+// made, and behind it, before they are used (some 45 cycles for each wait less).
+template <int A, int B>
+__device__ __forceinline__ void settle(f32x4 (&c)[A][B]) {
+#pragma unroll
+  for (int i = 0; i < A * B; ++i) asm volatile("" : "+v"(c[i / B][i % B]));
+  settle(c[0][0]);
+#pragma unroll
+  for (int i = 0; i < A * B; ++i) asm volatile("" : "+v"(c[i / B][i % B]));
+}
+
 // Four fp32 values as NP parts of four bf16.
 template <int NP>
 __device__ __forceinline__ void split4(f32x4 v, uint2 (&p)[NP]) {
@@ -146,7 +157,7 @@ __device__ __forceinline__ void store_frag(void* base, size_t frag, int lane, ui
 // everything is loaded at once, unconditionally, and T takes A's place in LDS (57
 // KB at 128 dimensions in bf16: two workgroups per CU): 2048 rows of 16 key and 32
 // value heads in 18.5 us.  With many, what it writes does: 465 MB of factors for
-// 16384 rows in 130 us, 4.2 TB/s with what it reads.
+// 16384 rows in 124 us, 5 TB/s with what it reads.
 // The first `short_blocks` workgroups take the short sequences, row by row: they
 // have the longest way, and no chunk waits for them.
 template <typename T, int DKT, int NPK, int NPO, int HB>
@@ -490,8 +501,9 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
 // the others leave in LDS.  So the chain never waits for memory: with its loads
 // its own, a third of its time went into their issue, 64 bytes a cycle and CU
 // (75 us instead of 57 for 2048 rows of 32 heads).  What bounds it is the way
-// from barrier to barrier, 1.75 us a chunk with one column tile and 2.6 with two;
-// the matrix cores are busy 17 to 19% of it.
+// from barrier to barrier, 1.7 us a chunk with one column tile and 2.5 with two;
+// the matrix cores are busy 17 to 19% of it.  A wave for all rows of a tile needs no
+// way through LDS, but its 132 products and their splits alone take 2.3 us.
 // A factor is used in one step only, so one copy of each is enough: the next
 // chunk's K arrives from the barrier behind step 1 to the one behind 3, K^T as
 // well, T from there to the next one.  Where they do not fit, the chain loads K,
@@ -671,12 +683,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
           get(sb, st, nc, b);
           o[nc][st & 1] = mfma_parts<NPO>(b, qf[st], o[nc][st & 1]);
         }
+      settle(o);
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc) {
-        settle(o[nc][0]);
-        settle(o[nc][1]);
-        o[nc][0] = (o[nc][0] + o[nc][1]) * pq;
-      }
+      for (int nc = 0; nc < NC; ++nc) o[nc][0] = (o[nc][0] + o[nc][1]) * pq;
       load_q();
       // K and K^T are there: only what was issued behind them, Q, may be under way
       if constexpr (M::stage) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KS * NPQ) : "memory");
@@ -691,8 +700,8 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
           get(ub, 1, nc, b);
           o[nc][0] = mfma_parts<NPO>(b, af[1], o[nc][0]);
         }
-        settle(o[nc][0]);
       }
+      settle(o);
       load_a();
       put_v(c + 1);
       if (c * kChunk + row < len) {
@@ -824,9 +833,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
       put(rb, w, nc, P3{}, x[nc]);
     }
     lds_barrier();
+    f32x4 u[NC][2] = {};
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
-      f32x4 u = {}, u1 = {};
       bf16x8 b[3], b1[3];
       get(rb, 0, nc, b);
       if (two) {
@@ -835,18 +844,19 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
         for (int i = 0; i < 3; ++i)
 #pragma unroll
           for (int j = 0; j < 3 - i; ++j) {
-            u = mfma16(tf[0][i], b[j], u);
-            u1 = mfma16(tf[1][i], b1[j], u1);
+            u[nc][0] = mfma16(tf[0][i], b[j], u[nc][0]);
+            u[nc][1] = mfma16(tf[1][i], b1[j], u[nc][1]);
           }
-        settle(u);
-        settle(u1);
-        u += u1;
       } else {
-        u = mfma_parts<3>(tf[0], b, u);
-        settle(u);
+        u[nc][0] = mfma_parts<3>(tf[0], b, u[nc][0]);
       }
-      put(gb, w, nc, P3{}, u * pr);
-      put(ub, w, nc, PO{}, u);
+    }
+    settle(u);
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+      u[nc][0] += u[nc][1];
+      put(gb, w, nc, P3{}, u[nc][0] * pr);
+      put(ub, w, nc, PO{}, u[nc][0]);
     }
     lds_barrier();
     if constexpr (M::stage) take_kt(lds + M::kt);
@@ -878,10 +888,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
       take_t(vws);
       take_kt(kws);
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int nc = 0; nc < NC; ++nc) settle(S[t][nc]);
+    settle(S);
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -922,8 +929,8 @@ hipError_t run(T, Layout<DKT, NPK, NPO>, const dmh_gated_delta& a, const SeqDev&
   const int64_t units = ((int64_t)s.num * a.v_heads + 7) / 8 * 8;
   const int rep = a.v_heads / a.k_heads;
   // Two column tiles per workgroup take 1.5 times as long as one (2048 rows of 32
-  // heads: 82 us instead of 56), so they pay where single tiles would come to
-  // more than one workgroup per CU (four long prompts: 408 us instead of 590).
+  // heads: 80 us instead of 55), so they pay where single tiles would come to
+  // more than one workgroup per CU (four long prompts: 386 us instead of 580).
   const int64_t longs = std::min<int64_t>(s.num, s.rows / min_rows);
   const bool pairs = longs * a.v_heads * ((a.v_dim + 15) / 16) > 256;
   const auto chain = pairs ? k_delta_chunks<T, DKT, 2, NPK, NPO>
