@@ -147,7 +147,8 @@ __device__ __forceinline__ Gates gates_of(const dmh_gated_delta& d, const RawGat
 // all of them, without a way through LDS.
 __device__ __forceinline__ float sum_eighths(float x) {
   const auto bits = [](float v) { return __builtin_bit_cast(unsigned, v); };
-  x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, (int)bits(x), 0x128, 0xF, 0xF, false));
+  const int eight = __builtin_amdgcn_update_dpp(0, (int)bits(x), 0x128, 0xF, 0xF, false);
+  x += __builtin_bit_cast(float, eight);
   auto p = __builtin_amdgcn_permlane16_swap(bits(x), bits(x), false, false);
   x = __builtin_bit_cast(float, (unsigned)p[0]) + __builtin_bit_cast(float, (unsigned)p[1]);
   p = __builtin_amdgcn_permlane32_swap(bits(x), bits(x), false, false);

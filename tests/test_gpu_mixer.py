@@ -192,6 +192,21 @@ def test_norm_many_rows(block):
     run_norm(block, 70001, 1, 16, torch.bfloat16, torch.bfloat16)
 
 
+@pytest.mark.parametrize("dim", [60, 96, 128, 130, 255, 260, 512])
+def test_norm_of_many_rows_is_that_of_few(block, dim):
+    """Many rows take half the lanes a row: the same sums, and right."""
+    rows = (1 << 21) // dim + 5
+    run_norm(block, rows, 1, dim, torch.bfloat16, torch.float32, residual=False)
+    g = gen("many", dim)
+    x, z, r = (rand(g, rows, 1, dim) for _ in range(3))
+    op = GatedNorm(block, dim, gate="silu", edge=True)
+    torch.cuda.synchronize()
+    many = op(x, torch.empty_like(x), torch.empty_like(x), gate=z, residual=r)
+    few = op(x[:9], torch.empty_like(x[:9]), torch.empty_like(x[:9]), gate=z[:9], residual=r[:9])
+    block.sync()
+    assert torch.equal(many[0][:9], few[0]) and torch.equal(many[1][:9], few[1])
+
+
 def test_norm_in_place_and_special_values(block):
     g = gen("place")
     x, z, r = (rand(g, 6, 1, 64) for _ in range(3))
