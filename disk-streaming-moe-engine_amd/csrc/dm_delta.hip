@@ -11,11 +11,10 @@
 //
 // Precision.  The state is fp32 and so are all sums; products run on the bf16
 // matrix cores with every fp32 factor split into bf16 parts of 8 bits each: x =
-// x0 + x1 + x2 to 2^-26.  What reaches the state keeps the products of parts i
-// and j with i + j < 3 (all 24 bits); what only reaches 16-bit outputs keeps i +
-// j < 2 (2^-17, against their 2^-9 or 2^-12).  Keys and queries enter the
-// products as they came (one part for bf16 rows, two for f16, three for f32),
-// their norms and decays as factors of rows in fp32.  Sums of log decays are
+// x0 + x1 + x2 to 2^-26, and the products of parts i and j with i + j < 3 kept (all
+// 24 bits).  Keys and queries enter the products as they came (one part for bf16
+// rows, two for f16, three for f32), their norms and decays as factors of rows in
+// fp32.  Sums of log decays are
 // kept in 64 bits: e^(G_i - G_j) of two large sums would lose what the
 // difference holds.
 #include <algorithm>
@@ -38,7 +37,7 @@ __device__ __forceinline__ int tile_of(int row_blk, int half) {
 constexpr size_t frag_bytes(int n) { return (size_t)n * 1024; }  // 64 lanes of 16 bytes
 
 // What k_delta_prep leaves per chunk: for each value head (I + A)^-1 diag(beta)
-// in three parts, the query-key matrix in NPO, and the rows' factors; for each
+// and the query-key matrix in three parts each, and the rows' factors; for each
 // key head K^T, K and Q (copied: rows a power of two apart meet in the same
 // channels of the L2, and read in place they hold up all the other loads: 2048
 // rows of 32 heads took 62 us instead of 57).
@@ -47,21 +46,20 @@ constexpr size_t frag_bytes(int n) { return (size_t)n * 1024; }  // 64 lanes of 
 // of 16 rows are a right factor as they stand, row 4 g + i of a step's first tile
 // is the lane group's dimension i, of its second one 4 + i.  At 64 dimensions a
 // wave of the chain has only one tile, and its step is half empty.
-template <int DKT, int NPK, int NPO>
+template <int DKT, int NPK>
 struct Layout {
   static constexpr int SW = DKT == 64 ? 16 : 32;
   static constexpr int KS = DKT / SW;
-  static constexpr int NPQ = NPK < NPO ? NPK : NPO;
   // the dimension that row m of tile t is
   static __device__ __forceinline__ int dim(int t, int m) {
     return SW == 32 ? 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3) : 16 * t + m;
   }
   static constexpr size_t qk = frag_bytes(kTiles * 3);
-  static constexpr size_t rows = qk + frag_bytes(kTiles * NPO);
+  static constexpr size_t rows = qk + frag_bytes(kTiles * 3);
   static constexpr size_t v_head = rows + 4 * kChunk * sizeof(float);
   static constexpr size_t k_rows = frag_bytes(DKT / 16 * 2 * NPK);
   static constexpr size_t q_rows = k_rows + frag_bytes(4 * KS * NPK);
-  static constexpr size_t k_head = q_rows + frag_bytes(4 * KS * NPQ);
+  static constexpr size_t k_head = q_rows + frag_bytes(4 * KS * NPK);
 };
 
 struct ChunkWork {
@@ -124,14 +122,14 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&p)[NP]) {
 }
 
 // c += a b over the parts whose product counts.
-template <int LIM, int NPA, int NPB>
+template <int NPA, int NPB>
 __device__ __forceinline__ f32x4 mfma_parts(const bf16x8 (&a)[NPA], const bf16x8 (&b)[NPB],
                                             f32x4 c) {
 #pragma unroll
   for (int i = 0; i < NPA; ++i)
 #pragma unroll
     for (int j = 0; j < NPB; ++j)
-      if (i + j < LIM) c = mfma16(a[i], b[j], c);
+      if (i + j < 3) c = mfma16(a[i], b[j], c);
   return c;
 }
 
@@ -160,14 +158,14 @@ __device__ __forceinline__ void store_frag(void* base, size_t frag, int lane, ui
 // 16384 rows in 124 us, 5 TB/s with what it reads.
 // The first `short_blocks` workgroups take the short sequences, row by row: they
 // have the longest way, and no chunk waits for them.
-template <typename T, int DKT, int NPK, int NPO, int HB>
+template <typename T, int DKT, int NPK, int HB>
 __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s, ChunkWork cw,
                                                     unsigned short_blocks) {
   if (blockIdx.x < short_blocks) {
     delta_rows<T, DKT / 8>(d, s, cw.min_rows - 1, blockIdx.x);
     return;
   }
-  using L = Layout<DKT, NPK, NPO>;
+  using L = Layout<DKT, NPK>;
   constexpr int KS = L::KS;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -284,7 +282,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
       qf[st][p] = __builtin_bit_cast(bf16x8, qp4[p]);
       if (group == 0) {
         store_frag(kws + L::k_rows, (w * KS + st) * NPK + p, lane, kp4[p]);
-        if (p < L::NPQ) store_frag(kws + L::q_rows, (w * KS + st) * L::NPQ + p, lane, qp4[p]);
+        store_frag(kws + L::q_rows, (w * KS + st) * NPK + p, lane, qp4[p]);
       }
     }
   }
@@ -341,8 +339,8 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
         bf16x8 b[NPK];
 #pragma unroll
         for (int p = 0; p < NPK; ++p) b[p] = load_key(j, st, p);
-        kk = mfma_parts<3>(b, kf[st], kk);
-        kq = mfma_parts<3>(b, qf[st], kq);
+        kk = mfma_parts(b, kf[st], kk);
+        kq = mfma_parts(b, qf[st], kq);
       }
       settle(kk);
       settle(kq);
@@ -362,13 +360,13 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
           q[r] = c0 + r <= qrow && here ? rq_row * (e * kq[r]) : 0.0f;
         }
         *reinterpret_cast<f32x4*>(am + i * kMat + qrow * kPad + c0) = a;
-        uint2 p[NPO];
-        split4<NPO>(q, p);
+        uint2 p[3];
+        split4<3>(q, p);
         uint8_t* const to = vws + i * L::v_head + L::qk +
                             (n + 16 * ((j & 1) * 2 + (g >> 1))) * 16 + (g & 1) * 8;
 #pragma unroll
-        for (int o = 0; o < NPO; ++o)
-          *reinterpret_cast<uint2*>(to + (tile_of(rb, j >> 1) * NPO + o) * 1024) = p[o];
+        for (int o = 0; o < 3; ++o)
+          *reinterpret_cast<uint2*>(to + (tile_of(rb, j >> 1) * 3 + o) * 1024) = p[o];
       }
     }
   };
@@ -388,8 +386,8 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
       *reinterpret_cast<f32x4*>(am + i * kMat + row * kPad + 16 * w + 16 + 4 * g) = f32x4{};
       uint8_t* const to = vws + i * L::v_head + L::qk + (n + 32 + 16 * (g >> 1)) * 16 + (g & 1) * 8;
 #pragma unroll
-      for (int o = 0; o < NPO; ++o)
-        *reinterpret_cast<uint2*>(to + (tile_of(w, w >> 1) * NPO + o) * 1024) = make_uint2(0, 0);
+      for (int o = 0; o < 3; ++o)
+        *reinterpret_cast<uint2*>(to + (tile_of(w, w >> 1) * 3 + o) * 1024) = make_uint2(0, 0);
     }
   }
   __syncthreads();
@@ -510,15 +508,15 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
 // T and K^T into registers itself.
 constexpr size_t kLds = 160 * 1024 - 512;
 
-template <int DKT, int NC, int NPK, int NPO>
+template <int DKT, int NC, int NPK>
 struct Shared {
-  using L = Layout<DKT, NPK, NPO>;
+  using L = Layout<DKT, NPK>;
   static constexpr int KS = L::KS;
   static constexpr size_t s = 0;                               // S: [step][column tile][part]
-  static constexpr size_t p = s + frag_bytes(KS * NC * NPO);   // P: [column tile][row block][wave]
+  static constexpr size_t p = s + frag_bytes(KS * NC * 3);     // P: [column tile][row block][wave]
   static constexpr size_t r = p + frag_bytes(16 * NC);         // R: [half][column tile][part]
   static constexpr size_t u = r + frag_bytes(3 * 2 * NC);      // U
-  static constexpr size_t g = u + frag_bytes(NPO * 2 * NC);    // U as S' takes it
+  static constexpr size_t g = u + frag_bytes(3 * 2 * NC);      // U as S' takes it
   static constexpr size_t v = g + frag_bytes(3 * 2 * NC);      // V: [row][column] fp32
   static constexpr int vp = 16 * NC + 4;  // a row's pitch: four rows apart, other banks
   static constexpr size_t f = v + (size_t)kChunk * vp * 4;     // factors of rows, twice
@@ -531,11 +529,11 @@ struct Shared {
   static constexpr size_t bytes = stage ? all : common;
 };
 
-template <typename T, int DKT, int NC, int NPK, int NPO>
+template <typename T, int DKT, int NC, int NPK>
 __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev s, ChunkWork cw) {
-  using L = Layout<DKT, NPK, NPO>;
-  using M = Shared<DKT, NC, NPK, NPO>;
-  constexpr int KS = L::KS, KW = KS / 4, NT = DKT / 64, NPQ = L::NPQ;
+  using L = Layout<DKT, NPK>;
+  using M = Shared<DKT, NC, NPK>;
+  constexpr int KS = L::KS, KW = KS / 4, NT = DKT / 64;
   constexpr int kKT = DKT / 16 * 2 * NPK;  // fragments of K^T
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3;
@@ -599,27 +597,27 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
   if (wave >= 4) {  // ---- loads, and the outputs of rows 16 w .. 16 w + 15
     // O and V are held transposed: a row (n) and four columns per lane
     const int col = cb * 16 * NC + 4 * g, row = 16 * w + n;
-    const uint32_t q_at = (uint32_t)L::q_rows + w * KS * NPQ * 1024 + at16;
-    const uint32_t a_at[2] = {(uint32_t)L::qk + tile_of(w, 0) * NPO * 1024 + at16,
-                              (uint32_t)L::qk + tile_of(w, two) * NPO * 1024 + at16};
+    const uint32_t q_at = (uint32_t)L::q_rows + w * KS * NPK * 1024 + at16;
+    const uint32_t a_at[2] = {(uint32_t)L::qk + tile_of(w, 0) * 3 * 1024 + at16,
+                              (uint32_t)L::qk + tile_of(w, two) * 3 * 1024 + at16};
     // the rows' factors in one load: of lane group 0 for R, 1 for O, 2 for U, 3 fade
     const uint32_t f_at = (uint32_t)L::rows + (g * kChunk + (g < 3 ? row : 0)) * 4;
     T* const o0 = static_cast<T*>(d.o) + (int64_t)(r.begin + row) * d.o_stride + h * d.v_dim + col;
     const T* const v0 = static_cast<const T*>(d.v) + (int64_t)r.begin * d.v_stride + h * d.v_dim;
-    bf16x8 qf[KS][NPQ], af[2][NPO];
+    bf16x8 qf[KS][NPK], af[2][3];
     float f;
     Vec<T, 4> v4[NC];  // (as it comes: a conversion would wait for it)
     const auto load_q = [&] {
 #pragma unroll
       for (int st = 0; st < KS; ++st)
 #pragma unroll
-        for (int i = 0; i < NPQ; ++i) qf[st][i] = frag(kws, q_at + (st * NPQ + i) * 1024);
+        for (int i = 0; i < NPK; ++i) qf[st][i] = frag(kws, q_at + (st * NPK + i) * 1024);
     };
     const auto load_a = [&] {
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
-        for (int i = 0; i < NPO; ++i) af[st][i] = frag(vws, a_at[st] + i * 1024);
+        for (int i = 0; i < 3; ++i) af[st][i] = frag(vws, a_at[st] + i * 1024);
     };
     const auto load_v = [&](int c) {
       f = *reinterpret_cast<const float*>(vws + f_at);
@@ -679,26 +677,26 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
       for (int st = 0; st < KS; ++st)
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
-          bf16x8 b[NPO];
+          bf16x8 b[3];
           get(sb, st, nc, b);
-          o[nc][st & 1] = mfma_parts<NPO>(b, qf[st], o[nc][st & 1]);
+          o[nc][st & 1] = mfma_parts(b, qf[st], o[nc][st & 1]);
         }
       settle(o);
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) o[nc][0] = (o[nc][0] + o[nc][1]) * pq;
       load_q();
       // K and K^T are there: only what was issued behind them, Q, may be under way
-      if constexpr (M::stage) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KS * NPQ) : "memory");
+      if constexpr (M::stage) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KS * NPK) : "memory");
       lds_barrier();  // 3
       if constexpr (M::stage) bring(vws, M::t, kTiles * 3);
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) {
-        bf16x8 b[NPO];
+        bf16x8 b[3];
         get(ub, 0, nc, b);
-        o[nc][0] = mfma_parts<NPO>(b, af[0], o[nc][0]);
+        o[nc][0] = mfma_parts(b, af[0], o[nc][0]);
         if (two) {
           get(ub, 1, nc, b);
-          o[nc][0] = mfma_parts<NPO>(b, af[1], o[nc][0]);
+          o[nc][0] = mfma_parts(b, af[1], o[nc][0]);
         }
       }
       settle(o);
@@ -735,17 +733,14 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
         S[t][nc][i] = in && !(c0 == 0 && r.fresh) ? sp[(size_t)dim * d.v_dim + 16 * nc] : 0.0f;
       }
   // row block t of a right factor to LDS
-  const auto put = [&](uint8_t* base, int t, int nc, auto parts, f32x4 x) {
-    constexpr int NP = decltype(parts)::value;
-    uint2 p[NP];
-    split4<NP>(x, p);
+  const auto put = [&](uint8_t* base, int t, int nc, f32x4 x) {
+    uint2 p[3];
+    split4<3>(x, p);
     const int at = (n + 16 * ((t & 1) * 2 + (g >> 1))) * 16 + (g & 1) * 8;
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
-      *reinterpret_cast<uint2*>(base + (((t >> 1) * NC + nc) * NP + i) * 1024 + at) = p[i];
+    for (int i = 0; i < 3; ++i)
+      *reinterpret_cast<uint2*>(base + (((t >> 1) * NC + nc) * 3 + i) * 1024 + at) = p[i];
   };
-  using P3 = std::integral_constant<int, 3>;
-  using PO = std::integral_constant<int, NPO>;
 
   // a factor: from LDS where a step begins, or into registers for the next chunk
   bf16x8 kf[4][KW][NPK], tf[2][3], gf[NT][2][NPK];
@@ -795,7 +790,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
           const uint4 q = make_uint4(lo[i].x, lo[i].y, hi[i].x, hi[i].y);
-          if (i < NPO) store_frag(sb, ((w * KW + kw) * NC + nc) * NPO + i, lane, q);
+          store_frag(sb, ((w * KW + kw) * NC + nc) * 3 + i, lane, q);
           b[i] = __builtin_bit_cast(bf16x8, q);
         }
 #pragma unroll
@@ -830,7 +825,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
       q[nc][0] = (q[nc][0] + q[nc][1]) + (q[nc][2] + q[nc][3]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[nc][i] = __builtin_fmaf(-pk[i], q[nc][0][i], x[nc][i]);
-      put(rb, w, nc, P3{}, x[nc]);
+      put(rb, w, nc, x[nc]);
     }
     lds_barrier();
     f32x4 u[NC][2] = {};
@@ -848,15 +843,15 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
             u[nc][1] = mfma16(tf[1][i], b1[j], u[nc][1]);
           }
       } else {
-        u[nc][0] = mfma_parts<3>(tf[0], b, u[nc][0]);
+        u[nc][0] = mfma_parts(tf[0], b, u[nc][0]);
       }
     }
     settle(u);
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
       u[nc][0] += u[nc][1];
-      put(gb, w, nc, P3{}, u[nc][0] * pr);
-      put(ub, w, nc, PO{}, u[nc][0]);
+      put(gb, w, nc, u[nc][0] * pr);
+      put(ub, w, nc, u[nc][0]);
     }
     lds_barrier();
     if constexpr (M::stage) take_kt(lds + M::kt);
@@ -906,10 +901,9 @@ __global__ __launch_bounds__(512) void k_delta_chunks(dmh_gated_delta d, SeqDev 
 template <typename T, typename F>
 auto with_dims(const dmh_gated_delta& a, F f) {
   constexpr int NPK = std::is_same_v<T, bf16_t> ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
-  constexpr int NPO = std::is_same_v<T, float> ? 3 : 2;
-  if (a.k_dim <= 64) return f(T{}, Layout<64, NPK, NPO>{});
-  if (a.k_dim <= 128) return f(T{}, Layout<128, NPK, NPO>{});
-  return f(T{}, Layout<256, NPK, NPO>{});
+  if (a.k_dim <= 64) return f(T{}, Layout<64, NPK>{});
+  if (a.k_dim <= 128) return f(T{}, Layout<128, NPK>{});
+  return f(T{}, Layout<256, NPK>{});
 }
 template <typename F>
 auto with_form(const dmh_gated_delta& a, F f) {
@@ -918,10 +912,10 @@ auto with_form(const dmh_gated_delta& a, F f) {
   return with_dims<float>(a, f);
 }
 
-template <typename T, int DKT, int NPK, int NPO>
-hipError_t run(T, Layout<DKT, NPK, NPO>, const dmh_gated_delta& a, const SeqDev& s,
+template <typename T, int DKT, int NPK>
+hipError_t run(T, Layout<DKT, NPK>, const dmh_gated_delta& a, const SeqDev& s,
                int min_rows, int64_t chunks, int64_t room, void* ws, hipStream_t st) {
-  using L = Layout<DKT, NPK, NPO>;
+  using L = Layout<DKT, NPK>;
   ChunkWork cw;
   cw.v_heads = static_cast<uint8_t*>(ws);
   cw.k_heads = cw.v_heads + (size_t)room * a.v_heads * L::v_head;
@@ -933,16 +927,16 @@ hipError_t run(T, Layout<DKT, NPK, NPO>, const dmh_gated_delta& a, const SeqDev&
   // more than one workgroup per CU (four long prompts: 386 us instead of 580).
   const int64_t longs = std::min<int64_t>(s.num, s.rows / min_rows);
   const bool pairs = longs * a.v_heads * ((a.v_dim + 15) / 16) > 256;
-  const auto chain = pairs ? k_delta_chunks<T, DKT, 2, NPK, NPO>
-                           : k_delta_chunks<T, DKT, 1, NPK, NPO>;
+  const auto chain = pairs ? k_delta_chunks<T, DKT, 2, NPK>
+                           : k_delta_chunks<T, DKT, 1, NPK>;
   const int64_t ncb = pairs ? (a.v_dim + 31) / 32 : (a.v_dim + 15) / 16;
   for (int64_t at = 0; at < chunks; at += room) {
     cw.rank0 = (int)at;
     cw.count = (int)(chunks - at < room ? chunks - at : room);
     const unsigned blocks = (unsigned)cw.count * a.k_heads * (rep > 1 ? (rep + 1) / 2 : 1);
     const unsigned rows = at == 0 ? delta_rows_blocks(a, s) : 0;
-    const auto prep = rep > 1 ? k_delta_prep<T, DKT, NPK, NPO, 2>
-                              : k_delta_prep<T, DKT, NPK, NPO, 1>;
+    const auto prep = rep > 1 ? k_delta_prep<T, DKT, NPK, 2>
+                              : k_delta_prep<T, DKT, NPK, 1>;
     prep<<<dim3(rows + blocks), 256, 0, st>>>(a, s, cw, rows);
     chain<<<dim3((unsigned)(units * ncb)), 512, 0, st>>>(a, s, cw);
   }

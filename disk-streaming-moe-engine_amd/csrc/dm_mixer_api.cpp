@@ -29,7 +29,7 @@ using dm::SeqDev;
 // row, 16 rows 23, 26 and 114, 32 rows 42, 45 and 210; as a chunk all of these
 // 17, 43 and 245 to 271.
 constexpr int kRowsMost = 16;
-// Chunks whose factors are in memory at once (40 KB to 130 KB a head).  Four
+// Chunks whose factors are in memory at once (40 KB to 330 KB a head).  Four
 // sequences of 16384 rows at 32 heads take 3.1 ms with 256, 1.81 ms with 512 and
 // 1.78 ms with 2048; one of 65536 rows 2.8, 2.7 and 2.6 ms.
 constexpr int64_t kChunkRoom = 512;

@@ -478,7 +478,7 @@ int dmh_moe_forward_gguf(dmh_ctx* ctx, int layer, const float* x, const float* r
  * error, before anything is written.
  *
  * The delta rule of sequences of more than 16 rows works in device memory of the
- * context (some 55 KB per value head and 64 rows at 128 dimensions in bf16, for
+ * context (some 61 KB per value head and 64 rows at 128 dimensions in bf16, for
  * 512 times 64 rows at once at most), kept from call to call: make a call of the
  * same sizes before one is captured.  Replays of graphs that one context captured
  * must not overlap each other or its other calls. */
