@@ -61,18 +61,43 @@ struct SeqRange {
   bool fresh, live;  // live: rows to work on and a state to keep
 };
 
-// Sequence i, with everything about it checked that this sequence alone shows.
-// report: record what is wrong with it (one workgroup per sequence does).
+// Whether an offset before sequence i lies behind `begin`, its first row.  What lies
+// before a sequence that is not skipped is that one's to find wrong, so the way back
+// ends there; offsets of skipped ones come eight at a time, as no load then waits for
+// the slot before it.  before, slot: the offset and slot of sequence i - 1.
+__device__ __forceinline__ bool offsets_fall(const SeqDev& s, int i, int begin, int before,
+                                             int slot) {
+  bool fall = before > begin, last = slot >= 0;
+  for (int j = i - 2; j >= 0 && !fall && !last; j -= 8) {
+    int off[8], slots[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      off[u] = s.off[max(j - u, 0)];
+      slots[u] = s.slots[max(j - u, 0)];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      fall = fall || (!last && off[u] > begin);
+      last = last || slots[u] >= 0;
+    }
+  }
+  return fall;
+}
+
+// Sequence i, with everything about it checked that it and the skipped ones before
+// it show.  report: record what is wrong with it (one workgroup per sequence does).
 __device__ __forceinline__ SeqRange seq_range(const SeqDev& s, int i, bool report) {
   SeqRange r;
   r.begin = s.off[i];
   r.end = s.off[i + 1];
   r.slot = s.slots ? s.slots[i] : i;
   r.fresh = s.fresh && s.fresh[i] != 0;
+  const int before = i ? s.off[i - 1] : 0, slot = i && s.slots ? s.slots[i - 1] : 0;
   r.live = r.slot >= 0;
   uint32_t kind = kSqCount;
   if (r.live) {
-    if (r.begin < 0 || r.end < r.begin || r.end > s.rows || (i && s.off[i - 1] > r.begin))
+    if (r.begin < 0 || r.end < r.begin || r.end > s.rows ||
+        offsets_fall(s, i, r.begin, before, slot))
       kind = kSqOffsets;
     else if (r.end - r.begin > s.max_len) kind = kSqLength;
     else if (r.slot >= s.slots_n) kind = kSqSlot;

@@ -470,8 +470,9 @@ int dmh_moe_forward_gguf(dmh_ctx* ctx, int layer, const float* x, const float* r
  *
  * With DMH_F_DEVICE the arrays are device memory, read when the kernels run, so
  * a captured graph takes each replay's values.  A sequence whose offsets
- * decrease or leave [0, total_tokens], that is longer than max_seq_len, or whose
- * slot is num_slots or more, is left out, and the next dmh_sync reports a
+ * decrease, also from those of skipped sequences before it, or leave
+ * [0, total_tokens], that is longer than max_seq_len, or whose slot is
+ * num_slots or more, is left out, and the next dmh_sync reports a
  * SEQUENCE_ERROR; what the sequences behind decreasing offsets give is not valid.
  * It also reports two sequences with rows that name one slot, whose state and
  * rows are then not valid.  With host memory the call itself fails with that
