@@ -377,16 +377,39 @@ class PortBlock:
     def __call__(self, x, mix, xn, x_mid, y):
         """x, xn, x_mid, y [rows][hidden] fp32 device tensors (xn and x_mid are
         overwritten); mix(xn) -> the mixer's output rows [rows][hidden], in fp32,
-        fp16 or bf16."""
+        fp16 or bf16.  The call takes its place in torch's current stream, as mix
+        does: where the block's is another one, each waits for the other."""
         for a, what in ((x, "x"), (xn, "xn"), (x_mid, "x_mid"), (y, "y")):
             if isinstance(a, np.ndarray) or _type(a) != F32 or a.shape != (x.shape[0], self._h) \
                     or not a.is_contiguous() or a.get_device() != self._blk.device:
                 raise _bad(f"{what} must be contiguous float32 rows of {self._h} on"
                            f" cuda:{self._blk.device}")
         rows = (x.shape[0], 1, self._h)
-        self._before(x.view(rows), y=xn.view(rows))
-        out = mix(xn)
-        self._after(out.reshape(rows), x_mid.view(rows), xn.view(rows), residual=x.view(rows))
-        self._blk.forward_device(self._layer, xn.data_ptr(), x.shape[0], y.data_ptr(),
-                                 residual_ptr=x_mid.data_ptr())
+        ours = theirs = None
+        if x.is_cuda:
+            import torch
+            theirs = torch.cuda.current_stream(x.device)
+            ours = torch.cuda.ExternalStream(self._blk.stream(), device=x.device)
+            if ours.cuda_stream == theirs.cuda_stream:
+                ours = None
+        if ours is not None:
+            ours.wait_stream(theirs)
+        try:
+            self._before(x.view(rows), y=xn.view(rows))
+            if ours is not None:
+                theirs.wait_stream(ours)
+            try:
+                # (a copy where the rows are no view, on the stream that made them)
+                out = mix(xn).reshape(rows)
+            finally:
+                if ours is not None:
+                    ours.wait_stream(theirs)
+            self._after(out, x_mid.view(rows), xn.view(rows), residual=x.view(rows))
+            self._blk.forward_device(self._layer, xn.data_ptr(), x.shape[0], y.data_ptr(),
+                                     residual_ptr=x_mid.data_ptr())
+        finally:
+            # (so what `out` was is free only when the block has read it: a tensor must
+            # not be recorded on a block's own stream, which may end before the tensor)
+            if ours is not None:
+                theirs.wait_stream(ours)
         return y

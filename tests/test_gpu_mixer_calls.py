@@ -58,3 +58,106 @@ def test_offsets_that_fall_between_skipped_sequences(block, op, off, slots, lost
     assert (state.cpu().double() - new).abs().max() < 1e-4
     for i in set(range(n)) - set(keep):
         assert torch.equal(state[i], old[i])
+
+
+def port_block(blk, rows=9):
+    from dismoen import PortBlock, synth
+    layer = synth.make_layer(**synth.CONFIG_TOY, seed=3)
+    blk.upload_layer(0, layer)
+    g = torch.Generator().manual_seed(rows)
+    h = layer.hidden
+    x, w = rand(g, rows, h), rand(g, h, 2 * h) * h ** -0.5
+    port = PortBlock(blk, 0, 1 + 0.1 * rand(g, h), 1 + 0.1 * rand(g, h))
+    arrays = [torch.zeros_like(x) for _ in range(3)]
+
+    def mix(v):
+        return (v @ w)[:, ::2].bfloat16().contiguous()
+
+    def want():  # everything in order by waiting for the device
+        def waited(v):
+            torch.cuda.synchronize()
+            out = mix(v)
+            torch.cuda.synchronize()
+            return out
+
+        torch.cuda.synchronize()
+        port(x, waited, *arrays)
+        torch.cuda.synchronize()
+        return [a.clone() for a in arrays]
+
+    return port, x, mix, arrays, want
+
+
+@pytest.mark.parametrize("view", [True, False])
+def test_port_block_and_torch_streams(view):
+    """On the block's own stream, with both streams busy: x, the mixer and y are in the
+    order of torch's current stream, and what the mixer returned is not reused before
+    the block has read it."""
+    from dismoen import MoEBlock
+    with MoEBlock(0) as blk:
+        port, x, mix, arrays, want = port_block(blk)
+        right = want()
+        busy = torch.randn(2048, 2048, device="cuda")
+        ours = torch.cuda.ExternalStream(blk.stream())
+        source = x.clone()
+
+        def work():
+            for _ in range(20):
+                torch.mm(busy, busy)
+
+        def slow(v):
+            out = mix(v)
+            work()
+            # (rows in another order of memory: the block takes a copy of them)
+            return out.clone() if view else out.unflatten(0, (3, 3)).permute(1, 0, 2) \
+                .contiguous().permute(1, 0, 2)
+
+        for other in (False, True):
+            stream = torch.cuda.Stream() if other else torch.cuda.current_stream()
+            for a in (x, *arrays):
+                a.zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(ours):
+                work()
+            with torch.cuda.stream(stream):
+                work()
+                x.copy_(source)
+                y = port(x, slow, *arrays)
+                junk = [torch.full((9, x.shape[1]), float("nan"), dtype=torch.bfloat16,
+                                   device="cuda") for _ in range(8)]
+                got = [a.clone() for a in arrays]
+            torch.cuda.synchronize()
+            blk.sync()
+            assert y is arrays[2] and junk[0].isnan().all()
+            for a, b in zip(got, right):
+                assert torch.equal(a, b)
+
+
+def test_port_block_captured():
+    """A capture of torch's stream takes in the block's own one."""
+    from dismoen import MoEBlock
+    with MoEBlock(0) as blk:
+        port, x, mix, arrays, want = port_block(blk)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        values = [x.clone(), x * 0.5 + 1, x.flip(0)]
+        right = []
+        for v in values:
+            x.copy_(v)
+            right.append(want())
+        with torch.cuda.stream(stream):  # (buffers of its sizes, libraries' handles)
+            port(x, mix, *arrays)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            port(x, mix, *arrays)
+        for _ in range(2):
+            for v, r in zip(values, right):
+                x.copy_(v)
+                for a in arrays:
+                    a.zero_()
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+                for a, b in zip(arrays, r):
+                    assert torch.equal(a, b)
+                blk.sync()
+        del graph
