@@ -370,9 +370,16 @@ class PortBlock:
 
     def __init__(self, blk, layer_idx: int, input_gamma=None, post_gamma=None, eps: float = 1e-6):
         self._blk, self._layer = blk, layer_idx
-        self._h = h = blk.dims[layer_idx][0]
+        self._h = h = self._hidden()
         self._before = GatedNorm(blk, h, post=False, edge=True, edge_gamma=input_gamma, eps=eps)
         self._after = GatedNorm(blk, h, post=False, edge=True, edge_gamma=post_gamma, eps=eps)
+
+    def _hidden(self) -> int:
+        """The width of the layer as it is now uploaded."""
+        dims = self._blk.dims.get(self._layer)
+        if dims is None:
+            raise _bad(f"layer {self._layer} is not an uploaded 4-bit layer")
+        return dims[0]
 
     def __call__(self, x, mix, xn, x_mid, y):
         """x, xn, x_mid, y [rows][hidden] fp32 device tensors (xn and x_mid are
@@ -384,6 +391,8 @@ class PortBlock:
                     or not a.is_contiguous() or a.get_device() != self._blk.device:
                 raise _bad(f"{what} must be contiguous float32 rows of {self._h} on"
                            f" cuda:{self._blk.device}")
+        if self._hidden() != self._h:
+            raise _bad(f"layer {self._layer} was replaced by one of {self._hidden()} elements a row")
         rows = (x.shape[0], 1, self._h)
         ours = theirs = None
         if x.is_cuda:
