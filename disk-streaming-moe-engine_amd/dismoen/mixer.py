@@ -18,6 +18,7 @@ theirs (MoEBlock.set_stream).
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import numpy as np
 
@@ -381,6 +382,13 @@ class PortBlock:
             raise _bad(f"layer {self._layer} is not an uploaded 4-bit layer")
         return dims[0]
 
+    def _mixed(self, out, rows):
+        """The mixer's output in the block's shape."""
+        shape = getattr(out, "shape", ())
+        if not shape or shape[-1] != self._h or math.prod(shape) != math.prod(rows):
+            raise _bad(f"mix must return {rows[0]} rows of {self._h}")
+        return out.reshape(rows)
+
     def __call__(self, x, mix, xn, x_mid, y):
         """x, xn, x_mid, y [rows][hidden] fp32 device tensors (xn and x_mid are
         overwritten); mix(xn) -> the mixer's output rows [rows][hidden], in fp32,
@@ -409,7 +417,7 @@ class PortBlock:
                 theirs.wait_stream(ours)
             try:
                 # (a copy where the rows are no view, on the stream that made them)
-                out = mix(xn).reshape(rows)
+                out = self._mixed(mix(xn), rows)
             finally:
                 if ours is not None:
                     ours.wait_stream(theirs)

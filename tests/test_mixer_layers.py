@@ -32,3 +32,14 @@ def test_port_block_needs_a_4_bit_layer():
     del blk.dims[0]
     with pytest.raises(DismoenError, match="CONFIG_ERROR.*not an uploaded"):
         run()
+
+
+def test_port_block_refuses_other_rows_of_the_mixer():
+    torch = pytest.importorskip("torch")
+    port = PortBlock(port_blk(dims={0: (8, 4, 2, 4, 4)}), 0)
+    rows = (6, 1, 8)
+    for shape in ((6, 8), (6, 1, 8), (2, 3, 8), (1, 6, 8)):
+        assert port._mixed(torch.zeros(shape), rows).shape == rows
+    for out in (None, 1.0, torch.zeros(5, 8), torch.zeros(8, 6), torch.zeros(48), torch.zeros(())):
+        with pytest.raises(DismoenError, match="CONFIG_ERROR.*mix must return 6 rows of 8"):
+            port._mixed(out, rows)
