@@ -158,10 +158,11 @@ class Stage {
     add(p, r.bytes());
     if (n_ > n) items_[n].out = &r;
   }
-  int in(dmh_ctx* c, hipStream_t st, const Err& err) {
+  // (check: makes the block alone)
+  int in(dmh_ctx* c, hipStream_t st, bool check, const Err& err) {
     void* base = nullptr;
     const int rc = dm::api_mixer_buffer(c, dm::kMixerStage, total_ ? total_ : 256, &base, err.p, err.n);
-    if (rc) return rc;
+    if (rc || check) return rc;
     for (int i = 0; i < n_; ++i) {
       Item& it = items_[i];
       void* d = static_cast<uint8_t*>(base) + it.at;
@@ -224,7 +225,7 @@ extern "C" {
 int dmh_short_conv_forward(dmh_ctx* c, const dmh_short_conv* args, const dmh_seq_batch* batch,
                            unsigned flags, char* errp, size_t errlen) {
   const Err err{errp, errlen, "short_conv"};
-  const bool dev = flags & DMH_F_DEVICE;
+  const bool dev = flags & DMH_F_DEVICE, check = flags & DMH_F_CHECK;
   if (!args) return err.arg("args is NULL");
   dmh_short_conv a = *args;
   if (!known(a.dtype)) return err.arg("unknown dtype");
@@ -256,8 +257,9 @@ int dmh_short_conv_forward(dmh_ctx* c, const dmh_short_conv* args, const dmh_seq
     stage.add_out(a.state, state);
     stage.add_out(a.y, y);
     stage_batch(stage, b);
-    if ((rc = stage.in(c, st, err))) return rc;
+    if ((rc = stage.in(c, st, check, err))) return rc;
   }
+  if (check) return DMH_OK;
   const hipError_t e = dm::launch_short_conv(a, seq_dev(b, status), st);
   if (e != hipSuccess) return err.hip(e);
   return dev ? DMH_OK : stage.out(st, err);
@@ -266,7 +268,7 @@ int dmh_short_conv_forward(dmh_ctx* c, const dmh_short_conv* args, const dmh_seq
 int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_seq_batch* batch,
                             unsigned flags, char* errp, size_t errlen) {
   const Err err{errp, errlen, "gated_delta"};
-  const bool dev = flags & DMH_F_DEVICE;
+  const bool dev = flags & DMH_F_DEVICE, check = flags & DMH_F_CHECK;
   if (!args) return err.arg("args is NULL");
   dmh_gated_delta a = *args;
   if (!known(a.dtype)) return err.arg("unknown dtype");
@@ -322,7 +324,7 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
     stage.add_out(a.state, state);
     stage.add_out(a.o, o);
     stage_batch(stage, b);
-    if ((rc = stage.in(c, st, err))) return rc;
+    if ((rc = stage.in(c, st, check, err))) return rc;
   }
   const SeqDev s = seq_dev(b, status);
   const int64_t chunks = b.max_seq_len > kRowsMost ? dm::delta_chunk_count(s, kRowsMost + 1) : 0;
@@ -331,6 +333,7 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
   if (chunks && (rc = dm::api_mixer_buffer(c, dm::kMixerChunks, room * dm::delta_chunk_bytes(a),
                                            &ws, errp, errlen)))
     return rc;
+  if (check) return DMH_OK;
   const hipError_t e = chunks ? dm::launch_delta(a, s, kRowsMost + 1, chunks, room, ws, st)
                               : dm::launch_delta_rows(a, s, st);
   if (e != hipSuccess) return err.hip(e);
@@ -340,7 +343,7 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
 int dmh_gated_norm_forward(dmh_ctx* c, const dmh_gated_norm* args, unsigned flags, char* errp,
                            size_t errlen) {
   const Err err{errp, errlen, "gated_norm"};
-  const bool dev = flags & DMH_F_DEVICE;
+  const bool dev = flags & DMH_F_DEVICE, check = flags & DMH_F_CHECK;
   if (!args) return err.arg("args is NULL");
   dmh_gated_norm a = *args;
   if (!known(a.dtype) || (a.stream_dtype != a.dtype && a.stream_dtype != DMH_DTYPE_F32))
@@ -384,8 +387,9 @@ int dmh_gated_norm_forward(dmh_ctx* c, const dmh_gated_norm* args, unsigned flag
     stage.add(a.gamma, 4 * (size_t)a.dim);
     stage.add(a.edge_gamma, 4 * (size_t)a.dim);
     stage.add(a.scale_vec, 4 * (size_t)w);
-    if ((rc = stage.in(c, st, err))) return rc;
+    if ((rc = stage.in(c, st, check, err))) return rc;
   }
+  if (check) return DMH_OK;
   const hipError_t e = dm::launch_gated_norm(a, st);
   if (e != hipSuccess) return err.hip(e);
   return dev ? DMH_OK : stage.out(st, err);

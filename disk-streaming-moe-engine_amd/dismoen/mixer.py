@@ -22,7 +22,7 @@ import math
 
 import numpy as np
 
-from ._lib import (DMH_F_DEVICE, DismoenError, DmhGatedDelta, DmhGatedNorm, DmhSeqBatch,
+from ._lib import (DMH_F_CHECK, DMH_F_DEVICE, DismoenError, DmhGatedDelta, DmhGatedNorm, DmhSeqBatch,
                    DmhShortConv, check, errbuf)
 
 F32, F16, BF16 = 0, 1, 2
@@ -196,19 +196,26 @@ class ShortConv(_Operator):
     def __call__(self, x, state, batch: SeqBatch, out):
         """out[t] for the rows x [rows][channels]; state [num_slots][width - 1]
         [channels], the last rows of each sequence, is brought up to date."""
-        c, t, w, e, blk = self._c, x.dtype, self.channels, self._err, self._blk
-        dev = None if self._side(x) else blk.device
+        self._go(batch, self._set(x, state, batch, out))
+        return out
+
+    def _set(self, x, state, batch, out):
+        """Fills the argument block from the arrays, which it checks; the call's flags."""
+        c, t, w = self._c, x.dtype, self.channels
+        dev = None if self._side(x) else self._blk.device
         c.dtype = code = _type(x)
         nx, c.x, c.x_stride = self._rows1(x, w, t, dev, "x")
         ny, c.y, c.y_stride = self._rows1(out, w, t, dev, "out")
         c.state = self._state(state, (self.width - 1, w), code, dev, batch)
         if min(nx, ny) < batch.total_tokens:
             raise _bad("x or out has fewer rows than total_tokens")
-        rc = blk._lib.dmh_short_conv_forward(blk.handle, self._ref, batch._ref,
-                                             0 if dev is None else DMH_F_DEVICE, e, 2048)
+        return 0 if dev is None else DMH_F_DEVICE
+
+    def _go(self, batch, flags):
+        blk, e = self._blk, self._err
+        rc = blk._lib.dmh_short_conv_forward(blk.handle, self._ref, batch._ref, flags, e, 2048)
         if rc:
             check(rc, e)
-        return out
 
 
 class GatedDelta(_Operator):
@@ -234,8 +241,12 @@ class GatedDelta(_Operator):
         """out[t] [v_heads][v_dim] for rows q, k [rows][k_heads][k_dim], v
         [rows][v_heads][v_dim] and gates a, b [rows][v_heads]; state [num_slots]
         [v_heads][k_dim][v_dim] fp32 is brought up to date."""
-        c, t, e, blk = self._c, v.dtype, self._err, self._blk
-        dev = None if self._side(v) else blk.device
+        self._go(batch, self._set(q, k, v, a, b, state, batch, out))
+        return out
+
+    def _set(self, q, k, v, a, b, state, batch, out):
+        c, t = self._c, v.dtype
+        dev = None if self._side(v) else self._blk.device
         c.dtype = _type(v)
         g = t if self._raw else a.dtype
         if not self._raw and _type(a) != F32:
@@ -251,11 +262,13 @@ class GatedDelta(_Operator):
         c.state = self._state(state, self._s, F32, dev, batch)
         if min(nq, nk, nv, na, nb, no) < batch.total_tokens:
             raise _bad("a row array has fewer rows than total_tokens")
-        rc = blk._lib.dmh_gated_delta_forward(blk.handle, self._ref, batch._ref,
-                                              0 if dev is None else DMH_F_DEVICE, e, 2048)
+        return 0 if dev is None else DMH_F_DEVICE
+
+    def _go(self, batch, flags):
+        blk, e = self._blk, self._err
+        rc = blk._lib.dmh_gated_delta_forward(blk.handle, self._ref, batch._ref, flags, e, 2048)
         if rc:
             check(rc, e)
-        return out
 
 
 class GatedNorm(_Operator):
@@ -288,13 +301,17 @@ class GatedNorm(_Operator):
     def __call__(self, x, stream=None, y=None, gate=None, residual=None):
         """Writes stream and (where `edge`) y, arrays of the rows' shape [rows]
         [groups][dim]; stream may be the residual itself."""
+        self._go(self._set(x, stream, y, gate, residual))
+        return stream, y
+
+    def _set(self, x, stream, y, gate, residual):
         if (gate is None) == self._gate or (y is None) == self._edge:
             raise _bad("gate and y are given exactly where the operator has them")
         out = y if stream is None else stream
         if out is None:
             raise _bad("neither stream nor y is given")
-        c, t, so, e, blk = self._c, x.dtype, out.dtype, self._err, self._blk
-        dev = None if self._side(x) else blk.device
+        c, t, so = self._c, x.dtype, out.dtype
+        dev = None if self._side(x) else self._blk.device
         c.dtype, c.stream_dtype = _type(x), _type(out)
         h, d = self._shape
         rows = self._rows
@@ -317,11 +334,13 @@ class GatedNorm(_Operator):
             m = m if k == n else k
         if m != n or n >= 1 << 31:
             raise _bad("the row arrays differ in their rows, or have 2^31 or more")
-        rc = blk._lib.dmh_gated_norm_forward(blk.handle, self._ref, 0 if dev is None else DMH_F_DEVICE,
-                                             e, 2048)
+        return 0 if dev is None else DMH_F_DEVICE
+
+    def _go(self, flags):
+        blk, e = self._blk, self._err
+        rc = blk._lib.dmh_gated_norm_forward(blk.handle, self._ref, flags, e, 2048)
         if rc:
             check(rc, e)
-        return stream, y
 
 
 class GatedDeltaMixer:
@@ -345,10 +364,11 @@ class GatedDeltaMixer:
         """out [rows][v_heads][v_dim], the input of the output projection, from the
         input projection's rows mixed [rows][channels], z [rows][v_heads][v_dim]
         and b, a [rows][v_heads].  work: rows like mixed, overwritten.  What out
-        holds in rows of no sequence has no meaning."""
+        holds in rows of no sequence has no meaning.  A call that is refused leaves
+        both states as they were."""
         n, kw = batch.total_tokens, self.k[0] * self.k[1]
         work, out = work[:n], out[:n]
-        self.conv(mixed, conv_state, batch, work)
+        flags = self.conv._set(mixed, conv_state, batch, work)
         if isinstance(work, np.ndarray):
             q, k, v = (np.lib.stride_tricks.as_strided(
                 work[:, at:], (n, *s), (work.strides[0], s[1] * work.itemsize, work.itemsize))
@@ -356,8 +376,14 @@ class GatedDeltaMixer:
         else:
             q, k, v = (work[:, at:at + s[0] * s[1]].unflatten(1, s)
                        for at, s in ((0, self.k), (kw, self.k), (2 * kw, self.v)))
-        self.delta(q, k, v, a, b, state, batch, out)
-        self.norm(out, out, gate=z[:n])
+        self.delta._set(q, k, v, a, b, state, batch, out)
+        self.norm._set(out, out, None, z[:n], None)
+        # (all that the library can refuse, before the first of them runs)
+        self.delta._go(batch, flags | DMH_F_CHECK)
+        self.norm._go(flags | DMH_F_CHECK)
+        self.conv._go(batch, flags)
+        self.delta._go(batch, flags)
+        self.norm._go(flags)
         return out
 
 

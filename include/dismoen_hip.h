@@ -456,6 +456,9 @@ int dmh_moe_forward_gguf(dmh_ctx* ctx, int layer, const float* x, const float* r
  * Rows (x, q, k, v, y, o, gates) have one of these types; weights, decays and
  * the delta rule's states are fp32, and everything is computed in fp32 or more
  * and rounded once, on output. */
+#define DMH_F_CHECK 0x80u /* these calls: check the arguments, make the device memory that
+                           * the call needs, and leave it at that; the call itself then
+                           * fails at a launch at most */
 #define DMH_DTYPE_F32 0
 #define DMH_DTYPE_F16 1
 #define DMH_DTYPE_BF16 2

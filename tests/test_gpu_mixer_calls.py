@@ -161,3 +161,59 @@ def test_port_block_captured():
                     assert torch.equal(a, b)
                 blk.sync()
         del graph
+
+
+def test_mixer_layer_refused_in_a_capture_changes_nothing():
+    """The layer's delta rule needs memory that a capture cannot make: none of the three
+    operators is recorded, and after a call of its sizes all are."""
+    from dismoen import GatedDeltaMixer, MoEBlock
+    g = torch.Generator().manual_seed(5)
+    t, (hk, hv, dk, dv), rows = torch.bfloat16, (1, 2, 64, 64), 70
+    ch = 2 * hk * dk + hv * dv
+    with MoEBlock(0) as blk:
+        mixer = GatedDeltaMixer(blk, hk, hv, dk, dv, rand(g, ch, 4), rand(g, hv), rand(g, hv),
+                                rand(g, dv))
+        off = torch.tensor([0, 20, 70], dtype=torch.int32).cuda()
+        batch = SeqBatch(off, rows, 50, 2)
+        mixed, z = rand(g, rows, ch, t=t), rand(g, rows, hv, dv, t=t)
+        a, b = rand(g, rows, hv, t=t), rand(g, rows, hv, t=t)
+        start = rand(g, 2, 3, ch, t=t), rand(g, 2, hv, dk, dv)
+        cs, st = start[0].clone(), start[1].clone()
+        work, out = torch.zeros_like(mixed), torch.zeros_like(z)
+        args = (mixed, z, b, a, cs, st, batch, work, out)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        mark = torch.zeros(1, device="cuda")
+        torch.cuda.synchronize()
+        blk.set_stream(stream.cuda_stream)
+        with torch.cuda.graph(graph, stream=stream):
+            with pytest.raises(DismoenError, match="before the capture"):
+                mixer(*args)
+            mark.add_(1)
+        blk.set_stream(None)
+        # and one that the library refuses: its output on the gates
+        with pytest.raises(DismoenError, match="overlap"):
+            mixer(mixed, z, b, out[:, 0, :hv], *args[4:])
+        blk.sync()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert mark.item() == 1 and not work.any() and not out.any()
+        assert torch.equal(cs, start[0]) and torch.equal(st, start[1])
+        mixer(*args)
+        blk.sync()
+        want = [x.clone() for x in (out, cs, st)]
+        graph = torch.cuda.CUDAGraph()
+        blk.set_stream(stream.cuda_stream)
+        with torch.cuda.graph(graph, stream=stream):
+            mixer(*args)
+        blk.set_stream(None)
+        for _ in range(3):
+            cs.copy_(start[0])
+            st.copy_(start[1])
+            out.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, y in zip((out, cs, st), want):
+                assert torch.equal(x, y)
+        blk.sync()
+        del graph

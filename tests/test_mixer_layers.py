@@ -1,9 +1,12 @@
 """The layer and the block made of the token mixer's operators: what they refuse, and
 that a refused call has changed nothing, without a GPU."""
 
+import ctypes as C
+
+import numpy as np
 import pytest
 
-from dismoen import DismoenError, PortBlock, lib
+from dismoen import DismoenError, GatedDeltaMixer, PortBlock, SeqBatch, lib
 
 
 def port_blk(**kw):
@@ -43,3 +46,54 @@ def test_port_block_refuses_other_rows_of_the_mixer():
     for out in (None, 1.0, torch.zeros(5, 8), torch.zeros(8, 6), torch.zeros(48), torch.zeros(())):
         with pytest.raises(DismoenError, match="CONFIG_ERROR.*mix must return 6 rows of 8"):
             port._mixed(out, rows)
+
+
+class Counted:
+    """The library without a device: which calls were to run, and the real checks of
+    those that were only to be checked (which end at the missing context)."""
+    CHECK = 0x80
+
+    def __init__(self):
+        self.ran = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            flags = args[-3]
+            if not flags & self.CHECK:
+                self.ran.append(name)
+                return 0
+            rc = getattr(lib(), name)(*args)
+            text = C.string_at(args[-2])
+            return 0 if rc and b"ctx is NULL" in text else rc
+        return call
+
+
+def test_mixer_refuses_before_anything_runs():
+    hk, hv, dk, dv, rows = 1, 2, 8, 8, 5
+    ch = 2 * hk * dk + hv * dv
+
+    def z(*shape, t=np.float32):
+        return np.zeros(shape, t)
+
+    fake = Counted()
+    blk = port_blk(_lib=fake)
+    mixer = GatedDeltaMixer(blk, hk, hv, dk, dv, z(ch, 4), z(hv), z(hv), z(dv))
+    batch = SeqBatch(np.array([0, 2, 5], np.int32), rows, 4, 3)
+    ok = dict(mixed=z(rows, ch), z=z(rows, hv, dv), b=z(rows, hv), a=z(rows, hv),
+              conv_state=z(3, 3, ch), state=z(3, hv, dk, dv), batch=batch, work=z(rows, ch),
+              out=z(rows, hv, dv))
+    mixer(**ok)
+    assert fake.ran == ["dmh_short_conv_forward", "dmh_gated_delta_forward",
+                        "dmh_gated_norm_forward"]
+    for name, other in (("z", z(rows - 1, hv, dv)), ("z", z(rows, hv, dv, t=np.float16)),
+                        ("a", z(rows, hv + 1)), ("b", z(rows - 1, hv)),
+                        ("state", z(3, hv, dk, dv + 8)), ("state", z(2, hv, dk, dv)),
+                        ("conv_state", z(3, 2, ch)), ("out", z(rows, hv, dv, t=np.float16)),
+                        ("out", z(rows - 1, hv, dv)), ("work", z(rows - 1, ch)),
+                        # what only the library sees: outputs on inputs
+                        ("out", ok["work"][:, :hv * dv].reshape(rows, hv, dv, copy=False)),
+                        ("out", ok["z"]), ("a", ok["out"][:, 0, :hv])):
+        fake.ran.clear()
+        with pytest.raises(DismoenError):
+            mixer(**{**ok, name: other})
+        assert not fake.ran, (name, other.shape)
