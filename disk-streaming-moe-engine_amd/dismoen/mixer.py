@@ -27,6 +27,7 @@ from ._lib import (DMH_F_CHECK, DMH_F_DEVICE, DismoenError, DmhGatedDelta, DmhGa
 
 F32, F16, BF16 = 0, 1, 2
 GATES = {None: 0, "silu": 1, "sigmoid": 2}
+_WRITTEN = ("out", "stream", "y")  # the names of row arrays that a call writes
 _TYPES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint16): BF16}
 
 
@@ -97,6 +98,8 @@ class _Operator:
         if device is None:
             if not isinstance(a, np.ndarray) or a.ndim != 3:
                 raise _bad(f"{what} must be a numpy array as the others, [rows][{heads}][{dim}]")
+            if what in _WRITTEN and not a.flags.writeable:
+                raise _bad(f"{what} is written, and the array is read-only")
             (n, h, d), (s, sh, sd), p = a.shape, _strides(a), a.ctypes.data
         else:
             try:
@@ -119,6 +122,8 @@ class _Operator:
         if device is None:
             if not isinstance(a, np.ndarray) or a.ndim != 2:
                 raise _bad(f"{what} must be a numpy array as the others, [rows][{dim}]")
+            if what in _WRITTEN and not a.flags.writeable:
+                raise _bad(f"{what} is written, and the array is read-only")
             (n, d), (s, sd), p = a.shape, _strides(a), a.ctypes.data
         else:
             try:
@@ -139,6 +144,8 @@ class _Operator:
                 or _type(a) != dtype or not (a.flags.c_contiguous if host else a.is_contiguous()) \
                 or (not host and a.get_device() != device):
             raise _bad(f"state must be a contiguous array [num_slots]{list(shape)}")
+        if host and not a.flags.writeable:
+            raise _bad("state is written, and the array is read-only")
         if batch.device != device:
             raise _bad("the batch's arrays are not where the call's are")
         return a.ctypes.data if host else a.data_ptr()

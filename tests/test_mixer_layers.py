@@ -6,7 +6,8 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from dismoen import DismoenError, GatedDeltaMixer, PortBlock, SeqBatch, lib
+from dismoen import (DismoenError, GatedDelta, GatedDeltaMixer, GatedNorm, PortBlock, SeqBatch,
+                     ShortConv, lib)
 
 
 def port_blk(**kw):
@@ -97,3 +98,32 @@ def test_mixer_refuses_before_anything_runs():
         with pytest.raises(DismoenError):
             mixer(**{**ok, name: other})
         assert not fake.ran, (name, other.shape)
+
+
+def test_host_arrays_that_are_written_must_be_writable():
+    """bytes, a broadcast value, a file mapped to be read: an operator that wrote there
+    would change what others hold, or end the process."""
+    blk = port_blk(_lib=Counted())
+    batch = SeqBatch(np.array([0, 2, 5], np.int32), 5, 4, 3)
+
+    def z(*shape):
+        return np.zeros(shape, np.float32)
+
+    def fixed(*shape):
+        return np.frombuffer(bytes(4 * int(np.prod(shape))), np.float32).reshape(shape)
+
+    conv, delta = ShortConv(blk, fixed(8, 4)), GatedDelta(blk, 1, 2, 8, 8, a_log=fixed(2))
+    norm = GatedNorm(blk, 4, 2, gamma=fixed(4), edge=True)
+    r, ins = fixed(5, 8), (fixed(5, 1, 8), fixed(5, 1, 8), fixed(5, 2, 8), fixed(5, 2), fixed(5, 2))
+    conv(r, z(3, 3, 8), batch, z(5, 8))
+    delta(*ins, z(3, 2, 8, 8), batch, z(5, 2, 8))
+    norm(fixed(3, 2, 4), z(3, 2, 4), z(3, 2, 4), residual=fixed(3, 2, 4))
+    for f in (lambda: conv(r, fixed(3, 3, 8), batch, z(5, 8)),
+              lambda: conv(r, z(3, 3, 8), batch, fixed(5, 8)),
+              lambda: conv(r, z(3, 3, 8), batch, np.broadcast_to(np.float32(0), (5, 8))),
+              lambda: delta(*ins, fixed(3, 2, 8, 8), batch, z(5, 2, 8)),
+              lambda: delta(*ins, z(3, 2, 8, 8), batch, fixed(5, 2, 8)),
+              lambda: norm(fixed(3, 2, 4), fixed(3, 2, 4), z(3, 2, 4)),
+              lambda: norm(fixed(3, 2, 4), None, fixed(3, 2, 4))):
+        with pytest.raises(DismoenError, match="CONFIG_ERROR"):
+            f()
