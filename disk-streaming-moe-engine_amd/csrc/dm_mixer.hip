@@ -4,6 +4,8 @@
 //
 // All three read their rows once, keep what they sum in fp32 registers and
 // round once on the way out; all are bound by the memory they touch.
+#include <algorithm>
+
 #include "dm_mixer_device.h"
 
 namespace dm {
@@ -104,9 +106,11 @@ __device__ __forceinline__ void conv_rows(const dmh_short_conv& a, const SeqDev&
 }
 
 template <typename T, int V, int W, int TOK>
-__global__ __launch_bounds__(256) void k_short_conv(dmh_short_conv a, SeqDev s, int col_blocks) {
+__global__ __launch_bounds__(256) void k_short_conv(dmh_short_conv a, SeqDev s, int col_blocks,
+                                                    int tile0) {
   const int tid = threadIdx.x;
-  const int tile = blockIdx.x / col_blocks, col = blockIdx.x - tile * col_blocks;
+  const int in_launch = blockIdx.x / col_blocks, col = blockIdx.x - in_launch * col_blocks;
+  const int tile = tile0 + in_launch;
   const int t0 = tile * TOK, t1 = min(t0 + TOK, s.rows);
 
   // the first sequence with a row at t0 or behind it
@@ -125,9 +129,9 @@ __global__ __launch_bounds__(256) void k_short_conv(dmh_short_conv a, SeqDev s, 
   else if (at - full < a.channels % V)
     conv_rows<T, 1, W>(a, s, full * V + at - full, t0, t1, q0);
 
-  // what is wrong with the call's sequences, spread over the first column of
-  // workgroups
-  if (col == 0 && tid < 64)
+  // what is wrong with the call's sequences, spread over the first launch's first
+  // column of workgroups
+  if (tile0 == 0 && col == 0 && tid < 64)
     for (int q = tile; q < s.num; q += gridDim.x / col_blocks) {
       const SeqRange r = seq_range(s, q, tid == 0);
       if (r.live && s.slots) report_shared_slot(s, q, r.slot, tid);
@@ -140,7 +144,9 @@ hipError_t conv_w(const dmh_short_conv& a, const SeqDev& s, hipStream_t st) {
   const int cb = (a.channels / V + a.channels % V + 255) / 256;
   const auto blocks = [&](int tok) { return (int64_t)cb * ((s.rows + tok - 1) / tok); };
   const auto run = [&](auto kernel, int tok) {
-    kernel<<<dim3((unsigned)blocks(tok)), 256, 0, st>>>(a, s, cb);
+    const int64_t tiles = blocks(tok) / cb, most = (1 << 23) / cb;  // 2^31 threads a launch
+    for (int64_t t = 0; t < tiles; t += most)
+      kernel<<<dim3((unsigned)(std::min(most, tiles - t) * cb)), 256, 0, st>>>(a, s, cb, (int)t);
   };
   // Longer tiles read the weights and the rows before them less often, as long
   // as they leave four workgroups per CU (256 CUs); below one per CU, rows one by

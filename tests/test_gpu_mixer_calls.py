@@ -217,3 +217,47 @@ def test_mixer_layer_refused_in_a_capture_changes_nothing():
                 assert torch.equal(x, y)
         blk.sync()
         del graph
+
+
+def test_conv_of_the_most_rows(block):
+    """2^30 - 1 rows, which take more than one launch: offsets in elements and bytes are
+    past 2^32, and the rows where a launch ends belong to a sequence that goes on."""
+    rows, ch, t = (1 << 30) - 1, 5, torch.float16
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 25 GB")
+    g = torch.Generator().manual_seed(30)
+    x = torch.empty(rows, ch, dtype=t, device="cuda")
+    y = torch.full_like(x, 7.0)
+    w = rand(g, ch, 4)
+    cuts = [0, 3, 1 << 20, (1 << 29) - 2, rows - 2]
+    spots = [0, 1 << 20, (1 << 29) - 70, rows - 150]  # rows looked at
+    part = rand(g, 150, ch, t=t)
+    x.zero_()
+    for at in spots:
+        x[at:at + 150] = part
+    start = rand(g, 4, 3, ch, t=t)
+    state = start.clone()
+    batch = SeqBatch(torch.tensor(cuts, dtype=torch.int32).cuda(), rows, rows, 4)
+    torch.cuda.synchronize()
+    ShortConv(block, w)(x, state, batch, y)
+    block.sync()
+    for at in spots:
+        lo = max(0, at - 3)
+        off = sorted({0, *(min(max(c - lo, 0), at + 150 - lo) for c in cuts)})
+        first = next(i for i in range(4) if cuts[i + 1] > lo)
+        # (the state of the first sequence here: its own, or the rows before)
+        old = torch.zeros(len(off) - 1, 3, ch, dtype=t)
+        for i in range(len(off) - 1):
+            seq = first + i
+            if seq < 4:
+                old[i] = start[seq].cpu() if cuts[seq] >= lo else \
+                    x[lo - 3:lo].cpu() if lo >= 3 and cuts[seq] <= lo - 3 else 0
+        want, _, size = R.conv(x[lo:at + 150], w, None, old, off)
+        inside = [r for r in range(at, at + 150) if r < cuts[4]]
+        R.close(y[inside], want[[r - lo for r in inside]], size[[r - lo for r in inside]], 12)
+    assert (y[cuts[4]:] == 7).all()
+    for i in range(4):
+        line = torch.cat([start[i], x[max(cuts[i], cuts[i + 1] - 3):cuts[i + 1]]])
+        assert torch.equal(state[i], line[-3:])
+    del x, y
+    torch.cuda.empty_cache()
