@@ -290,8 +290,11 @@ int dmh_gated_delta_forward(dmh_ctx* c, const dmh_gated_delta* args, const dmh_s
   if (!a.q || !a.k || !a.v || !a.a || !a.b || !a.state || !a.o)
     return err.arg("q, k, v, a, b, state or o is NULL");
   if (!aligned(a.state, 16)) return err.arg("state must be 16-byte aligned");
-  // (2^32 threads are the most that a launch holds)
-  if ((int64_t)b.num_seqs * a.v_heads * ((a.v_dim + 15) / 16) >= (int64_t)1 << 23)
+  // (a launch holds fewer than 2^32 threads; that of the chunks, of 512 a unit, counts
+  // its units in eights)
+  int64_t units = (int64_t)b.num_seqs * a.v_heads;
+  if (b.max_seq_len > kRowsMost) units = (units + 7) / 8 * 8;
+  if (units * ((a.v_dim + 15) / 16) >= (int64_t)1 << 23)
     return err(DMH_ERR_CONFIG, "CONFIG_ERROR", "too many sequences for one call: %d", b.num_seqs);
   const size_t es = elem(a.dtype), gs = a.a_log ? es : 4;
   const int64_t kw = (int64_t)a.k_heads * a.k_dim, vw = (int64_t)a.v_heads * a.v_dim;

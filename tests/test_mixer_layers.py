@@ -6,6 +6,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
+import test_mixer_refusals as T
 from dismoen import (DismoenError, GatedDelta, GatedDeltaMixer, GatedNorm, PortBlock, SeqBatch,
                      ShortConv, lib)
 
@@ -127,3 +128,17 @@ def test_host_arrays_that_are_written_must_be_writable():
               lambda: norm(fixed(3, 2, 4), None, fixed(3, 2, 4))):
         with pytest.raises(DismoenError, match="CONFIG_ERROR"):
             f()
+
+
+def test_sequences_that_one_launch_holds():
+    """The launch of the chunks counts units in eights: the last few below 2^23 are too
+    many for it, and not for the one row by row."""
+    for seqs, max_len, fits in (((1 << 23) - 1, 16, True), (1 << 23, 16, False),
+                                ((1 << 23) - 1, 17, False), ((1 << 23) - 8, 17, True),
+                                ((1 << 23) - 7, 17, False)):
+        b = T.batch(max_len=max_len)
+        b.num_seqs = b.num_slots = seqs
+        # (addresses apart from each other, which the host does not read)
+        far = {f: (2 + i) << 40 for i, f in enumerate([*"qkvabo", "state"])}
+        rc, text = T.call("gated_delta", T.delta(v_heads=1, **far), b, T.F_DEVICE)
+        assert ("ctx is NULL" if fits else "too many sequences") in text, (seqs, max_len, text)
