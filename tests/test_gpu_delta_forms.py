@@ -79,3 +79,31 @@ def test_forms(block, k_dim, hk, hv, v_dim, t):
         op(*(y[at] for y in ins), one, SeqBatch(i32(0, length), length, length, 1), alone)
         block.sync()
         assert torch.equal(alone, o[at]) and torch.equal(one[0], state[i]), length
+
+
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES)
+def test_a_prompt_among_single_tokens(block, t):
+    """The sequences of one row outnumber the chunked ones by far, on both sides of them."""
+    lens = [1] * 70 + [150] + [1] * 40 + [0, 70] + [1] * 9
+    hk, hv, dk, dv, n, rows = 2, 4, 64, 64, len(lens), sum(lens)
+    g = torch.Generator().manual_seed(9)
+    q, k = (torch.randn((rows, hk, dk), generator=g).to(t) for _ in range(2))
+    v = torch.randn((rows, hv, dv), generator=g).to(t)
+    a, b = -torch.rand((rows, hv), generator=g), torch.rand((rows, hv), generator=g)
+    start = torch.randn((n, hv, dk, dv), generator=g) * 0.3
+    slots = torch.randperm(n, generator=g).int()
+    off = [sum(lens[:i]) for i in range(n + 1)]
+    o, state = torch.zeros((rows, hv, dv), dtype=t, device="cuda"), start.cuda()
+    ins = [x.cuda() for x in (q, k, v, a, b)]
+    batch = SeqBatch(i32(*off), rows, max(lens), n, slots=slots.cuda())
+    torch.cuda.synchronize()
+    GatedDelta(block, hk, hv, dk, dv)(*ins, state, batch, o)
+    block.sync()
+    for i in range(n):
+        at, slot = slice(off[i], off[i + 1]), int(slots[i])
+        if not lens[i]:
+            assert torch.equal(state[slot].cpu(), start[slot])
+            continue
+        worst = D.check(o[at], state[slot], q[at], k[at], v[at], a[at].double(), b[at].double(),
+                        start[slot])
+        assert max(worst) <= 1, (i, worst)

@@ -261,3 +261,28 @@ def test_conv_of_the_most_rows(block):
         assert torch.equal(state[i], line[-3:])
     del x, y
     torch.cuda.empty_cache()
+
+
+def test_mixer_layer_on_host_arrays(block):
+    """The layer on numpy arrays gives the device tensors' bits, and leaves what is
+    behind total_tokens."""
+    from dismoen import GatedDeltaMixer
+    g = torch.Generator().manual_seed(8)
+    (hk, hv, dk, dv), rows = (1, 2, 64, 64), 60
+    ch = 2 * hk * dk + hv * dv
+    p = [rand(g, ch, 4), rand(g, hv), rand(g, hv), rand(g, dv)]
+    ins = [rand(g, rows + 4, ch), rand(g, rows + 4, hv, dv), rand(g, rows, hv), rand(g, rows, hv)]
+    cs, st = rand(g, 3, 3, ch), rand(g, 3, hv, dk, dv)
+    work, out = torch.full((rows + 4, ch), 3.0).cuda(), torch.full((rows + 4, hv, dv), 3.0).cuda()
+    off = torch.tensor([0, 1, 40, 60], dtype=torch.int32)
+    host = [x.cpu().numpy().copy() for x in (*ins, cs, st)]
+    hwork, hout = work.cpu().numpy().copy(), out.cpu().numpy().copy()
+    torch.cuda.synchronize()
+    GatedDeltaMixer(block, hk, hv, dk, dv, *p)(*ins, cs, st, SeqBatch(off.cuda(), rows, 39, 3),
+                                               work, out)
+    block.sync()
+    GatedDeltaMixer(block, hk, hv, dk, dv, *(x.cpu().numpy() for x in p))(
+        *host, SeqBatch(off.numpy(), rows, 39, 3), hwork, hout)
+    for a, b in ((out, hout), (work, hwork), (cs, host[4]), (st, host[5])):
+        assert torch.equal(a.cpu(), torch.from_numpy(b))
+    assert (hout[rows:] == 3).all() and (hwork[rows:] == 3).all()
