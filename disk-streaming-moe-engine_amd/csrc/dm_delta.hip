@@ -39,8 +39,8 @@ constexpr size_t frag_bytes(int n) { return (size_t)n * 1024; }  // 64 lanes of 
 // What k_delta_prep leaves per chunk: for each value head (I + A)^-1 diag(beta)
 // and the query-key matrix in three parts each, and the rows' factors; for each
 // key head K^T, K and Q (copied: rows a power of two apart meet in the same
-// channels of the L2, and read in place they hold up all the other loads: 2048
-// rows of 32 heads took 62 us instead of 57).
+// channels of the L2, and read in place they hold up all the other loads: a tenth
+// of the chain's time for 2048 rows of 32 heads).
 // The key dimension comes in steps of a matrix product, SW dimensions each, of
 // which lane group g of a factor has SW / 4 in a row.  In the state, whose tiles
 // of 16 rows are a right factor as they stand, row 4 g + i of a step's first tile
@@ -154,8 +154,8 @@ __device__ __forceinline__ void store_frag(void* base, size_t frag, int lane, ui
 // With few chunks the way through loads, products and substitution bounds it, so
 // everything is loaded at once, unconditionally, and T takes A's place in LDS (57
 // KB at 128 dimensions in bf16: two workgroups per CU): 2048 rows of 16 key and 32
-// value heads in 18.5 us.  With many, what it writes does: 465 MB of factors for
-// 16384 rows in 124 us, 5 TB/s with what it reads.
+// value heads in 18.5 us.  With many, what it writes does: 516 MB of factors for
+// 16384 rows in 133 us, 5 TB/s with what it reads.
 // The first `short_blocks` workgroups take the short sequences, row by row: they
 // have the longest way, and no chunk waits for them.
 template <typename T, int DKT, int NPK, int HB>
@@ -497,11 +497,12 @@ __global__ __launch_bounds__(256) void k_delta_prep(dmh_gated_delta d, SeqDev s,
 // from memory into LDS, without registers where they fit (M::stage), and make the
 // outputs of 16 rows each, O = e^G Q S + (Q K^T) U, from the parts of S and U that
 // the others leave in LDS.  So the chain never waits for memory: with its loads
-// its own, a third of its time went into their issue, 64 bytes a cycle and CU
-// (75 us instead of 57 for 2048 rows of 32 heads).  What bounds it is the way
-// from barrier to barrier, 1.7 us a chunk with one column tile and 2.5 with two;
-// the matrix cores are busy 17 to 19% of it.  A wave for all rows of a tile needs no
-// way through LDS, but its 132 products and their splits alone take 2.3 us.
+// its own, it took a third longer: their issue, 64 bytes a cycle and CU.  What
+// bounds it is the way from barrier to barrier, 1.9 us a chunk with one column tile
+// (2048 rows of 32 heads: 60 us) and 2.8 to 3.2 with two; the matrix cores are busy
+// 18 to 20% of it.  Outputs from two parts instead of three take 0.2 us a chunk less
+// and lose what lies below 2^-17 of their terms.  A wave for all rows of a tile
+// needs no way through LDS, but its 132 products and their splits alone take 2.3 us.
 // A factor is used in one step only, so one copy of each is enough: the next
 // chunk's K arrives from the barrier behind step 1 to the one behind 3, K^T as
 // well, T from there to the next one.  Where they do not fit, the chain loads K,
@@ -923,8 +924,8 @@ hipError_t run(T, Layout<DKT, NPK>, const dmh_gated_delta& a, const SeqDev& s,
   const int64_t units = ((int64_t)s.num * a.v_heads + 7) / 8 * 8;
   const int rep = a.v_heads / a.k_heads;
   // Two column tiles per workgroup take 1.5 times as long as one (2048 rows of 32
-  // heads: 80 us instead of 55), so they pay where single tiles would come to
-  // more than one workgroup per CU (four long prompts: 386 us instead of 580).
+  // heads: 91 us instead of 60), so they pay where single tiles would come to
+  // more than one workgroup per CU (four long prompts: 449 us instead of 630).
   const int64_t longs = std::min<int64_t>(s.num, s.rows / min_rows);
   const bool pairs = longs * a.v_heads * ((a.v_dim + 15) / 16) > 256;
   const auto chain = pairs ? k_delta_chunks<T, DKT, 2, NPK>

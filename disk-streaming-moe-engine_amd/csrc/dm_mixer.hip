@@ -25,7 +25,7 @@ hipError_t with_type(int dtype, F f) {
 // read and replaced by the workgroup with its first row, which also computes all
 // rows that need the old state (the first W - 1, also where they reach past its
 // rows): no other workgroup touches the state, so nothing has to wait.  Bound by
-// the rows' bytes: 16384 rows of 8192 f16 channels in 123 us, 4.4 TB/s.
+// the rows' bytes: 16384 rows of 8192 f16 channels in 121 us, 4.4 TB/s.
 template <typename T, int V, int W>
 __device__ __forceinline__ void conv_rows(const dmh_short_conv& a, const SeqDev& s, int ch, int t0,
                                           int t1, int first_seq) {
@@ -192,7 +192,7 @@ __device__ __forceinline__ float row_sum(const float (&s)[N], float* part) {
 // each, so that both norms run on the one read of it.  All loads come first and
 // are whole; the one lane whose elements pass the end of the group reads and
 // writes them one by one.  Bound by the rows' bytes: 16384 rows of 2048, bf16
-// into an fp32 stream and its norm, in 92 us, 5.1 TB/s.
+// into an fp32 stream and its norm, in 94 us, 5.0 TB/s.
 template <typename T, typename S, int LPR, int V, int N>
 __global__ __launch_bounds__(256) void k_gated_norm(dmh_gated_norm a, int64_t unit0) {
   __shared__ float part[4];

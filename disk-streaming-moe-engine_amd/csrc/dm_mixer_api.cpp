@@ -25,13 +25,13 @@ namespace {
 using dm::SeqDev;
 
 // Sequences of up to kRowsMost rows take the delta rule row by row.  Measured for
-// 1, 8 and 64 sequences at 32 heads of 128: 8 rows take 14, 17 and 68 us row by
-// row, 16 rows 23, 26 and 114, 32 rows 42, 45 and 210; as a chunk all of these
-// 17, 43 and 245 to 271.
+// 1, 8 and 64 sequences at 32 heads of 128: 8 rows take 14, 16 and 74 us row by
+// row, 16 rows 23, 26 and 115, 32 rows 41, 44 and 212; as a chunk all of these
+// 18, 44 and 253 to 278.
 constexpr int kRowsMost = 16;
 // Chunks whose factors are in memory at once (40 KB to 330 KB a head).  Four
-// sequences of 16384 rows at 32 heads take 3.1 ms with 256, 1.81 ms with 512 and
-// 1.78 ms with 2048; one of 65536 rows 2.8, 2.7 and 2.6 ms.
+// sequences of 16384 rows at 32 heads take 3.4 ms with 256, 1.99 ms with 512 and
+// 1.96 ms with 2048; one of 65536 rows 2.9, 2.8 and 2.8 ms.
 constexpr int64_t kChunkRoom = 512;
 // Rows of a call, whose numbers the kernels count on from in 32 bits.
 constexpr int32_t kRowsLimit = 1 << 30;

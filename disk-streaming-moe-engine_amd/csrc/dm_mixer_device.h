@@ -189,7 +189,7 @@ __device__ __forceinline__ float sum_eighths(float x) {
 // one.  A row's three sums of squares and eight column sums are then added over
 // the eight row groups.  One read and one write of the state bound a single row
 // per sequence: 128 bytes per row and wave, whole lines; 250 sequences of 32
-// heads, 1.05 GB, in 162 us, 6.5 TB/s.  Further rows are bound by the instructions
+// heads, 1.05 GB, in 167 us, 6.3 TB/s.  Further rows are bound by the instructions
 // of a wave, 620 a row: 1.15 us.
 // Sequences of more than max_rows rows (64 at most) are left alone; block: of the workgroups
 // that delta_rows_blocks counts.
@@ -305,7 +305,7 @@ __device__ __forceinline__ void delta_rows(const dmh_gated_delta& d, const SeqDe
   }
   if (!col_in) return;
   // Past the L2, since it is read again in the model's next step: 250 sequences of
-  // 32 heads in 162 us instead of 182 (32 of them: 21.7 and 21.2).
+  // 32 heads in 167 us instead of 182 (32 of them: 21.7 and 21.2).
 #pragma unroll
   for (int i = 0; i < B; ++i) {
     if (row0 + 8 * i >= d.k_dim) break;
