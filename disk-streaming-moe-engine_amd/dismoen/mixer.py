@@ -13,7 +13,7 @@ block's stream and returns at once; errors in the sequences are reported by
 MoEBlock.sync()), or numpy arrays, all of them (the call is synchronous; bf16
 rows are their uint16 bit patterns).  Outputs are arrays of the caller's.  A
 block's stream is its own: order work of other streams against it, or give it
-theirs (MoEBlock.set_stream).
+theirs (MoEBlock.set_stream).  PortBlock does so for torch's current stream.
 """
 from __future__ import annotations
 

@@ -1,5 +1,6 @@
 """The token mixer's calls at the edges of what they take: device batches whose offsets
-fall between skipped sequences."""
+fall between skipped sequences, the port block beside torch's streams and captured, a
+layer that is refused, the most rows, a layer on host arrays."""
 import pytest
 import torch
 
