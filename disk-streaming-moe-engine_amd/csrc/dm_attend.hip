@@ -1,0 +1,775 @@
+// dm_attend.hip -- causal attention over the 4-bit cache.
+//
+// A unit is one key head of a sequence with up to 16 MT of its query rows (a row is one
+// token and one of the R query heads that share the key head).  A wave takes 32
+// tokens of the context a step:
+//   S^T = K Q^T   on the matrix cores; the codes become bf16 in registers, exactly
+//   P   = e^(scale S - m) with m the running maximum of each row
+//   O^T += V^T P^T
+// With S and O transposed, lane (n, quad) holds row n of S for tokens 4 quad .. + 3
+// and 16 + 4 quad .. + 3, which is what the second product takes from it: P passes
+// through no other lane, and each row's maximum and factor lie in its own lanes.
+//
+// What is rounded: queries of 16 or 32 bits enter as one to three bf16 parts that hold
+// all of them, P as two parts (16 bits of it) for rows of 16 bits and three (24) for
+// fp32; sums and maxima are fp32.
+#include <algorithm>
+#include <type_traits>
+
+#include "dm_cache_device.h"
+
+namespace dm {
+namespace {
+
+template <typename F>
+hipError_t with_type(int dtype, F f) {
+  if (dtype == DMH_DTYPE_BF16) return f(bf16_t{});
+  if (dtype == DMH_DTYPE_F16) return f(half_t{});
+  return f(float{});
+}
+
+// A matrix product's result may be read only some cycles after its issue; the compiler
+// counts instructions for that, but not across the end of a loop.
+template <int A, int B>
+__device__ __forceinline__ void settle(f32x4 (&c)[A][B]) {
+#pragma unroll
+  for (int i = 0; i < A * B; ++i) asm volatile("" : "+v"(c[i / B][i % B]));
+  asm volatile("s_nop 7\n\ts_nop 7" : "+v"(c[0][0]));
+#pragma unroll
+  for (int i = 0; i < A * B; ++i) asm volatile("" : "+v"(c[i / B][i % B]));
+}
+
+constexpr int kStep = 32;   // tokens of a step
+constexpr int kTile = 128;  // tokens of a step of four waves
+constexpr float kNone = -3e38f;  // the maximum of a row that has seen no token
+
+struct AttendDev {
+  dmh_attention a;
+  CacheDev c;
+  SeqDev s;
+  int rep;       // query heads per key head
+  int few_rows;  // sequences of up to so many rows are k_attend_few's
+  int blocks;    // row blocks of a unit there, at most
+  float c2;      // scale * log2(e)
+  float* part;   // the workgroups' unfinished units
+  int4* meta;    // by unit: first workgroup, how many, its first one's place, -
+};
+
+// N words at any word's address.
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint32_t u2v __attribute__((ext_vector_type(2), aligned(4)));
+  int i = 0;
+#pragma unroll
+  for (; i + 4 <= N; i += 4) {
+    const u4 v = *reinterpret_cast<const u4*>(p + 4 * i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[i + j] = v[j];
+  }
+  if (N % 4 >= 2) {
+    const u2v v = *reinterpret_cast<const u2v*>(p + 4 * i);
+    w[i] = v[0];
+    w[i + 1] = v[1];
+    i += 2;
+  }
+  if (N % 2) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+}
+// NB bytes at a multiple of their number (of 16 bytes that belong to the same array).
+template <int NB>
+__device__ __forceinline__ void load_scales(const uint8_t* p, uint32_t (&w)[(NB + 3) / 4]) {
+  if constexpr (NB == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else if constexpr (NB == 6) {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    w[0] = h[0] | (uint32_t)h[1] << 16;
+    w[1] = h[2];
+  } else if constexpr (NB == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (NB == 3) {
+    w[0] = p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16;
+  } else if constexpr (NB == 2) {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else {
+    w[0] = p[0];
+  }
+}
+// Byte i of a word as an exponent field.
+__device__ __forceinline__ uint32_t exponent(uint32_t w, int i) {
+  return (i == 3 ? w >> 24 : (w >> (8 * i)) & 0xFFu) << 23;
+}
+
+__device__ __forceinline__ float max_quads(float x) {
+  const auto bits = [](float v) { return __builtin_bit_cast(unsigned, v); };
+  auto p = __builtin_amdgcn_permlane16_swap(bits(x), bits(x), false, false);
+  x = fmaxf(u2f(p[0]), u2f(p[1]));
+  p = __builtin_amdgcn_permlane32_swap(bits(x), bits(x), false, false);
+  return fmaxf(u2f(p[0]), u2f(p[1]));
+}
+__device__ __forceinline__ float sum_quads(float x) {
+  const auto bits = [](float v) { return __builtin_bit_cast(unsigned, v); };
+  auto p = __builtin_amdgcn_permlane16_swap(bits(x), bits(x), false, false);
+  x = u2f(p[0]) + u2f(p[1]);
+  p = __builtin_amdgcn_permlane32_swap(bits(x), bits(x), false, false);
+  return u2f(p[0]) + u2f(p[1]);
+}
+
+// x as PARTS bf16 values whose sum it is, to 8 bits each.
+template <int PARTS>
+__device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&out)[PARTS]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+      if (p + 1 < PARTS) {
+        r[2 * i] -= bf16lo(w[i]);
+        r[2 * i + 1] -= bf16hi(w[i]);
+      }
+    }
+    out[p] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+
+// The codes and scales of a step, as they come.
+template <int NB>
+struct Held {
+  static constexpr int VS = CacheLay<NB>::pow2 ? 1 : NB;
+  uint32_t k[2][NB], v[2][NB], ks[2][(NB + 3) / 4], vs[2][VS];
+};
+
+template <typename T, int NB, int MT>
+struct Wave {
+  using L = CacheLay<NB>;
+  static constexpr int QP = std::is_same<T, bf16_t>::value ? 1 : std::is_same<T, half_t>::value ? 2 : 3;
+  static constexpr int PP = std::is_same<T, float>::value ? 3 : 2;
+  bf16x8 q[MT][QP][NB];
+  f32x4 o[MT][2 * NB];
+  float m[MT], l[MT];  // in units of log2; l of this lane's tokens
+  int seen[MT];        // the last position that the row sees, -1: no such row
+
+  // the unit
+  const uint8_t *codes, *scales;
+  const int32_t* table;
+  size_t value_at;  // regions from a head's keys to its values
+  int head, shift, num_pages, heads, len;
+  bool bad;
+
+  // Rows row0 .. row0 + 16 MT - 1 of the sequence's n * rep.
+  __device__ __forceinline__ void begin(const AttendDev& d, const CacheSeq& s, int h, int row0) {
+    const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+    codes = d.c.codes;
+    scales = d.c.scales;
+    table = d.c.pages + (int64_t)s.slot * d.c.max_pages;
+    head = h;
+    heads = d.c.heads;
+    shift = d.c.page_shift;
+    num_pages = d.c.num_pages;
+    len = s.past + s.n;
+    bad = false;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int row = row0 + 16 * i + n, t = row / d.rep;
+      const bool in = t < s.n;
+      seen[i] = in ? s.past + t : -1;
+      m[i] = kNone;
+      l[i] = 0.0f;
+      const T* p = static_cast<const T*>(d.a.q) + (int64_t)(s.begin + (in ? t : 0)) * d.a.q_stride +
+                   (int64_t)(h * d.rep + (in ? row - t * d.rep : 0)) * d.a.q_head_stride + 8 * quad;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        float f[8];
+        bf16x8 w[QP];
+        load_f32<8>(p + 32 * j, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = in ? f[e] : 0.0f;
+        split<QP>(f, w);
+#pragma unroll
+        for (int e = 0; e < QP; ++e) q[i][e][j] = w[e];
+      }
+#pragma unroll
+      for (int j = 0; j < 2 * NB; ++j) o[i][j] = f32x4{};
+    }
+  }
+
+  __device__ __forceinline__ int page(int t) const {  // of a uniform position
+    return table[min(t, len - 1) >> shift];
+  }
+
+  __device__ __forceinline__ void load(Held<NB>& w, int t0, int p0, int p1) {
+    const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      int p = a ? p1 : p0;
+      if ((unsigned)p >= (unsigned)num_pages) {
+        bad = true;
+        p = 0;
+      }
+      // (the second 16 may lie behind the last page: those of the first are read again)
+      const int t = t0 + 16 * a < len ? t0 + 16 * a : t0;
+      const size_t pos = t & ((1 << shift) - 1);
+      const size_t key = (((size_t)p * 2) * heads + head) << shift;
+      const size_t value = key + ((size_t)heads << shift);
+      load_words<NB>(codes + (key + pos) * L::row + (unsigned)(n * L::row + quad * NB * 4), w.k[a]);
+      load_words<NB>(codes + (value + pos) * L::row + (unsigned)(quad * (4 * L::row) + n * (4 * NB)),
+                     w.v[a]);
+      load_scales<NB>(scales + (key + pos) * NB + (unsigned)(n * NB), w.ks[a]);
+      const uint8_t* vs = scales + (value + pos) * NB + (unsigned)(quad * (4 * NB));
+      if constexpr (L::pow2) w.vs[a][0] = *reinterpret_cast<const uint32_t*>(vs + (n * NB / 16) * 4);
+      else load_words<Held<NB>::VS>(vs, w.vs[a]);
+    }
+  }
+
+  // MASK: some row does not see some token of the step.
+  template <bool MASK>
+  __device__ __forceinline__ void step(const AttendDev& d, Held<NB>& w, int t0) {
+    const int quad = (threadIdx.x & 63) >> 4;
+    f32x4 s[MT][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) s[i][a] = f32x4{};
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const uint32_t x = exponent(w.ks[a][j / 4], j % 4), c = w.k[a][j];
+        const bf16x8 k = __builtin_bit_cast(
+            bf16x8, make_uint4(held_pair<0>(c, x), held_pair<1>(c, x), held_pair<2>(c, x),
+                               held_pair<3>(c, x)));
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < QP; ++e) s[i][a] = mfma16(k, q[i][e][j], s[i][a]);
+      }
+    }
+    bf16x8 p[MT][PP];
+    uint32_t visible[MT][4];  // 1.0 of each token that the row sees
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      float z[8];
+      float most = -__builtin_inff();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        z[e] = s[i][e / 4][e % 4];
+        if (MASK && t0 + 16 * (e / 4) + 4 * quad + e % 4 > seen[i]) z[e] = -__builtin_inff();
+        most = fmaxf(most, z[e]);
+      }
+      if (MASK) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = t0 + 16 * (e / 2) + 4 * quad + e % 2 * 2;
+          visible[i][e] = (t <= seen[i] ? 0x3F80u : 0u) | (t + 1 <= seen[i] ? 0x3F800000u : 0u);
+        }
+      }
+      const float now = fmaxf(m[i], max_quads(most) * d.c2);
+      if (__any(now != m[i])) {
+        const float f = __builtin_amdgcn_exp2f(m[i] - now);
+        l[i] *= f;
+#pragma unroll
+        for (int j = 0; j < 2 * NB; ++j) o[i][j] *= f;
+        m[i] = now;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], d.c2, -now));
+        l[i] += z[e];
+      }
+      split<PP>(z, p[i]);
+    }
+    // A value held as NaN would reach the rows that do not see it (0 * NaN): it enters
+    // as 0, and rows that see it are made NaN behind the products.
+    uint32_t vs[2][Held<NB>::VS];
+    bool nan = false;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int g = 0; g < Held<NB>::VS; ++g) {
+        uint32_t x = w.vs[a][g];
+        if (MASK) {  // tokens behind the last one are not there
+          const int left = len - (t0 + 16 * a + 4 * quad);
+          x = left >= 4 ? x : left <= 0 ? 0u : x & ((1u << (8 * left)) - 1);
+        }
+        vs[a][g] = x;
+        // a byte of 255: x & (x >> 4 ...) by bytes is costlier than a carry out of +1
+        const uint32_t y = ~x;
+        nan = nan || (((y - 0x01010101u) & ~y & 0x80808080u) != 0);
+      }
+    const bool some = __any(nan);
+    if (some) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        uint32_t mark[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t x = vs[e / 2][L::pow2 ? 0 : b] >> (16 * (e % 2));
+          mark[e] = ((x & 0xFFu) == 0xFFu ? 0x3F80u : 0u) | ((x & 0xFF00u) == 0xFF00u ? 0x3F800000u : 0u);
+        }
+        const bf16x8 a = __builtin_bit_cast(bf16x8, make_uint4(mark[0], mark[1], mark[2], mark[3]));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          uint32_t v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = MASK ? visible[i][e] : 0x3F803F80u;
+          const f32x4 hit = mfma16(
+              a, __builtin_bit_cast(bf16x8, make_uint4(v[0], v[1], v[2], v[3])), f32x4{});
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float add = hit[e] > 0.0f ? __builtin_nanf("") : 0.0f;
+            o[i][2 * b][e] += add;
+            o[i][2 * b + 1][e] += add;
+          }
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int g = 0; g < Held<NB>::VS; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((vs[a][g] >> (8 * e) & 0xFFu) == 0xFFu) vs[a][g] &= ~(0xFFu << (8 * e));
+    }
+    // (a pair that every row of the wave takes as it is: two tokens of one element)
+    uint32_t x[8];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      if (b == 0 || !L::pow2) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = exponent(vs[e / 4][L::pow2 ? 0 : b], e % 4);
+      }
+      uint32_t pair[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int at = (e % 4) * NB + b;
+        const uint32_t c = w.v[e / 4][at / 4];
+        pair[e] = at % 4 == 0 ? held_pair<0>(c, x[e]) : at % 4 == 1 ? held_pair<1>(c, x[e])
+                  : at % 4 == 2 ? held_pair<2>(c, x[e]) : held_pair<3>(c, x[e]);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t sel = half ? 0x07060302u : 0x05040100u;
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_perm(pair[2 * e + 1], pair[2 * e], sel);
+        const bf16x8 a = __builtin_bit_cast(bf16x8, make_uint4(v[0], v[1], v[2], v[3]));
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < PP; ++e)
+            o[i][2 * b + half] = mfma16(a, p[i][e], o[i][2 * b + half]);
+      }
+    }
+  }
+
+  // Steps t0, t0 + stride, ... below end.
+  __device__ __forceinline__ void run(const AttendDev& d, int t0, int end, int stride, int past) {
+    if (t0 >= end) return;
+    Held<NB> w;
+    load(w, t0, page(t0), page(t0 + 16));
+    int p0 = page(t0 + stride), p1 = page(t0 + stride + 16);
+    for (; t0 < end; t0 += stride) {
+      const Held<NB> now = w;
+      if (t0 + stride < end) {
+        load(w, t0 + stride, p0, p1);
+        p0 = page(t0 + 2 * stride);
+        p1 = page(t0 + 2 * stride + 16);
+      }
+      Held<NB> cur = now;
+      if (t0 + kStep - 1 > past) step<true>(d, cur, t0);
+      else step<false>(d, cur, t0);
+    }
+    settle(o);
+  }
+
+  // Elements that lane quad holds of its row: f(element, four values e, e + 1 ...) in
+  // ascending runs.  o[i][j][e] is element elem(quad, j, e).
+  __device__ __forceinline__ static int elem(int quad, int j, int e) {
+    return L::pow2 ? (4 * quad + e) * 2 * NB + j : 32 * (j / 2) + 8 * quad + 2 * e + j % 2;
+  }
+};
+
+// ---- few rows: contexts divided over the workgroups -------------------------------------
+// All tiles of 128 tokens of all units, one behind the other, are divided evenly over
+// the workgroups, so that one long context and many short ones fill the device alike; a
+// workgroup's four waves take the steps of its tiles in turn and join what they have
+// through LDS.  A unit that lies in one workgroup is done there, others leave O, m and
+// l of their parts for k_attend_join.
+struct Share {
+  int64_t total, lo, hi;  // tiles in all, this workgroup's
+  int groups;
+};
+__device__ __forceinline__ int64_t share_at(int64_t total, int groups, int w) {
+  return total / groups * w + total % groups * w / groups;
+}
+
+__device__ __forceinline__ int tiles_of(const AttendDev& d, const CacheSeq& q, int rows_per_block,
+                                        int* blocks) {
+  const int64_t rows = (int64_t)q.n * d.rep;
+  if (!q.n || rows > d.few_rows) return *blocks = 0;
+  *blocks = ((int)rows + rows_per_block - 1) / rows_per_block;
+  return (q.past + q.n + kTile - 1) / kTile;
+}
+
+template <int D, int ROWS>
+constexpr int part_floats() { return ROWS * (D + 2); }
+
+template <typename T>
+__device__ __forceinline__ void finish(const AttendDev& d, const CacheSeq& s, int h, int row, int e0,
+                                       const float (&v)[4], float l) {
+  const int t = row / d.rep, hq = h * d.rep + (row - t * d.rep);
+  const int64_t tok = s.begin + t;
+  float r[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = v[e] / l;
+  if (d.a.gate) {
+    float g[4];
+    load_f32<4>(static_cast<const T*>(d.a.gate) + tok * d.a.gate_stride +
+                    hq * d.a.gate_head_stride + e0, g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] *= sigmoid_hw(g[e]);
+  }
+  store_f32<4>(static_cast<T*>(d.a.o) + tok * d.a.o_stride + hq * d.a.o_head_stride + e0, r);
+}
+
+template <typename T, int NB, int MT>
+__global__ __launch_bounds__(256) void k_attend_few(AttendDev d) {
+  using W = Wave<T, NB, MT>;
+  constexpr int D = 32 * NB, ROWS = 16 * MT;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = blockIdx.x;
+
+  __shared__ int64_t ends[256];  // tiles to the end of each of 256 sequences
+  __shared__ CacheSeq seqs[256];
+  __shared__ int64_t wsum[4];
+  __shared__ float om[4][ROWS], ol[4][ROWS];
+  __shared__ __align__(16) float oo[4][16][D + 4];
+
+  // The tiles of 256 sequences from i0 on, summed up in ends; their sum.
+  const auto count = [&](int i0) {
+    CacheSeq q = {};
+    int64_t mine = 0;
+    if (i0 + tid < d.s.num) {
+      q = cache_seq(d.c, d.s, i0 + tid, group == 0);
+      int blocks;
+      const int tiles = tiles_of(d, q, ROWS, &blocks);
+      mine = (int64_t)tiles * blocks * d.c.heads;
+    }
+    int64_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int64_t x = __shfl_up(sum, o);
+      if (lane >= o) sum += x;
+    }
+    __syncthreads();
+    if (lane == 63) wsum[wave] = sum;
+    seqs[tid] = q;
+    __syncthreads();
+    int64_t before = 0;
+    for (int i = 0; i < wave; ++i) before += wsum[i];
+    ends[tid] = before + sum;
+    __syncthreads();
+    return ends[255];
+  };
+
+  int64_t total = count(0);
+  for (int i0 = 256; i0 < d.s.num; i0 += 256) total += count(i0);
+  const int groups = (int)min<int64_t>(gridDim.x, total);
+  if (group >= groups) return;
+  const int64_t lo = share_at(total, groups, group), hi = share_at(total, groups, group + 1);
+  int64_t base = 0, at = lo;
+  int slot = 0;  // unfinished units of this workgroup so far
+  for (int i0 = 0; i0 < d.s.num && at < hi; i0 += 256) {
+    const int64_t sum = d.s.num > 256 ? count(i0) : total;
+    int i = 0;
+    while (at < hi && at < base + sum) {
+      // the sequence that tile `at` lies in
+      int step = 128;
+      for (i = 0; step; step /= 2)
+        if (base + ends[i + step - 1] <= at) i += step;
+      i = __builtin_amdgcn_readfirstlane(i);
+      const CacheSeq q = seqs[i];
+      const int64_t first = base + (i ? ends[i - 1] : 0);
+      int blocks;
+      const int tiles = tiles_of(d, q, ROWS, &blocks);
+      const int unit = (int)((at - first) / tiles);
+      const int64_t unit_at = first + (int64_t)unit * tiles;
+      const int h = unit / blocks, block = unit - h * blocks;
+      const int ta = (int)(at - unit_at), tb = (int)min<int64_t>(tiles, hi - unit_at);
+
+      W w;
+      w.begin(d, q, h, block * ROWS);
+      w.run(d, ta * kTile + wave * kStep, min(tb * kTile, w.len), kTile, q.past);
+      if (w.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)(i0 + i), kSqPage));
+
+      const bool whole = ta == 0 && tb == tiles;
+      const int n = lane & 15, quad = lane >> 4;
+      float* const part = d.part + (size_t)(2 * group + slot) * part_floats<D, ROWS>();
+      const int64_t mi = ((int64_t)(i0 + i) * d.c.heads + h) * d.blocks + block;
+      if (!whole && ta == 0 && tid == 0) {
+        // the workgroup of the unit's last tile: the last one that begins before it
+        const int64_t last = unit_at + tiles - 1;
+        int g = (int)(last * groups / total);
+        while (share_at(total, groups, g) > last) --g;
+        while (share_at(total, groups, g + 1) <= last) ++g;
+        d.meta[mi] = make_int4(group, g - group + 1, 2 * group + slot, 0);
+      } else if (whole && tid == 0) {
+        d.meta[mi] = make_int4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int b = 0; b < MT; ++b) {
+        __syncthreads();
+        const float l = sum_quads(w.l[b]);
+        if (quad == 0) {
+          om[wave][16 * b + n] = w.m[b];
+          ol[wave][16 * b + n] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * NB; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) oo[wave][n][W::elem(quad, j, e)] = w.o[b][j][e];
+        __syncthreads();
+        for (int x = tid; x < 16 * D / 4; x += 256) {
+          const int r = x / (D / 4), e0 = x % (D / 4) * 4;
+          const int row = block * ROWS + 16 * b + r;
+          if (row >= q.n * d.rep) break;
+          float f[4], m = kNone, sum_l = 0.0f, v[4] = {};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) m = fmaxf(m, om[k][16 * b + r]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            f[k] = __builtin_amdgcn_exp2f(om[k][16 * b + r] - m);
+            sum_l += f[k] * ol[k][16 * b + r];
+            const f32x4 y = *reinterpret_cast<const f32x4*>(&oo[k][r][e0]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(f[k], y[e], v[e]);
+          }
+          if (whole) {
+            finish<T>(d, q, h, row, e0, v, sum_l);
+          } else {
+            *reinterpret_cast<f32x4*>(part + (16 * b + r) * D + e0) = f32x4{v[0], v[1], v[2], v[3]};
+            if (e0 == 0) {
+              part[ROWS * D + 16 * b + r] = m;
+              part[ROWS * D + ROWS + 16 * b + r] = sum_l;
+            }
+          }
+        }
+      }
+      slot += !whole;
+      at = unit_at + tb;
+      __syncthreads();
+    }
+    base += sum;
+  }
+}
+
+// The parts of a unit joined: a workgroup takes one row and 64 of its elements, 16
+// threads of 4 elements, 16 parts at a time.
+template <typename T, int NB, int MT>
+__global__ __launch_bounds__(256) void k_attend_join(AttendDev d) {
+  constexpr int D = 32 * NB, ROWS = 16 * MT, COLS = (D + 63) / 64;
+  const int tid = threadIdx.x, x = tid & 15, y = tid >> 4;
+  int u = blockIdx.x;
+  const int col = u % COLS * 64 + 4 * x;
+  u /= COLS;
+  const int r = u % ROWS;
+  u /= ROWS;
+  const int block = u % d.blocks, h = u / d.blocks % d.c.heads;
+  const int seq = u / d.blocks / d.c.heads;
+  const CacheSeq q = cache_seq(d.c, d.s, seq, false);
+  int blocks;
+  if (!tiles_of(d, q, ROWS, &blocks) || block >= blocks) return;
+  const int row = block * ROWS + r;
+  if (row >= q.n * d.rep) return;
+  const int4 meta = d.meta[u];
+  if (meta.y == 0) return;
+  constexpr int P = part_floats<D, ROWS>();
+  // a workgroup's parts lie at 2 g and 2 g + 1; all but the first begin with this unit
+  const auto part = [&](int i) {
+    return d.part + (size_t)(i ? 2 * (meta.x + i) : meta.z) * P;
+  };
+  float m = kNone, l = 0.0f;
+  f32x4 v = {};
+  for (int i = y; i < meta.y; i += 16) {
+    const float* p = part(i);
+    const float pm = p[ROWS * D + r], pl = p[ROWS * D + ROWS + r];
+    f32x4 o = {};
+    if (col < D) o = *reinterpret_cast<const f32x4*>(p + r * D + col);
+    const float now = fmaxf(m, pm);
+    const float a = __builtin_amdgcn_exp2f(m - now), b = __builtin_amdgcn_exp2f(pm - now);
+    m = now;
+    l = a * l + b * pl;
+    v = a * v + b * o;
+  }
+  __shared__ float sm[16][16], sl[16][16];
+  __shared__ f32x4 so[16][16];
+  sm[y][x] = m;
+  sl[y][x] = l;
+  so[y][x] = v;
+  __syncthreads();
+  if (y || col >= D) return;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = fmaxf(m, sm[i][x]);
+  l = 0.0f;
+  v = f32x4{};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float f = __builtin_amdgcn_exp2f(sm[i][x] - m);
+    l = __builtin_fmaf(f, sl[i][x], l);
+    v = f * so[i][x] + v;
+  }
+  const float out[4] = {v[0], v[1], v[2], v[3]};
+  finish<T>(d, q, h, row, col, out, l);
+}
+
+// ---- many rows ------------------------------------------------------------------------------
+// A workgroup takes 64 MT rows of a unit, each of its waves 16 MT of them with the whole
+// context up to its last row; the waves read the same codes at about the same time.
+template <typename T, int NB, int MT>
+__global__ __launch_bounds__(256) void k_attend_many(AttendDev d) {
+  using W = Wave<T, NB, MT>;
+  constexpr int ROWS = 64 * MT;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // the sequence and block of rows: the last blocks, of the longest contexts, first
+  __shared__ int64_t wsum[4];
+  __shared__ int found[2];
+  const int h = blockIdx.x % d.c.heads;
+  const int64_t mine = gridDim.x / d.c.heads - 1 - blockIdx.x / d.c.heads;
+  if (tid == 0) found[0] = -1;
+  int64_t base = 0;
+  for (int i0 = 0; i0 < d.s.num; i0 += 256) {
+    int n = 0;
+    if (i0 + tid < d.s.num) {
+      const CacheSeq q = cache_seq(d.c, d.s, i0 + tid, blockIdx.x == 0);
+      const int64_t rows = (int64_t)q.n * d.rep;
+      n = rows > d.few_rows ? (int)((rows + ROWS - 1) / ROWS) : 0;
+    }
+    int64_t sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int64_t x = __shfl_up(sum, o);
+      if (lane >= o) sum += x;
+    }
+    __syncthreads();
+    if (lane == 63) wsum[wave] = sum;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) sum += wsum[i];
+    if (mine >= base + sum - n && mine < base + sum) {
+      found[0] = i0 + tid;
+      found[1] = (int)(mine - (base + sum - n));
+    }
+    base += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    if (base > mine) break;
+  }
+  __syncthreads();
+  const int seq = __builtin_amdgcn_readfirstlane(found[0]);
+  if (seq < 0) return;
+  const CacheSeq q = cache_seq(d.c, d.s, seq, false);
+  const int64_t row0 = (int64_t)found[1] * ROWS + wave * (16 * MT), rows = (int64_t)q.n * d.rep;
+  if (row0 >= rows) return;
+  W w;
+  w.begin(d, q, h, (int)row0);
+  const int last = (int)((min(row0 + 16 * MT, rows) - 1) / d.rep);
+  w.run(d, 0, q.past + last + 1, kStep, q.past + (int)(row0 / d.rep));
+  if (w.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)seq, kSqPage));
+  const int n = lane & 15, quad = lane >> 4;
+#pragma unroll
+  for (int b = 0; b < MT; ++b) {
+    const float l = sum_quads(w.l[b]);
+    const int64_t row = row0 + 16 * b + n;
+    if (row >= rows) continue;
+    if constexpr (W::L::pow2 && NB >= 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < 2 * NB; j += 4) {
+          const float v[4] = {w.o[b][j][e], w.o[b][j + 1][e], w.o[b][j + 2][e], w.o[b][j + 3][e]};
+          finish<T>(d, q, h, (int)row, W::elem(quad, j, e), v, l);
+        }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e += 2)
+#pragma unroll
+        for (int j = 0; j < 2 * NB; j += 2) {
+          const float v[4] = {w.o[b][j][e], w.o[b][j + 1][e], w.o[b][j][e + 1], w.o[b][j + 1][e + 1]};
+          finish<T>(d, q, h, (int)row, W::elem(quad, j, e), v, l);
+        }
+    }
+  }
+}
+
+constexpr int kGroups = 512;  // workgroups of k_attend_few
+constexpr int64_t kMostBlocks = 1 << 23;  // workgroups of a launch, of 2^31 threads
+
+// Rows of a sequence that k_attend_few takes, in blocks of 16 or 32.
+int few_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, int mt) {
+  const int64_t rep = a.q_heads / c.kv_heads;
+  const int64_t most = std::max<int64_t>(rep, std::min<int64_t>(64, s.max_len * rep));
+  return (int)((most + 16 * mt - 1) / (16 * mt));
+}
+int few_tiles(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
+  const int64_t rep = a.q_heads / c.kv_heads;
+  return c.dim <= 128 && s.max_len * rep > 16 ? 2 : 1;
+}
+
+// Workgroups of k_attend_many and of k_attend_join, at most.
+constexpr int many_tiles(int dim) { return dim > 128 ? 1 : 2; }
+int64_t many_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
+  const int64_t rep = a.q_heads / c.kv_heads;
+  return (s.rows * rep / (64 * many_tiles(c.dim)) + std::min(s.num, s.rows)) * c.kv_heads;
+}
+int64_t join_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, int mt) {
+  return (int64_t)s.num * c.kv_heads * few_blocks(a, c, s, mt) * 16 * mt * ((c.dim + 63) / 64);
+}
+
+}  // namespace
+
+bool attend_fits(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
+  return many_blocks(a, c, s) < kMostBlocks &&
+         join_blocks(a, c, s, few_tiles(a, c, s)) < kMostBlocks;
+}
+
+size_t attend_bytes(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
+  const int mt = few_tiles(a, c, s);
+  return (size_t)2 * kGroups * (16 * mt) * (c.dim + 2) * 4 +
+         sizeof(int4) * s.num * c.kv_heads * few_blocks(a, c, s, mt);
+}
+
+hipError_t launch_attend(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, void* ws,
+                         hipStream_t st) {
+  AttendDev d = {a, cache_dev(c), s};
+  d.rep = a.q_heads / c.kv_heads;
+  d.few_rows = std::max(d.rep, 64);
+  d.c2 = (float)((double)a.scale * 1.4426950408889634);
+  const int mt = few_tiles(a, c, s);
+  d.blocks = few_blocks(a, c, s, mt);
+  d.part = static_cast<float*>(ws);
+  d.meta = reinterpret_cast<int4*>(d.part + (size_t)2 * kGroups * (16 * mt) * (c.dim + 2));
+  return with_type(a.dtype, [&](auto t) {
+    return with_blocks(c.dim, [&](auto nb) {
+      using T = decltype(t);
+      constexpr int NB = decltype(nb)::value;
+      if ((int64_t)s.max_len * d.rep > d.few_rows) {
+        k_attend_many<T, NB, many_tiles(32 * NB)>
+            <<<(unsigned)many_blocks(a, c, s), 256, 0, st>>>(d);
+      }
+      const auto few = [&](auto m) {
+        constexpr int MT = decltype(m)::value;
+        k_attend_few<T, NB, MT><<<kGroups, 256, 0, st>>>(d);
+        k_attend_join<T, NB, MT><<<(unsigned)join_blocks(a, c, s, MT), 256, 0, st>>>(d);
+      };
+      if constexpr (NB <= 4) {
+        if (mt == 2) few(std::integral_constant<int, 2>{});
+      }
+      if (mt == 1) few(std::integral_constant<int, 1>{});
+      return hipGetLastError();
+    });
+  });
+}
+
+}  // namespace dm

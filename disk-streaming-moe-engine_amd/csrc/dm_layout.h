@@ -104,7 +104,8 @@ enum : uint32_t {  // kinds
   kEkBadId = 4,     // an expert id outside [0, E) given to the experts entry point
   kEkRecheck = 15,  // fused decode: a non-finite output whose first failing check is re-derived
   kGkLogit = 0, kGkRange = 1,                       // shared gate
-  kSqOffsets = 0, kSqLength = 1, kSqSlot = 2, kSqTwice = 3, kSqCount = 4,  // sequences
+  kSqOffsets = 0, kSqLength = 1, kSqSlot = 2, kSqTwice = 3, kSqPast = 4, kSqPage = 5,
+  kSqCount = 6,                                     // sequences
 };
 constexpr uint64_t kNoError = ~0ull;
 

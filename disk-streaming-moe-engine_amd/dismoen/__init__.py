@@ -7,4 +7,5 @@ from ._lib import DismoenError, LIB_PATH, lib  # noqa: F401
 from .layers import MoEBlock, RouterConfig, RoutingInfo  # noqa: F401
 from .mixer import (GatedDelta, GatedDeltaMixer, GatedNorm, PortBlock, SeqBatch,  # noqa: F401
                     ShortConv)
+from .attention import AttentionMixer, CacheAttention, KVCache  # noqa: F401
 from . import formats, gguf, synth  # noqa: F401

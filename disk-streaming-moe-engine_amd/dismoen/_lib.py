@@ -39,7 +39,8 @@ EXPORTS = (
     "dmh_upload_moe_layer_gguf", "dmh_free_layer_gguf", "dmh_moe_forward_gguf",
     "dmh_set_layer_norm", "dmh_port_moe_forward", "dmh_moe_forward_noalloc",
     "dmh_set_spin_limit", "dmh_sync_fallbacks", "dmh_xcd_rotation", "dmh_short_conv_forward",
-    "dmh_gated_delta_forward", "dmh_gated_norm_forward",
+    "dmh_gated_delta_forward", "dmh_gated_norm_forward", "dmh_kv_write", "dmh_kv_read",
+    "dmh_attention_forward",
 )
 
 
@@ -105,6 +106,24 @@ class DmhGatedNorm(C.Structure):
                 + [(n, C.c_int64) for n in ("x_stride", "gate_stride", "residual_stride",
                                             "stream_stride", "y_stride")]
                 + [(n, C.c_void_p) for n in ("gamma", "edge_gamma", "scale_vec")])
+
+
+class DmhKvCache(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("kv_heads", "dim", "page_size", "num_pages", "max_pages")]
+                + [(n, C.c_void_p) for n in ("codes", "scales", "pages", "past")])
+
+
+class DmhKvRows(C.Structure):
+    _fields_ = ([("dtype", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p)]
+                + [(n, C.c_int64) for n in ("k_stride", "k_head_stride", "v_stride",
+                                            "v_head_stride")])
+
+
+class DmhAttention(C.Structure):
+    _fields_ = ([("dtype", C.c_int32), ("q_heads", C.c_int32), ("scale", C.c_float)]
+                + [(n, C.c_void_p) for n in ("q", "gate", "o")]
+                + [(n, C.c_int64) for n in ("q_stride", "q_head_stride", "gate_stride",
+                                            "gate_head_stride", "o_stride", "o_head_stride")])
 
 
 class DismoenError(RuntimeError):
@@ -194,6 +213,9 @@ def lib():
     L.dmh_short_conv_forward.argtypes = [vp, vp, vp, u32, vp, sz]
     L.dmh_gated_delta_forward.argtypes = [vp, vp, vp, u32, vp, sz]
     L.dmh_gated_norm_forward.argtypes = [vp, vp, u32, vp, sz]
+    for name in ("write", "read"):
+        getattr(L, "dmh_kv_" + name).argtypes = [vp, vp, vp, vp, u32, vp, sz]
+    L.dmh_attention_forward.argtypes = [vp, vp, vp, vp, u32, vp, sz]
     _lib = L
     return L
 

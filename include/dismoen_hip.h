@@ -593,6 +593,81 @@ typedef struct {
 int dmh_gated_norm_forward(dmh_ctx* ctx, const dmh_gated_norm* args, unsigned flags, char* err,
                            size_t errlen);
 
+/* ---- the full-attention layers: a cache in 4 bits, and attention over it ------------
+ * Keys and values of earlier tokens are held in pages.  Each row of a head is cut
+ * into blocks of 32 elements; a block is held as one power of two and 32 codes of 4
+ * bits (OCP MX, E2M1 with an E8M0 scale): with 2^X the smallest that leaves no
+ * |element| above 7 * 2^X, X from -120 to 125, an element is element / 2^X rounded to
+ * the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} (ties to the even code, above 6 to 6),
+ * and the scale's byte is X + 127.  A block with an element that is not finite is held
+ * as NaN (byte 255).  What the cache holds is exact in bf16 and in fp32.
+ *
+ * Page p has codes[p][0][h] and scales[p][0][h], the keys of head h at its page_size
+ * positions, and codes[p][1][h], scales[p][1][h], the values.  The order of the bytes
+ * within one of these is the library's own (dmh_kv_write writes it, the other calls
+ * read it); a page may be copied as a whole.  The positions of slot s lie in pages
+ * pages[s][0], pages[s][1], ...; past[s] is how many it held before the call's rows.
+ * Row t of a sequence with slot s is its token at position past[s] + t (fresh: at t,
+ * whatever past says).  No call changes pages or past: the caller adds a step's rows
+ * to past when all layers have had theirs, and may let slots share pages that no
+ * call writes.
+ *
+ * In device memory a sequence whose past is negative, or whose tokens are more than
+ * max_pages pages hold, is left out, and one that names a page outside [0, num_pages)
+ * where the call needs it has rows that are not valid, or not written; the next
+ * dmh_sync reports a SEQUENCE_ERROR. */
+typedef struct {
+  int32_t kv_heads;        /* 1 to 1024 */
+  int32_t dim;             /* of a head: 32, 64, 96, 128, 192 or 256 */
+  int32_t page_size;       /* positions of a page: a power of two from 16 on */
+  int32_t num_pages;
+  int32_t max_pages;       /* of a slot; max_pages * page_size at most 2^30 */
+  uint8_t* codes;          /* [num_pages][2][kv_heads][page_size][dim / 2], 16-byte aligned */
+  uint8_t* scales;         /* [num_pages][2][kv_heads][page_size][dim / 32], 16-byte aligned */
+  const int32_t* pages;    /* [num_slots][max_pages] */
+  const int32_t* past;     /* [num_slots] */
+} dmh_kv_cache;
+
+/* Rows of keys and values; strides in elements between rows and between heads.  A
+ * row's heads lie within its stride. */
+typedef struct {
+  int32_t dtype;
+  void* k;                 /* [total_tokens][kv_heads][dim] */
+  void* v;
+  int64_t k_stride, k_head_stride, v_stride, v_head_stride;
+} dmh_kv_rows;
+
+/* Rows into the cache, and out of it: the positions are those of the rows, so a batch
+ * whose sequences are all fresh reads slots from their beginning.  Two sequences of a
+ * writing call must not name one slot; k and v are not changed by it. */
+int dmh_kv_write(dmh_ctx* ctx, const dmh_kv_cache* cache, const dmh_kv_rows* rows,
+                 const dmh_seq_batch* batch, unsigned flags, char* err, size_t errlen);
+int dmh_kv_read(dmh_ctx* ctx, const dmh_kv_cache* cache, const dmh_kv_rows* rows,
+                const dmh_seq_batch* batch, unsigned flags, char* err, size_t errlen);
+
+/* Causal attention of rows over the cache, which holds their own keys and values
+ * already: the row at position p, query head h with key head h / (q_heads / kv_heads),
+ *   z_j = scale * q . k_j,   o = sum_j e^(z_j) v_j / sum_j e^(z_j),   j = 0 .. p,
+ * and where gate is set o is multiplied by sigmoid(gate).  Positions behind p do not
+ * enter, whatever they hold.  The bits of a row's result may differ with the rest of
+ * the batch, which the work on long contexts is divided over.
+ *
+ * The calls work in device memory of the context of a fixed size, kept from call to
+ * call: make one before one is captured.  Replays of graphs that one context captured
+ * must not overlap each other or its other calls. */
+typedef struct {
+  int32_t dtype;           /* of q, gate and o */
+  int32_t q_heads;         /* a multiple of kv_heads, up to 4096 */
+  float scale;             /* > 0 */
+  const void* q;           /* [total_tokens][q_heads][dim] */
+  const void* gate;        /* the same, or NULL */
+  void* o;
+  int64_t q_stride, q_head_stride, gate_stride, gate_head_stride, o_stride, o_head_stride;
+} dmh_attention;
+
+int dmh_attention_forward(dmh_ctx* ctx, const dmh_attention* args, const dmh_kv_cache* cache,
+                          const dmh_seq_batch* batch, unsigned flags, char* err, size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif
