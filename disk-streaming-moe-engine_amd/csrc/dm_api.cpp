@@ -24,6 +24,7 @@
 #include "dm_gguf.h"
 #include "dm_grouped.h"
 #include "dm_kernels.h"
+#include "dm_linear.h"
 #include "dm_layout.h"
 
 using dm::LayerDev;
@@ -289,7 +290,12 @@ struct dmh_ctx {
     bool captured = false;
   } mixer[dm::kMixerBuffers];
   std::vector<void*> mixer_held;
+  std::vector<dmh_linear*> linears;
   ~dmh_ctx() {
+    for (dmh_linear* l : linears) {
+      (void)hipFree(l->buf);
+      delete l;
+    }
     for (const MixerBuf& b : mixer)
       if (b.p) (void)hipFree(b.p);
     for (void* p : mixer_held) (void)hipFree(p);
@@ -420,6 +426,44 @@ int dm::api_mixer_begin(dmh_ctx* c, hipStream_t* st, unsigned long long** status
   *st = c->cur;
   *status = c->status + kMixerSlot;
   return DMH_OK;
+}
+
+int dm::api_upload_begin(dmh_ctx* c, hipStream_t* st, unsigned long long** vkey, char* err,
+                         size_t errlen) {
+  HIP_TRY(hipSetDevice(c->device));
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  HIP_TRY(hipStreamIsCapturing(c->cur, &cap));
+  if (cap != hipStreamCaptureStatusNone)
+    return set_err(err, errlen, DMH_ERR_INVALID_ARG,
+                   "{\"error_type\":\"CONFIG_ERROR\",\"detail\":\"weights cannot be uploaded while"
+                   " the stream is being captured\",\"stage\":\"linear\"}");
+  *st = c->cur;
+  *vkey = c->vkey;
+  return DMH_OK;
+}
+
+int dm::api_malloc(size_t bytes, void** p, char* err, size_t errlen) {
+  const hipError_t e = dev_malloc(p, bytes);
+  if (e == hipSuccess) return DMH_OK;
+  *p = nullptr;
+  (void)hipGetLastError();  // (the failed allocation is not the next launch's error)
+  return set_err(err, errlen, DMH_ERR_NO_MEMORY, "hipMalloc(%zu): %s", bytes, hipGetErrorString(e));
+}
+
+int dm::api_keep_linear(dmh_ctx* c, dmh_linear* l, char* err, size_t errlen) {
+  try {
+    c->linears.push_back(l);
+  } catch (const std::bad_alloc&) {
+    return set_err(err, errlen, DMH_ERR_NO_MEMORY, "out of host memory");
+  }
+  return DMH_OK;
+}
+
+bool dm::api_drop_linear(dmh_ctx* c, dmh_linear* l) {
+  const auto it = std::find(c->linears.begin(), c->linears.end(), l);
+  if (it == c->linears.end()) return false;
+  c->linears.erase(it);
+  return hipSetDevice(c->device) == hipSuccess;
 }
 
 int dm::api_mixer_buffer(dmh_ctx* c, MixerBuffer which, size_t bytes, void** p, char* err,

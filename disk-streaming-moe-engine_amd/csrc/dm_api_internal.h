@@ -28,6 +28,17 @@ int api_mixer_buffer(dmh_ctx* c, MixerBuffer which, size_t bytes, void** p, char
 // The text of a key that these calls recorded.
 int api_mixer_error(unsigned long long key, char* err, size_t errlen);
 
+// ---- what the linear layers' entry points (dm_linear_api.cpp) use besides --------
+// Makes the context's device current for an upload, which a capture cannot hold; its
+// stream and the word that checks of weights report to.
+int api_upload_begin(dmh_ctx* c, hipStream_t* st, unsigned long long** vkey, char* err,
+                     size_t errlen);
+// Device memory on the current device.
+int api_malloc(size_t bytes, void** p, char* err, size_t errlen);
+// The context's linear layers, which end with it at the latest.
+int api_keep_linear(dmh_ctx* c, dmh_linear* l, char* err, size_t errlen);
+bool api_drop_linear(dmh_ctx* c, dmh_linear* l);
+
 }  // namespace dm
 
 #endif

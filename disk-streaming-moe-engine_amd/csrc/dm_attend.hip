@@ -478,7 +478,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendDev d) {
 
   int64_t total = count(0);
   for (int i0 = 256; i0 < d.s.num; i0 += 256) total += count(i0);
-  const int groups = (int)min<int64_t>(gridDim.x, total);
+  const int groups = (int)least(gridDim.x, total);
   if (group >= groups) return;
   const int64_t lo = share_at(total, groups, group), hi = share_at(total, groups, group + 1);
   int64_t base = 0, at = lo;
@@ -499,7 +499,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendDev d) {
       const int unit = (int)((at - first) / tiles);
       const int64_t unit_at = first + (int64_t)unit * tiles;
       const int h = unit / blocks, block = unit - h * blocks;
-      const int ta = (int)(at - unit_at), tb = (int)min<int64_t>(tiles, hi - unit_at);
+      const int ta = (int)(at - unit_at), tb = (int)least(tiles, hi - unit_at);
 
       W w;
       w.begin(d, q, h, block * ROWS);
@@ -674,7 +674,7 @@ __global__ __launch_bounds__(256) void k_attend_many(AttendDev d) {
   if (row0 >= rows) return;
   W w;
   w.begin(d, q, h, (int)row0);
-  const int last = (int)((min(row0 + 16 * MT, rows) - 1) / d.rep);
+  const int last = (int)((least(row0 + 16 * MT, rows) - 1) / d.rep);
   w.run(d, 0, q.past + last + 1, kStep, q.past + (int)(row0 / d.rep));
   if (w.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)seq, kSqPage));
   const int n = lane & 15, quad = lane >> 4;

@@ -9,6 +9,9 @@
 
 namespace dm {
 
+// (HIP's min of a 64-bit and a 32-bit integer is a double)
+__device__ __forceinline__ int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
+
 // ---- row types ----------------------------------------------------------------
 typedef _Float16 half_t;
 typedef __bf16 bf16_t;

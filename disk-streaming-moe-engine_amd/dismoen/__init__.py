@@ -8,4 +8,5 @@ from .layers import MoEBlock, RouterConfig, RoutingInfo  # noqa: F401
 from .mixer import (GatedDelta, GatedDeltaMixer, GatedNorm, PortBlock, SeqBatch,  # noqa: F401
                     ShortConv)
 from .attention import AttentionMixer, CacheAttention, KVCache  # noqa: F401
+from .linear import QuantLinear  # noqa: F401
 from . import formats, gguf, synth  # noqa: F401

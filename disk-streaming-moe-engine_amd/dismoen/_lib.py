@@ -40,7 +40,7 @@ EXPORTS = (
     "dmh_set_layer_norm", "dmh_port_moe_forward", "dmh_moe_forward_noalloc",
     "dmh_set_spin_limit", "dmh_sync_fallbacks", "dmh_xcd_rotation", "dmh_short_conv_forward",
     "dmh_gated_delta_forward", "dmh_gated_norm_forward", "dmh_kv_write", "dmh_kv_read",
-    "dmh_attention_forward",
+    "dmh_attention_forward", "dmh_upload_linear", "dmh_free_linear", "dmh_linear_forward",
 )
 
 
@@ -124,6 +124,17 @@ class DmhAttention(C.Structure):
                 + [(n, C.c_void_p) for n in ("q", "gate", "o")]
                 + [(n, C.c_int64) for n in ("q_stride", "q_head_stride", "gate_stride",
                                             "gate_head_stride", "o_stride", "o_head_stride")])
+
+
+class DmhLinearWeights(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("out_features", "in_features", "group_size")]
+                + [(n, C.c_void_p) for n in ("scales", "packed", "bias")])
+
+
+class DmhLinearRows(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "out_dtype", "rows")]
+                + [("x", C.c_void_p), ("x_stride", C.c_int64), ("y", C.c_void_p),
+                   ("y_stride", C.c_int64)])
 
 
 class DismoenError(RuntimeError):
@@ -216,6 +227,9 @@ def lib():
     for name in ("write", "read"):
         getattr(L, "dmh_kv_" + name).argtypes = [vp, vp, vp, vp, u32, vp, sz]
     L.dmh_attention_forward.argtypes = [vp, vp, vp, vp, u32, vp, sz]
+    L.dmh_upload_linear.argtypes = [vp, vp, u32, C.POINTER(vp), C.c_char_p, sz]
+    L.dmh_free_linear.argtypes = [vp, vp]
+    L.dmh_linear_forward.argtypes = [vp, vp, vp, u32, vp, sz]
     _lib = L
     return L
 

@@ -668,6 +668,43 @@ typedef struct {
 int dmh_attention_forward(dmh_ctx* ctx, const dmh_attention* args, const dmh_kv_cache* cache,
                           const dmh_seq_batch* batch, unsigned flags, char* err, size_t errlen);
 
+/* ---- linear layers with 4-bit weights ------------------------------------------------
+ * The projections around both kinds of mixer, and the model's head: y = W x + bias with
+ * W [out_features][in_features] in the quant model's layout (fp16 scales, then packed
+ * codes, groups along in_features), each weight the bf16 value that dmh_dequant_q4_bf16
+ * gives.  dmh_upload_linear copies and re-tiles the weights once (they may be freed when
+ * it returns) and refuses what dequantising refuses, with its text.  The handle is the
+ * context's: dmh_free_linear or dmh_destroy ends it.  flags: DMH_F_DEVICE, the arrays
+ * are device memory, whose writes the caller has waited for. */
+typedef struct dmh_linear dmh_linear;
+typedef struct {
+  int32_t out_features;    /* 1 to 2^24 */
+  int32_t in_features;     /* a multiple of group_size, up to 2^20 */
+  int32_t group_size;      /* 32, 64, 128 or 256 */
+  const uint16_t* scales;  /* [out_features * in_features / group_size] fp16 bits */
+  const uint8_t* packed;   /* [out_features * in_features / 2] */
+  const float* bias;       /* [out_features], or NULL */
+} dmh_linear_weights;
+
+int dmh_upload_linear(dmh_ctx* ctx, const dmh_linear_weights* w, unsigned flags, dmh_linear** out,
+                      char* err, size_t errlen);
+int dmh_free_linear(dmh_ctx* ctx, dmh_linear* linear);
+
+/* Rows x [rows][in_features] of dtype to y [rows][out_features] of out_dtype (dtype or
+ * DMH_DTYPE_F32).  Products are exact, sums fp32, and y is rounded once; strides are in
+ * elements between rows. */
+typedef struct {
+  int32_t dtype, out_dtype;
+  int32_t rows;
+  const void* x;
+  int64_t x_stride;
+  void* y;
+  int64_t y_stride;
+} dmh_linear_rows;
+
+int dmh_linear_forward(dmh_ctx* ctx, const dmh_linear* linear, const dmh_linear_rows* rows,
+                       unsigned flags, char* err, size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,159 @@
+"""Linear layers with 4-bit weights, against 64-bit products with the dequantiser's weights.
+
+Tolerance: half a step of the output's type, plus roundings of 2^-24 of the sum of the
+products' sizes: products are exact, a sum is taken 32 columns at a time (at most 6
+roundings each) and over at most 8192 / 32 of these, in up to 16 waves and joined: 8 for
+each part of x (of at most three) and each 128 columns of a wave's share cover sums that
+grow one way; random ones stay far below.  STEPS counts 256 sums of one rounding each and
+their inner 6, times three parts, at the largest size tested here (k of 4224: 132 sums)."""
+import zlib
+
+import numpy as np
+import pytest
+import torch
+
+import mixer_ref as M
+from dismoen import DismoenError, QuantLinear
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def gen(*seed):
+    return torch.Generator().manual_seed(zlib.crc32(repr(seed).encode()))
+
+
+def weights(g, n, k, group):
+    q = torch.randint(-7, 8, (n, k), generator=g)
+    scales = (torch.rand(n * k // group, generator=g) * 0.01 + 1e-3).half()
+    flat = (q & 15).flatten().to(torch.uint8)
+    packed = flat[0::2] | (flat[1::2] << 4)
+    w = (q.view(n, -1, group).float() * scales.float().view(n, -1, 1)).bfloat16().double()
+    return w.view(n, k), scales, packed
+
+
+def check(got, x, w, bias, k):
+    xd = x.double().cpu()
+    want = xd @ w.T
+    size = xd.abs() @ w.abs().T
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    parts = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}[x.dtype]
+    M.close(got, want, size, parts * (k / 32 + 8) + 8)
+
+
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("n,k,group", [(1, 32, 32), (16, 128, 128), (17, 96, 32), (50, 320, 64),
+                                       (515, 4224, 32), (2048, 256, 256), (129, 1024, 128)])
+@pytest.mark.parametrize("rows", [1, 3, 16, 17, 33, 64, 65, 200])
+def test_linear(block, rows, n, k, group, t):
+    g = gen(n, k, rows)
+    w, scales, packed = weights(g, n, k, group)
+    bias = torch.randn(n, generator=g) if rows % 2 else None
+    x = torch.randn((rows, k), generator=g).to(t)
+    lin = QuantLinear(block, n, k, scales.cuda(), packed.cuda(), group,
+                      bias=None if bias is None else bias.cuda())
+    for out in {t, torch.float32}:
+        # strided rows: x from a wider projection, y into one
+        wide = torch.full((rows + 1, k + 40), float("nan"), dtype=t, device="cuda")
+        wide[:rows, 8:8 + k] = x
+        y = torch.full((rows + 1, n + 5), 3.0, dtype=out, device="cuda")
+        torch.cuda.synchronize()
+        assert lin(wide[:rows, 8:8 + k], y[:rows, 2:2 + n]) is not None
+        block.sync()
+        check(y[:rows, 2:2 + n], x, w, bias, k)
+        assert (y[rows:] == 3).all() and (y[:, :2] == 3).all() and (y[:, 2 + n:] == 3).all()
+    lin.close()
+
+
+def test_rows_of_many_tiles(block):
+    """Many rows of x through a layer of many rows and an odd size."""
+    g = gen("many")
+    n, k, rows = 1111, 544, 1300
+    w, scales, packed = weights(g, n, k, 32)
+    lin = QuantLinear(block, n, k, scales.cuda(), packed.cuda(), 32)
+    for t in TYPES.values():
+        x = torch.randn((rows, k), generator=g).to(t).cuda()
+        y = torch.empty(rows, n, dtype=t, device="cuda")
+        torch.cuda.synchronize()
+        lin(x, y)
+        block.sync()
+        check(y, x, w, None, k)
+
+
+def test_rows_do_not_meet(block):
+    """A row that is not finite makes its own results so, and no other's."""
+    g = gen("nan")
+    w, scales, packed = weights(g, 64, 256, 64)
+    lin = QuantLinear(block, 64, 256, scales.cuda(), packed.cuda(), 64)
+    for rows in (5, 40, 300):
+        x = torch.randn((rows, 256), generator=g).bfloat16()
+        clean, x[2, 100] = x.clone(), float("nan")
+        y, z = (torch.empty(rows, 64, device="cuda") for _ in range(2))
+        a, b = x.cuda(), clean.cuda()
+        torch.cuda.synchronize()
+        lin(a, y)
+        lin(b, z)
+        block.sync()
+        assert y[2].isnan().all()
+        keep = [i for i in range(rows) if i != 2]
+        assert torch.equal(y[keep], z[keep])
+
+
+def test_host_arrays(block):
+    """numpy weights and rows give the device's bits."""
+    g = gen("host")
+    n, k, rows = 70, 160, 9
+    w, scales, packed = weights(g, n, k, 32)
+    bias = torch.randn(n, generator=g)
+    x = torch.randn((rows, k), generator=g)
+    y = torch.empty(rows, n, device="cuda")
+    xd = x.cuda()
+    dev = QuantLinear(block, n, k, scales.cuda(), packed.cuda(), 32, bias=bias.cuda())
+    torch.cuda.synchronize()
+    dev(xd, y)
+    block.sync()
+    host = QuantLinear(block, n, k, scales.numpy(), packed.numpy(), 32, bias=bias.numpy())
+    out = np.full((rows, n), 2, np.float32)
+    host(x.numpy(), out)
+    assert np.array_equal(out, y.cpu().numpy())
+
+
+def test_refused_weights(block):
+    """What the dequantiser refuses, the upload refuses with its text."""
+    g = gen("bad")
+    _, scales, packed = weights(g, 8, 64, 32)
+    bad = packed.clone()
+    bad[100] = 0x18
+    def changed(i, v):
+        s = scales.clone()
+        s[i] = v
+        return s
+
+    for s, p, text in ((scales, bad, "reserved nibble"),
+                       (changed(5, 0.0), packed, "non-positive at group 5"),
+                       (changed(3, float("inf")), packed, "NaN or Inf at group 3"),
+                       (changed(7, -1.0), packed, "non-positive at group 7")):
+        with pytest.raises(DismoenError, match=text) as e:
+            QuantLinear(block, 8, 64, s.numpy(), p.numpy(), 32)
+        assert e.value.code == 5
+    QuantLinear(block, 8, 64, scales.numpy(), packed.numpy(), 32).close()
+
+
+def test_from_a_quant_model(block, tmp_path):
+    from dismoen import formats
+    g = gen("file")
+    w, scales, packed = weights(g, 96, 128, 32)
+    path = str(tmp_path / "model.bin")
+    formats.write_quant_file(path, "m", [("a.weight", [96, 128], scales.numpy().view(np.uint16),
+                                          packed.numpy())], 32)
+    with formats.scan_quant_file(path) as index:
+        lin = QuantLinear.from_quant_model(block, index, "a.weight")
+        with pytest.raises(DismoenError, match="not in the quant model"):
+            QuantLinear.from_quant_model(block, index, "b.weight")
+    x, y = torch.randn((4, 128), generator=g).cuda(), torch.empty(4, 96, device="cuda")
+    torch.cuda.synchronize()
+    lin(x, y)
+    block.sync()
+    check(y, x, w, None, 128)
