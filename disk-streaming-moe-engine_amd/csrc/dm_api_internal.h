@@ -22,7 +22,7 @@ int api_mixer_begin(dmh_ctx* c, hipStream_t* st, unsigned long long** status, ch
 // Device memory of the context, kept and grown from call to call.  A buffer
 // whose address a captured graph holds is not freed when it grows, and none is
 // made while the stream is being captured (DMH_ERR_INVALID_ARG).
-enum MixerBuffer { kMixerStage, kMixerChunks, kMixerParts, kMixerBuffers };
+enum MixerBuffer { kMixerStage, kMixerChunks, kMixerParts, kMixerSplit, kMixerBuffers };
 int api_mixer_buffer(dmh_ctx* c, MixerBuffer which, size_t bytes, void** p, char* err,
                      size_t errlen);
 // The text of a key that these calls recorded.

@@ -103,68 +103,298 @@ __device__ __forceinline__ void store_out(const LinearDev& l, const dmh_linear_r
 }
 
 // ---- few rows -------------------------------------------------------------------------
-// A workgroup takes 16 rows of W and 16 NT rows of x; its waves take W's chunks of 128
-// columns in turn and add up through LDS.  Bound by W's bytes.
-template <typename T, typename O, int NT, int WAVES>
+// A workgroup takes 16 AT rows of W and 16 NT rows of x; its waves take W's chunks of 128
+// columns in turn, one of them on its way ahead of the products, and add up through LDS.
+// Bound by W's bytes.
+template <typename T, typename O, int AT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinearDev l, dmh_linear_rows r) {
   constexpr int P = parts_of<T>();
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rb = blockIdx.x;
+  const int rb0 = blockIdx.x * AT;
   const int64_t t0 = (int64_t)blockIdx.y * (16 * NT);
   const T* x[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
     x[i] = static_cast<const T*>(r.x) + least(t0 + 16 * i + n, r.rows - 1) * r.x_stride + 8 * quad;
-  const uint8_t* const nib = l.nib + a16_nib_offset(l.chunks, rb, 0, lane);
-  const uint16_t* const sc = l.sc + a16_sc_offset(l.chunks, rb, 0, n);
-  f32x4 acc[NT] = {};
+  const uint8_t* nib[AT];
+  const uint16_t* sc[AT];
+#pragma unroll
+  for (int j = 0; j < AT; ++j) {
+    const int rb = min(rb0 + j, l.row_blocks - 1);
+    nib[j] = l.nib + a16_nib_offset(l.chunks, rb, 0, lane);
+    sc[j] = l.sc + a16_sc_offset(l.chunks, rb, 0, n);
+  }
+  uint4 w[AT];
+  uint2 s[AT];
+  const auto load = [&](size_t g) {
+#pragma unroll
+    for (int j = 0; j < AT; ++j) {
+      w[j] = *reinterpret_cast<const uint4*>(nib[j] + g * 1024);
+      s[j] = *reinterpret_cast<const uint2*>(sc[j] + g * 64);
+    }
+  };
+  f32x4 acc[AT][NT] = {};
+  if (wave < l.chunks) load(wave);
   for (int g = wave; g < l.chunks; g += WAVES) {
-    const uint4 w4 = *reinterpret_cast<const uint4*>(nib + (size_t)g * 1024);
-    const uint2 s2 = *reinterpret_cast<const uint2*>(sc + (size_t)g * 64);
-    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-    const uint32_t s[4] = {s2.x & 0xFFFFu, s2.x >> 16, s2.y & 0xFFFFu, s2.y >> 16};
+    uint4 wn[AT];
+    uint2 sn[AT];
+#pragma unroll
+    for (int j = 0; j < AT; ++j) {
+      wn[j] = w[j];
+      sn[j] = s[j];
+    }
+    load(min(g + WAVES, l.chunks - 1));
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int col = g * kQuadCols + c * kGroup;
       if (col >= l.k) break;
-      const bf16x8 a = dequant8(w[c], fp16_bits_to_f32(s[c]));
+      bf16x8 b[NT][P];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        bf16x8 b[P];
-        load_parts<T, P>(x[i] + col, b);
+      for (int i = 0; i < NT; ++i) load_parts<T, P>(x[i] + col, b[i]);
 #pragma unroll
-        for (int p = 0; p < P; ++p) acc[i] = mfma16(a, b[p], acc[i]);
+      for (int j = 0; j < AT; ++j) {
+        const uint32_t word = c == 0 ? wn[j].x : c == 1 ? wn[j].y : c == 2 ? wn[j].z : wn[j].w;
+        const uint32_t half = c < 2 ? sn[j].x : sn[j].y;
+        const bf16x8 a = dequant8(word, fp16_bits_to_f32(c % 2 ? half >> 16 : half & 0xFFFFu));
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int p = 0; p < P; ++p) acc[j][i] = mfma16(a, b[i][p], acc[j][i]);
       }
     }
   }
-  __shared__ f32x4 red[WAVES][NT][64];
+  __shared__ f32x4 red[WAVES][AT][NT][64];
   // (a product's result is read some cycles after its issue, which the compiler does not
   // count over the end of a loop)
 #pragma unroll
-  for (int i = 0; i < NT; ++i) asm volatile("s_nop 7\n\ts_nop 7" : "+v"(acc[i]));
+  for (int j = 0; j < AT; ++j)
 #pragma unroll
-  for (int i = 0; i < NT; ++i) red[wave][i][lane] = acc[i];
+    for (int i = 0; i < NT; ++i) {
+      asm volatile("s_nop 7\n\ts_nop 7" : "+v"(acc[j][i]));
+      red[wave][j][i][lane] = acc[j][i];
+    }
   __syncthreads();
-  for (int i = wave; i < NT; i += WAVES) {
-    f32x4 v = red[0][i][lane];
+  for (int i = wave; i < AT * NT; i += WAVES) {
+    f32x4 v = red[0][i / NT][i % NT][lane];
 #pragma unroll
-    for (int k = 1; k < WAVES; ++k) v += red[k][i][lane];
-    store_out<O>(l, r, t0 + 16 * i + n, rb * kTileRows + 4 * quad, v);
+    for (int k = 1; k < WAVES; ++k) v += red[k][i / NT][i % NT][lane];
+    store_out<O>(l, r, t0 + 16 * (i % NT) + n, (rb0 + i / NT) * kTileRows + 4 * quad, v);
   }
 }
 
+// ---- many rows --------------------------------------------------------------------------
+// A workgroup takes 64 AT rows of W and 16 BT rows of x.  Each of its four waves has
+// 16 AT rows of W of its own, whose codes it makes into operands once, and all rows of
+// x, 128 columns of which pass through LDS at a time by direct loads, one stage ahead.
+// Segment s (16 bytes) of row t lies at s ^ (t % 16), so that the 16 rows of an operand
+// lie in different banks.  Bound by the matrix cores.
+template <typename O, int AT, int BT>
+__global__ __launch_bounds__(256, 2) void k_linear_many(LinearDev l, dmh_linear_rows r,
+                                                        const uint16_t* __restrict__ xb,
+                                                        int64_t x_stride, int64_t part_stride,
+                                                        int parts, int wtiles, int ttiles) {
+  constexpr int ROWS = 16 * BT, STAGE = ROWS * 256;
+  __shared__ __align__(16) uint8_t lds[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // workgroups come to the XCDs in turn: each gets a run of tiles, rows of x fastest
+  const int all = wtiles * ttiles, per = (all + 7) / 8;
+  const int tile = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+  if ((int)(blockIdx.x / 8) >= per || tile >= all) return;
+  const int wt = tile / ttiles, tt = tile - wt * ttiles;
+  const int rb0 = (wt * 4 + wave) * AT;
+  const int64_t t0 = (int64_t)tt * ROWS;
+
+  // steps: the whole chunks of each part, then the last ones that are not whole
+  const int whole = l.k / kQuadCols, steps = whole * parts;
+  const int all_steps = l.chunks * parts;
+  const auto chunk_of = [&](int step) { return step < steps ? step % whole : whole; };
+  const auto part_of = [&](int step) { return step < steps ? step / whole : step - steps; };
+
+  // this lane's part of a stage: 16 bytes of every fourth row
+  const uint32_t base = lds_u32(lds);
+  const auto fetch = [&](int step, int buf) {
+    const int g = chunk_of(step);
+    const uint16_t* const x = xb + part_of(step) * part_stride + g * kQuadCols;
+#pragma unroll
+    for (int i = 0; i < BT; ++i) {
+      const int row = 16 * i + 4 * wave + quad;  // a wave brings 4 rows, 256 bytes each
+      const int seg = n ^ (row & 15);
+      // (columns behind the last are not used; they are read from the row itself)
+      const int col = min(8 * seg, l.k - 8 - g * kQuadCols);
+      dma16_lds(x + least(t0 + row, r.rows - 1) * x_stride + col,
+                base + buf * STAGE + (16 * i + 4 * wave) * 256);
+    }
+  };
+  const uint8_t* nib[AT];
+  const uint16_t* sc[AT];
+#pragma unroll
+  for (int a = 0; a < AT; ++a) {
+    const int rb = min(rb0 + a, l.row_blocks - 1);
+    nib[a] = l.nib + a16_nib_offset(l.chunks, rb, 0, lane);
+    sc[a] = l.sc + a16_sc_offset(l.chunks, rb, 0, n);
+  }
+  uint4 w[AT];
+  uint2 s[AT];
+  f32x4 acc[AT][BT] = {};
+  const auto weights = [&](int step) {
+    const size_t g = chunk_of(step);
+#pragma unroll
+    for (int a = 0; a < AT; ++a) {
+      w[a] = *reinterpret_cast<const uint4*>(nib[a] + g * 1024);
+      s[a] = *reinterpret_cast<const uint2*>(sc[a] + g * 64);
+    }
+  };
+  // Brings the next step on its way and does this one's `groups` of 32 columns.
+  const auto go = [&](int i, int groups) {
+    uint4 wn[AT];
+    uint2 sn[AT];
+#pragma unroll
+    for (int a = 0; a < AT; ++a) {
+      wn[a] = w[a];
+      sn[a] = s[a];
+    }
+    wait_vm();
+    __syncthreads();
+    if (i + 1 < all_steps) {
+      fetch(i + 1, (i + 1) & 1);
+      weights(i + 1);
+    }
+    const uint8_t* const x = lds + (i & 1) * STAGE;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (c >= groups) break;
+      bf16x8 a[AT], b[BT];
+#pragma unroll
+      for (int j = 0; j < BT; ++j)
+        b[j] = *reinterpret_cast<const bf16x8*>(x + (16 * j + n) * 256 + ((4 * c + quad) ^ n) * 16);
+#pragma unroll
+      for (int j = 0; j < AT; ++j) {
+        const uint32_t word = c == 0 ? wn[j].x : c == 1 ? wn[j].y : c == 2 ? wn[j].z : wn[j].w;
+        const uint32_t half = c < 2 ? sn[j].x : sn[j].y;
+        a[j] = dequant8(word, fp16_bits_to_f32(c % 2 ? half >> 16 : half & 0xFFFFu));
+      }
+#pragma unroll
+      for (int j = 0; j < AT; ++j)
+#pragma unroll
+        for (int k = 0; k < BT; ++k) acc[j][k] = mfma16(a[j], b[k], acc[j][k]);
+    }
+  };
+  fetch(0, 0);
+  weights(0);
+  for (int i = 0; i < steps; ++i) go(i, 4);
+  for (int i = steps; i < all_steps; ++i) go(i, (l.k - whole * kQuadCols) / kGroup);
+#pragma unroll
+  for (int j = 0; j < AT; ++j)
+#pragma unroll
+    for (int k = 0; k < BT; ++k) asm volatile("" : "+v"(acc[j][k]));
+  asm volatile("s_nop 7\n\ts_nop 7" : "+v"(acc[0][0]));
+#pragma unroll
+  for (int j = 0; j < AT; ++j) {
+    if (rb0 + j >= l.row_blocks) break;
+#pragma unroll
+    for (int k = 0; k < BT; ++k) {
+      asm volatile("" : "+v"(acc[j][k]));
+      store_out<O>(l, r, t0 + 16 * k + n, (rb0 + j) * kTileRows + 4 * quad, acc[j][k]);
+    }
+  }
+}
+
+// Rows of x as bf16 parts, [parts][rows][k].
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_split(const T* x, int64_t stride, int k, int64_t rows,
+                                                      uint16_t* out) {
+  constexpr int P = parts_of<T>();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = k / 8;
+  if (i >= rows * per) return;
+  const int64_t row = i / per;
+  const int col = (int)(i - row * per) * 8;
+  bf16x8 p[P];
+  load_parts<T, P>(x + row * stride + col, p);
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+    *reinterpret_cast<bf16x8*>(out + (j * rows + row) * k + col) = p[j];
+}
+
+template <typename T>
+bool direct(const dmh_linear_rows& r) {  // whether the kernel can bring x into LDS as it is
+  return std::is_same<T, bf16_t>::value && (uintptr_t)r.x % 16 == 0 && r.x_stride % 8 == 0;
+}
+
 template <typename T, typename O>
-hipError_t run(const LinearDev& l, const dmh_linear_rows& r, hipStream_t st) {
-  const auto few = [&](auto nt) {
-    constexpr int NT = decltype(nt)::value;
-    const dim3 grid(l.row_blocks, (r.rows + 16 * NT - 1) / (16 * NT));
-    k_linear_few<T, O, NT, 4><<<grid, 256, 0, st>>>(l, r);
+hipError_t many(const LinearDev& l, const dmh_linear_rows& r, void* ws, hipStream_t st) {
+  constexpr int P = parts_of<T>();
+  const uint16_t* xb = static_cast<const uint16_t*>(r.x);
+  int64_t x_stride = r.x_stride;
+  if (!direct<T>(r)) {
+    const int64_t n = (int64_t)r.rows * (l.k / 8);
+    uint16_t* const out = static_cast<uint16_t*>(ws);
+    k_linear_split<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(static_cast<const T*>(r.x),
+                                                                  r.x_stride, l.k, r.rows, out);
+    xb = out;
+    x_stride = l.k;
+  }
+  const auto go = [&](auto at, auto bt) {
+    constexpr int AT = decltype(at)::value, BT = decltype(bt)::value;
+    const int wt = (l.row_blocks + 4 * AT - 1) / (4 * AT);
+    const int tt = (r.rows + 16 * BT - 1) / (16 * BT);
+    const unsigned blocks = (unsigned)(((int64_t)wt * tt + 7) / 8 * 8);
+    k_linear_many<O, AT, BT><<<blocks, 256, 0, st>>>(l, r, xb, x_stride, r.rows * x_stride, P, wt, tt);
+  };
+  // Tiles of 192 by 128 take the least from memory for their products, as long as there
+  // are enough of them; 128 by 64 fill the device sooner.  9216 x 2048, 512, 1024 and
+  // 2048 rows: 33, 51 and 88 us with the large ones, 35, 57 and 106 with the small; 2048
+  // x 4096, 1024 rows (88 large tiles): 55 and 32.
+  using std::integral_constant;
+  const int64_t large = (int64_t)((l.row_blocks + 11) / 12) * ((r.rows + 127) / 128);
+  if (large >= 192) go(integral_constant<int, 3>{}, integral_constant<int, 8>{});
+  else go(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+  return hipGetLastError();
+}
+
+// Tiles of 16 by 16 outputs.
+int64_t units(const LinearDev& l, const dmh_linear_rows& r) {
+  return (int64_t)l.row_blocks * ((r.rows + 15) / 16);
+}
+// Up to how many of them waves without LDS in between are the faster: 2048 x 4096 at 512
+// rows (4096 tiles) 22 us, and 31 through LDS; 9216 x 2048 at 128 (4608) 18.9 and 18.0, at
+// 256 (9216) 30 and 24.  32 rows and fewer are bound by W's bytes, which they read once.
+bool few_rows(const LinearDev& l, const dmh_linear_rows& r) {
+  return r.rows <= 32 || units(l, r) <= 4608;
+}
+
+template <typename T, typename O>
+hipError_t run(const LinearDev& l, const dmh_linear_rows& r, void* ws, hipStream_t st) {
+  if (!few_rows(l, r)) return many<T, O>(l, r, ws, st);
+  const auto few = [&](auto at, auto nt, auto waves) {
+    constexpr int AT = decltype(at)::value, NT = decltype(nt)::value, W = decltype(waves)::value;
+    const dim3 grid((l.row_blocks + AT - 1) / AT, (r.rows + 16 * NT - 1) / (16 * NT));
+    k_linear_few<T, O, AT, NT, W><<<grid, 64 * W, 0, st>>>(l, r);
     return hipGetLastError();
   };
-  if (r.rows <= 16) return few(std::integral_constant<int, 1>{});
-  if (r.rows <= 32) return few(std::integral_constant<int, 2>{});
-  return few(std::integral_constant<int, 4>{});
+  using std::integral_constant;
+  const integral_constant<int, 1> one{};
+  const integral_constant<int, 2> two{};
+  const integral_constant<int, 4> four{};
+  const integral_constant<int, 8> eight{};
+  // More tiles to a workgroup reuse what is loaded and dequantised, more workgroups and
+  // waves load sooner.  One row: 2048 x 4096 4.3 us with 16 waves and 4.7 with 8, 9216 x
+  // 2048 5.7 with 8 and 6.5 with two tiles; five rows of 100000 x 2048 32 us with two
+  // tiles and 41 with one.  32 rows of 2048 x 4096 6.9 us with one tile, 7.4 with two; 64
+  // rows 7.6 with two, 11.0 with one; 128 rows 10.1 with four, 12.4 with two; of 9216 x
+  // 2048 32 rows 8.6 with four times two, 64 rows 13.0, with one 17.
+  const int64_t u = units(l, r);
+  if (r.rows <= 16) {
+    if (l.row_blocks < 256) return few(one, one, integral_constant<int, 16>{});
+    if (l.row_blocks < 1024) return few(one, one, eight);
+    return few(two, one, four);
+  }
+  if (u < 512) return few(one, one, eight);
+  if (u < 1024) return few(two, one, eight);
+  if (u < 2048) return r.rows <= 32 ? few(four, two, eight) : few(four, one, eight);
+  return few(four, two, four);
 }
 
 }  // namespace
@@ -178,11 +408,20 @@ hipError_t launch_linear_pack(const uint16_t* scales, const uint8_t* packed, int
   return hipGetLastError();
 }
 
-hipError_t launch_linear(const LinearDev& l, const dmh_linear_rows& r, hipStream_t st) {
+size_t linear_bytes(const LinearDev& l, const dmh_linear_rows& r) {
+  if (few_rows(l, r)) return 0;
+  const size_t n = (size_t)r.rows * l.k * 2;
+  if (r.dtype == DMH_DTYPE_F32) return parts_of<float>() * n;
+  if (r.dtype == DMH_DTYPE_F16) return parts_of<half_t>() * n;
+  return direct<bf16_t>(r) ? 0 : n;
+}
+
+hipError_t launch_linear(const LinearDev& l, const dmh_linear_rows& r, void* ws, hipStream_t st) {
   const bool f32 = r.out_dtype == DMH_DTYPE_F32;
-  if (r.dtype == DMH_DTYPE_F32) return run<float, float>(l, r, st);
-  if (r.dtype == DMH_DTYPE_F16) return f32 ? run<half_t, float>(l, r, st) : run<half_t, half_t>(l, r, st);
-  return f32 ? run<bf16_t, float>(l, r, st) : run<bf16_t, bf16_t>(l, r, st);
+  if (r.dtype == DMH_DTYPE_F32) return run<float, float>(l, r, ws, st);
+  if (r.dtype == DMH_DTYPE_F16)
+    return f32 ? run<half_t, float>(l, r, ws, st) : run<half_t, half_t>(l, r, ws, st);
+  return f32 ? run<bf16_t, float>(l, r, ws, st) : run<bf16_t, bf16_t>(l, r, ws, st);
 }
 
 }  // namespace dm

@@ -130,8 +130,11 @@ int dmh_linear_forward(dmh_ctx* c, const dmh_linear* l, const dmh_linear_rows* r
     stage.add_out(r.y, y);
     if ((rc = stage.in(c, st, check, err))) return rc;
   }
+  void* ws = nullptr;
+  const size_t need = linear_bytes(l->dev, r);
+  if (need && (rc = api_mixer_buffer(c, kMixerSplit, need, &ws, errp, errlen))) return rc;
   if (check) return DMH_OK;
-  const hipError_t e = launch_linear(l->dev, r, st);
+  const hipError_t e = launch_linear(l->dev, r, ws, st);
   if (e != hipSuccess) return err.hip(e);
   return dev ? DMH_OK : stage.out(st, err);
 }

@@ -67,10 +67,11 @@ def test_linear(block, rows, n, k, group, t):
     lin.close()
 
 
-def test_rows_of_many_tiles(block):
-    """Many rows of x through a layer of many rows and an odd size."""
+@pytest.mark.parametrize("n,k,rows", [(1111, 544, 1300), (2401, 160, 2500), (33000, 64, 30),
+                                      (1024, 96, 40), (1024, 128, 33), (4100, 32, 25)])
+def test_rows_of_many_tiles(block, n, k, rows):
+    """Many rows of x, and layers of many rows, of odd sizes."""
     g = gen("many")
-    n, k, rows = 1111, 544, 1300
     w, scales, packed = weights(g, n, k, 32)
     lin = QuantLinear(block, n, k, scales.cuda(), packed.cuda(), 32)
     for t in TYPES.values():
