@@ -137,13 +137,73 @@ __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&out)[PARTS])
   }
 }
 
-// The codes and scales of a step, as they come.
+// Where a unit's bytes lie.  All of it is the same in a wave: addresses are a scalar base
+// and the lane's own 32 bits.
 template <int NB>
-struct Held {
-  static constexpr int VS = CacheLay<NB>::pow2 ? 1 : NB;
-  uint32_t k[2][NB], v[2][NB], ks[2][(NB + 3) / 4], vs[2][VS];
+struct Unit {
+  const uint8_t *codes, *scales;
+  const int32_t* table;  // the slot's pages
+  size_t page_bytes, head_bytes, value_bytes;  // of codes; scales have a 16th
+  int shift, num_pages, len;
+  bool bad;  // a page was not one of the cache's
+  __device__ __forceinline__ void begin(const AttendDev& d, const CacheSeq& s, int h) {
+    codes = d.c.codes;
+    scales = d.c.scales;
+    table = d.c.pages + (int64_t)s.slot * d.c.max_pages;
+    shift = d.c.page_shift;
+    value_bytes = ((size_t)d.c.heads << shift) * (16 * NB);
+    page_bytes = 2 * value_bytes;
+    head_bytes = ((size_t)h << shift) * (16 * NB);
+    num_pages = d.c.num_pages;
+    len = s.past + s.n;
+    bad = false;
+  }
+  __device__ __forceinline__ int page(int t) const {  // of a uniform position
+    return __builtin_amdgcn_readfirstlane(table[min(t, len - 1) >> shift]);
+  }
+  // The keys' codes of position t, in page p.
+  __device__ __forceinline__ size_t at(int p, int t) {
+    if ((unsigned)p >= (unsigned)num_pages) {
+      bad = true;
+      p = 0;
+    }
+    return p * page_bytes + head_bytes + (size_t)(t & ((1 << shift) - 1)) * (16 * NB);
+  }
 };
 
+// Scales of the values of four tokens (a byte each) without those behind the last token.
+__device__ __forceinline__ uint32_t present(uint32_t x, int left) {
+  return left >= 4 ? x : left <= 0 ? 0u : x & ((1u << (8 * left)) - 1);
+}
+// Whether a byte is 255, and the word with such bytes 0.
+__device__ __forceinline__ bool any_nan(uint32_t x) {
+  const uint32_t y = ~x;
+  return ((y - 0x01010101u) & ~y & 0x80808080u) != 0;
+}
+__device__ __forceinline__ uint32_t no_nan(uint32_t x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if ((x >> (8 * e) & 0xFFu) == 0xFFu) x &= ~(0xFFu << (8 * e));
+  return x;
+}
+// 1.0 for each NaN of the eight tokens whose scales two words hold, as an operand.
+__device__ __forceinline__ bf16x8 nan_marks(uint32_t x0, uint32_t x1) {
+  uint32_t mark[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t x = (e < 2 ? x0 : x1) >> (16 * (e % 2));
+    mark[e] = ((x & 0xFFu) == 0xFFu ? 0x3F80u : 0u) | ((x & 0xFF00u) == 0xFF00u ? 0x3F800000u : 0u);
+  }
+  return __builtin_bit_cast(bf16x8, make_uint4(mark[0], mark[1], mark[2], mark[3]));
+}
+
+// One word of a key's codes as an operand.
+__device__ __forceinline__ bf16x8 key_operand(uint32_t c, uint32_t scale) {
+  return __builtin_bit_cast(bf16x8, make_uint4(held_pair<0>(c, scale), held_pair<1>(c, scale),
+                                               held_pair<2>(c, scale), held_pair<3>(c, scale)));
+}
+// 16 MT rows of a unit on their way through the context: queries, running maxima and
+// sums, and outputs.
 template <typename T, int NB, int MT>
 struct Wave {
   using L = CacheLay<NB>;
@@ -154,25 +214,9 @@ struct Wave {
   float m[MT], l[MT];  // in units of log2; l of this lane's tokens
   int seen[MT];        // the last position that the row sees, -1: no such row
 
-  // the unit
-  const uint8_t *codes, *scales;
-  const int32_t* table;
-  size_t value_at;  // regions from a head's keys to its values
-  int head, shift, num_pages, heads, len;
-  bool bad;
-
   // Rows row0 .. row0 + 16 MT - 1 of the sequence's n * rep.
   __device__ __forceinline__ void begin(const AttendDev& d, const CacheSeq& s, int h, int row0) {
     const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
-    codes = d.c.codes;
-    scales = d.c.scales;
-    table = d.c.pages + (int64_t)s.slot * d.c.max_pages;
-    head = h;
-    heads = d.c.heads;
-    shift = d.c.page_shift;
-    num_pages = d.c.num_pages;
-    len = s.past + s.n;
-    bad = false;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int row = row0 + 16 * i + n, t = row / d.rep;
@@ -198,57 +242,29 @@ struct Wave {
     }
   }
 
-  __device__ __forceinline__ int page(int t) const {  // of a uniform position
-    return table[min(t, len - 1) >> shift];
-  }
-
-  __device__ __forceinline__ void load(Held<NB>& w, int t0, int p0, int p1) {
-    const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      int p = a ? p1 : p0;
-      if ((unsigned)p >= (unsigned)num_pages) {
-        bad = true;
-        p = 0;
-      }
-      // (the second 16 may lie behind the last page: those of the first are read again)
-      const int t = t0 + 16 * a < len ? t0 + 16 * a : t0;
-      const size_t pos = t & ((1 << shift) - 1);
-      const size_t key = (((size_t)p * 2) * heads + head) << shift;
-      const size_t value = key + ((size_t)heads << shift);
-      load_words<NB>(codes + (key + pos) * L::row + (unsigned)(n * L::row + quad * NB * 4), w.k[a]);
-      load_words<NB>(codes + (value + pos) * L::row + (unsigned)(quad * (4 * L::row) + n * (4 * NB)),
-                     w.v[a]);
-      load_scales<NB>(scales + (key + pos) * NB + (unsigned)(n * NB), w.ks[a]);
-      const uint8_t* vs = scales + (value + pos) * NB + (unsigned)(quad * (4 * NB));
-      if constexpr (L::pow2) w.vs[a][0] = *reinterpret_cast<const uint32_t*>(vs + (n * NB / 16) * 4);
-      else load_words<Held<NB>::VS>(vs, w.vs[a]);
-    }
-  }
-
-  // MASK: some row does not see some token of the step.
-  template <bool MASK>
-  __device__ __forceinline__ void step(const AttendDev& d, Held<NB>& w, int t0) {
+  // The 32 tokens from t0 on.  MASK: some row does not see some of them.
+  //   key(a, j)               operand j of the keys of the a-th 16 tokens
+  //   value(b, first, second) operands of elements 2 b and 2 b + 1 of the values
+  //   nan, marks(b)           whether a value is held as NaN, and which: such a value would
+  //                           reach the rows that do not see it (0 * NaN), so it enters as
+  //                           0, and rows that see it are made NaN behind the products
+  template <bool MASK, typename K, typename V, typename M>
+  __device__ __forceinline__ void step(float c2, int t0, K key, V value, bool nan, M marks) {
     const int quad = (threadIdx.x & 63) >> 4;
     f32x4 s[MT][2];
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int i = 0; i < MT; ++i) s[i][0] = s[i][1] = f32x4{};
 #pragma unroll
-      for (int i = 0; i < MT; ++i) s[i][a] = f32x4{};
+    for (int j = 0; j < NB; ++j) {
+      const bf16x8 k[2] = {key(0, j), key(1, j)};
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        const uint32_t x = exponent(w.ks[a][j / 4], j % 4), c = w.k[a][j];
-        const bf16x8 k = __builtin_bit_cast(
-            bf16x8, make_uint4(held_pair<0>(c, x), held_pair<1>(c, x), held_pair<2>(c, x),
-                               held_pair<3>(c, x)));
+      for (int e = 0; e < QP; ++e)
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int e = 0; e < QP; ++e) s[i][a] = mfma16(k, q[i][e][j], s[i][a]);
-      }
+          for (int a = 0; a < 2; ++a) s[i][a] = mfma16(k[a], q[i][e][j], s[i][a]);
     }
     bf16x8 p[MT][PP];
-    uint32_t visible[MT][4];  // 1.0 of each token that the row sees
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       float z[8];
@@ -259,14 +275,7 @@ struct Wave {
         if (MASK && t0 + 16 * (e / 4) + 4 * quad + e % 4 > seen[i]) z[e] = -__builtin_inff();
         most = fmaxf(most, z[e]);
       }
-      if (MASK) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = t0 + 16 * (e / 2) + 4 * quad + e % 2 * 2;
-          visible[i][e] = (t <= seen[i] ? 0x3F80u : 0u) | (t + 1 <= seen[i] ? 0x3F800000u : 0u);
-        }
-      }
-      const float now = fmaxf(m[i], max_quads(most) * d.c2);
+      const float now = fmaxf(m[i], max_quads(most) * c2);
       if (__any(now != m[i])) {
         const float f = __builtin_amdgcn_exp2f(m[i] - now);
         l[i] *= f;
@@ -276,45 +285,24 @@ struct Wave {
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], d.c2, -now));
+        z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], c2, -now));
         l[i] += z[e];
       }
       split<PP>(z, p[i]);
     }
-    // A value held as NaN would reach the rows that do not see it (0 * NaN): it enters
-    // as 0, and rows that see it are made NaN behind the products.
-    uint32_t vs[2][Held<NB>::VS];
-    bool nan = false;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int g = 0; g < Held<NB>::VS; ++g) {
-        uint32_t x = w.vs[a][g];
-        if (MASK) {  // tokens behind the last one are not there
-          const int left = len - (t0 + 16 * a + 4 * quad);
-          x = left >= 4 ? x : left <= 0 ? 0u : x & ((1u << (8 * left)) - 1);
-        }
-        vs[a][g] = x;
-        // a byte of 255: x & (x >> 4 ...) by bytes is costlier than a carry out of +1
-        const uint32_t y = ~x;
-        nan = nan || (((y - 0x01010101u) & ~y & 0x80808080u) != 0);
-      }
-    const bool some = __any(nan);
-    if (some) {
+    if (nan) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        uint32_t mark[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t x = vs[e / 2][L::pow2 ? 0 : b] >> (16 * (e % 2));
-          mark[e] = ((x & 0xFFu) == 0xFFu ? 0x3F80u : 0u) | ((x & 0xFF00u) == 0xFF00u ? 0x3F800000u : 0u);
-        }
-        const bf16x8 a = __builtin_bit_cast(bf16x8, make_uint4(mark[0], mark[1], mark[2], mark[3]));
+        const bf16x8 a = marks(b);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          uint32_t v[4];
+          uint32_t v[4];  // 1.0 of each token that the row sees
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = MASK ? visible[i][e] : 0x3F803F80u;
+          for (int e = 0; e < 4; ++e) {
+            const int t = t0 + 16 * (e / 2) + 4 * quad + e % 2 * 2;
+            v[e] = MASK ? (t <= seen[i] ? 0x3F80u : 0u) | (t + 1 <= seen[i] ? 0x3F800000u : 0u)
+                        : 0x3F803F80u;
+          }
           const f32x4 hit = mfma16(
               a, __builtin_bit_cast(bf16x8, make_uint4(v[0], v[1], v[2], v[3])), f32x4{});
 #pragma unroll
@@ -325,72 +313,127 @@ struct Wave {
           }
         }
       }
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int g = 0; g < Held<NB>::VS; ++g)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if ((vs[a][g] >> (8 * e) & 0xFFu) == 0xFFu) vs[a][g] &= ~(0xFFu << (8 * e));
     }
-    // (a pair that every row of the wave takes as it is: two tokens of one element)
-    uint32_t x[8];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      if (b == 0 || !L::pow2) {
+      bf16x8 v[2];
+      value(b, v[0], v[1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = exponent(vs[e / 4][L::pow2 ? 0 : b], e % 4);
-      }
-      uint32_t pair[8];
+      for (int e = 0; e < PP; ++e)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int at = (e % 4) * NB + b;
-        const uint32_t c = w.v[e / 4][at / 4];
-        pair[e] = at % 4 == 0 ? held_pair<0>(c, x[e]) : at % 4 == 1 ? held_pair<1>(c, x[e])
-                  : at % 4 == 2 ? held_pair<2>(c, x[e]) : held_pair<3>(c, x[e]);
-      }
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t sel = half ? 0x07060302u : 0x05040100u;
-        uint32_t v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_perm(pair[2 * e + 1], pair[2 * e], sel);
-        const bf16x8 a = __builtin_bit_cast(bf16x8, make_uint4(v[0], v[1], v[2], v[3]));
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int e = 0; e < PP; ++e)
-            o[i][2 * b + half] = mfma16(a, p[i][e], o[i][2 * b + half]);
-      }
+          for (int i = 0; i < MT; ++i)
+            o[i][2 * b + half] = mfma16(v[half], p[i][e], o[i][2 * b + half]);
     }
   }
 
-  // Steps t0, t0 + stride, ... below end.
-  __device__ __forceinline__ void run(const AttendDev& d, int t0, int end, int stride, int past) {
-    if (t0 >= end) return;
-    Held<NB> w;
-    load(w, t0, page(t0), page(t0 + 16));
-    int p0 = page(t0 + stride), p1 = page(t0 + stride + 16);
-    for (; t0 < end; t0 += stride) {
-      const Held<NB> now = w;
-      if (t0 + stride < end) {
-        load(w, t0 + stride, p0, p1);
-        p0 = page(t0 + 2 * stride);
-        p1 = page(t0 + 2 * stride + 16);
-      }
-      Held<NB> cur = now;
-      if (t0 + kStep - 1 > past) step<true>(d, cur, t0);
-      else step<false>(d, cur, t0);
-    }
-    settle(o);
-  }
-
-  // Elements that lane quad holds of its row: f(element, four values e, e + 1 ...) in
-  // ascending runs.  o[i][j][e] is element elem(quad, j, e).
+  // Element of o[i][j][e].
   __device__ __forceinline__ static int elem(int quad, int j, int e) {
     return L::pow2 ? (4 * quad + e) * 2 * NB + j : 32 * (j / 2) + 8 * quad + 2 * e + j % 2;
   }
 };
+
+// The codes and scales of 32 tokens, as they come.
+template <int NB>
+struct Held {
+  using L = CacheLay<NB>;
+  static constexpr int VS = L::pow2 ? 1 : NB;
+  uint32_t k[2][NB], v[2][NB], ks[2][(NB + 3) / 4], vs[2][VS];
+
+  __device__ __forceinline__ void load(Unit<NB>& u, int t0, int p0, int p1) {
+    const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      // (the second 16 may lie behind the last page: those of the first are read again)
+      const size_t at = u.at(a ? p1 : p0, t0 + 16 * a < u.len ? t0 + 16 * a : t0);
+      load_words<NB>(u.codes + at + (unsigned)(n * L::row + quad * NB * 4), k[a]);
+      load_words<NB>(u.codes + at + u.value_bytes + (unsigned)(quad * (4 * L::row) + n * (4 * NB)), v[a]);
+      load_scales<NB>(u.scales + at / 16 + (unsigned)(n * NB), ks[a]);
+      load_value_scales(u, at, vs[a]);
+    }
+  }
+  __device__ __forceinline__ static void load_value_scales(const Unit<NB>& u, size_t at,
+                                                           uint32_t (&x)[VS]) {
+    const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+    const uint8_t* const p = u.scales + (at + u.value_bytes) / 16;
+    if constexpr (L::pow2)
+      x[0] = *reinterpret_cast<const uint32_t*>(p + (unsigned)(quad * (4 * NB) + n * NB / 16 * 4));
+    else load_words<VS>(p + (unsigned)(quad * (4 * NB)), x);
+  }
+};
+
+// Steps t0, t0 + stride, ... below end, straight from memory, the next step's bytes on
+// their way.
+template <typename T, int NB, int MT>
+__device__ __forceinline__ void run_steps(Wave<T, NB, MT>& w, Unit<NB>& u, float c2, int t0, int end,
+                                          int stride, int past) {
+  using H = Held<NB>;
+  const int quad = (threadIdx.x & 63) >> 4;
+  if (t0 >= end) return;
+  H next;
+  next.load(u, t0, u.page(t0), u.page(t0 + 16));
+  int p0 = u.page(t0 + stride), p1 = u.page(t0 + stride + 16);
+  // (steps that every row sees all of come first, in a loop of their own: as two ways in
+  // one loop they took twice the registers)
+  const auto one = [&](auto mask) {
+    constexpr bool MASK = decltype(mask)::value;
+    const H h = next;
+    if (t0 + stride < end) {
+      next.load(u, t0 + stride, p0, p1);
+      p0 = u.page(t0 + 2 * stride);
+      p1 = u.page(t0 + 2 * stride + 16);
+    }
+    uint32_t vs[2][H::VS], clean[2][H::VS];
+    bool nan = false;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int g = 0; g < H::VS; ++g) {
+        vs[a][g] = MASK ? present(h.vs[a][g], u.len - (t0 + 16 * a + 4 * quad)) : h.vs[a][g];
+        clean[a][g] = vs[a][g];
+        nan = nan || any_nan(vs[a][g]);
+      }
+    nan = __any(nan);
+    if (nan) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int g = 0; g < H::VS; ++g) clean[a][g] = no_nan(vs[a][g]);
+    }
+    uint32_t x[8];
+    w.template step<MASK>(
+        c2, t0,
+        [&](int a, int j) { return key_operand(h.k[a][j], exponent(h.ks[a][j / 4], j % 4)); },
+        [&](int b, bf16x8& first, bf16x8& second) {
+          uint32_t c[8];
+          if (b == 0 || !H::L::pow2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = exponent(clean[e / 4][H::L::pow2 ? 0 : b], e % 4);
+          }
+          uint32_t pair[8], f[4], g[4];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int at = (e % 4) * NB + b;
+            c[e] = h.v[e / 4][at / 4];
+            pair[e] = at % 4 == 0 ? held_pair<0>(c[e], x[e]) : at % 4 == 1 ? held_pair<1>(c[e], x[e])
+                      : at % 4 == 2 ? held_pair<2>(c[e], x[e]) : held_pair<3>(c[e], x[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[e] = __builtin_amdgcn_perm(pair[2 * e + 1], pair[2 * e], 0x05040100u);
+            g[e] = __builtin_amdgcn_perm(pair[2 * e + 1], pair[2 * e], 0x07060302u);
+          }
+          first = __builtin_bit_cast(bf16x8, make_uint4(f[0], f[1], f[2], f[3]));
+          second = __builtin_bit_cast(bf16x8, make_uint4(g[0], g[1], g[2], g[3]));
+        },
+        nan, [&](int b) { return nan_marks(vs[0][H::L::pow2 ? 0 : b], vs[1][H::L::pow2 ? 0 : b]); });
+    t0 += stride;
+  };
+  while (t0 < end && t0 + kStep - 1 <= past) one(std::false_type{});
+  while (t0 < end) one(std::true_type{});
+  settle(w.o);
+}
 
 // ---- few rows: contexts divided over the workgroups -------------------------------------
 // All tiles of 128 tokens of all units, one behind the other, are divided evenly over
@@ -417,26 +460,36 @@ __device__ __forceinline__ int tiles_of(const AttendDev& d, const CacheSeq& q, i
 template <int D, int ROWS>
 constexpr int part_floats() { return ROWS * (D + 2); }
 
+// A row of the results: where it goes, its gate's place and the factor 1 / l.
 template <typename T>
-__device__ __forceinline__ void finish(const AttendDev& d, const CacheSeq& s, int h, int row, int e0,
-                                       const float (&v)[4], float l) {
-  const int t = row / d.rep, hq = h * d.rep + (row - t * d.rep);
-  const int64_t tok = s.begin + t;
-  float r[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) r[e] = v[e] / l;
-  if (d.a.gate) {
-    float g[4];
-    load_f32<4>(static_cast<const T*>(d.a.gate) + tok * d.a.gate_stride +
-                    hq * d.a.gate_head_stride + e0, g);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] *= sigmoid_hw(g[e]);
+struct Result {
+  const T* gate;
+  T* o;
+  float f;
+  __device__ __forceinline__ Result(const AttendDev& d, const CacheSeq& s, int h, int row, float l) {
+    const int t = row / d.rep, hq = h * d.rep + (row - t * d.rep);
+    const int64_t tok = s.begin + t;
+    gate = d.a.gate ? static_cast<const T*>(d.a.gate) + tok * d.a.gate_stride + hq * d.a.gate_head_stride
+                    : nullptr;
+    o = static_cast<T*>(d.a.o) + tok * d.a.o_stride + hq * d.a.o_head_stride;
+    f = 1.0f / l;
   }
-  store_f32<4>(static_cast<T*>(d.a.o) + tok * d.a.o_stride + hq * d.a.o_head_stride + e0, r);
-}
+  __device__ __forceinline__ void store(int e0, const float (&v)[4]) const {
+    float r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = v[e] * f;
+    if (gate) {
+      float g[4];
+      load_f32<4>(gate + e0, g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] *= sigmoid_hw(g[e]);
+    }
+    store_f32<4>(o + e0, r);
+  }
+};
 
 template <typename T, int NB, int MT>
-__global__ __launch_bounds__(256) void k_attend_few(AttendDev d) {
+__global__ __launch_bounds__(256, 2) void k_attend_few(AttendDev d) {
   using W = Wave<T, NB, MT>;
   constexpr int D = 32 * NB, ROWS = 16 * MT;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -502,9 +555,11 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendDev d) {
       const int ta = (int)(at - unit_at), tb = (int)least(tiles, hi - unit_at);
 
       W w;
+      Unit<NB> u;
+      u.begin(d, q, h);
       w.begin(d, q, h, block * ROWS);
-      w.run(d, ta * kTile + wave * kStep, min(tb * kTile, w.len), kTile, q.past);
-      if (w.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)(i0 + i), kSqPage));
+      run_steps(w, u, d.c2, ta * kTile + wave * kStep, min(tb * kTile, u.len), kTile, q.past);
+      if (u.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)(i0 + i), kSqPage));
 
       const bool whole = ta == 0 && tb == tiles;
       const int n = lane & 15, quad = lane >> 4;
@@ -549,7 +604,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendDev d) {
             for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(f[k], y[e], v[e]);
           }
           if (whole) {
-            finish<T>(d, q, h, row, e0, v, sum_l);
+            Result<T>(d, q, h, row, sum_l).store(e0, v);
           } else {
             *reinterpret_cast<f32x4*>(part + (16 * b + r) * D + e0) = f32x4{v[0], v[1], v[2], v[3]};
             if (e0 == 0) {
@@ -623,31 +678,159 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendDev d) {
     v = f * so[i][x] + v;
   }
   const float out[4] = {v[0], v[1], v[2], v[3]};
-  finish<T>(d, q, h, row, col, out, l);
+  Result<T>(d, q, h, row, l).store(col, out);
 }
 
 // ---- many rows ------------------------------------------------------------------------------
-// A workgroup takes 64 MT rows of a unit, each of its waves 16 MT of them with the whole
-// context up to its last row; the waves read the same codes at about the same time.
+// A workgroup takes 128 rows of a unit, 16 MT for each wave, and its context 64 tokens at a
+// time.  The waves share the work of making codes into operands, which pass through LDS
+// in the order in which a wave reads them: 64 lanes of 16 bytes each.  One buffer is
+// filled while the other is read, and the codes of the tokens behind those are on their way.
+template <int NB, int NW>
+struct Share64 {
+  using L = CacheLay<NB>;
+  static constexpr int JK = 4 * NB / NW;             // key words of a lane: tile wave % 4
+  static constexpr int JV = (2 * NB + NW - 1) / NW;  // value bytes: 32 tokens of wave % 2
+  static constexpr bool word = NB == 8;  // a wave's bytes of a token lie in one word
+  static constexpr int VW = word ? 4 : NB, VS = Held<NB>::VS;
+  static constexpr int buffer = 8 * NB * 1024;
+  uint32_t k[JK], ks[(NB + 3) / 4], v[2][VW], vs[2][VS];
+
+  // The pages of this wave's tokens: of its keys, and of its values' two 16s.
+  struct Pages {
+    int k, v[2];
+  };
+  __device__ __forceinline__ static Pages pages(const Unit<NB>& u, int wave, int t0) {
+    return {u.page(t0 + 16 * (wave % 4)),
+            {u.page(t0 + 32 * (wave % 2)), u.page(t0 + 32 * (wave % 2) + 16)}};
+  }
+  __device__ __forceinline__ void load(Unit<NB>& u, int wave, int t0, const Pages& p) {
+    const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+    // (behind the last token, its own 16 are read again)
+    const int last = (u.len - 1) & ~15;
+    const size_t key = u.at(p.k, min(t0 + 16 * (wave % 4), last));
+    load_words<JK>(u.codes + key + (unsigned)(n * L::row + (quad * NB + wave / 4 * JK) * 4), k);
+    load_scales<NB>(u.scales + key / 16 + (unsigned)(n * NB), ks);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const size_t at = u.at(p.v[a], min(t0 + 32 * (wave % 2) + 16 * a, last));
+      const uint8_t* const c = u.codes + at + u.value_bytes;
+      const unsigned mine = quad * (4 * L::row) + n * (4 * NB);
+      if constexpr (word) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[a][e] = *reinterpret_cast<const uint32_t*>(c + (mine + e * NB + wave / 2 * JV / 4 * 4));
+      } else {
+        load_words<VW>(c + mine, v[a]);
+      }
+      Held<NB>::load_value_scales(u, at, vs[a]);
+    }
+  }
+
+  // The scales of the values, as they count.
+  __device__ __forceinline__ void value_scales(const Unit<NB>& u, int t32, uint32_t (&x)[2][VS]) const {
+    const int quad = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int g = 0; g < VS; ++g) x[a][g] = present(vs[a][g], u.len - (t32 + 16 * a + 4 * quad));
+  }
+
+  // Into a buffer: operands (tile, j) of the keys, then (32 tokens, 2 b + half) of the
+  // values; whether a value is NaN.
+  __device__ __forceinline__ bool store(const Unit<NB>& u, int wave, int t0, uint8_t* lds) const {
+    const int lane = threadIdx.x & 63;
+    bf16x8* const out = reinterpret_cast<bf16x8*>(lds) + lane;
+#pragma unroll
+    for (int i = 0; i < JK; ++i) {
+      const int j = wave / 4 * JK + i;
+      uint32_t x;
+      if constexpr (NW == 4) x = exponent(ks[i / 4], i % 4);
+      else x = ((uint32_t)((ks[0] | (uint64_t)ks[1] << 32) >> (8 * j)) & 0xFFu) << 23;
+      out[((wave % 4) * NB + j) * 64] = key_operand(k[i], x);
+    }
+    uint32_t x[2][VS];
+    value_scales(u, t0 + 32 * (wave % 2), x);
+    bool nan = false;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int g = 0; g < VS; ++g) nan = nan || any_nan(x[a][g]);
+    nan = __any(nan);
+    if (nan) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int g = 0; g < VS; ++g) x[a][g] = no_nan(x[a][g]);
+    }
+    // (bytes by uniform shifts: which ones a wave has is not known when this is compiled)
+#pragma unroll
+    for (int i = 0; i < JV; ++i) {
+      const int b = wave / 2 * JV + i;
+      if (b >= NB) break;
+      uint32_t pair[8], f[4], g[4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t c, s;
+        if constexpr (word) {
+          c = v[e / 4][e % 4] >> (8 * (b % 4));
+        } else if constexpr (NB == 4) {
+          c = v[e / 4][e % 4] >> (8 * b);
+        } else {
+          const int at = (e % 4) * NB + b;
+          c = 0;
+#pragma unroll
+          for (int y = 0; y < VW; ++y)
+            if (at / 4 == y) c = v[e / 4][y] >> (8 * (at % 4));
+        }
+        if constexpr (L::pow2) {
+          s = exponent(x[e / 4][0], e % 4);
+        } else {
+          uint32_t y = 0;
+#pragma unroll
+          for (int z = 0; z < VS; ++z)
+            if (z == b) y = x[e / 4][z];
+          s = exponent(y, e % 4);
+        }
+        pair[e] = held_pair<0>(c, s);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[e] = __builtin_amdgcn_perm(pair[2 * e + 1], pair[2 * e], 0x05040100u);
+        g[e] = __builtin_amdgcn_perm(pair[2 * e + 1], pair[2 * e], 0x07060302u);
+      }
+      const int at = 4 * NB + (wave % 2) * 2 * NB + 2 * b;
+      out[at * 64] = __builtin_bit_cast(bf16x8, make_uint4(f[0], f[1], f[2], f[3]));
+      out[(at + 1) * 64] = __builtin_bit_cast(bf16x8, make_uint4(g[0], g[1], g[2], g[3]));
+    }
+    return nan;
+  }
+};
+
+constexpr int kManyRows = 128;
+
 template <typename T, int NB, int MT>
-__global__ __launch_bounds__(256) void k_attend_many(AttendDev d) {
+__global__ __launch_bounds__(4 * kManyRows / MT, 2) void k_attend_many(AttendDev d) {
+  constexpr int NW = kManyRows / (16 * MT);
   using W = Wave<T, NB, MT>;
-  constexpr int ROWS = 64 * MT;
+  using S = Share64<NB, NW>;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // the sequence and block of rows: the last blocks, of the longest contexts, first
-  __shared__ int64_t wsum[4];
+  __shared__ __align__(16) uint8_t lds[2][S::buffer];
+  __shared__ int nans[2][NW];
+  __shared__ int64_t wsum[NW];
   __shared__ int found[2];
+  // the sequence and block of rows: the last blocks, of the longest contexts, first
   const int h = blockIdx.x % d.c.heads;
   const int64_t mine = gridDim.x / d.c.heads - 1 - blockIdx.x / d.c.heads;
   if (tid == 0) found[0] = -1;
   int64_t base = 0;
-  for (int i0 = 0; i0 < d.s.num; i0 += 256) {
+  for (int i0 = 0; i0 < d.s.num; i0 += 64 * NW) {
     int n = 0;
     if (i0 + tid < d.s.num) {
       const CacheSeq q = cache_seq(d.c, d.s, i0 + tid, blockIdx.x == 0);
       const int64_t rows = (int64_t)q.n * d.rep;
-      n = rows > d.few_rows ? (int)((rows + ROWS - 1) / ROWS) : 0;
+      n = rows > d.few_rows ? (int)((rows + kManyRows - 1) / kManyRows) : 0;
     }
     int64_t sum = n;
 #pragma unroll
@@ -658,38 +841,104 @@ __global__ __launch_bounds__(256) void k_attend_many(AttendDev d) {
     __syncthreads();
     if (lane == 63) wsum[wave] = sum;
     __syncthreads();
-    for (int i = 0; i < wave; ++i) sum += wsum[i];
+    int64_t all = 0;
+    for (int i = 0; i < NW; ++i) {
+      if (i < wave) sum += wsum[i];
+      all += wsum[i];
+    }
     if (mine >= base + sum - n && mine < base + sum) {
       found[0] = i0 + tid;
       found[1] = (int)(mine - (base + sum - n));
     }
-    base += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    base += all;
     if (base > mine) break;
   }
   __syncthreads();
   const int seq = __builtin_amdgcn_readfirstlane(found[0]);
   if (seq < 0) return;
   const CacheSeq q = cache_seq(d.c, d.s, seq, false);
-  const int64_t row0 = (int64_t)found[1] * ROWS + wave * (16 * MT), rows = (int64_t)q.n * d.rep;
-  if (row0 >= rows) return;
+  const int64_t rows = (int64_t)q.n * d.rep;
+  const int64_t block0 = (int64_t)__builtin_amdgcn_readfirstlane(found[1]) * kManyRows;
+  const int64_t row0 = block0 + wave * (16 * MT);
+  const int end = q.past + (int)((least(block0 + kManyRows, rows) - 1) / d.rep) + 1;
+  const int first_seen = q.past + (int)(block0 / d.rep);
+  const int last_seen = row0 < rows ? q.past + (int)((least(row0 + 16 * MT, rows) - 1) / d.rep) : -1;
   W w;
-  w.begin(d, q, h, (int)row0);
-  const int last = (int)((least(row0 + 16 * MT, rows) - 1) / d.rep);
-  w.run(d, 0, q.past + last + 1, kStep, q.past + (int)(row0 / d.rep));
-  if (w.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)seq, kSqPage));
+  Unit<NB> u;
+  u.begin(d, q, h);
+  w.begin(d, q, h, (int)least(row0, rows));
+  S raw;
+  raw.load(u, wave, 0, S::pages(u, wave, 0));
+  typename S::Pages pages = S::pages(u, wave, 64);
+  {
+    const bool nan = raw.store(u, wave, 0, lds[0]);
+    if (lane == 0) nans[0][wave] = nan;
+  }
+  raw.load(u, wave, 64, pages);
+  pages = S::pages(u, wave, 128);
+  __syncthreads();
+  int t0 = 0, buf = 0;
+  const auto tokens = [&](auto mask) {
+    if (t0 + 64 < end) {
+      const bool nan = raw.store(u, wave, t0 + 64, lds[buf ^ 1]);
+      if (lane == 0) nans[buf ^ 1][wave] = nan;
+      raw.load(u, wave, t0 + 128, pages);
+      pages = S::pages(u, wave, t0 + 192);
+    }
+    const bf16x8* const in = reinterpret_cast<const bf16x8*>(lds[buf]) + lane;
+#pragma unroll 1
+    for (int g = 0; g < 2; ++g) {
+      const int t = t0 + 32 * g;
+      if (t > last_seen) break;
+      int nan = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) nan |= nans[buf][i];
+      w.template step<decltype(mask)::value>(
+            d.c2, t, [&](int a, int j) { return in[((2 * g + a) * NB + j) * 64]; },
+            [&](int b, bf16x8& first, bf16x8& second) {
+              first = in[(4 * NB + g * 2 * NB + 2 * b) * 64];
+              second = in[(4 * NB + g * 2 * NB + 2 * b + 1) * 64];
+            },
+            __builtin_amdgcn_readfirstlane(nan) != 0,
+            [&](int b) {  // (rare: the scales once more)
+              uint32_t x[2];
+#pragma unroll
+              for (int a = 0; a < 2; ++a) {
+                uint32_t y[S::VS];
+                const int at = min(t + 16 * a, (u.len - 1) & ~15);
+                Held<NB>::load_value_scales(u, u.at(u.page(at), at), y);
+                x[a] = 0;
+#pragma unroll
+                for (int z = 0; z < S::VS; ++z)
+                  if (S::L::pow2 || z == b) x[a] = y[z];
+                x[a] = present(x[a], u.len - (t + 16 * a + 4 * (lane >> 4)));
+              }
+              return nan_marks(x[0], x[1]);
+            });
+    }
+    __syncthreads();
+    t0 += 64;
+    buf ^= 1;
+  };
+  // (steps that every row sees all of, then the others)
+  while (t0 < end && t0 + 63 <= first_seen) tokens(std::false_type{});
+  while (t0 < end) tokens(std::true_type{});
+  settle(w.o);
+  if (u.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)seq, kSqPage));
   const int n = lane & 15, quad = lane >> 4;
 #pragma unroll
   for (int b = 0; b < MT; ++b) {
     const float l = sum_quads(w.l[b]);
     const int64_t row = row0 + 16 * b + n;
     if (row >= rows) continue;
+    const Result<T> out(d, q, h, (int)row, l);
     if constexpr (W::L::pow2 && NB >= 2) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int j = 0; j < 2 * NB; j += 4) {
           const float v[4] = {w.o[b][j][e], w.o[b][j + 1][e], w.o[b][j + 2][e], w.o[b][j + 3][e]};
-          finish<T>(d, q, h, (int)row, W::elem(quad, j, e), v, l);
+          out.store(W::elem(quad, j, e), v);
         }
     } else {
 #pragma unroll
@@ -697,7 +946,7 @@ __global__ __launch_bounds__(256) void k_attend_many(AttendDev d) {
 #pragma unroll
         for (int j = 0; j < 2 * NB; j += 2) {
           const float v[4] = {w.o[b][j][e], w.o[b][j + 1][e], w.o[b][j][e + 1], w.o[b][j + 1][e + 1]};
-          finish<T>(d, q, h, (int)row, W::elem(quad, j, e), v, l);
+          out.store(W::elem(quad, j, e), v);
         }
     }
   }
@@ -718,10 +967,9 @@ int few_tiles(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
 }
 
 // Workgroups of k_attend_many and of k_attend_join, at most.
-constexpr int many_tiles(int dim) { return dim > 128 ? 1 : 2; }
 int64_t many_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
   const int64_t rep = a.q_heads / c.kv_heads;
-  return (s.rows * rep / (64 * many_tiles(c.dim)) + std::min(s.num, s.rows)) * c.kv_heads;
+  return (s.rows * rep / kManyRows + std::min(s.num, s.rows)) * c.kv_heads;
 }
 int64_t join_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, int mt) {
   return (int64_t)s.num * c.kv_heads * few_blocks(a, c, s, mt) * 16 * mt * ((c.dim + 63) / 64);
@@ -755,8 +1003,9 @@ hipError_t launch_attend(const dmh_attention& a, const dmh_kv_cache& c, const Se
       using T = decltype(t);
       constexpr int NB = decltype(nb)::value;
       if ((int64_t)s.max_len * d.rep > d.few_rows) {
-        k_attend_many<T, NB, many_tiles(32 * NB)>
-            <<<(unsigned)many_blocks(a, c, s), 256, 0, st>>>(d);
+        constexpr int MT = NB > 4 ? 1 : 2;
+        k_attend_many<T, NB, MT>
+            <<<(unsigned)many_blocks(a, c, s), 4 * kManyRows / MT, 0, st>>>(d);
       }
       const auto few = [&](auto m) {
         constexpr int MT = decltype(m)::value;
