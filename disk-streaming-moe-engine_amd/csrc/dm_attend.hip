@@ -43,6 +43,13 @@ constexpr int kStep = 32;   // tokens of a step
 constexpr int kTile = 128;  // tokens of a step of four waves
 constexpr float kNone = -3e38f;  // the maximum of a row that has seen no token
 
+// What k_attend_few leaves to k_attend_join of a unit.
+struct Meta {
+  int group, parts, place;  // the first workgroup with a part, how many, and that one's place
+  int begin, n;             // the sequence's rows
+  int pad[3];
+};
+
 struct AttendDev {
   dmh_attention a;
   CacheDev c;
@@ -52,7 +59,7 @@ struct AttendDev {
   int blocks;    // row blocks of a unit there, at most
   float c2;      // scale * log2(e)
   float* part;   // the workgroups' unfinished units
-  int4* meta;    // by unit: first workgroup, how many, its first one's place, -
+  struct Meta* meta;  // by unit
 };
 
 // N words at any word's address.
@@ -158,11 +165,12 @@ struct Unit {
     len = s.past + s.n;
     bad = false;
   }
-  __device__ __forceinline__ int page(int t) const {  // of a uniform position
-    return __builtin_amdgcn_readfirstlane(table[min(t, len - 1) >> shift]);
-  }
+  // The page of a position, the same in all lanes (at() sees to that: here it would wait for
+  // this load and the codes' before it).
+  __device__ __forceinline__ int page(int t) const { return table[min(t, len - 1) >> shift]; }
   // The keys' codes of position t, in page p.
   __device__ __forceinline__ size_t at(int p, int t) {
+    p = __builtin_amdgcn_readfirstlane(p);
     if ((unsigned)p >= (unsigned)num_pages) {
       bad = true;
       p = 0;
@@ -511,6 +519,10 @@ __global__ __launch_bounds__(256, 2) void k_attend_few(AttendDev d) {
       int blocks;
       const int tiles = tiles_of(d, q, ROWS, &blocks);
       mine = (int64_t)tiles * blocks * d.c.heads;
+      // (units that nobody works on, of which each call's other ones may have left something)
+      if (group == 0)
+        for (int u = 0; u < d.c.heads * d.blocks; ++u)
+          if (u % d.blocks >= blocks) d.meta[(int64_t)(i0 + tid) * d.c.heads * d.blocks + u].parts = 0;
     }
     int64_t sum = mine;
 #pragma unroll
@@ -565,15 +577,13 @@ __global__ __launch_bounds__(256, 2) void k_attend_few(AttendDev d) {
       const int n = lane & 15, quad = lane >> 4;
       float* const part = d.part + (size_t)(2 * group + slot) * part_floats<D, ROWS>();
       const int64_t mi = ((int64_t)(i0 + i) * d.c.heads + h) * d.blocks + block;
-      if (!whole && ta == 0 && tid == 0) {
+      if (ta == 0 && tid == 0) {
         // the workgroup of the unit's last tile: the last one that begins before it
         const int64_t last = unit_at + tiles - 1;
         int g = (int)(last * groups / total);
         while (share_at(total, groups, g) > last) --g;
         while (share_at(total, groups, g + 1) <= last) ++g;
-        d.meta[mi] = make_int4(group, g - group + 1, 2 * group + slot, 0);
-      } else if (whole && tid == 0) {
-        d.meta[mi] = make_int4(0, 0, 0, 0);
+        d.meta[mi] = {group, whole ? 0 : g - group + 1, 2 * group + slot, q.begin, q.n, {}};
       }
 #pragma unroll
       for (int b = 0; b < MT; ++b) {
@@ -622,63 +632,56 @@ __global__ __launch_bounds__(256, 2) void k_attend_few(AttendDev d) {
   }
 }
 
-// The parts of a unit joined: a workgroup takes one row and 64 of its elements, 16
-// threads of 4 elements, 16 parts at a time.
+// The parts of a unit joined: a workgroup takes one row, D / 4 threads of 4 elements, as
+// many parts at a time as it has threads for.
 template <typename T, int NB, int MT>
-__global__ __launch_bounds__(256) void k_attend_join(AttendDev d) {
-  constexpr int D = 32 * NB, ROWS = 16 * MT, COLS = (D + 63) / 64;
-  const int tid = threadIdx.x, x = tid & 15, y = tid >> 4;
-  int u = blockIdx.x;
-  const int col = u % COLS * 64 + 4 * x;
-  u /= COLS;
-  const int r = u % ROWS;
-  u /= ROWS;
-  const int block = u % d.blocks, h = u / d.blocks % d.c.heads;
-  const int seq = u / d.blocks / d.c.heads;
-  const CacheSeq q = cache_seq(d.c, d.s, seq, false);
-  int blocks;
-  if (!tiles_of(d, q, ROWS, &blocks) || block >= blocks) return;
+__global__ __launch_bounds__(256) void k_attend_join(AttendDev d, int rows_per_unit) {
+  constexpr int D = 32 * NB, ROWS = 16 * MT, X = D / 4, Y = 256 / X;
+  const int tid = threadIdx.x, x = tid % X, y = tid / X;
+  const int unit = blockIdx.x / rows_per_unit, r = blockIdx.x - unit * rows_per_unit;
+  const Meta meta = d.meta[unit];
+  if (meta.parts == 0) return;
+  const int block = unit % d.blocks, h = unit / d.blocks % d.c.heads;
   const int row = block * ROWS + r;
-  if (row >= q.n * d.rep) return;
-  const int4 meta = d.meta[u];
-  if (meta.y == 0) return;
+  if (row >= meta.n * d.rep) return;
   constexpr int P = part_floats<D, ROWS>();
-  // a workgroup's parts lie at 2 g and 2 g + 1; all but the first begin with this unit
-  const auto part = [&](int i) {
-    return d.part + (size_t)(i ? 2 * (meta.x + i) : meta.z) * P;
-  };
   float m = kNone, l = 0.0f;
   f32x4 v = {};
-  for (int i = y; i < meta.y; i += 16) {
-    const float* p = part(i);
-    const float pm = p[ROWS * D + r], pl = p[ROWS * D + ROWS + r];
-    f32x4 o = {};
-    if (col < D) o = *reinterpret_cast<const f32x4*>(p + r * D + col);
-    const float now = fmaxf(m, pm);
-    const float a = __builtin_amdgcn_exp2f(m - now), b = __builtin_amdgcn_exp2f(pm - now);
-    m = now;
-    l = a * l + b * pl;
-    v = a * v + b * o;
+  if (y < Y) {  // (D of 96 and 192 leave some threads over)
+    for (int i = y; i < meta.parts; i += Y) {
+      // (a workgroup's parts lie at 2 g and 2 g + 1; all but the first begin with this unit)
+      const float* p = d.part + (size_t)(i ? 2 * (meta.group + i) : meta.place) * P;
+      const float pm = p[ROWS * D + r], pl = p[ROWS * D + ROWS + r];
+      const f32x4 o = *reinterpret_cast<const f32x4*>(p + r * D + 4 * x);
+      const float now = fmaxf(m, pm);
+      const float a = __builtin_amdgcn_exp2f(m - now), b = __builtin_amdgcn_exp2f(pm - now);
+      m = now;
+      l = a * l + b * pl;
+      v = a * v + b * o;
+    }
   }
-  __shared__ float sm[16][16], sl[16][16];
-  __shared__ f32x4 so[16][16];
-  sm[y][x] = m;
-  sl[y][x] = l;
-  so[y][x] = v;
+  __shared__ float sm[Y][X], sl[Y][X];
+  __shared__ f32x4 so[Y][X];
+  if (y < Y) {
+    sm[y][x] = m;
+    sl[y][x] = l;
+    so[y][x] = v;
+  }
   __syncthreads();
-  if (y || col >= D) return;
+  if (y) return;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = fmaxf(m, sm[i][x]);
+  for (int i = 1; i < Y; ++i) m = fmaxf(m, sm[i][x]);
   l = 0.0f;
   v = f32x4{};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < Y; ++i) {
     const float f = __builtin_amdgcn_exp2f(sm[i][x] - m);
     l = __builtin_fmaf(f, sl[i][x], l);
     v = f * so[i][x] + v;
   }
   const float out[4] = {v[0], v[1], v[2], v[3]};
-  Result<T>(d, q, h, row, l).store(col, out);
+  const CacheSeq q = {meta.begin, meta.n, 0, 0};
+  Result<T>(d, q, h, row, l).store(4 * x, out);
 }
 
 // ---- many rows ------------------------------------------------------------------------------
@@ -971,8 +974,12 @@ int64_t many_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev&
   const int64_t rep = a.q_heads / c.kv_heads;
   return (s.rows * rep / kManyRows + std::min(s.num, s.rows)) * c.kv_heads;
 }
+// (of a unit's rows as many as sequences can have)
+int join_rows(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, int mt) {
+  return (int)std::min<int64_t>(16 * mt, (int64_t)s.max_len * (a.q_heads / c.kv_heads));
+}
 int64_t join_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, int mt) {
-  return (int64_t)s.num * c.kv_heads * few_blocks(a, c, s, mt) * 16 * mt * ((c.dim + 63) / 64);
+  return (int64_t)s.num * c.kv_heads * few_blocks(a, c, s, mt) * join_rows(a, c, s, mt);
 }
 
 }  // namespace
@@ -985,7 +992,7 @@ bool attend_fits(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s)
 size_t attend_bytes(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
   const int mt = few_tiles(a, c, s);
   return (size_t)2 * kGroups * (16 * mt) * (c.dim + 2) * 4 +
-         sizeof(int4) * s.num * c.kv_heads * few_blocks(a, c, s, mt);
+         sizeof(Meta) * s.num * c.kv_heads * few_blocks(a, c, s, mt);
 }
 
 hipError_t launch_attend(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, void* ws,
@@ -997,7 +1004,7 @@ hipError_t launch_attend(const dmh_attention& a, const dmh_kv_cache& c, const Se
   const int mt = few_tiles(a, c, s);
   d.blocks = few_blocks(a, c, s, mt);
   d.part = static_cast<float*>(ws);
-  d.meta = reinterpret_cast<int4*>(d.part + (size_t)2 * kGroups * (16 * mt) * (c.dim + 2));
+  d.meta = reinterpret_cast<Meta*>(d.part + (size_t)2 * kGroups * (16 * mt) * (c.dim + 2));
   return with_type(a.dtype, [&](auto t) {
     return with_blocks(c.dim, [&](auto nb) {
       using T = decltype(t);
@@ -1010,7 +1017,8 @@ hipError_t launch_attend(const dmh_attention& a, const dmh_kv_cache& c, const Se
       const auto few = [&](auto m) {
         constexpr int MT = decltype(m)::value;
         k_attend_few<T, NB, MT><<<kGroups, 256, 0, st>>>(d);
-        k_attend_join<T, NB, MT><<<(unsigned)join_blocks(a, c, s, MT), 256, 0, st>>>(d);
+        k_attend_join<T, NB, MT><<<(unsigned)join_blocks(a, c, s, MT), 256, 0, st>>>(
+            d, join_rows(a, c, s, MT));
       };
       if constexpr (NB <= 4) {
         if (mt == 2) few(std::integral_constant<int, 2>{});
