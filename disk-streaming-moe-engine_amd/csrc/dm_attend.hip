@@ -250,39 +250,44 @@ struct Wave {
     }
   }
 
-  // The 32 tokens from t0 on.  MASK: some row does not see some of them.
-  //   key(a, j)               operand j of the keys of the a-th 16 tokens
-  //   value(b, first, second) operands of elements 2 b and 2 b + 1 of the values
-  //   nan, marks(b)           whether a value is held as NaN, and which: such a value would
-  //                           reach the rows that do not see it (0 * NaN), so it enters as
-  //                           0, and rows that see it are made NaN behind the products
-  template <bool MASK, typename K, typename V, typename M>
+  // The 16 TILES tokens from t0 on.  MASK: some row does not see some of them.
+  //   key(a, j)                  operand j of the keys of the a-th 16 tokens
+  //   value(g, b, first, second) operands of elements 2 b and 2 b + 1 of the values of the
+  //                              g-th 32 tokens
+  //   nan, marks(g, b)           whether a value is held as NaN, and which: such a value would
+  //                              reach the rows that do not see it (0 * NaN), so it enters as
+  //                              0, and rows that see it are made NaN behind the products
+  template <bool MASK, int TILES, typename K, typename V, typename M>
   __device__ __forceinline__ void step(float c2, int t0, K key, V value, bool nan, M marks) {
     const int quad = (threadIdx.x & 63) >> 4;
-    f32x4 s[MT][2];
+    f32x4 s[MT][TILES];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) s[i][0] = s[i][1] = f32x4{};
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int a = 0; a < TILES; ++a) s[i][a] = f32x4{};
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const bf16x8 k[2] = {key(0, j), key(1, j)};
+      bf16x8 k[TILES];
+#pragma unroll
+      for (int a = 0; a < TILES; ++a) k[a] = key(a, j);
 #pragma unroll
       for (int e = 0; e < QP; ++e)
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int a = 0; a < 2; ++a) s[i][a] = mfma16(k[a], q[i][e][j], s[i][a]);
+          for (int a = 0; a < TILES; ++a) s[i][a] = mfma16(k[a], q[i][e][j], s[i][a]);
     }
-    bf16x8 p[MT][PP];
+    bf16x8 p[MT][TILES / 2][PP];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      float z[8];
       float most = -__builtin_inff();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        z[e] = s[i][e / 4][e % 4];
-        if (MASK && t0 + 16 * (e / 4) + 4 * quad + e % 4 > seen[i]) z[e] = -__builtin_inff();
-        most = fmaxf(most, z[e]);
-      }
+      for (int a = 0; a < TILES; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (MASK && t0 + 16 * a + 4 * quad + e > seen[i]) s[i][a][e] = -__builtin_inff();
+          most = fmaxf(most, s[i][a][e]);
+        }
       const float now = fmaxf(m[i], max_quads(most) * c2);
       if (__any(now != m[i])) {
         const float f = __builtin_amdgcn_exp2f(m[i] - now);
@@ -292,48 +297,56 @@ struct Wave {
         m[i] = now;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], c2, -now));
-        l[i] += z[e];
+      for (int g = 0; g < TILES / 2; ++g) {
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * g + e / 4][e % 4], c2, -now));
+          l[i] += z[e];
+        }
+        split<PP>(z, p[i][g]);
       }
-      split<PP>(z, p[i]);
     }
     if (nan) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const bf16x8 a = marks(b);
+      for (int g = 0; g < TILES / 2; ++g)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          uint32_t v[4];  // 1.0 of each token that the row sees
+        for (int b = 0; b < NB; ++b) {
+          const bf16x8 a = marks(g, b);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int t = t0 + 16 * (e / 2) + 4 * quad + e % 2 * 2;
-            v[e] = MASK ? (t <= seen[i] ? 0x3F80u : 0u) | (t + 1 <= seen[i] ? 0x3F800000u : 0u)
-                        : 0x3F803F80u;
-          }
-          const f32x4 hit = mfma16(
-              a, __builtin_bit_cast(bf16x8, make_uint4(v[0], v[1], v[2], v[3])), f32x4{});
+          for (int i = 0; i < MT; ++i) {
+            uint32_t v[4];  // 1.0 of each token that the row sees
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float add = hit[e] > 0.0f ? __builtin_nanf("") : 0.0f;
-            o[i][2 * b][e] += add;
-            o[i][2 * b + 1][e] += add;
+            for (int e = 0; e < 4; ++e) {
+              const int t = t0 + 32 * g + 16 * (e / 2) + 4 * quad + e % 2 * 2;
+              v[e] = MASK ? (t <= seen[i] ? 0x3F80u : 0u) | (t + 1 <= seen[i] ? 0x3F800000u : 0u)
+                          : 0x3F803F80u;
+            }
+            const f32x4 hit = mfma16(
+                a, __builtin_bit_cast(bf16x8, make_uint4(v[0], v[1], v[2], v[3])), f32x4{});
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float add = hit[e] > 0.0f ? __builtin_nanf("") : 0.0f;
+              o[i][2 * b][e] += add;
+              o[i][2 * b + 1][e] += add;
+            }
           }
         }
+    }
+#pragma unroll
+    for (int g = 0; g < TILES / 2; ++g)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        bf16x8 v[2];
+        value(g, b, v[0], v[1]);
+#pragma unroll
+        for (int e = 0; e < PP; ++e)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+              o[i][2 * b + half] = mfma16(v[half], p[i][g][e], o[i][2 * b + half]);
       }
-    }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      bf16x8 v[2];
-      value(b, v[0], v[1]);
-#pragma unroll
-      for (int e = 0; e < PP; ++e)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-            o[i][2 * b + half] = mfma16(v[half], p[i][e], o[i][2 * b + half]);
-    }
   }
 
   // Element of o[i][j][e].
@@ -410,10 +423,10 @@ __device__ __forceinline__ void run_steps(Wave<T, NB, MT>& w, Unit<NB>& u, float
         for (int g = 0; g < H::VS; ++g) clean[a][g] = no_nan(vs[a][g]);
     }
     uint32_t x[8];
-    w.template step<MASK>(
+    w.template step<MASK, 2>(
         c2, t0,
         [&](int a, int j) { return key_operand(h.k[a][j], exponent(h.ks[a][j / 4], j % 4)); },
-        [&](int b, bf16x8& first, bf16x8& second) {
+        [&](int, int b, bf16x8& first, bf16x8& second) {
           uint32_t c[8];
           if (b == 0 || !H::L::pow2) {
 #pragma unroll
@@ -435,7 +448,7 @@ __device__ __forceinline__ void run_steps(Wave<T, NB, MT>& w, Unit<NB>& u, float
           first = __builtin_bit_cast(bf16x8, make_uint4(f[0], f[1], f[2], f[3]));
           second = __builtin_bit_cast(bf16x8, make_uint4(g[0], g[1], g[2], g[3]));
         },
-        nan, [&](int b) { return nan_marks(vs[0][H::L::pow2 ? 0 : b], vs[1][H::L::pow2 ? 0 : b]); });
+        nan, [&](int, int b) { return nan_marks(vs[0][H::L::pow2 ? 0 : b], vs[1][H::L::pow2 ? 0 : b]); });
     t0 += stride;
   };
   while (t0 < end && t0 + kStep - 1 <= past) one(std::false_type{});
@@ -889,35 +902,32 @@ __global__ __launch_bounds__(4 * kManyRows / MT, 2) void k_attend_many(AttendDev
       pages = S::pages(u, wave, t0 + 192);
     }
     const bf16x8* const in = reinterpret_cast<const bf16x8*>(lds[buf]) + lane;
-#pragma unroll 1
-    for (int g = 0; g < 2; ++g) {
-      const int t = t0 + 32 * g;
-      if (t > last_seen) break;
+    if (t0 <= last_seen) {
       int nan = 0;
 #pragma unroll
       for (int i = 0; i < NW; ++i) nan |= nans[buf][i];
-      w.template step<decltype(mask)::value>(
-            d.c2, t, [&](int a, int j) { return in[((2 * g + a) * NB + j) * 64]; },
-            [&](int b, bf16x8& first, bf16x8& second) {
-              first = in[(4 * NB + g * 2 * NB + 2 * b) * 64];
-              second = in[(4 * NB + g * 2 * NB + 2 * b + 1) * 64];
-            },
-            __builtin_amdgcn_readfirstlane(nan) != 0,
-            [&](int b) {  // (rare: the scales once more)
-              uint32_t x[2];
+      w.template step<decltype(mask)::value, 4>(
+          d.c2, t0, [&](int a, int j) { return in[(a * NB + j) * 64]; },
+          [&](int g, int b, bf16x8& first, bf16x8& second) {
+            first = in[(4 * NB + g * 2 * NB + 2 * b) * 64];
+            second = in[(4 * NB + g * 2 * NB + 2 * b + 1) * 64];
+          },
+          __builtin_amdgcn_readfirstlane(nan) != 0,
+          [&](int g, int b) {  // (rare: the scales once more)
+            uint32_t x[2];
 #pragma unroll
-              for (int a = 0; a < 2; ++a) {
-                uint32_t y[S::VS];
-                const int at = min(t + 16 * a, (u.len - 1) & ~15);
-                Held<NB>::load_value_scales(u, u.at(u.page(at), at), y);
-                x[a] = 0;
+            for (int a = 0; a < 2; ++a) {
+              uint32_t y[S::VS];
+              const int t = t0 + 32 * g + 16 * a, at = min(t, (u.len - 1) & ~15);
+              Held<NB>::load_value_scales(u, u.at(u.page(at), at), y);
+              x[a] = 0;
 #pragma unroll
-                for (int z = 0; z < S::VS; ++z)
-                  if (S::L::pow2 || z == b) x[a] = y[z];
-                x[a] = present(x[a], u.len - (t + 16 * a + 4 * (lane >> 4)));
-              }
-              return nan_marks(x[0], x[1]);
-            });
+              for (int z = 0; z < S::VS; ++z)
+                if (S::L::pow2 || z == b) x[a] = y[z];
+              x[a] = present(x[a], u.len - (t + 4 * (lane >> 4)));
+            }
+            return nan_marks(x[0], x[1]);
+          });
     }
     __syncthreads();
     t0 += 64;
