@@ -47,7 +47,7 @@ constexpr float kNone = -3e38f;  // the maximum of a row that has seen no token
 struct Meta {
   int group, parts, place;  // the first workgroup with a part, how many, and that one's place
   int begin, n;             // the sequence's rows
-  int pad[3];
+  int head, block, pad;     // (of k_attend_many's units)
 };
 
 struct AttendDev {
@@ -210,6 +210,62 @@ __device__ __forceinline__ bf16x8 key_operand(uint32_t c, uint32_t scale) {
   return __builtin_bit_cast(bf16x8, make_uint4(held_pair<0>(c, scale), held_pair<1>(c, scale),
                                                held_pair<2>(c, scale), held_pair<3>(c, scale)));
 }
+// A row of the results: where it goes, its gate's place and the factor 1 / l.
+template <typename T>
+struct Result {
+  const T* gate;
+  T* o;
+  float f;
+  __device__ __forceinline__ Result(const AttendDev& d, const CacheSeq& s, int h, int row, float l) {
+    const int t = row / d.rep, hq = h * d.rep + (row - t * d.rep);
+    const int64_t tok = s.begin + t;
+    gate = d.a.gate ? static_cast<const T*>(d.a.gate) + tok * d.a.gate_stride + hq * d.a.gate_head_stride
+                    : nullptr;
+    o = static_cast<T*>(d.a.o) + tok * d.a.o_stride + hq * d.a.o_head_stride;
+    f = 1.0f / l;
+  }
+  __device__ __forceinline__ Vec<T, 4> gates(int e0) const {
+    return gate ? load_raw<4>(gate + e0) : Vec<T, 4>{};
+  }
+  __device__ __forceinline__ void store(int e0, const float (&v)[4], Vec<T, 4> g) const {
+    float r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = v[e] * f;
+    if (gate) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] *= sigmoid_hw((float)g[e]);
+    }
+    store_f32<4>(o + e0, r);
+  }
+};
+
+// The JG j from j0 on of a row's outputs that this lane holds, in runs of four elements;
+// all of their gates are requested before the first is used.
+template <typename T, int NB, int JG>
+__device__ __forceinline__ void store_lane(int quad, int j0, const f32x4 (&o)[JG],
+                                           const Result<T>& out) {
+  constexpr bool pow2 = CacheLay<NB>::pow2, runs = pow2 && NB >= 2;
+  const auto place = [&](int i) {  // of run i: four j of one e, or two j of two e
+    const int j = j0 + (runs ? i % (JG / 4) * 4 : i % (JG / 2) * 2);
+    const int e = runs ? i / (JG / 4) : i / (JG / 2) * 2;
+    return pow2 ? (4 * quad + e) * 2 * NB + j : 32 * (j / 2) + 8 * quad + 2 * e + j % 2;
+  };
+  Vec<T, 4> gate[JG] = {};
+  if (out.gate) {
+#pragma unroll
+    for (int i = 0; i < JG; ++i) gate[i] = load_raw<4>(out.gate + place(i));
+  }
+#pragma unroll
+  for (int i = 0; i < JG; ++i) {
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[k] = runs ? o[i % (JG / 4) * 4 + k][i / (JG / 4)]
+                  : o[i % (JG / 2) * 2 + k % 2][i / (JG / 2) * 2 + k / 2];
+    out.store(place(i), v, gate[i]);
+  }
+}
+
 // 16 MT rows of a unit on their way through the context: queries, running maxima and
 // sums, and outputs.
 template <typename T, int NB, int MT>
@@ -349,6 +405,10 @@ struct Wave {
       }
   }
 
+  __device__ __forceinline__ void results(int i, const Result<T>& out) const {
+    store_lane<T, NB, 2 * NB>((threadIdx.x & 63) >> 4, 0, o[i], out);
+  }
+
   // Element of o[i][j][e].
   __device__ __forceinline__ static int elem(int quad, int j, int e) {
     return L::pow2 ? (4 * quad + e) * 2 * NB + j : 32 * (j / 2) + 8 * quad + 2 * e + j % 2;
@@ -481,34 +541,6 @@ __device__ __forceinline__ int tiles_of(const AttendDev& d, const CacheSeq& q, i
 template <int D, int ROWS>
 constexpr int part_floats() { return ROWS * (D + 2); }
 
-// A row of the results: where it goes, its gate's place and the factor 1 / l.
-template <typename T>
-struct Result {
-  const T* gate;
-  T* o;
-  float f;
-  __device__ __forceinline__ Result(const AttendDev& d, const CacheSeq& s, int h, int row, float l) {
-    const int t = row / d.rep, hq = h * d.rep + (row - t * d.rep);
-    const int64_t tok = s.begin + t;
-    gate = d.a.gate ? static_cast<const T*>(d.a.gate) + tok * d.a.gate_stride + hq * d.a.gate_head_stride
-                    : nullptr;
-    o = static_cast<T*>(d.a.o) + tok * d.a.o_stride + hq * d.a.o_head_stride;
-    f = 1.0f / l;
-  }
-  __device__ __forceinline__ void store(int e0, const float (&v)[4]) const {
-    float r[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = v[e] * f;
-    if (gate) {
-      float g[4];
-      load_f32<4>(gate + e0, g);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] *= sigmoid_hw(g[e]);
-    }
-    store_f32<4>(o + e0, r);
-  }
-};
-
 template <typename T, int NB, int MT>
 __global__ __launch_bounds__(256, 2) void k_attend_few(AttendDev d) {
   using W = Wave<T, NB, MT>;
@@ -596,7 +628,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_few(AttendDev d) {
         int g = (int)(last * groups / total);
         while (share_at(total, groups, g) > last) --g;
         while (share_at(total, groups, g + 1) <= last) ++g;
-        d.meta[mi] = {group, whole ? 0 : g - group + 1, 2 * group + slot, q.begin, q.n, {}};
+        d.meta[mi] = {group, whole ? 0 : g - group + 1, 2 * group + slot, q.begin, q.n, h, block, 0};
       }
 #pragma unroll
       for (int b = 0; b < MT; ++b) {
@@ -627,7 +659,8 @@ __global__ __launch_bounds__(256, 2) void k_attend_few(AttendDev d) {
             for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(f[k], y[e], v[e]);
           }
           if (whole) {
-            Result<T>(d, q, h, row, sum_l).store(e0, v);
+            const Result<T> out(d, q, h, row, sum_l);
+            out.store(e0, v, out.gates(e0));
           } else {
             *reinterpret_cast<f32x4*>(part + (16 * b + r) * D + e0) = f32x4{v[0], v[1], v[2], v[3]};
             if (e0 == 0) {
@@ -694,7 +727,8 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendDev d, int rows_per_u
   }
   const float out[4] = {v[0], v[1], v[2], v[3]};
   const CacheSeq q = {meta.begin, meta.n, 0, 0};
-  Result<T>(d, q, h, row, l).store(4 * x, out);
+  const Result<T> to(d, q, h, row, l);
+  to.store(4 * x, out, to.gates(4 * x));
 }
 
 // ---- many rows ------------------------------------------------------------------------------
@@ -824,151 +858,278 @@ struct Share64 {
 };
 
 constexpr int kManyRows = 128;
+constexpr double kUnitCost = 320;   // of beginning and ending a unit, in tokens of its context
+constexpr double kShareCost = 512;  // the least that is worth a workgroup
+
+// The units of a sequence, a head's blocks of rows one behind the other, on a line whose
+// lengths are what they cost: about the tokens of the context up to a block's last row.
+// Workgroups take equal shares of the line.  All of them compute a place on it by the
+// same operations, so they agree on who has which part of a unit.
+struct Line {
+  int blocks;       // of a head
+  double one, per;  // block b costs one + per * (b + 1)
+  __device__ __forceinline__ Line(const AttendDev& d, const CacheSeq& q) {
+    const int64_t rows = (int64_t)q.n * d.rep;
+    blocks = rows > d.few_rows ? (int)((rows + kManyRows - 1) / kManyRows) : 0;
+    one = kUnitCost + q.past;
+    per = (double)kManyRows / d.rep;
+  }
+  __device__ __forceinline__ double to(int b) const {  // the blocks before b
+    return b * one + per * (0.5 * b * (b + 1.0));
+  }
+};
+
+// Places of a unit's part: of 16 rows and j, 64 lanes of four outputs; then the rows' m, l.
+template <int NB>
+__device__ __forceinline__ size_t many_part(int place) {
+  return (size_t)place * kManyRows * (32 * NB + 2);
+}
 
 template <typename T, int NB, int MT>
 __global__ __launch_bounds__(4 * kManyRows / MT, 2) void k_attend_many(AttendDev d) {
-  constexpr int NW = kManyRows / (16 * MT);
+  constexpr int NW = kManyRows / (16 * MT), D = 32 * NB;
   using W = Wave<T, NB, MT>;
   using S = Share64<NB, NW>;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = blockIdx.x;
   __shared__ __align__(16) uint8_t lds[2][S::buffer];
   __shared__ int nans[2][NW];
-  __shared__ int64_t wsum[NW];
-  __shared__ int found[2];
-  // the sequence and block of rows: the last blocks, of the longest contexts, first
-  const int h = blockIdx.x % d.c.heads;
-  const int64_t mine = gridDim.x / d.c.heads - 1 - blockIdx.x / d.c.heads;
-  if (tid == 0) found[0] = -1;
-  int64_t base = 0;
-  for (int i0 = 0; i0 < d.s.num; i0 += 64 * NW) {
-    int n = 0;
+  __shared__ double wsum[NW], ends[64 * NW];
+  __shared__ CacheSeq seqs[64 * NW];
+
+  // The lengths of as many sequences as there are threads, from i0 on, summed up in ends.
+  const auto count = [&](int i0) {
+    CacheSeq q = {};
+    double sum = 0.0;
     if (i0 + tid < d.s.num) {
-      const CacheSeq q = cache_seq(d.c, d.s, i0 + tid, blockIdx.x == 0);
-      const int64_t rows = (int64_t)q.n * d.rep;
-      n = rows > d.few_rows ? (int)((rows + kManyRows - 1) / kManyRows) : 0;
+      q = cache_seq(d.c, d.s, i0 + tid, group == 0);
+      const Line line(d, q);
+      sum = d.c.heads * line.to(line.blocks);
     }
-    int64_t sum = n;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
-      const int64_t x = __shfl_up(sum, o);
+      const double x = __shfl_up(sum, o);
       if (lane >= o) sum += x;
     }
     __syncthreads();
     if (lane == 63) wsum[wave] = sum;
+    seqs[tid] = q;
     __syncthreads();
-    int64_t all = 0;
-    for (int i = 0; i < NW; ++i) {
-      if (i < wave) sum += wsum[i];
-      all += wsum[i];
-    }
-    if (mine >= base + sum - n && mine < base + sum) {
-      found[0] = i0 + tid;
-      found[1] = (int)(mine - (base + sum - n));
-    }
-    base += all;
-    if (base > mine) break;
-  }
-  __syncthreads();
-  const int seq = __builtin_amdgcn_readfirstlane(found[0]);
-  if (seq < 0) return;
-  const CacheSeq q = cache_seq(d.c, d.s, seq, false);
-  const int64_t rows = (int64_t)q.n * d.rep;
-  const int64_t block0 = (int64_t)__builtin_amdgcn_readfirstlane(found[1]) * kManyRows;
-  const int64_t row0 = block0 + wave * (16 * MT);
-  const int end = q.past + (int)((least(block0 + kManyRows, rows) - 1) / d.rep) + 1;
-  const int first_seen = q.past + (int)(block0 / d.rep);
-  const int last_seen = row0 < rows ? q.past + (int)((least(row0 + 16 * MT, rows) - 1) / d.rep) : -1;
-  W w;
-  Unit<NB> u;
-  u.begin(d, q, h);
-  w.begin(d, q, h, (int)least(row0, rows));
-  S raw;
-  raw.load(u, wave, 0, S::pages(u, wave, 0));
-  typename S::Pages pages = S::pages(u, wave, 64);
-  {
-    const bool nan = raw.store(u, wave, 0, lds[0]);
-    if (lane == 0) nans[0][wave] = nan;
-  }
-  raw.load(u, wave, 64, pages);
-  pages = S::pages(u, wave, 128);
-  __syncthreads();
-  int t0 = 0, buf = 0;
-  const auto tokens = [&](auto mask) {
-    if (t0 + 64 < end) {
-      const bool nan = raw.store(u, wave, t0 + 64, lds[buf ^ 1]);
-      if (lane == 0) nans[buf ^ 1][wave] = nan;
-      raw.load(u, wave, t0 + 128, pages);
-      pages = S::pages(u, wave, t0 + 192);
-    }
-    const bf16x8* const in = reinterpret_cast<const bf16x8*>(lds[buf]) + lane;
-    if (t0 <= last_seen) {
-      int nan = 0;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) nan |= nans[buf][i];
-      w.template step<decltype(mask)::value, 4>(
-          d.c2, t0, [&](int a, int j) { return in[(a * NB + j) * 64]; },
-          [&](int g, int b, bf16x8& first, bf16x8& second) {
-            first = in[(4 * NB + g * 2 * NB + 2 * b) * 64];
-            second = in[(4 * NB + g * 2 * NB + 2 * b + 1) * 64];
-          },
-          __builtin_amdgcn_readfirstlane(nan) != 0,
-          [&](int g, int b) {  // (rare: the scales once more)
-            uint32_t x[2];
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-              uint32_t y[S::VS];
-              const int t = t0 + 32 * g + 16 * a, at = min(t, (u.len - 1) & ~15);
-              Held<NB>::load_value_scales(u, u.at(u.page(at), at), y);
-              x[a] = 0;
-#pragma unroll
-              for (int z = 0; z < S::VS; ++z)
-                if (S::L::pow2 || z == b) x[a] = y[z];
-              x[a] = present(x[a], u.len - (t + 4 * (lane >> 4)));
-            }
-            return nan_marks(x[0], x[1]);
-          });
-    }
+    double before = 0.0;
+    for (int i = 0; i < wave; ++i) before += wsum[i];
+    ends[tid] = before + sum;
     __syncthreads();
-    t0 += 64;
-    buf ^= 1;
+    return ends[64 * NW - 1];
   };
-  // (steps that every row sees all of, then the others)
-  while (t0 < end && t0 + 63 <= first_seen) tokens(std::false_type{});
-  while (t0 < end) tokens(std::true_type{});
-  settle(w.o);
-  if (u.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)seq, kSqPage));
-  const int n = lane & 15, quad = lane >> 4;
-#pragma unroll
-  for (int b = 0; b < MT; ++b) {
-    const float l = sum_quads(w.l[b]);
-    const int64_t row = row0 + 16 * b + n;
-    if (row >= rows) continue;
-    const Result<T> out(d, q, h, (int)row, l);
-    if constexpr (W::L::pow2 && NB >= 2) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int j = 0; j < 2 * NB; j += 4) {
-          const float v[4] = {w.o[b][j][e], w.o[b][j + 1][e], w.o[b][j + 2][e], w.o[b][j + 3][e]};
-          out.store(W::elem(quad, j, e), v);
+  double total = count(0);
+  for (int i0 = 64 * NW; i0 < d.s.num; i0 += 64 * NW) total += count(i0);
+  const int groups = (int)fmin(ceil(total / kShareCost), (double)gridDim.x);
+  if (tid == 0) d.meta[group].parts = 0;
+  if (group >= groups) return;
+  const auto share = [&](int w) { return total * w / groups; };
+  const double hi = group + 1 < groups ? share(group + 1) : total;
+  double at = share(group), base = 0.0;
+  int slot = 0;  // unfinished units of this workgroup so far
+  for (int i0 = 0; i0 < d.s.num && at < hi; i0 += 64 * NW) {
+    const double sum = d.s.num > 64 * NW ? count(i0) : total;
+    while (at < hi && at < base + sum) {
+      // the sequence, head and block that `at` lies in, and where that begins and ends
+      int i = 0;
+      for (int step = 32 * NW; step; step /= 2)
+        if (base + ends[i + step - 1] <= at) i += step;
+      i = __builtin_amdgcn_readfirstlane(i);
+      const CacheSeq q = seqs[i];
+      const Line line(d, q);
+      const double first = base + (i ? ends[i - 1] : 0.0), head = line.to(line.blocks);
+      int h = min((int)((at - first) / head), d.c.heads - 1);
+      while (h > 0 && first + h * head > at) --h;
+      while (h + 1 < d.c.heads && first + (h + 1) * head <= at) ++h;
+      int b = 0;
+      for (int step = 1 << (31 - __clz(line.blocks)); step; step /= 2)
+        if (b + step < line.blocks && first + h * head + line.to(b + step) <= at) b += step;
+      h = __builtin_amdgcn_readfirstlane(h);
+      b = __builtin_amdgcn_readfirstlane(b);
+      const double begin = first + h * head + line.to(b);
+      const double end = b + 1 < line.blocks   ? first + h * head + line.to(b + 1)
+                         : h + 1 < d.c.heads ? first + (h + 1) * head
+                                             : base + ends[i];
+      const int64_t rows = (int64_t)q.n * d.rep, block0 = (int64_t)b * kManyRows;
+      const int64_t row0 = block0 + wave * (16 * MT);
+      const int tokens = q.past + (int)((least(block0 + kManyRows, rows) - 1) / d.rep) + 1;
+      const int steps = (tokens + 63) / 64;
+      const auto step_at = [&](double x) {
+        return min((int)((x - begin) / (end - begin) * steps), steps);
+      };
+      const bool starts = at == begin, whole = starts && hi >= end;
+      const int from = __builtin_amdgcn_readfirstlane(starts ? 0 : step_at(at));
+      const int to = __builtin_amdgcn_readfirstlane(hi >= end ? steps : step_at(hi));
+
+      const int first_seen = q.past + (int)(block0 / d.rep);
+      const int last_seen =
+          row0 < rows ? q.past + (int)((least(row0 + 16 * MT, rows) - 1) / d.rep) : -1;
+      W w;
+      Unit<NB> u;
+      u.begin(d, q, h);
+      w.begin(d, q, h, (int)least(row0, rows));
+      int t0 = 64 * from, buf = 0;
+      const int stop = 64 * to;
+      S raw;
+      typename S::Pages pages;
+      if (t0 < stop) {
+        raw.load(u, wave, t0, S::pages(u, wave, t0));
+        pages = S::pages(u, wave, t0 + 64);
+        const bool nan = raw.store(u, wave, t0, lds[0]);
+        if (lane == 0) nans[0][wave] = nan;
+        raw.load(u, wave, t0 + 64, pages);
+        pages = S::pages(u, wave, t0 + 128);
+      }
+      __syncthreads();
+      const auto tile = [&](auto mask) {
+        if (t0 + 64 < stop) {
+          const bool nan = raw.store(u, wave, t0 + 64, lds[buf ^ 1]);
+          if (lane == 0) nans[buf ^ 1][wave] = nan;
+          raw.load(u, wave, t0 + 128, pages);
+          pages = S::pages(u, wave, t0 + 192);
         }
-    } else {
+        const bf16x8* const in = reinterpret_cast<const bf16x8*>(lds[buf]) + lane;
+        if (t0 <= last_seen) {
+          int nan = 0;
 #pragma unroll
-      for (int e = 0; e < 4; e += 2)
+          for (int k = 0; k < NW; ++k) nan |= nans[buf][k];
+          w.template step<decltype(mask)::value, 4>(
+              d.c2, t0, [&](int a, int j) { return in[(a * NB + j) * 64]; },
+              [&](int g, int b, bf16x8& v0, bf16x8& v1) {
+                v0 = in[(4 * NB + g * 2 * NB + 2 * b) * 64];
+                v1 = in[(4 * NB + g * 2 * NB + 2 * b + 1) * 64];
+              },
+              __builtin_amdgcn_readfirstlane(nan) != 0,
+              [&](int g, int b) {  // (rare: the scales once more)
+                uint32_t x[2];
 #pragma unroll
-        for (int j = 0; j < 2 * NB; j += 2) {
-          const float v[4] = {w.o[b][j][e], w.o[b][j + 1][e], w.o[b][j][e + 1], w.o[b][j + 1][e + 1]};
-          out.store(W::elem(quad, j, e), v);
+                for (int a = 0; a < 2; ++a) {
+                  uint32_t y[S::VS];
+                  const int t = t0 + 32 * g + 16 * a, near = min(t, (u.len - 1) & ~15);
+                  Held<NB>::load_value_scales(u, u.at(u.page(near), near), y);
+                  x[a] = 0;
+#pragma unroll
+                  for (int z = 0; z < S::VS; ++z)
+                    if (S::L::pow2 || z == b) x[a] = y[z];
+                  x[a] = present(x[a], u.len - (t + 4 * quad));
+                }
+                return nan_marks(x[0], x[1]);
+              });
         }
+        __syncthreads();
+        t0 += 64;
+        buf ^= 1;
+      };
+      // (steps that every row sees all of, then the others)
+      while (t0 < stop && t0 + 63 <= first_seen) tile(std::false_type{});
+      while (t0 < stop) tile(std::true_type{});
+      settle(w.o);
+      if (u.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)(i0 + i), kSqPage));
+      if (starts && !whole && tid == 0) {
+        int g = min((int)(end / total * groups), groups);  // the first whose share begins behind
+        while (g > group + 1 && share(g - 1) >= end) --g;
+        while (g < groups && share(g) < end) ++g;
+        d.meta[group] = {group, g - group, 2 * group + slot, q.begin, q.n, h, b, 0};
+      }
+      float* const part = d.part + many_part<NB>(2 * group + slot);
+#pragma unroll
+      for (int k = 0; k < MT; ++k) {
+        const float l = sum_quads(w.l[k]);
+        const int64_t row = row0 + 16 * k + n;
+        if (whole) {
+          if (row < rows) w.results(k, Result<T>(d, q, h, (int)row, l));
+        } else {
+          const int of = wave * MT + k;
+#pragma unroll
+          for (int j = 0; j < 2 * NB; ++j)
+            *reinterpret_cast<f32x4*>(part + ((size_t)(of * 2 * NB + j) * 64 + lane) * 4) = w.o[k][j];
+          if (quad == 0) {
+            part[kManyRows * D + 16 * of + n] = w.m[k];
+            part[kManyRows * D + kManyRows + 16 * of + n] = l;
+          }
+        }
+      }
+      slot += !whole;
+      at = end;
     }
+    base += sum;
   }
+}
+
+// The parts of a unit joined: a workgroup takes 16 rows and JG of the j of their outputs, each of
+// its waves every fourth part.
+template <int NB>
+constexpr int join_js() { return CacheLay<NB>::pow2 && NB >= 2 ? 4 : 2; }
+
+template <typename T, int NB>
+__global__ __launch_bounds__(256) void k_attend_many_join(AttendDev d) {
+  constexpr int D = 32 * NB, JG = join_js<NB>();
+  using L = CacheLay<NB>;
+  const Meta meta = d.meta[blockIdx.x];
+  if (meta.parts == 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, quad = lane >> 4, wave = tid >> 6;
+  const int of = blockIdx.y / (2 * NB / JG), j0 = blockIdx.y % (2 * NB / JG) * JG;
+  const int64_t row = (int64_t)meta.block * kManyRows + 16 * of + n;
+  const int64_t rows = (int64_t)meta.n * d.rep;
+  if (row - n >= rows) return;
+  float m = kNone, l = 0.0f;
+  f32x4 v[JG] = {};
+  for (int i = wave; i < meta.parts; i += 4) {
+    // (a workgroup's parts lie at 2 g and 2 g + 1; all but the first begin with this unit)
+    const float* const p = d.part + many_part<NB>(i ? 2 * (meta.group + i) : meta.place);
+    const float pm = p[kManyRows * D + 16 * of + n], pl = p[kManyRows * D + kManyRows + 16 * of + n];
+    f32x4 o[JG];
+#pragma unroll
+    for (int j = 0; j < JG; ++j)
+      o[j] = *reinterpret_cast<const f32x4*>(p + ((size_t)(of * 2 * NB + j0 + j) * 64 + lane) * 4);
+    const float now = fmaxf(m, pm);
+    const float a = __builtin_amdgcn_exp2f(m - now), b = __builtin_amdgcn_exp2f(pm - now);
+    m = now;
+    l = a * l + b * pl;
+#pragma unroll
+    for (int j = 0; j < JG; ++j) v[j] = a * v[j] + b * o[j];
+  }
+  __shared__ float sm[4][64], sl[4][64];
+  __shared__ f32x4 so[4][JG][64];
+  sm[wave][lane] = m;
+  sl[wave][lane] = l;
+#pragma unroll
+  for (int j = 0; j < JG; ++j) so[wave][j][lane] = v[j];
+  __syncthreads();
+  if (wave || row >= rows) return;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = fmaxf(m, sm[i][lane]);
+  l = 0.0f;
+#pragma unroll
+  for (int j = 0; j < JG; ++j) v[j] = f32x4{};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float f = __builtin_amdgcn_exp2f(sm[i][lane] - m);
+    l = __builtin_fmaf(f, sl[i][lane], l);
+#pragma unroll
+    for (int j = 0; j < JG; ++j) v[j] = f * so[i][j][lane] + v[j];
+  }
+  const CacheSeq q = {meta.begin, meta.n, 0, 0};
+  const Result<T> out(d, q, meta.head, (int)row, l);
+  store_lane<T, NB, JG>(quad, j0, v, out);
 }
 
 constexpr int kGroups = 512;  // workgroups of k_attend_few
 constexpr int64_t kMostBlocks = 1 << 23;  // workgroups of a launch, of 2^31 threads
 
-// Rows of a sequence that k_attend_few takes, in blocks of 16 or 32.
+// Workgroups of k_attend_many: one a CU where its LDS fills that, else two.
+int many_groups(int dim) { return dim > 128 ? 256 : 512; }
+
+// Rows (tokens times query heads of a key head) up to which a sequence is k_attend_few's.
+int few_limit(const dmh_attention& a, const dmh_kv_cache& c) {
+  return std::max(a.q_heads / c.kv_heads, 64);
+}
+
+// Blocks of 16 or 32 rows of a unit of k_attend_few.
 int few_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, int mt) {
   const int64_t rep = a.q_heads / c.kv_heads;
   const int64_t most = std::max<int64_t>(rep, std::min<int64_t>(64, s.max_len * rep));
@@ -979,11 +1140,7 @@ int few_tiles(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
   return c.dim <= 128 && s.max_len * rep > 16 ? 2 : 1;
 }
 
-// Workgroups of k_attend_many and of k_attend_join, at most.
-int64_t many_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
-  const int64_t rep = a.q_heads / c.kv_heads;
-  return (s.rows * rep / kManyRows + std::min(s.num, s.rows)) * c.kv_heads;
-}
+// Workgroups of k_attend_join.
 // (of a unit's rows as many as sequences can have)
 int join_rows(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, int mt) {
   return (int)std::min<int64_t>(16 * mt, (int64_t)s.max_len * (a.q_heads / c.kv_heads));
@@ -995,34 +1152,39 @@ int64_t join_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev&
 }  // namespace
 
 bool attend_fits(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
-  return many_blocks(a, c, s) < kMostBlocks &&
-         join_blocks(a, c, s, few_tiles(a, c, s)) < kMostBlocks;
+  return join_blocks(a, c, s, few_tiles(a, c, s)) < kMostBlocks;
 }
 
+// (the kernels for few and for many rows come one after the other and share the place)
+size_t attend_parts(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
+  const size_t few = (size_t)kGroups * 16 * few_tiles(a, c, s);
+  const bool any = (int64_t)s.max_len * (a.q_heads / c.kv_heads) > few_limit(a, c);
+  return 2 * std::max(few, any ? (size_t)many_groups(c.dim) * kManyRows : 0) * (c.dim + 2);
+}
 size_t attend_bytes(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
-  const int mt = few_tiles(a, c, s);
-  return (size_t)2 * kGroups * (16 * mt) * (c.dim + 2) * 4 +
-         sizeof(Meta) * s.num * c.kv_heads * few_blocks(a, c, s, mt);
+  const size_t units = (size_t)s.num * c.kv_heads * few_blocks(a, c, s, few_tiles(a, c, s));
+  return attend_parts(a, c, s) * 4 + sizeof(Meta) * std::max(units, (size_t)many_groups(c.dim));
 }
 
 hipError_t launch_attend(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, void* ws,
                          hipStream_t st) {
   AttendDev d = {a, cache_dev(c), s};
   d.rep = a.q_heads / c.kv_heads;
-  d.few_rows = std::max(d.rep, 64);
+  d.few_rows = few_limit(a, c);
   d.c2 = (float)((double)a.scale * 1.4426950408889634);
   const int mt = few_tiles(a, c, s);
   d.blocks = few_blocks(a, c, s, mt);
   d.part = static_cast<float*>(ws);
-  d.meta = reinterpret_cast<Meta*>(d.part + (size_t)2 * kGroups * (16 * mt) * (c.dim + 2));
+  d.meta = reinterpret_cast<Meta*>(d.part + attend_parts(a, c, s));
   return with_type(a.dtype, [&](auto t) {
     return with_blocks(c.dim, [&](auto nb) {
       using T = decltype(t);
       constexpr int NB = decltype(nb)::value;
       if ((int64_t)s.max_len * d.rep > d.few_rows) {
         constexpr int MT = NB > 4 ? 1 : 2;
-        k_attend_many<T, NB, MT>
-            <<<(unsigned)many_blocks(a, c, s), 4 * kManyRows / MT, 0, st>>>(d);
+        const int groups = many_groups(c.dim);
+        k_attend_many<T, NB, MT><<<groups, 4 * kManyRows / MT, 0, st>>>(d);
+        k_attend_many_join<T, NB><<<dim3(groups, 16 * NB / join_js<NB>()), 256, 0, st>>>(d);
       }
       const auto few = [&](auto m) {
         constexpr int MT = decltype(m)::value;
