@@ -566,8 +566,15 @@ __device__ __forceinline__ int tiles_of(const AttendDev& d, const CacheSeq& q, i
 template <int D, int ROWS>
 constexpr int part_floats() { return ROWS * (D + 2); }
 
+// Waves a SIMD and workgroups a CU: three where the registers hold them (128 elements of bf16
+// 134 -> 130 us, 64 102 -> 96; 128 of f16, whose queries take twice the registers, 38 -> 44).
+template <typename T>
+constexpr int few_waves(int dim, int mt) {
+  return mt == 1 && (dim <= 64 || (dim <= 128 && std::is_same<T, bf16_t>::value)) ? 3 : 2;
+}
+
 template <typename T, int NB, int MT>
-__global__ __launch_bounds__(256, 2) void k_attend_few(AttendDev d) {
+__global__ __launch_bounds__(256, few_waves<T>(32 * NB, MT)) void k_attend_few(AttendDev d) {
   using W = Wave<T, NB, MT>;
   constexpr int D = 32 * NB, ROWS = 16 * MT;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -1154,7 +1161,13 @@ __global__ __launch_bounds__(256) void k_attend_many_join(AttendDev d) {
   store_lane<T, NB, JG>(quad, j0, v, out);
 }
 
-constexpr int kGroups = 512;  // workgroups of k_attend_few
+// Workgroups of k_attend_few: as many as there is room for.
+int few_groups(int dtype, int dim, int mt) {
+  const int waves = dtype == DMH_DTYPE_BF16  ? few_waves<bf16_t>(dim, mt)
+                    : dtype == DMH_DTYPE_F16 ? few_waves<half_t>(dim, mt)
+                                             : few_waves<float>(dim, mt);
+  return 256 * waves;
+}
 constexpr int64_t kMostBlocks = 1 << 23;  // workgroups of a launch, of 2^31 threads
 
 // Workgroups of k_attend_many: one a CU where its LDS fills that, else two.
@@ -1193,7 +1206,8 @@ bool attend_fits(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s)
 
 // (the kernels for few and for many rows come one after the other and share the place)
 size_t attend_parts(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
-  const size_t few = (size_t)kGroups * 16 * few_tiles(a, c, s);
+  const int mt = few_tiles(a, c, s);
+  const size_t few = (size_t)few_groups(a.dtype, c.dim, mt) * 16 * mt;
   const bool any = (int64_t)s.max_len * (a.q_heads / c.kv_heads) > few_limit(a, c);
   return 2 * std::max(few, any ? (size_t)many_groups(c.dim) * kManyRows : 0) * (c.dim + 2);
 }
@@ -1224,7 +1238,7 @@ hipError_t launch_attend(const dmh_attention& a, const dmh_kv_cache& c, const Se
       }
       const auto few = [&](auto m) {
         constexpr int MT = decltype(m)::value;
-        k_attend_few<T, NB, MT><<<kGroups, 256, 0, st>>>(d);
+        k_attend_few<T, NB, MT><<<few_groups(a.dtype, c.dim, MT), 256, 0, st>>>(d);
         k_attend_join<T, NB, MT><<<(unsigned)join_blocks(a, c, s, MT), 256, 0, st>>>(
             d, join_rows(a, c, s, MT));
       };
