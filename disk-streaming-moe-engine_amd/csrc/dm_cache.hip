@@ -2,8 +2,11 @@
 //
 // A thread takes 8 elements of one head's row, four threads a block of 32: they agree
 // on its largest element and its scale, and each makes one word of codes.  The
-// hardware converts both ways (round to nearest even, above 6 to 6), so the bytes
-// bound both kernels.
+// hardware converts both ways (round to nearest even, above 6 to 6).  A workgroup first
+// finds where its rows lie in the cache, a chain of four loads one behind the other, and
+// then has up to 16 words for each thread, four on their way at a time: bound by
+// that chain for few rows and by bytes for many (16384 rows of 8 heads of 128 in f16, 86
+// MB: 38 us with one word a thread).
 #include <algorithm>
 #include <type_traits>
 
@@ -53,16 +56,166 @@ __device__ __forceinline__ uint32_t load_value(const uint8_t* region, size_t pos
   }
 }
 
-template <typename T, int NB, bool WRITE>
-__global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqDev s,
-                                                 int64_t block0) {
+// Eight elements of a row and their place in the cache.
+template <typename T, int NB>
+struct Word {
   using L = CacheLay<NB>;
+  T* x;
+  uint8_t *codes, *scale;
+  size_t pos;
+  int u;
+  bool value, in;  // in: there is such a row
+  // in_row: words of keys of all heads, then of values.
+  __device__ __forceinline__ Word() {}
+  __device__ __forceinline__ Word(const CacheDev& c, const dmh_kv_rows& r, bool in, int t, int in_row,
+                                  int page, int pos)
+      : pos(pos), in(in) {
+    const int half = c.heads * 4 * NB;
+    value = in_row >= half;
+    in_row -= value ? half : 0;
+    const int head = in_row / (4 * NB);
+    u = in_row - head * (4 * NB);
+    const size_t region = region_of(c, page, value, head) << c.page_shift;
+    codes = c.codes + region * L::row;
+    scale = c.scales + region * NB + (value ? L::value_scale(pos, u >> 2) : L::key_scale(pos, u >> 2));
+    x = static_cast<T*>(value ? r.v : r.k) + (int64_t)t * (value ? r.v_stride : r.k_stride) +
+        head * (value ? r.v_head_stride : r.k_head_stride) + 8 * u;
+  }
+  // (four lanes with the words of one block together)
+  __device__ __forceinline__ void write(Vec<T, 8> raw) const {
+    float f[8];
+    to_f32<8>(raw, f);
+    uint32_t most = 0;  // as bits: a NaN is larger than any number
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, f2u(f[i]) & 0x7FFFFFFFu);
+    most = max(most, (uint32_t)__shfl_xor((int)most, 1));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+    // 2^X with |x| <= 7 * 2^X: X = floor(log2) - 2, or one more above 1.75 * 2^floor
+    const int e = (int)(most >> 23) - 2 + ((most & 0x7FFFFFu) > 0x600000u);
+    const bool finite = most < 0x7F800000u;
+    const uint32_t byte = finite ? (uint32_t)min(max(e, 7), 252) : 255u;
+    const float unit = u2f((finite ? byte : 127u) << 23);
+    uint32_t z = 0;
+    z = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(z, f[0], f[1], unit, 0);
+    z = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(z, f[2], f[3], unit, 1);
+    z = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(z, f[4], f[5], unit, 2);
+    z = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(z, f[6], f[7], unit, 3);
+    z = finite ? z : 0u;
+    if (!in) return;
+    if (value) store_value<NB>(codes, pos, u, z);
+    else *reinterpret_cast<uint32_t*>(codes + L::key_word(pos, u)) = z;
+    if ((u & 3) == 0) *scale = (uint8_t)byte;
+  }
+  __device__ __forceinline__ void fetch(uint32_t& z, uint32_t& unit) const {
+    z = unit = 0;
+    if (!in) return;
+    z = value ? load_value<NB>(codes, pos, u)
+              : *reinterpret_cast<const uint32_t*>(codes + L::key_word(pos, u));
+    unit = (uint32_t)*scale << 23;
+  }
+  __device__ __forceinline__ void read(uint32_t z, uint32_t unit) const {
+    if (!in) return;
+    const uint32_t p[4] = {held_pair<0>(z, unit), held_pair<1>(z, unit), held_pair<2>(z, unit),
+                           held_pair<3>(z, unit)};
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = bf16lo(p[i]);
+      f[2 * i + 1] = bf16hi(p[i]);
+    }
+    store_f32<8>(x, f);
+  }
+};
+
+constexpr int kMostWords = 16;                        // of a thread
+constexpr int kMostRows = 256 * kMostWords / 8 + 2;   // of a workgroup, at 8 words a row
+
+template <typename T, int NB, bool WRITE>
+__global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqDev s, int words,
+                                                 int64_t block0) {
   const int tid = threadIdx.x;
-  constexpr int per_head = 4 * NB;
-  const int per_row = 2 * c.heads * per_head;
-  const int64_t at = (block0 + blockIdx.x) * 256;
+  const int per_row = 2 * c.heads * 4 * NB;
+  const int64_t block = block0 + blockIdx.x;
+  const int64_t first = block * (256 * words);
   // (fewer than 2^30 rows)
-  const int t0 = (int)(at / per_row), t = (int)((at + tid) / per_row);
+  const int t0 = (int)least(first / per_row, s.rows);
+  const int t1 = (int)least((first + 256 * words - 1) / per_row + 1, s.rows);
+
+  __shared__ int found;
+  __shared__ struct { int begin, end, past, slot, seq; } part[kMostRows];
+  __shared__ int page_of_row[kMostRows], pos_of_row[kMostRows];
+  if (tid == 0) found = 0;
+  if (block < s.num && tid < 64) {
+    // what is wrong with the call's sequences, a workgroup each
+    const CacheSeq q = cache_seq(c, s, (int)block, tid == 0);
+    if (WRITE && q.n && s.slots) report_shared_slot(s, (int)block, q.slot, tid);
+  }
+  __syncthreads();
+  // the sequences with rows here
+  for (int i = tid; i < s.num; i += 256) {
+    if (s.off[i] >= t1 || s.off[i + 1] <= t0) continue;
+    const CacheSeq q = cache_seq(c, s, i, false);
+    if (!q.n) continue;
+    // (ones that overlap, which nothing is said about, may be more than there is room for)
+    const int at = atomicAdd(&found, 1);
+    if (at < kMostRows) part[at] = {q.begin, q.begin + q.n, q.past, q.slot, i};
+  }
+  __syncthreads();
+  const int parts = min(found, kMostRows);
+  for (int t = t0 + tid; t < t1; t += 256) {
+    int page = -1, pos = 0;
+    for (int i = 0; i < parts; ++i) {
+      if (t < part[i].begin || t >= part[i].end) continue;
+      pos = part[i].past + (t - part[i].begin);
+      page = page_of(c, part[i].slot, pos);
+      if (page < 0) record_err(s.status, err_key(kPhSeq, 0, 0, (uint32_t)part[i].seq, kSqPage));
+      break;
+    }
+    page_of_row[t - t0] = page;
+    pos_of_row[t - t0] = pos & ((1 << c.page_shift) - 1);
+  }
+  __syncthreads();
+
+  const auto word = [&](int k) {
+    const int64_t i = first + 256 * k + tid;
+    const int64_t row = i / per_row;
+    const int t = (int)least(row, s.rows);
+    const bool in = t < t1 && page_of_row[t - t0] >= 0;
+    const int at = in ? t - t0 : 0;
+    return Word<T, NB>(c, r, in, in ? t : 0, (int)(i - row * per_row), in ? page_of_row[at] : 0,
+                       in ? pos_of_row[at] : 0);
+  };
+  constexpr int B = 4;
+  for (int k0 = 0; k0 < words; k0 += B) {
+    Word<T, NB> w[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      w[b] = word(min(k0 + b, words - 1));
+      w[b].in = w[b].in && k0 + b < words;
+    }
+    if constexpr (WRITE) {
+      Vec<T, 8> raw[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) raw[b] = w[b].in ? load_raw<8>(w[b].x) : Vec<T, 8>{};
+#pragma unroll
+      for (int b = 0; b < B; ++b) w[b].write(raw[b]);
+    } else {
+      uint32_t z[B], unit[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) w[b].fetch(z[b], unit[b]);
+#pragma unroll
+      for (int b = 0; b < B; ++b) w[b].read(z[b], unit[b]);
+    }
+  }
+}
+
+// The same with one word a thread, each of which finds its own row: no way through LDS.
+template <typename T, int NB, bool WRITE>
+__global__ __launch_bounds__(256) void k_kv_few(CacheDev c, dmh_kv_rows r, SeqDev s) {
+  const int tid = threadIdx.x;
+  const int per_row = 2 * c.heads * 4 * NB;
+  const int64_t i = (int64_t)blockIdx.x * 256 + tid;
+  const int t0 = (int)least((i - tid) / per_row, s.rows), t = (int)least(i / per_row, s.rows);
 
   // the first sequence with a row at t0 or behind it, then this row's
   __shared__ int first_seq;
@@ -73,14 +226,9 @@ __global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqD
   if (j0 < s.num) atomicMin(&first_seq, j0);
   __syncthreads();
   int q = first_seq;
-  if (block0 + blockIdx.x < s.num) {
-    // what is wrong with the call's sequences, a workgroup each (and those behind the
-    // last workgroup: the launch has as many as there are sequences at least)
-    if (tid < 64) {
-      const int i = (int)(block0 + blockIdx.x);
-      const CacheSeq cs = cache_seq(c, s, i, tid == 0);
-      if (WRITE && cs.n && s.slots) report_shared_slot(s, i, cs.slot, tid);
-    }
+  if ((int)blockIdx.x < s.num && tid < 64) {
+    const CacheSeq cs = cache_seq(c, s, blockIdx.x, tid == 0);
+    if (WRITE && cs.n && s.slots) report_shared_slot(s, blockIdx.x, cs.slot, tid);
   }
   if (t >= s.rows) return;
   while (q < s.num && s.off[q + 1] <= t) ++q;
@@ -93,52 +241,14 @@ __global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqD
     record_err(s.status, err_key(kPhSeq, 0, 0, (uint32_t)q, kSqPage));
     return;
   }
-  int in_row = (int)(at + tid - (int64_t)t * per_row);
-  const int kind = in_row >= per_row / 2;
-  in_row -= kind * (per_row / 2);
-  const int head = in_row / per_head, u = in_row - head * per_head;
-  const size_t region = region_of(c, page, kind, head) << c.page_shift;
-  const size_t in_page = pos & ((1 << c.page_shift) - 1);
-  uint8_t* const codes = c.codes + region * L::row;
-  uint8_t* const scales = c.scales + region * NB;
-  uint8_t* const scale = scales + (kind ? L::value_scale(in_page, u >> 2) : L::key_scale(in_page, u >> 2));
-  T* const x = static_cast<T*>(kind ? r.v : r.k) + (int64_t)t * (kind ? r.v_stride : r.k_stride) +
-               head * (kind ? r.v_head_stride : r.k_head_stride) + 8 * u;
+  const Word<T, NB> w(c, r, true, t, (int)(i - (int64_t)t * per_row), page,
+                      pos & ((1 << c.page_shift) - 1));
   if constexpr (WRITE) {
-    float f[8];
-    load_f32<8>(x, f);
-    uint32_t most = 0;  // as bits: a NaN is larger than any number
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, f2u(f[i]) & 0x7FFFFFFFu);
-    most = max(most, (uint32_t)__shfl_xor((int)most, 1));
-    most = max(most, (uint32_t)__shfl_xor((int)most, 2));
-    // 2^X with |x| <= 7 * 2^X: X = floor(log2) - 2, or one more above 1.75 * 2^floor
-    const int e = (int)(most >> 23) - 2 + ((most & 0x7FFFFFu) > 0x600000u);
-    const bool finite = most < 0x7F800000u;
-    const uint32_t byte = finite ? (uint32_t)min(max(e, 7), 252) : 255u;
-    const float unit = u2f((finite ? byte : 127u) << 23);
-    uint32_t w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[0], f[1], unit, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2], f[3], unit, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4], f[5], unit, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6], f[7], unit, 3);
-    w = finite ? w : 0u;
-    if (kind) store_value<NB>(codes, in_page, u, w);
-    else *reinterpret_cast<uint32_t*>(codes + L::key_word(in_page, u)) = w;
-    if ((u & 3) == 0) *scale = (uint8_t)byte;
+    w.write(load_raw<8>(w.x));
   } else {
-    const uint32_t w = kind ? load_value<NB>(codes, in_page, u)
-                            : *reinterpret_cast<const uint32_t*>(codes + L::key_word(in_page, u));
-    const uint32_t unit = (uint32_t)*scale << 23;
-    const uint32_t p[4] = {held_pair<0>(w, unit), held_pair<1>(w, unit), held_pair<2>(w, unit),
-                           held_pair<3>(w, unit)};
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = bf16lo(p[i]);
-      f[2 * i + 1] = bf16hi(p[i]);
-    }
-    store_f32<8>(x, f);
+    uint32_t z, unit;
+    w.fetch(z, unit);
+    w.read(z, unit);
   }
 }
 
@@ -148,12 +258,21 @@ hipError_t run(const dmh_kv_cache& c, const dmh_kv_rows& r, const SeqDev& s, hip
     return with_blocks(c.dim, [&](auto nb) {
       using T = decltype(t);
       constexpr int NB = decltype(nb)::value;
-      const int64_t threads = (int64_t)s.rows * 2 * c.kv_heads * 4 * NB;
-      const int64_t blocks = std::max<int64_t>((threads + 255) / 256, s.num);
+      const int64_t all = (int64_t)s.rows * 2 * c.kv_heads * 4 * NB;  // words
+      // as many to a thread as leave four workgroups a CU (32 rows of 2 heads of 256: 4.4 us
+      // with none, which the first kernel does in 6.5)
+      const int words = (int)std::min<int64_t>(kMostWords, all / (256 * 1024));
+      if (words == 0 && s.num < 4096) {
+        const int64_t blocks = std::max<int64_t>((all + 255) / 256, s.num);
+        k_kv_few<T, NB, WRITE><<<(unsigned)blocks, 256, 0, st>>>(cache_dev(c), r, s);
+        return hipGetLastError();
+      }
+      const int some = std::max(words, 1);
+      const int64_t blocks = std::max<int64_t>((all + 256 * some - 1) / (256 * some), s.num);
       constexpr int64_t most = 1 << 23;  // 2^31 threads a launch
       for (int64_t b = 0; b < blocks; b += most)
         k_kv_rows<T, NB, WRITE><<<(unsigned)std::min(most, blocks - b), 256, 0, st>>>(
-            cache_dev(c), r, s, b);
+            cache_dev(c), r, s, some, b);
       return hipGetLastError();
     });
   });
