@@ -258,7 +258,7 @@ struct Result {
     for (int e = 0; e < 4; ++e) r[e] = v[e] * f;
     if (gate) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] *= sigmoid_hw((float)g[e]);
+      for (int e = 0; e < 4; ++e) r[e] *= sigmoid_all((float)g[e]);
     }
     store_f32<4>(o + e0, r);
   }

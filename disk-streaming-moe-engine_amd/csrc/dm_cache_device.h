@@ -15,6 +15,13 @@ __device__ __forceinline__ uint32_t held_pair(uint32_t codes, uint32_t scale) {
       uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, u2f(scale), BYTE));
 }
 
+// 1 / (1 + e^-z), also where it is below fp32's normal numbers, which the hardware's
+// reciprocal takes for 0.
+__device__ __forceinline__ float sigmoid_all(float z) {
+  const float e = expf(-__builtin_fabsf(z));
+  return (z < 0.0f ? e : 1.0f) / (1.0f + e);
+}
+
 // A sequence's rows and the tokens before them, with everything about it checked that
 // no page needs.
 struct CacheSeq {
