@@ -62,13 +62,12 @@ constexpr int parts_of() {
 
 // Eight elements as PARTS bf16 values whose sum each is.
 template <typename T, int PARTS>
-__device__ __forceinline__ void load_parts(const T* p, bf16x8 (&out)[PARTS]) {
+__device__ __forceinline__ void to_parts(Vec<T, 8> v, bf16x8 (&out)[PARTS]) {
   if constexpr (PARTS == 1) {
-    const Vec<T, 8> v = load_raw<8>(p);
     out[0] = __builtin_bit_cast(bf16x8, v);
   } else {
     float r[8];
-    load_f32<8>(p, r);
+    to_f32<8>(v, r);
 #pragma unroll
     for (int q = 0; q < PARTS; ++q) {
       uint32_t w[4];
@@ -145,13 +144,22 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinearDev l, dmh_line
       sn[j] = s[j];
     }
     load(min(g + WAVES, l.chunks - 1));
+    // (rows that are not there are not read: their lines would cost as much as the others')
+    Vec<T, 8> raw[4][NT] = {};
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if (t0 + 16 * i + n < r.rows) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          raw[c][i] = load_raw<8>(x[i] + min(g * kQuadCols + c * kGroup, l.k - kGroup));
+      }
+    }
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int col = g * kQuadCols + c * kGroup;
-      if (col >= l.k) break;
+      if (g * kQuadCols + c * kGroup >= l.k) break;
       bf16x8 b[NT][P];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) load_parts<T, P>(x[i] + col, b[i]);
+      for (int i = 0; i < NT; ++i) to_parts<T, P>(raw[c][i], b[i]);
 #pragma unroll
       for (int j = 0; j < AT; ++j) {
         const uint32_t word = c == 0 ? wn[j].x : c == 1 ? wn[j].y : c == 2 ? wn[j].z : wn[j].w;
@@ -312,7 +320,7 @@ __global__ __launch_bounds__(256) void k_linear_split(const T* x, int64_t stride
   const int64_t row = i / per;
   const int col = (int)(i - row * per) * 8;
   bf16x8 p[P];
-  load_parts<T, P>(x + row * stride + col, p);
+  to_parts<T, P>(load_raw<8>(x + row * stride + col), p);
 #pragma unroll
   for (int j = 0; j < P; ++j)
     *reinterpret_cast<bf16x8*>(out + (j * rows + row) * k + col) = p[j];
@@ -389,6 +397,7 @@ hipError_t run(const LinearDev& l, const dmh_linear_rows& r, void* ws, hipStream
   if (r.rows <= 16) {
     if (l.row_blocks < 256) return few(one, one, integral_constant<int, 16>{});
     if (l.row_blocks < 1024) return few(one, one, eight);
+    if (l.row_blocks >= 4096 && (r.rows > 8 || parts_of<T>() > 1)) return few(four, one, four);
     return few(two, one, four);
   }
   if (u < 512) return few(one, one, eight);
