@@ -5,8 +5,8 @@
 // hardware converts both ways (round to nearest even, above 6 to 6).  A workgroup first
 // finds where its rows lie in the cache, a chain of four loads one behind the other, and
 // then has up to 16 words for each thread, four on their way at a time: bound by
-// that chain for few rows and by bytes for many (16384 rows of 8 heads of 128 in f16, 86
-// MB: 38 us with one word a thread).
+// that chain for few rows (32 of 2 heads of 256: 5 us) and by bytes for many (16384 rows of 8
+// heads of 128 in f16, 86 MB: 26 us, 3.3 TB/s, and 38 with one word a thread).
 #include <algorithm>
 #include <type_traits>
 

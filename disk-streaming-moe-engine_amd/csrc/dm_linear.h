@@ -27,6 +27,8 @@ inline int linear_chunks(int k) { return (k + kQuadCols - 1) / kQuadCols; }
 hipError_t launch_linear_pack(const uint16_t* scales, const uint8_t* packed, int n, int k, int group,
                               uint8_t* nib, uint16_t* sc, unsigned long long* vkey, hipStream_t st);
 
+// Whether a launch holds the call's work.
+bool linear_fits(const LinearDev& l, const dmh_linear_rows& r);
 // ws: linear_bytes of device memory (0: none), 16-byte aligned.
 size_t linear_bytes(const LinearDev& l, const dmh_linear_rows& r);
 hipError_t launch_linear(const LinearDev& l, const dmh_linear_rows& r, void* ws, hipStream_t st);

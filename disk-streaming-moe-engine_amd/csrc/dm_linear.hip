@@ -417,6 +417,13 @@ hipError_t launch_linear_pack(const uint16_t* scales, const uint8_t* packed, int
   return hipGetLastError();
 }
 
+bool linear_fits(const LinearDev& l, const dmh_linear_rows& r) {
+  if (few_rows(l, r)) return true;
+  constexpr int64_t most = 1 << 23;  // workgroups of a launch, of 2^31 threads
+  return (int64_t)((l.row_blocks + 7) / 8) * ((r.rows + 63) / 64) < most &&
+         (int64_t)r.rows * (l.k / 8) < most * 256;
+}
+
 size_t linear_bytes(const LinearDev& l, const dmh_linear_rows& r) {
   if (few_rows(l, r)) return 0;
   const size_t n = (size_t)r.rows * l.k * 2;

@@ -120,6 +120,8 @@ int dmh_linear_forward(dmh_ctx* c, const dmh_linear* l, const dmh_linear_rows* r
   const Rows y{r.y, r.rows, l->dev.n, r.y_stride, elem(r.out_dtype)};
   if (!x.ok() || !y.ok()) return err.arg("a stride is shorter than its row, or an array is misaligned");
   if (overlap(x, y)) return err.arg("x and y must not overlap");
+  if (!linear_fits(l->dev, r))
+    return err(DMH_ERR_CONFIG, "CONFIG_ERROR", "too many rows for one call: %d", r.rows);
   hipStream_t st;
   unsigned long long* status;
   int rc = api_mixer_begin(c, &st, &status, errp, errlen);

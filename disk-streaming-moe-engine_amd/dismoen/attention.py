@@ -69,7 +69,7 @@ class KVCache(_Heads):
         for a, shape, kind, what in (
                 (codes, (n, 2, h, page, half), "uint8", "codes"),
                 (scales, (n, 2, h, page, half // 16), "uint8", "scales"),
-                (pages, (self.num_slots, *pages.shape[1:2]), "int32", "pages"),
+                (pages, (self.num_slots, pages.shape[-1]), "int32", "pages"),
                 (past, (self.num_slots,), "int32", "past")):
             if isinstance(a, np.ndarray) is not host or tuple(a.shape) != shape \
                     or str(a.dtype).split(".")[-1] != kind or not _packed(a.shape, _strides(a)):

@@ -173,6 +173,20 @@ def test_attention_arguments(kw, code, text):
     assert rc == code and text in got, got
 
 
+def test_rows_past_32_bits():
+    """Rows count tokens times query heads of a key head."""
+    c = cache(kv_heads=1, past=(0, 0, 0), max_pages=1 << 26)
+    big = dict(q_heads=4096, q=ptr(64), o=ptr(64, 16), dtype=0)
+    strides = {k: 4096 * 64 for k in ("q_stride", "o_stride")}
+    a = attention(**big, **strides)
+    b = batch(offsets=(0, 1), total=1 << 18, max_len=1)
+    a.o = a.q + (1 << 40)  # (never touched: the call is refused)
+    rc, got = call("dmh_attention_forward", a, c, b, F_DEVICE)
+    assert rc == 2 and "too many rows" in got, got
+    b.total_tokens = (1 << 18) - 1
+    assert CTX[1] in call("dmh_attention_forward", a, c, b, F_DEVICE)[1]
+
+
 def test_nulls():
     for name, make in CALLS.items():
         assert call(name, None, cache(), batch())[0] == 1
@@ -238,6 +252,7 @@ def arrays(**kw):
     ({"scales": np.zeros((6, 2, 2, 16, 4), np.uint8)[..., ::2]}, "scales must be"),
     ({"pages": np.zeros((2, 4), np.int32)}, "pages must be"),
     ({"pages": np.zeros((3, 4), np.int64)}, "pages must be"),
+    ({"pages": np.zeros(3, np.int32)}, "pages must be"),
     ({"past": np.zeros(3, np.uint32)}, "past must be"),
 ])
 def test_python_arrays(kw, text):

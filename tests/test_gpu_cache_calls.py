@@ -229,13 +229,18 @@ def test_captured(lens):
         k, v, q, out = (rand(g, rows, h, dim) for h in (heads, heads, qh, qh))
         mix, b = AttentionMixer(blk, qh), c.batch()
         start = c.codes.clone(), c.scales.clone()
+        mark = torch.zeros(1, device="cuda")
         stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
         blk.set_stream(stream.cuda_stream)
         with torch.cuda.graph(graph, stream=stream):  # no memory for it yet: nothing is recorded
             with pytest.raises(DismoenError, match="before the capture"):
                 mix(q, k, v, c.cache, b, out)
+            mark.add_(1)
         blk.set_stream(None)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert mark.item() == 1 and torch.equal(c.codes, start[0]) and torch.equal(c.scales, start[1])
         mix(q, k, v, c.cache, b, out)
         blk.sync()
         graph = torch.cuda.CUDAGraph()

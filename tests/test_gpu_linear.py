@@ -158,3 +158,65 @@ def test_from_a_quant_model(block, tmp_path):
     lin(x, y)
     block.sync()
     check(y, x, w, None, 128)
+
+
+def test_too_many_rows(block):
+    """More tiles than a launch holds are refused before anything is read."""
+    import ctypes as C
+
+    from dismoen._lib import DmhLinearRows
+    g = gen("too many")
+    _, scales, packed = weights(g, 1000, 64, 32)
+    lin = QuantLinear(block, 1000, 64, scales.cuda(), packed.cuda(), 32)
+    e = C.create_string_buffer(512)
+    r = DmhLinearRows(2, 2, (1 << 30) - 1, 1 << 44, 64, 1 << 46, 1000)  # (addresses of nothing)
+    rc = block._lib.dmh_linear_forward(block.handle, lin._l, C.addressof(r), 1, e, 512)
+    assert rc == 2 and b"too many rows" in e.value
+
+
+@pytest.mark.parametrize("rows", [3, 40, 700])
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES)
+def test_captured(rows, t):
+    """Replays take new rows and give the bits of the same call made at once; one that needs
+    memory which a capture cannot make is refused."""
+    from dismoen import MoEBlock
+    g = gen("captured", rows)
+    with MoEBlock(0) as blk:
+        w, scales, packed = weights(g, 2100, 256, 32)
+        lin = QuantLinear(blk, 2100, 256, scales.cuda(), packed.cuda(), 32)
+        x, y = torch.zeros(rows, 256, dtype=t, device="cuda"), torch.zeros(rows, 2100, device="cuda")
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        mark = torch.zeros(1, device="cuda")
+        torch.cuda.synchronize()
+        if rows == 700 and t is not torch.bfloat16:
+            blk.set_stream(stream.cuda_stream)
+            with torch.cuda.graph(graph, stream=stream):
+                with pytest.raises(DismoenError, match="before the capture"):
+                    lin(x, y)
+                mark.add_(1)
+            blk.set_stream(None)
+            graph = torch.cuda.CUDAGraph()
+        lin(x, y)
+        blk.sync()
+        blk.set_stream(stream.cuda_stream)
+        with torch.cuda.graph(graph, stream=stream):
+            with pytest.raises(DismoenError, match="being captured"):
+                QuantLinear(blk, 2100, 256, scales.numpy(), packed.numpy(), 32)
+            lin(x, y)
+        blk.set_stream(None)
+        for _ in range(3):
+            x.copy_(torch.randn((rows, 256), generator=g))
+            y.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = y.clone()
+            torch.cuda.synchronize()
+            lin(x, y)
+            blk.sync()
+            assert torch.equal(got, y)
+            check(y, x, w, None, 256)
+        del graph
+        lin.close()
+        with pytest.raises(DismoenError, match="linear layer is NULL"):
+            lin(x, y)
