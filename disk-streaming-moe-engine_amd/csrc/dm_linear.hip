@@ -191,6 +191,93 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinearDev l, dmh_line
   }
 }
 
+// ---- few rows of a large W ----------------------------------------------------------------
+// Workgroups that stay: each takes a run of W's row blocks, its waves CW chunks of 128
+// columns each.  A wave holds its chunks of x as operands in registers the whole time, so that
+// x is read and taken apart once a workgroup instead of once in every 16 AT rows of W, and
+// W's next row blocks are on their way over the joins through LDS, two row blocks at a time
+// (four: up to 2 us slower).  Bound by W's bytes: 100003 x 2048, five rows, 26.8 us in bf16
+// (4.3 TB/s), 29.9 in f16, 33.4 in fp32; with one chunk after the other by k_linear_few 31.4,
+// 38.9 and 44.6.
+constexpr int kJoinTiles = 2;
+template <typename T, typename O, int CW>
+__global__ __launch_bounds__(1024, 4) void k_linear_run(LinearDev l, dmh_linear_rows r) {
+  constexpr int P = parts_of<T>(), JT = kJoinTiles;
+  extern __shared__ f32x4 red[];  // [2][JT][waves][64]
+  const int waves = blockDim.x / 64;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lo = (int)((int64_t)l.row_blocks * blockIdx.x / gridDim.x);
+  const int hi = (int)((int64_t)l.row_blocks * (blockIdx.x + 1) / gridDim.x);
+  uint4 w[JT][CW];
+  uint2 s[JT][CW];
+  const auto load = [&](int j, int rb) {
+#pragma unroll
+    for (int i = 0; i < CW; ++i) {
+      const int g = min(wave * CW + i, l.chunks - 1);
+      // (read once and not again before the next call: not kept in L2 over what is)
+      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+      const u32x4 a = __builtin_nontemporal_load(
+          reinterpret_cast<const u32x4*>(l.nib + a16_nib_offset(l.chunks, rb, g, lane)));
+      w[j][i] = make_uint4(a.x, a.y, a.z, a.w);
+      s[j][i] = *reinterpret_cast<const uint2*>(l.sc + a16_sc_offset(l.chunks, rb, g, n));
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < JT; ++j)
+    if (lo + j < hi) load(j, lo + j);
+  // (rows and columns that are not there are 0)
+  bf16x8 b[CW][4][P];
+  {
+    const T* const x = static_cast<const T*>(r.x) + least(n, r.rows - 1) * r.x_stride + 8 * quad;
+    Vec<T, 8> raw[CW][4] = {};
+#pragma unroll
+    for (int i = 0; i < CW; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int col = (wave * CW + i) * kQuadCols + c * kGroup;
+        if (n < r.rows && col < l.k) raw[i][c] = load_raw<8>(x + col);
+      }
+#pragma unroll
+    for (int i = 0; i < CW; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) to_parts<T, P>(raw[i][c], b[i][c]);
+  }
+  int buf = 0, turn = wave;  // the waves add up in turn, JT of them at a time
+  for (int t = lo; t < hi; t += JT, buf ^= 1) {
+    f32x4 acc[JT] = {};
+#pragma unroll
+    for (int j = 0; j < JT; ++j) {
+      if (t + j >= hi) break;
+#pragma unroll
+      for (int i = 0; i < CW; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t word = c == 0 ? w[j][i].x : c == 1 ? w[j][i].y : c == 2 ? w[j][i].z : w[j][i].w;
+          const uint32_t half = c < 2 ? s[j][i].x : s[j][i].y;
+          const bf16x8 a = dequant8(word, fp16_bits_to_f32(c % 2 ? half >> 16 : half & 0xFFFFu));
+#pragma unroll
+          for (int p = 0; p < P; ++p) acc[j] = mfma16(a, b[i][c][p], acc[j]);
+        }
+      if (t + JT + j < hi) load(j, t + JT + j);
+      // (a product's result is read some cycles after its issue, which the compiler does not
+      // count over the end of a block)
+      asm volatile("s_nop 7\n\ts_nop 7" : "+v"(acc[j]));
+      red[((buf * JT + j) * waves + wave) * 64 + lane] = acc[j];
+    }
+    __syncthreads();
+    for (; turn < JT; turn += waves) {
+      if (t + turn >= hi) continue;
+      const f32x4* const from = red + (buf * JT + turn) * waves * 64 + lane;
+      f32x4 v = from[0];
+#pragma unroll 4
+      for (int k = 1; k < waves; ++k) v += from[k * 64];
+      store_out<O>(l, r, n, (t + turn) * kTileRows + 4 * quad, v);
+    }
+    turn -= JT;
+  }
+}
+
 // ---- many rows --------------------------------------------------------------------------
 // A workgroup takes 64 AT rows of W and 16 BT rows of x.  Each of its four waves has
 // 16 AT rows of W of its own, whose codes it makes into operands once, and all rows of
@@ -373,9 +460,41 @@ bool few_rows(const LinearDev& l, const dmh_linear_rows& r) {
   return r.rows <= 32 || units(l, r) <= 4608;
 }
 
+// Chunks of W a wave of k_linear_run takes and the waves that takes.  Two chunks of fp32 rows
+// do not fit its registers.
+template <typename T>
+int run_chunks(const LinearDev& l) {
+  return l.chunks > 8 && parts_of<T>() < 3 ? 2 : 1;
+}
+template <typename T>
+int run_waves(const LinearDev& l) {
+  return (l.chunks + run_chunks<T>(l) - 1) / run_chunks<T>(l);
+}
+// Whether that kernel is the faster: a CU's 16 waves have to be in use (nine to eleven
+// waves leave the others empty: 65536 x 2496 29 us, and 22.6 with k_linear_few), and W needs enough rows to
+// read and take apart x for, fewer the more parts that takes.  In bf16 2048 row blocks, one
+// row of 16384 x 2048 7.2 us and 7.1, five of 32768 x 2048 11.4 and 11.6; in f16 half as many,
+// one row of 9216 x 2048 8.6 and 8.3, of 16384 x 2048 9.0 and 9.7; in fp32 a quarter,
+// 9216 x 2048 7.9 and 10.3.
+template <typename T>
+bool stays(const LinearDev& l, const dmh_linear_rows& r) {
+  const int waves = run_waves<T>(l);
+  return r.rows <= 16 && waves <= 16 && 16 / waves * waves >= 12 &&
+         l.row_blocks >= 2048 >> (parts_of<T>() - 1);
+}
+
 template <typename T, typename O>
 hipError_t run(const LinearDev& l, const dmh_linear_rows& r, void* ws, hipStream_t st) {
   if (!few_rows(l, r)) return many<T, O>(l, r, ws, st);
+  if (stays<T>(l, r)) {
+    const auto stay = [&](auto k) {
+      const int waves = run_waves<T>(l);
+      k<<<16 / waves * 256, 64 * waves, 2 * kJoinTiles * waves * 64 * sizeof(f32x4), st>>>(l, r);
+      return hipGetLastError();
+    };
+    if (run_chunks<T>(l) == 1) return stay(k_linear_run<T, O, 1>);
+    if constexpr (parts_of<T>() < 3) return stay(k_linear_run<T, O, 2>);
+  }
   const auto few = [&](auto at, auto nt, auto waves) {
     constexpr int AT = decltype(at)::value, NT = decltype(nt)::value, W = decltype(waves)::value;
     const dim3 grid((l.row_blocks + AT - 1) / AT, (r.rows + 16 * NT - 1) / (16 * NT));
@@ -389,15 +508,16 @@ hipError_t run(const LinearDev& l, const dmh_linear_rows& r, void* ws, hipStream
   const integral_constant<int, 8> eight{};
   // More tiles to a workgroup reuse what is loaded and dequantised, more workgroups and
   // waves load sooner.  One row: 2048 x 4096 4.3 us with 16 waves and 4.7 with 8, 9216 x
-  // 2048 5.7 with 8 and 6.5 with two tiles; five rows of 100000 x 2048 32 us with two
-  // tiles and 41 with one.  32 rows of 2048 x 4096 6.9 us with one tile, 7.4 with two; 64
-  // rows 7.6 with two, 11.0 with one; 128 rows 10.1 with four, 12.4 with two; of 9216 x
-  // 2048 32 rows 8.6 with four times two, 64 rows 13.0, with one 17.
+  // 2048 5.7 with 8 and 6.5 with two tiles; five rows of 65536 x 8192 65 us with four tiles
+  // or two and 82 with one, 16 rows 65 with four, 79 with two.  32 rows of 2048 x 4096 6.9 us
+  // with one tile, 7.4 with two; 64 rows 7.6 with two, 11.0 with one; 128 rows 10.1 with
+  // four, 12.4 with two; of 9216 x 2048 32 rows 8.6 with four times two, 64 rows 13.0, with
+  // one 17.
   const int64_t u = units(l, r);
   if (r.rows <= 16) {
     if (l.row_blocks < 256) return few(one, one, integral_constant<int, 16>{});
     if (l.row_blocks < 1024) return few(one, one, eight);
-    if (l.row_blocks >= 4096 && (r.rows > 8 || parts_of<T>() > 1)) return few(four, one, four);
+    if (l.row_blocks >= 4096) return few(four, one, four);
     return few(two, one, four);
   }
   if (u < 512) return few(one, one, eight);

@@ -83,6 +83,40 @@ def test_rows_of_many_tiles(block, n, k, rows):
         check(y, x, w, None, k)
 
 
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("n,k", [(32753, 32), (32768, 352), (33001, 1024), (32790, 1184), (32769, 1632),
+                                 (40000, 2048), (32785, 2080), (32777, 4064), (32768, 4160)])
+def test_few_rows_of_large_layers(block, n, k, t):
+    """One to 17 rows of layers that take many tiles a workgroup, of whole and odd sizes: rows
+    apart, rows that are not finite, and nothing written beside the results."""
+    g = gen("large", n, k)
+    w, scales, packed = weights(g, n, k, 32)
+    bias = torch.randn(n, generator=g)
+    lin = QuantLinear(block, n, k, scales.cuda(), packed.cuda(), 32, bias=bias.cuda())
+    plain = QuantLinear(block, n, k, scales.cuda(), packed.cuda(), 32)
+    for rows, out, layer in ((1, t, lin), (5, torch.float32, plain), (16, t, plain), (17, t, lin)):
+        x = torch.randn((rows, k), generator=g).to(t)
+        wide = torch.full((rows + 1, k + 40), float("nan"), dtype=t, device="cuda")
+        wide[:rows, 8:8 + k] = x
+        y = torch.full((rows + 1, n + 5), 3.0, dtype=out, device="cuda")
+        torch.cuda.synchronize()
+        layer(wide[:rows, 8:8 + k], y[:rows, 2:2 + n])
+        block.sync()
+        check(y[:rows, 2:2 + n], x, w, bias if layer is lin else None, k)
+        assert (y[rows:] == 3).all() and (y[:, :2] == 3).all() and (y[:, 2 + n:] == 3).all()
+        if rows == 5:
+            clean = y.clone()
+            wide[2, 8 + k - 1] = float("nan")
+            torch.cuda.synchronize()
+            layer(wide[:rows, 8:8 + k], y[:rows, 2:2 + n])
+            block.sync()
+            assert y[2, 2:2 + n].isnan().all()
+            y[2] = clean[2]
+            assert torch.equal(y, clean)
+    lin.close()
+    plain.close()
+
+
 def test_rows_do_not_meet(block):
     """A row that is not finite makes its own results so, and no other's."""
     g = gen("nan")
