@@ -73,7 +73,9 @@ __device__ __forceinline__ void to_parts(Vec<T, 8> v, bf16x8 (&out)[PARTS]) {
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+        // (fp32 values are cut off first, as the largest have no bf16 above them)
+        w[i] = PARTS == 3 && q == 0 ? f2u(r[2 * i]) >> 16 | (f2u(r[2 * i + 1]) & 0xFFFF0000u)
+                                    : pack_bf16x2(r[2 * i], r[2 * i + 1]);
         r[2 * i] -= bf16lo(w[i]);
         r[2 * i + 1] -= bf16hi(w[i]);
       }

@@ -691,8 +691,9 @@ int dmh_upload_linear(dmh_ctx* ctx, const dmh_linear_weights* w, unsigned flags,
 int dmh_free_linear(dmh_ctx* ctx, dmh_linear* linear);
 
 /* Rows x [rows][in_features] of dtype to y [rows][out_features] of out_dtype (dtype or
- * DMH_DTYPE_F32).  Products are exact, sums fp32, and y is rounded once; strides are in
- * elements between rows. */
+ * DMH_DTYPE_F32).  Products are exact, but for parts of x below 2^-126, which count as 0;
+ * sums are fp32, and y is rounded once.  An element that is not finite makes the results of
+ * its row so, NaN where x is not bf16, and no other's.  Strides are in elements between rows. */
 typedef struct {
   int32_t dtype, out_dtype;
   int32_t rows;

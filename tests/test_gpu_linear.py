@@ -194,6 +194,31 @@ def test_from_a_quant_model(block, tmp_path):
     check(y, x, w, None, 128)
 
 
+@pytest.mark.parametrize("rows", [1, 16, 20, 400])
+@pytest.mark.parametrize("n", [200, 20000, 33000])
+def test_largest_values(block, n, rows):
+    """The largest fp32 value, which has no bf16 above it; infinities stay in their row."""
+    if n * rows > 4 << 20:
+        n = 1500
+    g = gen("largest", n)
+    w, scales, packed = weights(g, n, 160, 32)
+    lin = QuantLinear(block, n, 160, scales.cuda(), packed.cuda(), 32)
+    for t in TYPES.values():
+        x = torch.randn((rows, 160), generator=g).to(t)
+        x[0, 77] = torch.finfo(t).max
+        x[rows - 1, 3] = -torch.finfo(t).max
+        y, z = (torch.empty(rows, n, device="cuda") for _ in range(2))
+        a, b = x.cuda(), x.cuda()
+        b[0, 100] = float("inf")
+        torch.cuda.synchronize()
+        lin(a, y)
+        lin(b, z)
+        block.sync()
+        check(y, x, w, None, 160)
+        assert not z[0].isfinite().any() and torch.equal(y[1:], z[1:])
+    lin.close()
+
+
 def test_too_many_rows(block):
     """More tiles than a launch holds are refused before anything is read."""
     import ctypes as C
