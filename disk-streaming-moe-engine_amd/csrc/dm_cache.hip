@@ -4,9 +4,11 @@
 // on its largest element and its scale, and each makes one word of codes.  The
 // hardware converts both ways (round to nearest even, above 6 to 6).  A workgroup first
 // finds where its rows lie in the cache, a chain of four loads one behind the other, and
-// then has up to 16 words for each thread, four on their way at a time: bound by
+// then has up to 16 words for each thread, two on their way at a time: bound by
 // that chain for few rows (32 of 2 heads of 256: 5 us) and by bytes for many (16384 rows of 8
-// heads of 128 in f16, 86 MB: 26 us, 3.3 TB/s, and 38 with one word a thread).
+// heads of 128 in f16, 86 MB: 25 us, 3.4 TB/s, and 38 with one word a thread).  Four words on
+// their way leave fewer waves a SIMD: 8192 rows of 4 heads of 64, there and back, 15.9 us, and
+// 13.6 with two.
 #include <algorithm>
 #include <type_traits>
 
@@ -113,6 +115,8 @@ struct Word {
               : *reinterpret_cast<const uint32_t*>(codes + L::key_word(pos, u));
     unit = (uint32_t)*scale << 23;
   }
+  // PAST: past the L2, which many rows would fill.
+  template <bool PAST>
   __device__ __forceinline__ void read(uint32_t z, uint32_t unit) const {
     if (!in) return;
     const uint32_t p[4] = {held_pair<0>(z, unit), held_pair<1>(z, unit), held_pair<2>(z, unit),
@@ -123,23 +127,34 @@ struct Word {
       f[2 * i] = bf16lo(p[i]);
       f[2 * i + 1] = bf16hi(p[i]);
     }
-    store_f32<8>(x, f);
+    if constexpr (PAST) {
+      Vec<T, 8> v;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (T)f[i];
+      __builtin_nontemporal_store(v, reinterpret_cast<Vec<T, 8>*>(x));
+    } else {
+      store_f32<8>(x, f);
+    }
   }
 };
 
 constexpr int kMostWords = 16;                        // of a thread
-constexpr int kMostRows = 256 * kMostWords / 8 + 2;   // of a workgroup, at 8 words a row
+constexpr int kMostRows = 256 * kMostWords / 8 + 8;   // of a workgroup, at 8 words a row
 
+// Words come four rows at a time, those of one head in the four rows together: what they hold
+// of values is one piece of the cache then.
 template <typename T, int NB, bool WRITE>
 __global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqDev s, int words,
                                                  int64_t block0) {
   const int tid = threadIdx.x;
-  const int per_row = 2 * c.heads * 4 * NB;
+  const uint32_t per_four = 4 * 2 * c.heads * 4 * NB;  // words of four rows
   const int64_t block = block0 + blockIdx.x;
   const int64_t first = block * (256 * words);
   // (fewer than 2^30 rows)
-  const int t0 = (int)least(first / per_row, s.rows);
-  const int t1 = (int)least((first + 256 * words - 1) / per_row + 1, s.rows);
+  const int q0 = (int)least(first / per_four, (s.rows + 3) / 4);
+  const uint32_t base = (uint32_t)least(first - (int64_t)q0 * per_four, per_four);
+  const int t0 = 4 * q0;
+  const int t1 = (int)least(t0 + 4 * (int64_t)((base + 256 * words - 1) / per_four + 1), s.rows);
 
   __shared__ int found;
   __shared__ struct { int begin, end, past, slot, seq; } part[kMostRows];
@@ -177,15 +192,16 @@ __global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqD
   __syncthreads();
 
   const auto word = [&](int k) {
-    const int64_t i = first + 256 * k + tid;
-    const int64_t row = i / per_row;
-    const int t = (int)least(row, s.rows);
+    const uint32_t i = base + 256 * k + tid, four = i / per_four, in_four = i - four * per_four;
+    const int in_head = in_four % (4 * 4 * NB);
+    const int t = t0 + 4 * (int)four + in_head / (4 * NB);
     const bool in = t < t1 && page_of_row[t - t0] >= 0;
     const int at = in ? t - t0 : 0;
-    return Word<T, NB>(c, r, in, in ? t : 0, (int)(i - row * per_row), in ? page_of_row[at] : 0,
+    return Word<T, NB>(c, r, in, in ? t : 0,
+                       in_four / (4 * 4 * NB) * (4 * NB) + in_head % (4 * NB), in ? page_of_row[at] : 0,
                        in ? pos_of_row[at] : 0);
   };
-  constexpr int B = 4;
+  constexpr int B = 2;
   for (int k0 = 0; k0 < words; k0 += B) {
     Word<T, NB> w[B];
 #pragma unroll
@@ -204,7 +220,7 @@ __global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqD
 #pragma unroll
       for (int b = 0; b < B; ++b) w[b].fetch(z[b], unit[b]);
 #pragma unroll
-      for (int b = 0; b < B; ++b) w[b].read(z[b], unit[b]);
+      for (int b = 0; b < B; ++b) w[b].template read<true>(z[b], unit[b]);
     }
   }
 }
@@ -248,7 +264,7 @@ __global__ __launch_bounds__(256) void k_kv_few(CacheDev c, dmh_kv_rows r, SeqDe
   } else {
     uint32_t z, unit;
     w.fetch(z, unit);
-    w.read(z, unit);
+    w.template read<false>(z, unit);
   }
 }
 
@@ -258,7 +274,7 @@ hipError_t run(const dmh_kv_cache& c, const dmh_kv_rows& r, const SeqDev& s, hip
     return with_blocks(c.dim, [&](auto nb) {
       using T = decltype(t);
       constexpr int NB = decltype(nb)::value;
-      const int64_t all = (int64_t)s.rows * 2 * c.kv_heads * 4 * NB;  // words
+      const int64_t all = (s.rows + (int64_t)3) / 4 * 4 * 2 * c.kv_heads * 4 * NB;  // words
       // as many to a thread as leave four workgroups a CU (32 rows of 2 heads of 256: 4.4 us
       // with none, which the first kernel does in 6.5)
       const int words = (int)std::min<int64_t>(kMostWords, all / (256 * 1024));

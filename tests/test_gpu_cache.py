@@ -120,6 +120,39 @@ def test_write_and_read(block, dim, t):
     assert int((c.scales != scales).sum()) <= rows * 2 * heads * dim // 32
 
 
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("heads,more", [(1, 1.01), (5, 1.5), (3, 3.7)])
+def test_many_rows_at_once(block, dim, t, heads, more):
+    """Calls of several words a thread, of sequences that begin and end anywhere among four
+    rows, hold what the definition gives, in rows with gaps between heads."""
+    g = gen("at once", dim, heads)
+    rows = int(more * 2 ** 20) // (heads * dim) + 3
+    lens = [1, 2, 3, 0, 517, 5, rows - 528]
+    c = Cache(block, g, [3, 0, 6, 9, 77, 2, 14], lens, heads, dim, 16)
+    k, v = (torch.full((rows + 5, heads + 1, dim), 7.0, dtype=t, device="cuda") for _ in range(2))
+    x = [spread(g, (rows, heads, dim), t) for _ in range(2)]
+    k[:rows, :heads], v[:rows, 1:] = x[0].cuda(), x[1].cuda()
+    out = [torch.full((rows + 5, heads + 1, dim), 3.0, dtype=t, device="cuda") for _ in range(2)]
+    before = c.codes.clone()
+    torch.cuda.synchronize()
+    c.cache.write(k[:, :heads], v[:, 1:], c.batch(pad=5))
+    c.cache.read(out[0][:, 1:], out[1][:, :heads], c.batch(pad=5))
+    block.sync()
+    for got, y in ((out[0][:, 1:], x[0]), (out[1][:, :heads], x[1])):
+        assert torch.equal(got[:rows].double().cpu(), R.held(y).to(t).double())
+    assert (out[0][:, 0] == 3).all() and (out[1][:, heads] == 3).all()
+    assert all((o[rows:] == 3).all() for o in out)
+    # rows of the pages in front of a sequence's and behind them stay
+    for slot, past, n in zip(c.slots.tolist(), c.past, lens):
+        for pos in (past - 1, past + n):
+            if pos < 0 or pos >= -(-(past + n) // 16) * 16:
+                continue
+            page = c.pages[slot, pos // 16].item()
+            # (a key's codes lie together, in the order of positions)
+            assert torch.equal(c.codes[page, 0, :, pos % 16], before[page, 0, :, pos % 16])
+
+
 @pytest.mark.parametrize("page", [16, 64, 1024])
 def test_write_in_steps(block, page):
     """Rows written one by one and a few at a time give the bytes of one call."""
