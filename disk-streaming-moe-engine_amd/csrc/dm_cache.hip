@@ -229,9 +229,10 @@ __global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqD
 template <typename T, int NB, bool WRITE>
 __global__ __launch_bounds__(256) void k_kv_few(CacheDev c, dmh_kv_rows r, SeqDev s) {
   const int tid = threadIdx.x;
-  const int per_row = 2 * c.heads * 4 * NB;
-  const int64_t i = (int64_t)blockIdx.x * 256 + tid;
-  const int t0 = (int)least((i - tid) / per_row, s.rows), t = (int)least(i / per_row, s.rows);
+  const uint32_t per_row = 2 * c.heads * 4 * NB;
+  const uint32_t i = blockIdx.x * 256 + tid;  // (2^20 at most)
+  const int t0 = min((int)(blockIdx.x * 256 / per_row), s.rows);
+  const int t = min((int)(i / per_row), s.rows);
 
   // the first sequence with a row at t0 or behind it, then this row's
   __shared__ int first_seq;
@@ -257,7 +258,7 @@ __global__ __launch_bounds__(256) void k_kv_few(CacheDev c, dmh_kv_rows r, SeqDe
     record_err(s.status, err_key(kPhSeq, 0, 0, (uint32_t)q, kSqPage));
     return;
   }
-  const Word<T, NB> w(c, r, true, t, (int)(i - (int64_t)t * per_row), page,
+  const Word<T, NB> w(c, r, true, t, (int)(i - t * per_row), page,
                       pos & ((1 << c.page_shift) - 1));
   if constexpr (WRITE) {
     w.write(load_raw<8>(w.x));
