@@ -6,9 +6,9 @@
 // finds where its rows lie in the cache, a chain of four loads one behind the other, and
 // then has up to 16 words for each thread, two on their way at a time: bound by
 // that chain for few rows (32 of 2 heads of 256: 5 us) and by bytes for many (16384 rows of 8
-// heads of 128 in f16, 86 MB: 25 us, 3.4 TB/s, and 38 with one word a thread).  Four words on
-// their way leave fewer waves a SIMD: 8192 rows of 4 heads of 64, there and back, 15.9 us, and
-// 13.6 with two.
+// heads of 128 in f16, 86 MB: 20 us, 4.3 TB/s; 25 where each word's place takes divisions, and
+// 38 with one word a thread).  Four words on their way leave fewer waves a SIMD: 8192
+// rows of 4 heads of 64, there and back, 14.2 us, and 12.9 with two.
 #include <algorithm>
 #include <type_traits>
 
@@ -58,6 +58,24 @@ __device__ __forceinline__ uint32_t load_value(const uint8_t* region, size_t pos
   }
 }
 
+// The size of the largest of eight elements, as fp32 bits: a NaN is larger than any number.
+template <typename T>
+__device__ __forceinline__ uint32_t largest(Vec<T, 8> raw) {
+  if constexpr (sizeof(T) == 2) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    const uint4 w = __builtin_bit_cast(uint4, raw);
+    const auto size = [](uint32_t x) { return __builtin_bit_cast(u16x2, x & 0x7FFF7FFFu); };
+    const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(size(w.x), size(w.y)),
+                                              __builtin_elementwise_max(size(w.z), size(w.w)));
+    return f2u((float)__builtin_bit_cast(T, m.x > m.y ? m.x : m.y));
+  } else {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, f2u(raw[i]) & 0x7FFFFFFFu);
+    return most;
+  }
+}
+
 // Eight elements of a row and their place in the cache.
 template <typename T, int NB>
 struct Word {
@@ -67,29 +85,34 @@ struct Word {
   size_t pos;
   int u;
   bool value, in;  // in: there is such a row
-  // in_row: words of keys of all heads, then of values.
   __device__ __forceinline__ Word() {}
-  __device__ __forceinline__ Word(const CacheDev& c, const dmh_kv_rows& r, bool in, int t, int in_row,
-                                  int page, int pos)
-      : pos(pos), in(in) {
+  // in_row: words of keys of all heads, then of values.
+  __device__ __forceinline__ Word(const CacheDev& c, const dmh_kv_rows& r, int t, int in_row, int page,
+                                  int pos)
+      : in(true) {
     const int half = c.heads * 4 * NB;
     value = in_row >= half;
     in_row -= value ? half : 0;
     const int head = in_row / (4 * NB);
     u = in_row - head * (4 * NB);
-    const size_t region = region_of(c, page, value, head) << c.page_shift;
+    place(c, region_of(c, page, value, head) << c.page_shift, pos);
+    x = row(r, t, head);
+  }
+  __device__ __forceinline__ T* row(const dmh_kv_rows& r, int t, int head) const {
+    return static_cast<T*>(value ? r.v : r.k) + (int64_t)t * (value ? r.v_stride : r.k_stride) +
+           head * (value ? r.v_head_stride : r.k_head_stride) + 8 * u;
+  }
+  // region: the tokens in front of a page's of this head.
+  __device__ __forceinline__ void place(const CacheDev& c, size_t region, int at) {
+    pos = at;
     codes = c.codes + region * L::row;
     scale = c.scales + region * NB + (value ? L::value_scale(pos, u >> 2) : L::key_scale(pos, u >> 2));
-    x = static_cast<T*>(value ? r.v : r.k) + (int64_t)t * (value ? r.v_stride : r.k_stride) +
-        head * (value ? r.v_head_stride : r.k_head_stride) + 8 * u;
   }
   // (four lanes with the words of one block together)
   __device__ __forceinline__ void write(Vec<T, 8> raw) const {
     float f[8];
     to_f32<8>(raw, f);
-    uint32_t most = 0;  // as bits: a NaN is larger than any number
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, f2u(f[i]) & 0x7FFFFFFFu);
+    uint32_t most = largest<T>(raw);
     most = max(most, (uint32_t)__shfl_xor((int)most, 1));
     most = max(most, (uint32_t)__shfl_xor((int)most, 2));
     // 2^X with |x| <= 7 * 2^X: X = floor(log2) - 2, or one more above 1.75 * 2^floor
@@ -139,22 +162,23 @@ struct Word {
 };
 
 constexpr int kMostWords = 16;                        // of a thread
-constexpr int kMostRows = 256 * kMostWords / 8 + 8;   // of a workgroup, at 8 words a row
+constexpr int kMostRows = 4 * kMostWords * 8;  // of a workgroup: four rows have 32 words or more
 
-// Words come four rows at a time, those of one head in the four rows together: what they hold
-// of values is one piece of the cache then.
+// A thread has the same word of every fourth row, so that only the page changes from one to
+// the next; the words of one head in four rows lie together, whose values are one piece of
+// the cache.  Where four rows have fewer than 256 words, `side` of them lie side by side;
+// where they have more, `chunks` workgroups share them.
 template <typename T, int NB, bool WRITE>
-__global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqDev s, int words,
-                                                 int64_t block0) {
+__global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqDev s, int words, int side,
+                                                 int chunks, int64_t block0) {
   const int tid = threadIdx.x;
-  const uint32_t per_four = 4 * 2 * c.heads * 4 * NB;  // words of four rows
+  const int per_four = 4 * 2 * c.heads * 4 * NB;
   const int64_t block = block0 + blockIdx.x;
-  const int64_t first = block * (256 * words);
+  const int64_t rows_at = block / chunks;
+  const int chunk = (int)(block - rows_at * chunks);
   // (fewer than 2^30 rows)
-  const int q0 = (int)least(first / per_four, (s.rows + 3) / 4);
-  const uint32_t base = (uint32_t)least(first - (int64_t)q0 * per_four, per_four);
-  const int t0 = 4 * q0;
-  const int t1 = (int)least(t0 + 4 * (int64_t)((base + 256 * words - 1) / per_four + 1), s.rows);
+  const int t0 = (int)least(rows_at * (4 * words * side), s.rows);
+  const int t1 = (int)least((int64_t)t0 + 4 * words * side, s.rows);
 
   __shared__ int found;
   __shared__ struct { int begin, end, past, slot, seq; } part[kMostRows];
@@ -191,24 +215,30 @@ __global__ __launch_bounds__(256) void k_kv_rows(CacheDev c, dmh_kv_rows r, SeqD
   }
   __syncthreads();
 
+  const int at = chunk * 256 + tid, beside = at / per_four, in_four = at - beside * per_four;
+  const int in_head = in_four % (4 * 4 * NB), mine = 4 * beside + in_head / (4 * NB);
+  Word<T, NB> first;
+  int head = in_four / (4 * 4 * NB);
+  first.value = head >= c.heads;
+  const size_t head_at = (size_t)head << c.page_shift, page_tokens = (size_t)(2 * c.heads) << c.page_shift;
+  head -= first.value ? c.heads : 0;
+  first.u = in_head % (4 * NB);
+  const int64_t step = 4 * side * (first.value ? r.v_stride : r.k_stride);
+  first.x = first.row(r, t0 + mine, head);
   const auto word = [&](int k) {
-    const uint32_t i = base + 256 * k + tid, four = i / per_four, in_four = i - four * per_four;
-    const int in_head = in_four % (4 * 4 * NB);
-    const int t = t0 + 4 * (int)four + in_head / (4 * NB);
-    const bool in = t < t1 && page_of_row[t - t0] >= 0;
-    const int at = in ? t - t0 : 0;
-    return Word<T, NB>(c, r, in, in ? t : 0,
-                       in_four / (4 * 4 * NB) * (4 * NB) + in_head % (4 * NB), in ? page_of_row[at] : 0,
-                       in ? pos_of_row[at] : 0);
+    Word<T, NB> w = first;
+    const int row = mine + 4 * side * k;
+    w.in = beside < side && k < words && t0 + row < t1 && page_of_row[row] >= 0;
+    const int from = w.in ? row : 0;
+    w.place(c, (w.in ? page_of_row[from] : 0) * page_tokens + head_at, pos_of_row[from]);
+    w.x = first.x + k * step;
+    return w;
   };
   constexpr int B = 2;
   for (int k0 = 0; k0 < words; k0 += B) {
     Word<T, NB> w[B];
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-      w[b] = word(min(k0 + b, words - 1));
-      w[b].in = w[b].in && k0 + b < words;
-    }
+    for (int b = 0; b < B; ++b) w[b] = word(k0 + b);
     if constexpr (WRITE) {
       Vec<T, 8> raw[B];
 #pragma unroll
@@ -258,7 +288,7 @@ __global__ __launch_bounds__(256) void k_kv_few(CacheDev c, dmh_kv_rows r, SeqDe
     record_err(s.status, err_key(kPhSeq, 0, 0, (uint32_t)q, kSqPage));
     return;
   }
-  const Word<T, NB> w(c, r, true, t, (int)(i - t * per_row), page,
+  const Word<T, NB> w(c, r, t, (int)(i - t * per_row), page,
                       pos & ((1 << c.page_shift) - 1));
   if constexpr (WRITE) {
     w.write(load_raw<8>(w.x));
@@ -275,7 +305,7 @@ hipError_t run(const dmh_kv_cache& c, const dmh_kv_rows& r, const SeqDev& s, hip
     return with_blocks(c.dim, [&](auto nb) {
       using T = decltype(t);
       constexpr int NB = decltype(nb)::value;
-      const int64_t all = (s.rows + (int64_t)3) / 4 * 4 * 2 * c.kv_heads * 4 * NB;  // words
+      const int64_t per_row = 2 * c.kv_heads * 4 * NB, all = s.rows * per_row;  // words
       // as many to a thread as leave four workgroups a CU (32 rows of 2 heads of 256: 4.4 us
       // with none, which the first kernel does in 6.5)
       const int words = (int)std::min<int64_t>(kMostWords, all / (256 * 1024));
@@ -284,12 +314,14 @@ hipError_t run(const dmh_kv_cache& c, const dmh_kv_rows& r, const SeqDev& s, hip
         k_kv_few<T, NB, WRITE><<<(unsigned)blocks, 256, 0, st>>>(cache_dev(c), r, s);
         return hipGetLastError();
       }
-      const int some = std::max(words, 1);
-      const int64_t blocks = std::max<int64_t>((all + 256 * some - 1) / (256 * some), s.num);
+      const int some = std::max(words, 1), per_four = (int)(4 * per_row);
+      const int side = std::max(256 / per_four, 1), chunks = (per_four + 255) / 256;
+      const int64_t blocks =
+          std::max<int64_t>((s.rows + (int64_t)(4 * some * side) - 1) / (4 * some * side) * chunks, s.num);
       constexpr int64_t most = 1 << 23;  // 2^31 threads a launch
       for (int64_t b = 0; b < blocks; b += most)
         k_kv_rows<T, NB, WRITE><<<(unsigned)std::min(most, blocks - b), 256, 0, st>>>(
-            cache_dev(c), r, s, some, b);
+            cache_dev(c), r, s, some, side, chunks, b);
       return hipGetLastError();
     });
   });
