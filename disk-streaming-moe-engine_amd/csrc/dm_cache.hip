@@ -6,7 +6,7 @@
 // finds where its rows lie in the cache, a chain of four loads one behind the other, and
 // then has up to 16 words for each thread, two on their way at a time: bound by
 // that chain for few rows (32 of 2 heads of 256: 5 us) and by bytes for many (16384 rows of 8
-// heads of 128 in f16, 86 MB: 20 us, 4.3 TB/s; 25 where each word's place takes divisions, and
+// heads of 128 in f16, 86 MB: 19 us, 4.5 TB/s; 25 where each word's place takes divisions, and
 // 38 with one word a thread).  Four words on their way leave fewer waves a SIMD: 8192
 // rows of 4 heads of 64, there and back, 14.2 us, and 12.9 with two.
 #include <algorithm>
