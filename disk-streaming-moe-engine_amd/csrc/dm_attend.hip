@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "dm_attend_walk.h"
 #include "dm_cache_device.h"
 
 namespace dm {
@@ -901,28 +902,6 @@ struct Share64 {
   }
 };
 
-constexpr int kManyRows = 128;
-constexpr double kUnitCost = 320;   // of beginning and ending a unit, in tokens of its context
-constexpr double kShareCost = 512;  // the least that is worth a workgroup
-
-// The units of a sequence, a head's blocks of rows one behind the other, on a line whose
-// lengths are what they cost: about the tokens of the context up to a block's last row.
-// Workgroups take equal shares of the line.  All of them compute a place on it by the
-// same operations, so they agree on who has which part of a unit.
-struct Line {
-  int blocks;       // of a head
-  double one, per;  // block b costs one + per * (b + 1)
-  __device__ __forceinline__ Line(const AttendDev& d, const CacheSeq& q) {
-    const int64_t rows = (int64_t)q.n * d.rep;
-    blocks = rows > d.few_rows ? (int)((rows + kManyRows - 1) / kManyRows) : 0;
-    one = kUnitCost + q.past;
-    per = (double)kManyRows / d.rep;
-  }
-  __device__ __forceinline__ double to(int b) const {  // the blocks before b
-    return b * one + per * (0.5 * b * (b + 1.0));
-  }
-};
-
 // Places of a unit's part: of 16 rows and j, 64 lanes of four outputs; then the rows' m, l.
 template <int NB>
 __device__ __forceinline__ size_t many_part(int place) {
@@ -939,76 +918,48 @@ __global__ __launch_bounds__(4 * kManyRows / MT, 2) void k_attend_many(AttendDev
   const int group = blockIdx.x;
   __shared__ __align__(16) uint8_t lds[2][S::buffer];
   __shared__ int nans[2][NW];
-  __shared__ double wsum[NW], ends[64 * NW];
+  __shared__ int64_t wsum[NW], ends[64 * NW];
   __shared__ CacheSeq seqs[64 * NW];
+  const ManyCost cost(d.rep, d.few_rows);
 
   // The lengths of as many sequences as there are threads, from i0 on, summed up in ends.
   const auto count = [&](int i0) {
     CacheSeq q = {};
-    double sum = 0.0;
+    int64_t sum = 0;
     if (i0 + tid < d.s.num) {
       q = cache_seq(d.c, d.s, i0 + tid, group == 0);
-      const Line line(d, q);
-      sum = d.c.heads * line.to(line.blocks);
+      sum = d.c.heads * ManyLine(cost, q.n, q.past).head();
     }
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
-      const double x = __shfl_up(sum, o);
+      const int64_t x = __shfl_up(sum, o);
       if (lane >= o) sum += x;
     }
     __syncthreads();
     if (lane == 63) wsum[wave] = sum;
     seqs[tid] = q;
     __syncthreads();
-    double before = 0.0;
+    int64_t before = 0;
     for (int i = 0; i < wave; ++i) before += wsum[i];
     ends[tid] = before + sum;
     __syncthreads();
     return ends[64 * NW - 1];
   };
-  double total = count(0);
+  int64_t total = count(0);
   for (int i0 = 64 * NW; i0 < d.s.num; i0 += 64 * NW) total += count(i0);
-  const int groups = (int)fmin(ceil(total / kShareCost), (double)gridDim.x);
+  const ManyShares shares(cost, total, (int)gridDim.x);
   if (tid == 0) d.meta[group].parts = 0;
-  if (group >= groups) return;
-  const auto share = [&](int w) { return total * w / groups; };
-  const double hi = group + 1 < groups ? share(group + 1) : total;
-  double at = share(group), base = 0.0;
-  int slot = 0;  // unfinished units of this workgroup so far
-  for (int i0 = 0; i0 < d.s.num && at < hi; i0 += 64 * NW) {
-    const double sum = d.s.num > 64 * NW ? count(i0) : total;
-    while (at < hi && at < base + sum) {
-      // the sequence, head and block that `at` lies in, and where that begins and ends
-      int i = 0;
-      for (int step = 32 * NW; step; step /= 2)
-        if (base + ends[i + step - 1] <= at) i += step;
-      i = __builtin_amdgcn_readfirstlane(i);
-      const CacheSeq q = seqs[i];
-      const Line line(d, q);
-      const double first = base + (i ? ends[i - 1] : 0.0), head = line.to(line.blocks);
-      int h = min((int)((at - first) / head), d.c.heads - 1);
-      while (h > 0 && first + h * head > at) --h;
-      while (h + 1 < d.c.heads && first + (h + 1) * head <= at) ++h;
-      int b = 0;
-      for (int step = 1 << (31 - __clz(line.blocks)); step; step /= 2)
-        if (b + step < line.blocks && first + h * head + line.to(b + step) <= at) b += step;
-      h = __builtin_amdgcn_readfirstlane(h);
-      b = __builtin_amdgcn_readfirstlane(b);
-      const double begin = first + h * head + line.to(b);
-      const double end = b + 1 < line.blocks   ? first + h * head + line.to(b + 1)
-                         : h + 1 < d.c.heads ? first + (h + 1) * head
-                                             : base + ends[i];
+  if (group >= shares.groups) return;
+  many_walk<64 * NW>(
+    cost, shares, group, d.s.num, ends, count, [&](int i) { return seqs[i]; },
+    [&](int i0, int i, const CacheSeq& q, const ManyPart& unit, int slot) {
+      const int h = __builtin_amdgcn_readfirstlane(unit.head);
+      const int b = __builtin_amdgcn_readfirstlane(unit.block);
+      const int from = __builtin_amdgcn_readfirstlane(unit.from);
+      const int to = __builtin_amdgcn_readfirstlane(unit.to);
+      const bool starts = unit.starts, whole = unit.whole;
       const int64_t rows = (int64_t)q.n * d.rep, block0 = (int64_t)b * kManyRows;
       const int64_t row0 = block0 + wave * (16 * MT);
-      const int tokens = q.past + (int)((least(block0 + kManyRows, rows) - 1) / d.rep) + 1;
-      const int steps = (tokens + 63) / 64;
-      const auto step_at = [&](double x) {
-        return min((int)((x - begin) / (end - begin) * steps), steps);
-      };
-      const bool starts = at == begin, whole = starts && hi >= end;
-      const int from = __builtin_amdgcn_readfirstlane(starts ? 0 : step_at(at));
-      const int to = __builtin_amdgcn_readfirstlane(hi >= end ? steps : step_at(hi));
-
       const int first_seen = q.past + (int)(block0 / d.rep);
       const int last_seen =
           row0 < rows ? q.past + (int)((least(row0 + 16 * MT, rows) - 1) / d.rep) : -1;
@@ -1073,12 +1024,8 @@ __global__ __launch_bounds__(4 * kManyRows / MT, 2) void k_attend_many(AttendDev
       while (t0 < stop) tile(std::true_type{});
       settle(w.o);
       if (u.bad) record_err(d.s.status, err_key(kPhSeq, 0, 0, (uint32_t)(i0 + i), kSqPage));
-      if (starts && !whole && tid == 0) {
-        int g = min((int)(end / total * groups), groups);  // the first whose share begins behind
-        while (g > group + 1 && share(g - 1) >= end) --g;
-        while (g < groups && share(g) < end) ++g;
-        d.meta[group] = {group, g - group, 2 * group + slot, q.begin, q.n, h, b, 0};
-      }
+      if (starts && !whole && tid == 0)
+        d.meta[group] = {group, shares.parts(group, unit.end), 2 * group + slot, q.begin, q.n, h, b, 0};
       float* const part = d.part + many_part<NB>(2 * group + slot);
 #pragma unroll
       for (int k = 0; k < MT; ++k) {
@@ -1097,11 +1044,7 @@ __global__ __launch_bounds__(4 * kManyRows / MT, 2) void k_attend_many(AttendDev
           }
         }
       }
-      slot += !whole;
-      at = end;
-    }
-    base += sum;
-  }
+    });
 }
 
 // The parts of a unit joined: a workgroup takes 16 rows and JG of the j of their outputs, each of
