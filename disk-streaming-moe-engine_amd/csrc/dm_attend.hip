@@ -125,7 +125,8 @@ __device__ __forceinline__ float sum_quads(float x) {
   return u2f(p[0]) + u2f(p[1]);
 }
 
-// x as PARTS bf16 values whose sum it is, to 8 bits each.
+// x as PARTS bf16 values whose sum it is, to 8 bits each.  (The first of three is cut off, not
+// rounded: the largest fp32 values have no bf16 above them.)
 template <int PARTS>
 __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&out)[PARTS]) {
   float r[8];
@@ -136,7 +137,8 @@ __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&out)[PARTS])
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+      w[i] = PARTS == 3 && p == 0 ? f2u(r[2 * i]) >> 16 | (f2u(r[2 * i + 1]) & 0xFFFF0000u)
+                                  : pack_bf16x2(r[2 * i], r[2 * i + 1]);
       if (p + 1 < PARTS) {
         r[2 * i] -= bf16lo(w[i]);
         r[2 * i + 1] -= bf16hi(w[i]);
