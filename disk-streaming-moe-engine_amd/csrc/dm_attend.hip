@@ -4,7 +4,7 @@
 // token and one of the R query heads that share the key head).  A wave takes 32
 // tokens of the context a step:
 //   S^T = K Q^T   on the matrix cores; the codes become bf16 in registers, exactly
-//   P   = e^(scale S - m) with m the running maximum of each row
+//   P   = e^(scale (S - m)) with m the running maximum of each row
 //   O^T += V^T P^T
 // With S and O transposed, lane (n, quad) holds row n of S for tokens 4 quad .. + 3
 // and 16 + 4 quad .. + 3, which is what the second product takes from it: P passes
@@ -42,7 +42,7 @@ __device__ __forceinline__ void settle(f32x4 (&c)[A][B]) {
 
 constexpr int kStep = 32;   // tokens of a step
 constexpr int kTile = 128;  // tokens of a step of four waves
-constexpr float kNone = -3e38f;  // the maximum of a row that has seen no token
+constexpr float kNone = -3.40282347e38f;  // the maximum of a row that has seen no token: no score is less
 
 // What k_attend_few leaves to k_attend_join of a unit.
 struct Meta {
@@ -304,7 +304,7 @@ struct Wave {
   static constexpr int PP = std::is_same<T, float>::value ? 3 : 2;
   bf16x8 q[MT][QP][NB];
   f32x4 o[MT][2 * NB];
-  float m[MT], l[MT];  // in units of log2; l of this lane's tokens
+  float m[MT], l[MT];  // m of scores before they are scaled; l of this lane's tokens
   int seen[MT];        // the last position that the row sees, -1: no such row
 
   // Rows row0 .. row0 + 16 MT - 1 of the sequence's n * rep.
@@ -373,9 +373,9 @@ struct Wave {
           if (MASK && t0 + 16 * a + 4 * quad + e > seen[i]) s[i][a][e] = -__builtin_inff();
           most = fmaxf(most, s[i][a][e]);
         }
-      const float now = fmaxf(m[i], max_quads(most) * c2);
+      const float now = fmaxf(m[i], max_quads(most));
       if (__any(now != m[i])) {
-        const float f = __builtin_amdgcn_exp2f(m[i] - now);
+        const float f = __builtin_amdgcn_exp2f((m[i] - now) * c2);
         l[i] *= f;
 #pragma unroll
         for (int j = 0; j < 2 * NB; ++j) o[i][j] *= f;
@@ -386,7 +386,9 @@ struct Wave {
         float z[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * g + e / 4][e % 4], c2, -now));
+          // (the difference first: the largest score's is 0 at any size, where a product's
+          // remainder would be more than fp32's exponents from 2^31 on)
+          z[e] = __builtin_amdgcn_exp2f((s[i][2 * g + e / 4][e % 4] - now) * c2);
           l[i] += z[e];
         }
         split_p<PP>(z, p[i][g]);
@@ -688,7 +690,7 @@ __global__ __launch_bounds__(256, few_waves<T>(32 * NB, MT)) void k_attend_few(A
           for (int k = 0; k < 4; ++k) m = fmaxf(m, om[k][16 * b + r]);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            f[k] = __builtin_amdgcn_exp2f(om[k][16 * b + r] - m);
+            f[k] = __builtin_amdgcn_exp2f((om[k][16 * b + r] - m) * d.c2);
             sum_l += f[k] * ol[k][16 * b + r];
             const f32x4 y = *reinterpret_cast<const f32x4*>(&oo[k][r][e0]);
 #pragma unroll
@@ -736,7 +738,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendDev d, int rows_per_u
       const float pm = p[ROWS * D + r], pl = p[ROWS * D + ROWS + r];
       const f32x4 o = *reinterpret_cast<const f32x4*>(p + r * D + 4 * x);
       const float now = fmaxf(m, pm);
-      const float a = __builtin_amdgcn_exp2f(m - now), b = __builtin_amdgcn_exp2f(pm - now);
+      const float a = __builtin_amdgcn_exp2f((m - now) * d.c2), b = __builtin_amdgcn_exp2f((pm - now) * d.c2);
       m = now;
       l = a * l + b * pl;
       v = a * v + b * o;
@@ -757,7 +759,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendDev d, int rows_per_u
   v = f32x4{};
 #pragma unroll
   for (int i = 0; i < Y; ++i) {
-    const float f = __builtin_amdgcn_exp2f(sm[i][x] - m);
+    const float f = __builtin_amdgcn_exp2f((sm[i][x] - m) * d.c2);
     l = __builtin_fmaf(f, sl[i][x], l);
     v = f * so[i][x] + v;
   }
@@ -1076,7 +1078,7 @@ __global__ __launch_bounds__(256) void k_attend_many_join(AttendDev d) {
     for (int j = 0; j < JG; ++j)
       o[j] = *reinterpret_cast<const f32x4*>(p + ((size_t)(of * 2 * NB + j0 + j) * 64 + lane) * 4);
     const float now = fmaxf(m, pm);
-    const float a = __builtin_amdgcn_exp2f(m - now), b = __builtin_amdgcn_exp2f(pm - now);
+    const float a = __builtin_amdgcn_exp2f((m - now) * d.c2), b = __builtin_amdgcn_exp2f((pm - now) * d.c2);
     m = now;
     l = a * l + b * pl;
 #pragma unroll
@@ -1097,7 +1099,7 @@ __global__ __launch_bounds__(256) void k_attend_many_join(AttendDev d) {
   for (int j = 0; j < JG; ++j) v[j] = f32x4{};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float f = __builtin_amdgcn_exp2f(sm[i][lane] - m);
+    const float f = __builtin_amdgcn_exp2f((sm[i][lane] - m) * d.c2);
     l = __builtin_fmaf(f, sl[i][lane], l);
 #pragma unroll
     for (int j = 0; j < JG; ++j) v[j] = f * so[i][j][lane] + v[j];

@@ -47,3 +47,36 @@ def test_largest_queries(block, dim, past, rows):
     for got, want, size, *_ in attend(block, past, rows, 6, 2, dim, torch.float32, scale, q, ctx):
         assert got.isfinite().all()
         M.close(got, want, size, STEPS[torch.float32])
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [2.0 ** 31, 1e12, 1e29, 1e30])
+@pytest.mark.parametrize("past,rows", [([0, 2, 0, 700], [1, 1, 2, 1]), ([0, 31], [150, 90])])
+def test_large_scores(block, past, rows, scale, t):
+    """Scores of 2^31 and more, where their rounding alone is more than fp32's exponents: a row is
+    the value of its largest score.  Some rows see negative scores alone."""
+    dim = 64
+    g = gen("scores", sum(rows), scale)
+    q = torch.randn((sum(rows), 6, dim), generator=g)
+    q[:, 1] = -q[:, 1].abs()
+    ctx = [torch.randn((2, p + n, 2, dim), generator=g) for p, n in zip(past, rows)]
+    for x in ctx:
+        x[0, :, 0] = x[0, :, 0].abs() + 0.5  # keys of query heads 0 to 2
+    at = 0
+    for i, (got, _, _, q, k, v) in enumerate(attend(block, past, rows, 6, 2, dim, t, scale, q, ctx)):
+        for r in range(rows[i]):
+            z = torch.einsum("hd,jhd->hj", q[r].double().cpu(),
+                             k[:past[i] + r + 1].repeat_interleave(3, 1))
+            top = z.topk(min(2, z.shape[1]), 1)
+            # two scores' errors, of 50 roundings of their terms each, must not change which is
+            # larger, and the difference has to leave nothing of the other's probability
+            terms = torch.einsum("hd,jhd->hj", q[r].double().cpu().abs(),
+                                 k[:past[i] + r + 1].abs().repeat_interleave(3, 1)).amax(1)
+            clear = torch.ones(6, dtype=torch.bool)
+            if z.shape[1] > 1:
+                gap = top.values[:, 0] - top.values[:, 1]
+                clear = gap > 100 * 2.0 ** -24 * terms + 2.0 ** 8 / scale
+            at += int(clear.sum())
+            want = v[top.indices[:, 0], torch.arange(6) // 3]
+            assert torch.equal(got[r].double().cpu()[clear], want.to(t).double()[clear])
+    assert at > 6 * sum(rows) * 0.95
