@@ -1154,16 +1154,17 @@ bool attend_fits(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s)
          join_blocks(a, c, s, few_tiles(a, c, s)) < kMostBlocks;
 }
 
-// (the kernels for few and for many rows come one after the other and share the place)
-size_t attend_parts(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
-  const int mt = few_tiles(a, c, s);
-  const size_t few = (size_t)few_groups(a.dtype, c.dim, mt) * 16 * mt;
-  const bool any = (int64_t)s.max_len * (a.q_heads / c.kv_heads) > few_limit(a, c);
-  return 2 * std::max(few, any ? (size_t)many_groups(c.dim) * kManyRows : 0) * (c.dim + 2);
+// The memory is the same for all lengths of sequences, so that any call of as many heads and
+// sequences may stand before one that is captured.  (The kernels for few and for many rows
+// come one after the other and share the place of parts; those for many rows, two of 128 rows
+// a workgroup, take more than two of 16 or 32.)
+size_t attend_parts(const dmh_kv_cache& c) {
+  static_assert(3 * 256 * 32 <= 256 * kManyRows, "three waves a SIMD of k_attend_few");
+  return (size_t)2 * many_groups(c.dim) * kManyRows * (c.dim + 2);
 }
 size_t attend_bytes(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
-  const size_t units = (size_t)s.num * c.kv_heads * few_blocks(a, c, s, few_tiles(a, c, s));
-  return attend_parts(a, c, s) * 4 + sizeof(Meta) * std::max(units, (size_t)many_groups(c.dim));
+  const size_t units = (size_t)s.num * c.kv_heads * ((few_limit(a, c) + 15) / 16);
+  return attend_parts(c) * 4 + sizeof(Meta) * std::max(units, (size_t)many_groups(c.dim));
 }
 
 hipError_t launch_attend(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, void* ws,
@@ -1175,7 +1176,7 @@ hipError_t launch_attend(const dmh_attention& a, const dmh_kv_cache& c, const Se
   const int mt = few_tiles(a, c, s);
   d.blocks = few_blocks(a, c, s, mt);
   d.part = static_cast<float*>(ws);
-  d.meta = reinterpret_cast<Meta*>(d.part + attend_parts(a, c, s));
+  d.meta = reinterpret_cast<Meta*>(d.part + attend_parts(c));
   return with_type(a.dtype, [&](auto t) {
     return with_blocks(c.dim, [&](auto nb) {
       using T = decltype(t);

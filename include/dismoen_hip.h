@@ -652,13 +652,14 @@ int dmh_kv_read(dmh_ctx* ctx, const dmh_kv_cache* cache, const dmh_kv_rows* rows
  * enter, whatever they hold.  The bits of a row's result may differ with the rest of
  * the batch, which the work on long contexts is divided over.
  *
- * The calls work in device memory of the context of a fixed size, kept from call to
- * call: make one before one is captured.  Replays of graphs that one context captured
- * must not overlap each other or its other calls. */
+ * The calls work in device memory of the context, kept from call to call, of a size that
+ * depends on the heads, dim and num_seqs and on no lengths: make a call of these before one is
+ * captured.  Replays of graphs that one context captured must not overlap each other or
+ * its other calls. */
 typedef struct {
   int32_t dtype;           /* of q, gate and o */
   int32_t q_heads;         /* a multiple of kv_heads, up to 4096 */
-  float scale;             /* > 0 */
+  float scale;             /* 1e-30 to 1e30 */
   const void* q;           /* [total_tokens][q_heads][dim] */
   const void* gate;        /* the same, or NULL */
   void* o;
