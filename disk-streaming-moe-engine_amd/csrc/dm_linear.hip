@@ -3,6 +3,7 @@
 // W's codes become bf16 operands of the matrix cores as they are read, each the
 // bf16 value that dequantising gives; rows of x that are not bf16 enter as two or three
 // bf16 parts that hold all of their bits, so products are exact and sums fp32.
+#include <algorithm>
 #include <type_traits>
 
 #include "dm_device.h"
@@ -12,12 +13,15 @@
 namespace dm {
 namespace {
 
+constexpr int64_t kMostBlocks = 1 << 23;  // workgroups of a launch, of 2^31 threads
+
 __global__ __launch_bounds__(256) void k_linear_pack(const uint16_t* __restrict__ scales,
                                                      const uint8_t* __restrict__ packed, int n, int k,
                                                      int group, uint8_t* __restrict__ nib,
                                                      uint16_t* __restrict__ sc, int chunks,
-                                                     int64_t lanes, unsigned long long* vkey) {
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                                                     int64_t block0, int64_t lanes,
+                                                     unsigned long long* vkey) {
+  const int64_t gid = (block0 + blockIdx.x) * 256 + threadIdx.x;
   if (gid >= lanes) return;
   const int lane = (int)(gid & 63);
   const int gq = (int)((gid >> 6) % chunks), rb = (int)((gid >> 6) / chunks);
@@ -534,16 +538,17 @@ hipError_t launch_linear_pack(const uint16_t* scales, const uint8_t* packed, int
                               uint8_t* nib, uint16_t* sc, unsigned long long* vkey, hipStream_t st) {
   const int chunks = linear_chunks(k);
   const int64_t lanes = (int64_t)linear_row_blocks(n) * chunks * 64;
-  k_linear_pack<<<(unsigned)((lanes + 255) / 256), 256, 0, st>>>(scales, packed, n, k, group, nib, sc,
-                                                                chunks, lanes, vkey);
+  const int64_t blocks = (lanes + 255) / 256;
+  for (int64_t b = 0; b < blocks; b += kMostBlocks)
+    k_linear_pack<<<(unsigned)std::min(kMostBlocks, blocks - b), 256, 0, st>>>(
+        scales, packed, n, k, group, nib, sc, chunks, b, lanes, vkey);
   return hipGetLastError();
 }
 
 bool linear_fits(const LinearDev& l, const dmh_linear_rows& r) {
   if (few_rows(l, r)) return true;
-  constexpr int64_t most = 1 << 23;  // workgroups of a launch, of 2^31 threads
-  return (int64_t)((l.row_blocks + 7) / 8) * ((r.rows + 63) / 64) < most &&
-         (int64_t)r.rows * (l.k / 8) < most * 256;
+  return (int64_t)((l.row_blocks + 7) / 8) * ((r.rows + 63) / 64) < kMostBlocks &&
+         (int64_t)r.rows * (l.k / 8) < kMostBlocks * 256;
 }
 
 size_t linear_bytes(const LinearDev& l, const dmh_linear_rows& r) {
