@@ -1121,7 +1121,11 @@ constexpr int64_t kMostBlocks = 1 << 23;  // workgroups of a launch, of 2^31 thr
 // Workgroups of k_attend_many: one a CU where its LDS fills that, else two.
 int many_groups(int dim) { return dim > 128 ? 256 : 512; }
 
-// Rows (tokens times query heads of a key head) up to which a sequence is k_attend_few's.
+// Rows (tokens times query heads of a key head) up to which a sequence is k_attend_few's.  8
+// sequences behind 80000 tokens in all, 16 heads on 2, bf16, at 24, 32, 40 and 64 rows: 18, 18, 20
+// and 21 us of 64 elements here, 39 to 44 by k_attend_many; 23, 24, 26 and 28 of 128, and 45 to 53;
+// 29, 29, 39 and 41 of 256, and 56 to 67.  One sequence behind 8000, 64 rows of 256: 25 and 48.
+// (At 96 and 128 rows the order is still the same: 28 and 31 for 45 and 47, 55 and 61 for 84 and 93.)
 int few_limit(const dmh_attention& a, const dmh_kv_cache& c) {
   return std::max(a.q_heads / c.kv_heads, 64);
 }
@@ -1132,6 +1136,11 @@ int few_blocks(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s, i
   const int64_t most = std::max<int64_t>(rep, std::min<int64_t>(64, s.max_len * rep));
   return (int)((most + 16 * mt - 1) / (16 * mt));
 }
+// Of how many 16s: one where sequences have 16 rows or fewer (two: 128 elements at 8 rows 18.1 ->
+// 19.5 us in bf16, 18.8 -> 29.9 in fp32), and of 256 elements, which leave no registers for two.
+// Two 16s make operands once: of 64 elements 64 rows take 21.3 us, one by one 23.2.  At 24 and 32
+// rows both take 18; of 128 elements two are slower there (22.4 and 21.2, in fp32 32.7 and 23.2, at
+// 64 rows 28.0 and 28.5, in fp32 38.9 and 32.6).
 int few_tiles(const dmh_attention& a, const dmh_kv_cache& c, const SeqDev& s) {
   const int64_t rep = a.q_heads / c.kv_heads;
   return c.dim <= 128 && s.max_len * rep > 16 ? 2 : 1;

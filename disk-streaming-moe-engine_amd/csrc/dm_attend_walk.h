@@ -23,8 +23,16 @@ namespace dm {
 
 constexpr int kManyRows = 128;       // rows of a block
 constexpr int kManyStep = 64;        // tokens of a step
-constexpr int64_t kUnitCost = 320;   // of beginning and ending a unit, in tokens of its context
-constexpr int64_t kShareCost = 512;  // the least that is worth a workgroup
+// What beginning and ending a unit costs, in tokens of its context, and the least that is given a
+// workgroup.  In us, 16 heads on 2 of 256 in bf16:
+//   unit  0, 160, 320, 640:        prefill of 2048 rows 247, 141, 124, 126; 4096 rows 596, 377, 301,
+//                                  312; 512 behind 16000 tokens 276, 273, 274, 271; 8 prompts of
+//                                  128 rows 169, 84, 74, 62
+//   share 128, 256, 512, 2048:     124, 126, 124, 154; 300, 300, 301, 300; 274, 274, 274, 275; 61, 63,
+//                                  74, 133; one prompt of 200 rows 39, 41, 58, 109
+// So few short prompts would take smaller shares, which change nothing for long ones.
+constexpr int64_t kUnitCost = 320;
+constexpr int64_t kShareCost = 512;
 
 // What a token costs, and by how much each block sees further than the one before it:
 // `rep` and 128, halved together while both can be (the tokens' cost is cut to a whole number

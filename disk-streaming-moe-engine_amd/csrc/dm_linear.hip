@@ -446,7 +446,7 @@ hipError_t many(const LinearDev& l, const dmh_linear_rows& r, void* ws, hipStrea
   };
   // Tiles of 192 by 128 take the least from memory for their products, as long as there
   // are enough of them; 128 by 64 fill the device sooner.  9216 x 2048, 512, 1024 and
-  // 2048 rows: 33, 51 and 88 us with the large ones, 35, 57 and 106 with the small; 2048
+  // 2048 rows: 33, 51 and 83 us with the large ones, 36, 59 and 107 with the small; 2048
   // x 4096, 1024 rows (88 large tiles): 55 and 32.
   using std::integral_constant;
   const int64_t large = (int64_t)((l.row_blocks + 11) / 12) * ((r.rows + 127) / 128);

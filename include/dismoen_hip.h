@@ -649,8 +649,12 @@ int dmh_kv_read(dmh_ctx* ctx, const dmh_kv_cache* cache, const dmh_kv_rows* rows
  * already: the row at position p, query head h with key head h / (q_heads / kv_heads),
  *   z_j = scale * q . k_j,   o = sum_j e^(z_j) v_j / sum_j e^(z_j),   j = 0 .. p,
  * and where gate is set o is multiplied by sigmoid(gate).  Positions behind p do not
- * enter, whatever they hold.  The bits of a row's result may differ with the rest of
- * the batch, which the work on long contexts is divided over.
+ * enter, whatever they hold.  Products are exact, but for parts of queries below 2^-126, which
+ * count as 0; sums are fp32, and a row with a q . k that fp32 does not hold may be NaN.  The
+ * bits of a row's result may differ with the rest of the batch, which the work on long contexts
+ * is divided over.  With R = q_heads / kv_heads a call is refused if total_tokens * R is 2^30
+ * or more, and may be if num_seqs * kv_heads * (r + 31) is 2^23 or more, r = min(max_seq_len * R,
+ * 64), or R where that is more.
  *
  * The calls work in device memory of the context, kept from call to call, of a size that
  * depends on the heads, dim and num_seqs and on no lengths: make a call of these before one is
@@ -694,7 +698,10 @@ int dmh_free_linear(dmh_ctx* ctx, dmh_linear* linear);
 /* Rows x [rows][in_features] of dtype to y [rows][out_features] of out_dtype (dtype or
  * DMH_DTYPE_F32).  Products are exact, but for parts of x below 2^-126, which count as 0;
  * sums are fp32, and y is rounded once.  An element that is not finite makes the results of
- * its row so, NaN where x is not bf16, and no other's.  Strides are in elements between rows. */
+ * its row so, NaN where x is not bf16, and no other's.  Strides are in elements between rows.
+ * Calls of many rows whose x is not bf16, or not 16-byte aligned, work in device memory of the
+ * context, kept from call to call: make one of the size before one is captured, and let
+ * replays of graphs that one context captured not overlap each other or its other calls. */
 typedef struct {
   int32_t dtype, out_dtype;
   int32_t rows;
